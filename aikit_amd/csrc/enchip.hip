@@ -20,14 +20,18 @@
 #include "attention_f32.h"
 #include "attention_flash.h"
 #include "encoder_ops.h"
+#include "gated.h"
 #include "gemm_f32.h"
+#include "gemm_gated.h"
 #include "gemm_persistent.h"
 #include "gemm_pieces.h"
 #include "gemm_q8w.h"
 #include "gemm_skinny.h"
+#include "rope.h"
 #include "topk.h"
 #include "kernels.h"
 #include "probes.h"
+#include "weight_only.h"
 
 namespace {
 
@@ -42,6 +46,20 @@ struct Weight {
     float *d_s = nullptr;   // [N]
     int64_t N = 0, K = 0, Np = 0, Kp = 0;
     bool inf_scale = false;  // some scale is +-inf: enchip_matmul_bt_q8 declines (see there)
+};
+
+// A weight of 4-bit codes and f16 group scales (enchip_weight4_register; weight_only.h).
+struct Weight4 {
+    int8_t *d_w = nullptr;    // [Np/64][Kp/32][64][16 B]
+    uint16_t *d_s = nullptr;  // f16 [Np/64][G][64]
+    int64_t N = 0, K = 0, group = 0, Np = 0, Kp = 0, G = 0;
+};
+
+// Rotary frequencies (enchip_rope_create).
+struct Rope {
+    double *d_turns = nullptr;  // [n] f_j / 2 pi
+    int64_t n = 0;              // pairs
+    float mscale = 1.0f;
 };
 
 thread_local std::string g_open_error = "no error";
@@ -119,6 +137,8 @@ struct enchip_ctx {
     int8_t *noalloc = nullptr;  // this device's address of `scratch` (NULL: unavailable)
     std::string noalloc_err;
     std::unordered_map<uint64_t, Weight> weights;
+    std::unordered_map<uint64_t, Weight4> weights4;  // handles of all kinds come from next_handle
+    std::unordered_map<uint64_t, Rope> ropes;
     // Attention kernels whose dynamic-LDS limit has been raised on this context's device
     // (hipFuncSetAttribute, once per kernel and byte count rather than once per launch).
     std::vector<std::pair<const void *, size_t>> lds_set;
@@ -894,6 +914,13 @@ int enchip_close(enchip_ctx *ctx) {
             (void)hipFree(kv.second.d_s);
         }
         ctx->weights.clear();
+        for (auto &kv : ctx->weights4) {
+            (void)hipFree(kv.second.d_w);
+            (void)hipFree(kv.second.d_s);
+        }
+        ctx->weights4.clear();
+        for (auto &kv : ctx->ropes) (void)hipFree(kv.second.d_turns);
+        ctx->ropes.clear();
         void *bufs[] = {ctx->d_aq,  ctx->d_as, ctx->d_a,     ctx->d_dst,     ctx->d_bias,
                         ctx->d_acc, ctx->d_fb, ctx->d_cand, ctx->d_hits};
         for (void *p : bufs)
@@ -2419,4 +2446,491 @@ int enchip_bias_act_rows_dev(enchip_ctx *ctx, float *d_x, int64_t ld, int64_t ro
                                d_bias);
     }
     return check_launch(ctx, "bias_act_rows");
+}
+
+// ---------------------------------------------------------------------------- rotary positions
+
+namespace {
+
+constexpr double kTwoPi = 6.283185307179586476925286766559;
+
+// Copies n frequencies to the device, in turns per position, under a new handle.
+int add_rope(enchip_ctx *ctx, const double *freqs, int64_t n, double mscale, enchip_rope *out) {
+    double turns[enchip::ROPE_MAX_PAIRS];
+    for (int64_t j = 0; j < n; ++j) {
+        if (!std::isfinite(freqs[j])) return fail(ctx, ENCHIP_ERR_ARG, "rope: frequency %lld is not finite", (long long)j);
+        turns[j] = freqs[j] / kTwoPi;
+    }
+    if (!std::isfinite(mscale) || !std::isfinite((float)mscale))
+        return fail(ctx, ENCHIP_ERR_ARG, "rope: mscale %g is not a finite f32", mscale);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    Rope r;
+    r.n = n;
+    r.mscale = (float)mscale;
+    size_t cap = 0;
+    if (int rc = ensure(ctx, &r.d_turns, &cap, (size_t)n * sizeof(double), false)) return rc;
+    const hipError_t e = hipMemcpy(r.d_turns, turns, (size_t)n * sizeof(double), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        (void)hipFree(r.d_turns);
+        return fail(ctx, ENCHIP_ERR_HIP, "rope upload: %s", hipGetErrorString(e));
+    }
+    try {
+        ctx->ropes[ctx->next_handle] = r;
+    } catch (const std::bad_alloc &) {
+        (void)hipFree(r.d_turns);
+        return fail(ctx, ENCHIP_ERR_OOM, "rope: out of host memory");
+    }
+    *out = ctx->next_handle++;
+    return ENCHIP_OK;
+}
+
+}  // namespace
+
+int enchip_rope_create(enchip_ctx *ctx, int64_t rot_dim, double base, int scaling, double factor, int64_t orig_len,
+                       enchip_rope *out) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (!out) return fail(ctx, ENCHIP_ERR_ARG, "rope_create: out is NULL");
+    *out = 0;
+    if (rot_dim < 2 || rot_dim % 2 != 0 || rot_dim > 2 * enchip::ROPE_MAX_PAIRS)
+        return fail(ctx, ENCHIP_ERR_ARG, "rope_create: rot_dim %lld must be even, from 2 to %d", (long long)rot_dim,
+                    2 * enchip::ROPE_MAX_PAIRS);
+    if (!(base > 0) || !std::isfinite(base)) return fail(ctx, ENCHIP_ERR_ARG, "rope_create: bad base %g", base);
+    if (scaling < ENCHIP_ROPE_NONE || scaling > ENCHIP_ROPE_YARN)
+        return fail(ctx, ENCHIP_ERR_ARG, "rope_create: bad scaling %d", scaling);
+    if (scaling != ENCHIP_ROPE_NONE && (!(factor >= 1) || !std::isfinite(factor)))
+        return fail(ctx, ENCHIP_ERR_ARG, "rope_create: factor %g must be at least 1", factor);
+    if (scaling == ENCHIP_ROPE_YARN && orig_len < 1)
+        return fail(ctx, ENCHIP_ERR_ARG, "rope_create: orig_len %lld must be positive", (long long)orig_len);
+    const double r = (double)rot_dim;
+    double b = base, mscale = 1.0;
+    if (scaling == ENCHIP_ROPE_NTK && rot_dim > 2) b = base * std::pow(factor, r / (r - 2.0));
+    if (scaling == ENCHIP_ROPE_YARN) mscale = 0.1 * std::log(factor) + 1.0;
+    double f[enchip::ROPE_MAX_PAIRS];
+    for (int64_t j = 0; j < rot_dim / 2; ++j) {
+        f[j] = std::pow(b, -2.0 * (double)j / r);
+        if (scaling == ENCHIP_ROPE_LINEAR) f[j] /= factor;
+        if (scaling == ENCHIP_ROPE_YARN) {
+            const double keep = std::min(1.0, std::max(0.0, ((double)orig_len * f[j] / kTwoPi - 1.0) / 31.0));
+            f[j] = f[j] * keep + f[j] / factor * (1.0 - keep);
+        }
+    }
+    return add_rope(ctx, f, rot_dim / 2, mscale, out);
+}
+
+int enchip_rope_create_freqs(enchip_ctx *ctx, const double *freqs, int64_t pairs, double mscale, enchip_rope *out) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (!out) return fail(ctx, ENCHIP_ERR_ARG, "rope_create_freqs: out is NULL");
+    *out = 0;
+    if (pairs < 1 || pairs > enchip::ROPE_MAX_PAIRS)
+        return fail(ctx, ENCHIP_ERR_ARG, "rope_create_freqs: %lld pairs, must be from 1 to %d", (long long)pairs,
+                    enchip::ROPE_MAX_PAIRS);
+    if (!freqs) return fail(ctx, ENCHIP_ERR_ARG, "rope_create_freqs: null pointer");
+    return add_rope(ctx, freqs, pairs, mscale, out);
+}
+
+int enchip_rope_release(enchip_ctx *ctx, enchip_rope h) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    auto it = ctx->ropes.find(h);
+    if (it == ctx->ropes.end()) return fail(ctx, ENCHIP_ERR_HANDLE, "unknown rope handle %llu", (unsigned long long)h);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    (void)hipFree(it->second.d_turns);
+    ctx->ropes.erase(it);
+    return ENCHIP_OK;
+}
+
+int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, const float *d_x, int64_t ldx, float *d_y,
+                         int64_t ldy, int64_t nseq, int64_t L, int64_t heads, int64_t head_dim, const int32_t *d_pos,
+                         int64_t pos0, void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    auto it = ctx->ropes.find(h);
+    if (it == ctx->ropes.end()) return fail(ctx, ENCHIP_ERR_HANDLE, "unknown rope handle %llu", (unsigned long long)h);
+    const Rope &r = it->second;
+    if (layout != ENCHIP_ROPE_HALF && layout != ENCHIP_ROPE_INTERLEAVED)
+        return fail(ctx, ENCHIP_ERR_ARG, "rope: bad layout %d", layout);
+    if (nseq < 0 || L < 0 || heads < 0 || head_dim < 2 * r.n || head_dim > 2 * enchip::ROPE_MAX_PAIRS || heads > 65536 ||
+        nseq > INT32_MAX || L > INT32_MAX || nseq * L > INT32_MAX ||
+        ldx < heads * head_dim || ldy < heads * head_dim)
+        return fail(ctx, ENCHIP_ERR_ARG,
+                    "rope: bad shape nseq=%lld L=%lld heads=%lld head_dim=%lld (%lld rotated, at most %d) ldx=%lld ldy=%lld",
+                    (long long)nseq, (long long)L, (long long)heads, (long long)head_dim, (long long)(2 * r.n),
+                    2 * enchip::ROPE_MAX_PAIRS, (long long)ldx, (long long)ldy);
+    if (!d_pos && (pos0 < -((int64_t)1 << 31) || pos0 > ((int64_t)1 << 31)))
+        return fail(ctx, ENCHIP_ERR_ARG, "rope: pos0=%lld past 32 bits", (long long)pos0);
+    if (d_x == d_y && ldx != ldy) return fail(ctx, ENCHIP_ERR_ARG, "rope: in place needs one pitch, not %lld and %lld",
+                                              (long long)ldx, (long long)ldy);
+    if (nseq == 0 || L == 0 || heads == 0) return ENCHIP_OK;
+    if (!d_x || !d_y) return fail(ctx, ENCHIP_ERR_ARG, "rope: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    const int64_t rows = nseq * L;
+    for (int64_t r0 = 0; r0 < rows; r0 += kRowChunk) {
+        const int64_t n = std::min(kRowChunk, rows - r0);
+#define ROPE_CALL(I)                                                                                                  \
+    hipLaunchKernelGGL(enchip::rope_rows<I>, dim3((unsigned)n), dim3(256), 0, s, d_x + r0 * ldx, ldx, d_y + r0 * ldy, \
+                       ldy, r.d_turns, r.mscale, d_pos ? d_pos + r0 : nullptr, pos0, r0, (int)L, n, (int)heads,       \
+                       (int)head_dim, (int)(2 * r.n))
+        if (layout == ENCHIP_ROPE_INTERLEAVED) ROPE_CALL(true);
+        else ROPE_CALL(false);
+#undef ROPE_CALL
+    }
+    return check_launch(ctx, "rope_rows");
+}
+
+// ---------------------------------------------------------------------------- 4-bit weights, gated projections
+
+namespace {
+
+int find_weight4(enchip_ctx *c, enchip_weight h, Weight4 **out) {
+    auto it = c->weights4.find(h);
+    if (it == c->weights4.end())
+        return fail(c, ENCHIP_ERR_HANDLE, "unknown 4-bit weight handle %llu", (unsigned long long)h);
+    *out = &it->second;
+    return ENCHIP_OK;
+}
+
+constexpr int64_t kMaxGateN = (int64_t)1 << 24;  // output channels: one launch covers them
+
+// What the weight-only products take of one or two weights of one shape.
+struct WoArgs {
+    int bits;
+    int64_t N, K, Np, Kp, cpg, G;  // cpg: 32-deep chunks per scale group
+    enchip::WoWeight w[2];
+};
+
+WoArgs wo_args(const Weight &a, const Weight &b) {
+    return {8, a.N, a.K, a.Np, a.Kp, 1, 1, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
+}
+
+WoArgs wo_args(const Weight4 &a, const Weight4 &b) {
+    return {4, a.N, a.K, a.Np, a.Kp, a.group / 32, a.G, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
+}
+
+// Enqueues C = A . W^T (4-bit), or the gated pair, after the caller checked the arguments.
+template <int BITS, bool GATED>
+int launch_wo(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda, const float *b0, const float *b1, int act,
+              float *C, int64_t ldc, int64_t M, hipStream_t s) {
+    using namespace enchip;
+    const int64_t units = p.Kp / (BITS == 4 ? 32 : 16);
+    const int tilesN = (int)((p.N + 15) / 16);
+    const int mb = M == 1 ? 1 : M == 2 ? 2 : 4;
+    const bool one = units <= 4 * WO_WAVES;
+    const int64_t rows = std::max<int64_t>(mb, (((int64_t)1 << 22) / tilesN) * mb);
+    for (int64_t r0 = 0; r0 < M; r0 += rows) {
+        const int64_t n = std::min(rows, M - r0);
+        const dim3 grid((unsigned)(((n + mb - 1) / mb) * tilesN));
+#define WO_CALL(MB, PF)                                                                                              \
+    hipLaunchKernelGGL((gemv_wo<BITS, MB, GATED, PF>), grid, dim3(64 * WO_WAVES), 0, s, A + r0 * lda, lda, p.w[0], p.w[1], \
+                       b0, b1, act, C + r0 * ldc, ldc, (int)n, (int)p.N, (int)p.K, (int)p.Kp, (int)p.cpg, (int)p.G, tilesN)
+        if (mb == 1 && one) WO_CALL(1, 1);
+        else if (mb == 1) WO_CALL(1, 4);
+        else if (mb == 2) WO_CALL(2, 2);
+        else WO_CALL(4, 2);
+#undef WO_CALL
+    }
+    return check_launch(c, "gemv_wo");
+}
+
+int check_rows(enchip_ctx *c, const char *what, int64_t M, int64_t N) {
+    if (M < 0 || M > kMaxDimF32 || M * N > ((int64_t)1 << 36))
+        return fail(c, ENCHIP_ERR_ARG, "%s: bad M=%lld for N=%lld", what, (long long)M, (long long)N);
+    return ENCHIP_OK;
+}
+
+int check_pitches(enchip_ctx *c, const char *what, int64_t lda, int64_t K, int64_t ldd, int64_t N) {
+    if (lda < K || ldd < N)
+        return fail(c, ENCHIP_ERR_ARG, "%s: pitches lda=%lld ldd=%lld must cover a row (K=%lld, N=%lld)", what,
+                    (long long)lda, (long long)ldd, (long long)K, (long long)N);
+    return ENCHIP_OK;
+}
+
+// The gate's code of an enchip_act, -1 for one that no gate takes.
+int gate_code(int act) {
+    return act == ENCHIP_ACT_SILU ? enchip::GATE_SILU : act == ENCHIP_ACT_GELU ? enchip::GATE_GELU : -1;
+}
+
+// The two int8 weights of a gated call.
+int find_gate(enchip_ctx *c, const char *what, enchip_weight hg, enchip_weight hu, Weight **g, Weight **u) {
+    int rc = find_weight(c, hg, g);
+    if (rc || (rc = find_weight(c, hu, u))) return rc;
+    if ((*g)->N != (*u)->N || (*g)->K != (*u)->K || (*g)->K == 0 || (*g)->N > kMaxGateN)
+        return fail(c, ENCHIP_ERR_ARG,
+                    "%s: the gate's weight is %lld x %lld, the up projection's %lld x %lld (one shape, K > 0, N <= 2^24)",
+                    what, (long long)(*g)->N, (long long)(*g)->K, (long long)(*u)->N, (long long)(*u)->K);
+    return ENCHIP_OK;
+}
+
+int find_gate(enchip_ctx *c, const char *what, enchip_weight hg, enchip_weight hu, Weight4 **g, Weight4 **u) {
+    int rc = find_weight4(c, hg, g);
+    if (rc || (rc = find_weight4(c, hu, u))) return rc;
+    if ((*g)->N != (*u)->N || (*g)->K != (*u)->K || (*g)->group != (*u)->group)
+        return fail(c, ENCHIP_ERR_ARG,
+                    "%s: the gate's weight is %lld x %lld in groups of %lld, the up projection's %lld x %lld of %lld (one shape)",
+                    what, (long long)(*g)->N, (long long)(*g)->K, (long long)(*g)->group, (long long)(*u)->N,
+                    (long long)(*u)->K, (long long)(*u)->group);
+    return ENCHIP_OK;
+}
+
+int check_gate_weight(enchip_ctx *c, const char *what, const Weight &w, int64_t M) { return check_q8w(c, what, w, M); }
+int check_gate_weight(enchip_ctx *c, const char *what, const Weight4 &w, int64_t M) { return check_rows(c, what, M, w.N); }
+
+// enchip_gated_q8_dev (W = Weight) and enchip_gated_q4_dev (W = Weight4).
+template <typename W>
+int gated_wo_dev(enchip_ctx *ctx, const char *what, enchip_weight gate, enchip_weight up, const float *d_a, int64_t lda,
+                 int64_t M, const float *bg, const float *bu, int act, float *d_dst, int64_t ldd, void *stream) {
+    std::lock_guard<std::mutex> g(ctx->mu);
+    W *wg, *wu;
+    int rc = find_gate(ctx, what, gate, up, &wg, &wu);
+    if (rc || (rc = check_gate_weight(ctx, what, *wg, M)) || (rc = check_gate_weight(ctx, what, *wu, M))) return rc;
+    if (gate_code(act) < 0) return fail(ctx, ENCHIP_ERR_ARG, "%s: act must be ENCHIP_ACT_SILU or ENCHIP_ACT_GELU, got %d", what, act);
+    if (M == 0) return ENCHIP_OK;
+    if ((rc = check_pitches(ctx, what, lda, wg->K, ldd, wg->N))) return rc;
+    if (!d_a || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "%s: null pointer", what);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    return launch_wo<std::is_same<W, Weight4>::value ? 4 : 8, true>(
+        ctx, wo_args(*wg, *wu), d_a, lda, bg, bu, gate_code(act), d_dst, ldd, M, s);
+}
+
+// The operands of a host gated call on the device: a in d_a, the biases in d_bias (N floats each).
+int gated_upload(enchip_ctx *ctx, const float *a, int64_t M, int64_t N, int64_t K, const float *bg, const float *bu,
+                 hipStream_t s) {
+    int rc;
+    if ((rc = ensure(ctx, &ctx->d_a, &ctx->a_cap, (size_t)(M * K) * sizeof(float)))) return rc;
+    if ((rc = ensure(ctx, &ctx->d_dst, &ctx->dst_cap, (size_t)(M * N) * sizeof(float)))) return rc;
+    if ((bg || bu) && (rc = ensure(ctx, &ctx->d_bias, &ctx->bias_cap, (size_t)(2 * N) * sizeof(float)))) return rc;
+    if ((rc = upload(ctx, ctx->d_a, a, (size_t)(M * K) * sizeof(float), s))) return rc;
+    if (bg && (rc = upload(ctx, ctx->d_bias, bg, (size_t)N * sizeof(float), s))) return rc;
+    if (bu && (rc = upload(ctx, ctx->d_bias + N, bu, (size_t)N * sizeof(float), s))) return rc;
+    return ENCHIP_OK;
+}
+
+template <typename W>
+int gated_wo_host(enchip_ctx *ctx, const char *what, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                  const float *bg, const float *bu, int act, float *dst) {
+    std::lock_guard<std::mutex> g(ctx->mu);
+    W *wg, *wu;
+    int rc = find_gate(ctx, what, gate, up, &wg, &wu);
+    if (rc || (rc = check_gate_weight(ctx, what, *wg, M)) || (rc = check_gate_weight(ctx, what, *wu, M))) return rc;
+    if (gate_code(act) < 0) return fail(ctx, ENCHIP_ERR_ARG, "%s: act must be ENCHIP_ACT_SILU or ENCHIP_ACT_GELU, got %d", what, act);
+    if (M == 0) return ENCHIP_OK;
+    if (!a || !dst) return fail(ctx, ENCHIP_ERR_ARG, "%s: null pointer", what);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = ctx->stream;
+    const int64_t N = wg->N, K = wg->K;
+    if ((rc = gated_upload(ctx, a, M, N, K, bg, bu, s))) return rc;
+    if ((rc = launch_wo<std::is_same<W, Weight4>::value ? 4 : 8, true>(
+             ctx, wo_args(*wg, *wu), ctx->d_a, K, bg ? ctx->d_bias : nullptr, bu ? ctx->d_bias + N : nullptr,
+             gate_code(act), ctx->d_dst, N, M, s)))
+        return rc;
+    if ((rc = download(ctx, dst, ctx->d_dst, (size_t)(M * N) * sizeof(float), s))) return rc;
+    HIP_TRY(ctx, hipStreamSynchronize(s));
+    return ENCHIP_OK;
+}
+
+// Enqueues the W8A8 gated pair on d_a [M][K] after the caller checked the arguments.
+int launch_gated_w8a8(enchip_ctx *c, const Weight &wg, const Weight &wu, const float *d_a, int64_t M, const float *bg,
+                      const float *bu, int act, float *d_dst, hipStream_t s) {
+    int rc;
+    if ((rc = ensure_act_scratch(c, M, wg.Kp))) return rc;
+    if ((rc = scratch_wait(c, s))) return rc;
+    if ((rc = launch_quant(c, d_a, M, wg.K, c->d_aq, wg.Kp, c->d_as, s, true))) return rc;
+    const enchip::GatePair p = {{wg.d_w, wu.d_w}, {wg.d_s, wu.d_s}, {bg, bu}};
+    const int pn = (int)((wg.N + 31) / 32);
+    const int64_t rows = std::max<int64_t>(32, (((int64_t)1 << 23) / pn) * 32);
+    for (int64_t r0 = 0; r0 < M; r0 += rows) {
+        const int64_t n = std::min(rows, M - r0);
+        hipLaunchKernelGGL((enchip::gated_w8a8_piece<32, 32, 4>), dim3((unsigned)((n + 31) / 32 * pn)), dim3(256), 0, s,
+                           c->d_aq + r0 * wg.Kp, c->d_as + r0, p, act, d_dst + r0 * wg.N, wg.N, (int)n, (int)wg.N,
+                           (int)wg.Kp, pn);
+    }
+    if ((rc = check_launch(c, "gated_w8a8"))) return rc;
+    return scratch_record(c, s);
+}
+
+}  // namespace
+
+int enchip_weight4_register(enchip_ctx *ctx, const uint8_t *codes, const uint16_t *scales, int64_t N, int64_t K,
+                            int64_t group, enchip_weight *out) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (!out) return fail(ctx, ENCHIP_ERR_ARG, "weight4_register: out is NULL");
+    *out = 0;
+    if (N <= 0 || K <= 0 || K > kMaxK || N > kMaxGateN || round_up(N, kColPad) * round_up(K, 64) > ((int64_t)1 << 36) ||
+        group < 32 || group % 32 != 0 || group > (1 << 20))
+        return fail(ctx, ENCHIP_ERR_ARG, "weight4_register: bad shape N=%lld K=%lld group=%lld (a multiple of 32)",
+                    (long long)N, (long long)K, (long long)group);
+    if (!codes || !scales) return fail(ctx, ENCHIP_ERR_ARG, "weight4_register: null pointer");
+    Weight4 w;
+    w.N = N;
+    w.K = K;
+    w.group = group;
+    w.Np = round_up(N, kColPad);
+    w.Kp = round_up(K, 64);
+    w.G = (K + group - 1) / group;
+    for (int64_t i = 0; i < N * w.G; ++i)
+        if ((scales[i] & 0x7c00) == 0x7c00)
+            return fail(ctx, ENCHIP_ERR_ARG, "weight4_register: scale %lld is not finite", (long long)i);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    const size_t cb = (size_t)(N * ((K + 1) / 2)), sb = (size_t)(N * w.G) * 2;
+    uint8_t *t_c = nullptr;
+    uint16_t *t_s = nullptr;
+    size_t c1 = 0, c2 = 0, c3 = 0, c4 = 0;
+    int rc;
+    if (!(rc = ensure(ctx, &w.d_w, &c1, (size_t)(w.Np * w.Kp / 2), false)) &&
+        !(rc = ensure(ctx, &w.d_s, &c2, (size_t)(w.Np * w.G) * 2, false)) && !(rc = ensure(ctx, &t_c, &c3, cb, false)) &&
+        !(rc = ensure(ctx, &t_s, &c4, sb, false))) {
+        hipStream_t s = ctx->stream;
+        if (!(rc = upload(ctx, t_c, codes, cb, s)) && !(rc = upload(ctx, t_s, scales, sb, s))) {
+            const int64_t tw = w.Np * w.Kp / 32, ts = w.Np * w.G;
+            hipLaunchKernelGGL(enchip::q4_image, dim3((unsigned)((tw + 255) / 256)), dim3(256), 0, s, t_c,
+                               reinterpret_cast<uint4 *>(w.d_w), (int)N, (int)K, (int)(w.Kp / 32), tw);
+            hipLaunchKernelGGL(enchip::q4_scales, dim3((unsigned)((ts + 255) / 256)), dim3(256), 0, s, t_s, w.d_s, (int)N,
+                               (int)w.G, ts);
+            rc = check_launch(ctx, "q4_image");
+        }
+        const hipError_t e = hipStreamSynchronize(s);  // also the caller's memory is no longer read
+        if (!rc && e != hipSuccess) rc = fail(ctx, ENCHIP_ERR_HIP, "weight4 upload: %s", hipGetErrorString(e));
+    }
+    if (t_c) (void)hipFree(t_c);
+    if (t_s) (void)hipFree(t_s);
+    if (!rc) try {
+            ctx->weights4[ctx->next_handle] = w;
+        } catch (const std::bad_alloc &) {
+            rc = fail(ctx, ENCHIP_ERR_OOM, "weight4_register: out of host memory");
+        }
+    if (rc) {
+        if (w.d_w) (void)hipFree(w.d_w);
+        if (w.d_s) (void)hipFree(w.d_s);
+        return rc;
+    }
+    *out = ctx->next_handle++;
+    return ENCHIP_OK;
+}
+
+int enchip_weight4_release(enchip_ctx *ctx, enchip_weight h) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight4 *w;
+    int rc = find_weight4(ctx, h, &w);
+    if (rc) return rc;
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    (void)hipFree(w->d_w);
+    (void)hipFree(w->d_s);
+    ctx->weights4.erase(h);
+    return ENCHIP_OK;
+}
+
+int enchip_weight4_shape(enchip_ctx *ctx, enchip_weight h, int64_t *N, int64_t *K, int64_t *group) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight4 *w;
+    int rc = find_weight4(ctx, h, &w);
+    if (rc) return rc;
+    if (N) *N = w->N;
+    if (K) *K = w->K;
+    if (group) *group = w->group;
+    return ENCHIP_OK;
+}
+
+int enchip_matmul_bt_q4(enchip_ctx *ctx, enchip_weight h, const float *a, int64_t M, float *dst) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight4 *w;
+    int rc = find_weight4(ctx, h, &w);
+    if (rc || (rc = check_rows(ctx, "matmul_bt_q4", M, w->N))) return rc;
+    if (M == 0) return ENCHIP_OK;
+    if (!dst || !a) return fail(ctx, ENCHIP_ERR_ARG, "matmul_bt_q4: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = ctx->stream;
+    if ((rc = gated_upload(ctx, a, M, w->N, w->K, nullptr, nullptr, s))) return rc;
+    if ((rc = launch_wo<4, false>(ctx, wo_args(*w, *w), ctx->d_a, w->K, nullptr, nullptr, 0, ctx->d_dst, w->N, M, s)))
+        return rc;
+    if ((rc = download(ctx, dst, ctx->d_dst, (size_t)(M * w->N) * sizeof(float), s))) return rc;
+    HIP_TRY(ctx, hipStreamSynchronize(s));
+    return ENCHIP_OK;
+}
+
+int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight h, const float *d_a, int64_t lda, int64_t M, float *d_dst,
+                            int64_t ldd, void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight4 *w;
+    int rc = find_weight4(ctx, h, &w);
+    if (rc || (rc = check_rows(ctx, "matmul_bt_q4_dev", M, w->N))) return rc;
+    if (M == 0) return ENCHIP_OK;
+    if ((rc = check_pitches(ctx, "matmul_bt_q4_dev", lda, w->K, ldd, w->N))) return rc;
+    if (!d_dst || !d_a) return fail(ctx, ENCHIP_ERR_ARG, "matmul_bt_q4_dev: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    return launch_wo<4, false>(ctx, wo_args(*w, *w), d_a, lda, nullptr, nullptr, 0, d_dst, ldd, M, s);
+}
+
+int enchip_gated_q8(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                    const float *bias_gate, const float *bias_up, int act, float *dst) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    return gated_wo_host<Weight>(ctx, "gated_q8", gate, up, a, M, bias_gate, bias_up, act, dst);
+}
+
+int enchip_gated_q8_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a, int64_t lda, int64_t M,
+                        const float *d_bias_gate, const float *d_bias_up, int act, float *d_dst, int64_t ldd,
+                        void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    return gated_wo_dev<Weight>(ctx, "gated_q8_dev", gate, up, d_a, lda, M, d_bias_gate, d_bias_up, act, d_dst, ldd, stream);
+}
+
+int enchip_gated_q4(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                    const float *bias_gate, const float *bias_up, int act, float *dst) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    return gated_wo_host<Weight4>(ctx, "gated_q4", gate, up, a, M, bias_gate, bias_up, act, dst);
+}
+
+int enchip_gated_q4_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a, int64_t lda, int64_t M,
+                        const float *d_bias_gate, const float *d_bias_up, int act, float *d_dst, int64_t ldd,
+                        void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    return gated_wo_dev<Weight4>(ctx, "gated_q4_dev", gate, up, d_a, lda, M, d_bias_gate, d_bias_up, act, d_dst, ldd, stream);
+}
+
+int enchip_w8a8_gated(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                      const float *bias_gate, const float *bias_up, int act, float *dst) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight *wg, *wu;
+    int rc = find_gate(ctx, "w8a8_gated", gate, up, &wg, &wu);
+    if (rc || (rc = check_rows(ctx, "w8a8_gated", M, wg->N))) return rc;
+    if (gate_code(act) < 0) return fail(ctx, ENCHIP_ERR_ARG, "w8a8_gated: act must be ENCHIP_ACT_SILU or ENCHIP_ACT_GELU, got %d", act);
+    if (M == 0) return ENCHIP_OK;
+    if (!a || !dst) return fail(ctx, ENCHIP_ERR_ARG, "w8a8_gated: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = ctx->stream;
+    const int64_t N = wg->N, K = wg->K;
+    if ((rc = gated_upload(ctx, a, M, N, K, bias_gate, bias_up, s))) return rc;
+    if ((rc = launch_gated_w8a8(ctx, *wg, *wu, ctx->d_a, M, bias_gate ? ctx->d_bias : nullptr,
+                                bias_up ? ctx->d_bias + N : nullptr, gate_code(act), ctx->d_dst, s)))
+        return rc;
+    if ((rc = download(ctx, dst, ctx->d_dst, (size_t)(M * N) * sizeof(float), s))) return rc;
+    HIP_TRY(ctx, hipStreamSynchronize(s));
+    return ENCHIP_OK;
+}
+
+int enchip_w8a8_gated_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a, int64_t M,
+                          const float *d_bias_gate, const float *d_bias_up, int act, float *d_dst, void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight *wg, *wu;
+    int rc = find_gate(ctx, "w8a8_gated_dev", gate, up, &wg, &wu);
+    if (rc || (rc = check_rows(ctx, "w8a8_gated_dev", M, wg->N))) return rc;
+    if (gate_code(act) < 0)
+        return fail(ctx, ENCHIP_ERR_ARG, "w8a8_gated_dev: act must be ENCHIP_ACT_SILU or ENCHIP_ACT_GELU, got %d", act);
+    if (M == 0) return ENCHIP_OK;
+    if (!d_a || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "w8a8_gated_dev: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    return launch_gated_w8a8(ctx, *wg, *wu, d_a, M, d_bias_gate, d_bias_up, gate_code(act), d_dst, s);
 }

@@ -22,14 +22,17 @@ import numpy as np
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libenchip.so")
 
 OK, ERR_NO_DEVICE, ERR_ARG, ERR_HIP, ERR_OOM, ERR_HANDLE = range(6)
-ACT_NONE, ACT_GELU, ACT_TANH = 0, 1, 2
+ACT_NONE, ACT_GELU, ACT_TANH, ACT_SILU = 0, 1, 2, 3
 ATT_F32, ATT_SPLIT_BF16, ATT_FLASH_BF16, ATT_FLASH_F16 = 0, 1, 2, 3  # enchip_att_products
 ATT_DEFAULT = ATT_FLASH_F16  # the library's default
 B_NK, B_KN = 0, 1  # enchip_matmul_bt_f32_dev b layouts: b[N,K] rows, b[K,N] rows
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1  # enchip_rope_layout
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3  # enchip_rope_scaling
 ABI_VERSION = 3
 
 # Every symbol include/enchip.h declares, with (restype, argtypes).
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_u64, _f64 = ctypes.c_uint64, ctypes.c_double
 _SIGNATURES = {
     "enchip_abi_version": (_int, []),
     "enchip_open": (_int, [_int, ctypes.POINTER(_vp)]),
@@ -77,6 +80,21 @@ _SIGNATURES = {
     "enchip_w8a8_linear_noalloc_dev": (_int, [_vp, ctypes.c_uint64, _vp, _i64, _vp, _int, _vp, _vp]),
     "enchip_matmul_bt_q8": (_int, [_vp, ctypes.c_uint64, _vp, _i64, _vp]),
     "enchip_matmul_bt_q8_dev": (_int, [_vp, ctypes.c_uint64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "enchip_rope_create": (_int, [_vp, _i64, _f64, _int, _f64, _i64, ctypes.POINTER(_u64)]),
+    "enchip_rope_create_freqs": (_int, [_vp, _vp, _i64, _f64, ctypes.POINTER(_u64)]),
+    "enchip_rope_release": (_int, [_vp, _u64]),
+    "enchip_rope_rows_dev": (_int, [_vp, _u64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "enchip_weight4_register": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, ctypes.POINTER(_u64)]),
+    "enchip_weight4_release": (_int, [_vp, _u64]),
+    "enchip_weight4_shape": (_int, [_vp, _u64, ctypes.POINTER(_i64), ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
+    "enchip_matmul_bt_q4": (_int, [_vp, _u64, _vp, _i64, _vp]),
+    "enchip_matmul_bt_q4_dev": (_int, [_vp, _u64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "enchip_gated_q8": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp]),
+    "enchip_gated_q8_dev": (_int, [_vp, _u64, _u64, _vp, _i64, _i64, _vp, _vp, _int, _vp, _i64, _vp]),
+    "enchip_gated_q4": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp]),
+    "enchip_gated_q4_dev": (_int, [_vp, _u64, _u64, _vp, _i64, _i64, _vp, _vp, _int, _vp, _i64, _vp]),
+    "enchip_w8a8_gated": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp]),
+    "enchip_w8a8_gated_dev": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp, _vp]),
 }
 SYMBOLS = tuple(_SIGNATURES)
 
@@ -140,6 +158,22 @@ class Weight:
     handle: int
     N: int
     K: int
+
+
+@dataclass(frozen=True)
+class Weight4:
+    """A registered weight of 4-bit codes and f16 group scales."""
+    handle: int
+    N: int
+    K: int
+    group: int
+
+
+@dataclass(frozen=True)
+class Rope:
+    """Rotary frequencies for the first rot_dim elements of a head."""
+    handle: int
+    rot_dim: int
 
 
 class Context:
@@ -430,3 +464,110 @@ class Context:
     def linear_dev(self, w: Weight, d_a: int, M: int, d_bias: int, act: int, d_dst: int, stream: int = 0) -> None:
         self._check(self._lib.enchip_w8a8_linear_dev(self._h, w.handle, d_a, M, d_bias or None, act, d_dst,
                                                      stream or None))
+
+    # -- rotary positions ---------------------------------------------------------
+    def rope(self, rot_dim: int, base: float = 10000.0, scaling: int = ROPE_NONE, factor: float = 1.0,
+             orig_len: int = 0) -> Rope:
+        """Frequencies base^(-2j / rot_dim), stretched as enchip_rope_scaling says."""
+        out = _u64()
+        self._check(self._lib.enchip_rope_create(self._h, rot_dim, base, scaling, factor, orig_len, ctypes.byref(out)))
+        return Rope(out.value, rot_dim)
+
+    def rope_from_freqs(self, freqs, mscale: float = 1.0) -> Rope:
+        """The caller's own frequencies (radians per position, one per pair)."""
+        f = np.ascontiguousarray(freqs, dtype=np.float64)
+        if f.ndim != 1:
+            raise ValueError(f"freqs shape {f.shape} is not one-dimensional")
+        out = _u64()
+        self._check(self._lib.enchip_rope_create_freqs(self._h, _ptr(f), f.size, mscale, ctypes.byref(out)))
+        return Rope(out.value, 2 * f.size)
+
+    def release_rope(self, r: Rope) -> None:
+        self._check(self._lib.enchip_rope_release(self._h, r.handle))
+
+    def rope_rows_dev(self, r: Rope, layout: int, d_x: int, ldx: int, d_y: int, ldy: int, nseq: int, L: int, heads: int,
+                      head_dim: int, d_pos: int = 0, pos0: int = 0, stream: int = 0) -> None:
+        """Rotates rows of heads (d_y == d_x: in place); positions d_pos (int32 per row) or pos0 + i."""
+        self._check(self._lib.enchip_rope_rows_dev(self._h, r.handle, layout, d_x or None, ldx, d_y or None, ldy, nseq, L,
+                                                   heads, head_dim, d_pos or None, pos0, stream or None))
+
+    # -- 4-bit weights and gated projections ------------------------------------------
+    def register_weight4(self, codes: np.ndarray, scales: np.ndarray, K: int, group: int) -> Weight4:
+        """codes uint8 [N, ceil(K/2)] (c - 8, low half first), scales float16 [N, ceil(K/group)]."""
+        codes = np.ascontiguousarray(codes, dtype=np.uint8)
+        scales = np.ascontiguousarray(scales, dtype=np.float16)
+        if codes.ndim != 2 or group < 1 or codes.shape[1] != (K + 1) // 2:
+            raise ValueError(f"codes shape {codes.shape} is not (N, {(K + 1) // 2})")
+        N = codes.shape[0]
+        if scales.shape != (N, -(-K // group)):
+            raise ValueError(f"scales shape {scales.shape} != ({N}, {-(-K // group)})")
+        out = _u64()
+        self._check(self._lib.enchip_weight4_register(self._h, _ptr(codes), _ptr(scales), N, K, group, ctypes.byref(out)))
+        return Weight4(out.value, N, K, group)
+
+    def release_weight4(self, w: Weight4) -> None:
+        self._check(self._lib.enchip_weight4_release(self._h, w.handle))
+
+    def weight4_shape(self, w: Weight4):
+        n, k, g = _i64(), _i64(), _i64()
+        self._check(self._lib.enchip_weight4_shape(self._h, w.handle, ctypes.byref(n), ctypes.byref(k), ctypes.byref(g)))
+        return n.value, k.value, g.value
+
+    def matmul_bt_q4(self, w: Weight4, a: np.ndarray) -> np.ndarray:
+        """f32 a[M, K] times the 4-bit weight w widened; the activations stay f32."""
+        a = np.ascontiguousarray(a, dtype=np.float32)
+        M = a.shape[0] if a.ndim == 2 else -1
+        if a.shape != (M, w.K):
+            raise ValueError(f"matmul_bt_q4: a shape {a.shape} != (M, {w.K})")
+        dst = np.empty((M, w.N), np.float32)
+        self._check(self._lib.enchip_matmul_bt_q4(self._h, w.handle, _ptr(a), M, _ptr(dst)))
+        return dst
+
+    def matmul_bt_q4_dev(self, w: Weight4, d_a: int, lda: int, M: int, d_dst: int, ldd: int, stream: int = 0) -> None:
+        self._check(self._lib.enchip_matmul_bt_q4_dev(self._h, w.handle, d_a or None, lda, M, d_dst or None, ldd,
+                                                      stream or None))
+
+    def _gated(self, call, gate, up, a, bias_gate, bias_up, act):
+        a = np.ascontiguousarray(a, dtype=np.float32)
+        M = a.shape[0] if a.ndim == 2 else -1
+        if a.shape != (M, gate.K):
+            raise ValueError(f"gated: a shape {a.shape} != (M, {gate.K})")
+        b = [None if x is None else np.ascontiguousarray(x, dtype=np.float32) for x in (bias_gate, bias_up)]
+        for x in b:
+            if x is not None and x.shape != (gate.N,):
+                raise ValueError(f"gated: bias shape {x.shape} != ({gate.N},)")
+        dst = np.empty((M, gate.N), np.float32)
+        self._check(call(self._h, gate.handle, up.handle, _ptr(a), M, _ptr(b[0]), _ptr(b[1]), act, _ptr(dst)))
+        return dst
+
+    def gated_q8(self, gate: Weight, up: Weight, a: np.ndarray, bias_gate: Optional[np.ndarray] = None,
+                 bias_up: Optional[np.ndarray] = None, act: int = ACT_SILU) -> np.ndarray:
+        """act(a Wg^T + bg) * (a Wu^T + bu), int8 weights, f32 activations."""
+        return self._gated(self._lib.enchip_gated_q8, gate, up, a, bias_gate, bias_up, act)
+
+    def gated_q4(self, gate: Weight4, up: Weight4, a: np.ndarray, bias_gate: Optional[np.ndarray] = None,
+                 bias_up: Optional[np.ndarray] = None, act: int = ACT_SILU) -> np.ndarray:
+        """gated_q8 with 4-bit weights."""
+        return self._gated(self._lib.enchip_gated_q4, gate, up, a, bias_gate, bias_up, act)
+
+    def w8a8_gated(self, gate: Weight, up: Weight, a: np.ndarray, bias_gate: Optional[np.ndarray] = None,
+                   bias_up: Optional[np.ndarray] = None, act: int = ACT_SILU) -> np.ndarray:
+        """gated_q8 with the activations quantized per token (once for both projections)."""
+        return self._gated(self._lib.enchip_w8a8_gated, gate, up, a, bias_gate, bias_up, act)
+
+    def gated_q8_dev(self, gate: Weight, up: Weight, d_a: int, lda: int, M: int, d_bias_gate: int, d_bias_up: int,
+                     act: int, d_dst: int, ldd: int, stream: int = 0) -> None:
+        self._check(self._lib.enchip_gated_q8_dev(self._h, gate.handle, up.handle, d_a or None, lda, M,
+                                                  d_bias_gate or None, d_bias_up or None, act, d_dst or None, ldd,
+                                                  stream or None))
+
+    def gated_q4_dev(self, gate: Weight4, up: Weight4, d_a: int, lda: int, M: int, d_bias_gate: int, d_bias_up: int,
+                     act: int, d_dst: int, ldd: int, stream: int = 0) -> None:
+        self._check(self._lib.enchip_gated_q4_dev(self._h, gate.handle, up.handle, d_a or None, lda, M,
+                                                  d_bias_gate or None, d_bias_up or None, act, d_dst or None, ldd,
+                                                  stream or None))
+
+    def w8a8_gated_dev(self, gate: Weight, up: Weight, d_a: int, M: int, d_bias_gate: int, d_bias_up: int, act: int,
+                       d_dst: int, stream: int = 0) -> None:
+        self._check(self._lib.enchip_w8a8_gated_dev(self._h, gate.handle, up.handle, d_a or None, M, d_bias_gate or None,
+                                                    d_bias_up or None, act, d_dst or None, stream or None))

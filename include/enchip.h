@@ -61,7 +61,8 @@ enum enchip_status {
 enum enchip_act {
     ENCHIP_ACT_NONE = 0,
     ENCHIP_ACT_GELU = 1, /* exact-erf GELU, linalg.GELUF32 */
-    ENCHIP_ACT_TANH = 2  /* linalg.TanhF32; enchip_bias_act_rows_dev only */
+    ENCHIP_ACT_TANH = 2, /* linalg.TanhF32; enchip_bias_act_rows_dev only */
+    ENCHIP_ACT_SILU = 3  /* x / (1 + e^-x); the gated projections only */
 };
 
 /* Layout of the b operand of enchip_matmul_bt_f32_dev. */
@@ -492,6 +493,104 @@ int enchip_ann_topk(enchip_ctx *ctx, enchip_weight index, const float *queries, 
  * scoring higher). Both routes give identical results. No reference counterpart: a
  * diagnostic. */
 int enchip_ann_topk_stats(enchip_ctx *ctx, int64_t *fused, int64_t *fallbacks);
+
+/* ---- rotary positions ----------------------------------------------------------
+ * Frequencies are made once: a handle holds f_j, j < rot_dim / 2, in 64 bits and an f32
+ * factor mscale of the rotated values. enchip_rope_rows_dev turns pair j of every head of the
+ * row at position p by the angle p f_j:
+ *   y1 = mscale (x1 cos - x2 sin),  y2 = mscale (x2 cos + x1 sin).
+ * The angle is formed and reduced in 64 bits, so a far position is as exact as a near one
+ * (about 2^-22 of the pair's length). The reference's rotary encoders keep a table in f32
+ * (encoder's NomicBERT forward); parity with its table's last bits is not pinned. */
+typedef uint64_t enchip_rope; /* opaque handle; 0 is never a valid handle */
+
+enum enchip_rope_layout {
+    ENCHIP_ROPE_HALF = 0,       /* pair j = elements (j, j + rot_dim / 2) of the head */
+    ENCHIP_ROPE_INTERLEAVED = 1 /* pair j = elements (2j, 2j + 1) */
+};
+
+/* How enchip_rope_create stretches f_j = base^(-2j / rot_dim) to contexts `factor` times as long
+ * as a model was trained on. */
+enum enchip_rope_scaling {
+    ENCHIP_ROPE_NONE = 0,   /* factor and orig_len are not read */
+    ENCHIP_ROPE_LINEAR = 1, /* f_j / factor */
+    ENCHIP_ROPE_NTK = 2,    /* base factor^(rot_dim / (rot_dim - 2)) in place of base (rot_dim > 2) */
+    ENCHIP_ROPE_YARN = 3    /* f_j (w + (1 - w) / factor), w = clamp((orig_len f_j / 2 pi - 1) / 31, 0, 1):
+                               pairs that turn over 32 times within orig_len keep their frequency, those
+                               that do not turn once are divided; mscale = 0.1 ln(factor) + 1 */
+};
+
+/* rot_dim even, 2 .. 1024; base > 0; factor >= 1; orig_len >= 1 (YARN). */
+int enchip_rope_create(enchip_ctx *ctx, int64_t rot_dim, double base, int scaling, double factor,
+                       int64_t orig_len, enchip_rope *out);
+
+/* The caller's own frequencies freqs[pairs] (rot_dim = 2 pairs) and mscale: any other schedule. */
+int enchip_rope_create_freqs(enchip_ctx *ctx, const double *freqs, int64_t pairs, double mscale,
+                             enchip_rope *out);
+int enchip_rope_release(enchip_ctx *ctx, enchip_rope rope);
+
+/* Rows z*L + i (sequence z < nseq, i < L) of `heads` heads of head_dim floats, at d_x + row*ldx,
+ * into d_y + row*ldy. Elements rot_dim .. head_dim of a head are copied. A row's position is
+ * d_pos[row] (any int32), or pos0 + i when d_pos is NULL. d_y == d_x with ldy == ldx rotates in
+ * place; otherwise the two hold no element in common. The query and key heads of fused
+ * [tokens, 3D] QKV rows are one call with heads = 2D / head_dim. head_dim <= 1024, heads <=
+ * 65536, nseq * L < 2^31. */
+int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope rope, int layout, const float *d_x, int64_t ldx,
+                         float *d_y, int64_t ldy, int64_t nseq, int64_t L, int64_t heads,
+                         int64_t head_dim, const int32_t *d_pos, int64_t pos0, void *stream);
+
+/* ---- 4-bit weights with group scales ---------------------------------------------
+ * codes[N][ceil(K / 2)]: two codes c in 0 .. 15 a byte, the lower k in the low half, each
+ * standing for c - 8 (the high half of an odd K's last byte is not read). scales[N][ceil(K /
+ * group)]: IEEE half bits, one for every `group` k's of a channel (a multiple of 32, at most
+ * 2^20; the last group may be short); an infinite or NaN scale is refused. The reference's
+ * 4-bit weights with f16 group scales are linalg's Q4 / gpu's gemv_w4a8_fwd (gpu/gemv_quant.cu:
+ * 40-93). The context keeps its own copy. Handles are not those of enchip_weight_register:
+ * each entry point takes its own kind. 0 < K <= 131072, 0 < N <= 2^24, N K <= 2^36 (rounded up to
+ * 256 and 64). */
+int enchip_weight4_register(enchip_ctx *ctx, const uint8_t *codes, const uint16_t *scales, int64_t N,
+                            int64_t K, int64_t group, enchip_weight *out);
+int enchip_weight4_release(enchip_ctx *ctx, enchip_weight w);
+int enchip_weight4_shape(enchip_ctx *ctx, enchip_weight w, int64_t *N, int64_t *K, int64_t *group);
+
+/* dst[m][n] = sum_k a[m][k] * (c[n][k] - 8) * scale[n][k / group] on host buffers, with f32
+ * activations (never quantized), as enchip_matmul_bt_q8 is for int8 weights: a group's sum is
+ * accumulated in f32 and scaled once, in an order of its own; the same gate against a float64
+ * dot product. */
+int enchip_matmul_bt_q4(enchip_ctx *ctx, enchip_weight w, const float *a, int64_t M, float *dst);
+
+/* Device form: d_a[M,K] with row pitch lda >= K, d_dst[M,N] with row pitch ldd >= N, on `stream`.
+ * Allocates nothing. */
+int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, int64_t lda, int64_t M,
+                            float *d_dst, int64_t ldd, void *stream);
+
+/* ---- gated projections ------------------------------------------------------------
+ * The first half of a gated feed-forward block (encoder/forward_q8.go:264-279 swigluMLPQ8, up to
+ * the down projection), both projections, the activation and the product in one call:
+ *   dst[m][n] = act(yg[m][n]) * yu[m][n],  y = a . W^T (+ bias[n], nullable).
+ * act: ENCHIP_ACT_SILU (x / (1 + e^-x)) or ENCHIP_ACT_GELU (linalg.GELUF32). Both weights have one
+ * shape (and group), K > 0, N <= 2^24; the same handle may be both. dst holds no element of a.
+ *   gated_q8    int8 weights, f32 activations: y as enchip_matmul_bt_q8 defines it
+ *   gated_q4    4-bit weights, f32 activations: y as enchip_matmul_bt_q4 defines it
+ *   w8a8_gated  int8 weights, activations quantized per token: y bit-identical to
+ *               enchip_w8a8_linear's, one quantization shared by both projections
+ * The device forms of gated_q8 and gated_q4 allocate nothing; w8a8_gated_dev uses the context's
+ * shared scratch, as enchip_w8a8_linear_dev does. */
+int enchip_gated_q8(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                    const float *bias_gate, const float *bias_up, int act, float *dst);
+int enchip_gated_q8_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a,
+                        int64_t lda, int64_t M, const float *d_bias_gate, const float *d_bias_up,
+                        int act, float *d_dst, int64_t ldd, void *stream);
+int enchip_gated_q4(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                    const float *bias_gate, const float *bias_up, int act, float *dst);
+int enchip_gated_q4_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a,
+                        int64_t lda, int64_t M, const float *d_bias_gate, const float *d_bias_up,
+                        int act, float *d_dst, int64_t ldd, void *stream);
+int enchip_w8a8_gated(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
+                      const float *bias_gate, const float *bias_up, int act, float *dst);
+int enchip_w8a8_gated_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a,
+                          int64_t M, const float *d_bias_gate, const float *d_bias_up, int act,
+                          float *d_dst, void *stream);
 
 /* Caps each growable device scratch buffer of the context at `bytes` (0, the default:
  * no cap). A call that would grow scratch past the cap declines with ENCHIP_ERR_OOM

@@ -1,0 +1,250 @@
+"""Rotary positions (enchip_rope_rows_dev) against the formula in 80-bit floats.
+
+The tolerance per element. The reduced angle is rounded to f32 (2^-25 of a half turn: pi 2^-25
+radians); sine and cosine are within 2 ulp of values below 1 (2^-23), times mscale (half an ulp);
+two products and their sum round once each. With the reference's own rounding that is under
+2^-21 m (|x1| + |x2|). The angle itself is p f_j in 64 bits, two roundings of f_j / 2 pi and one
+of the product: |p| f_j 2^-51 radians. Elements that are not rotated are copied bit for bit."""
+import math
+
+import numpy as np
+import pytest
+
+from aikit_amd import enchip
+
+pytestmark = pytest.mark.gpu
+
+
+def say(msg):
+    print(f"[case] {msg}", flush=True)
+
+
+def freqs(r, base=1e4, scaling=enchip.ROPE_NONE, factor=1.0, orig=0):
+    """(f_j [r/2], mscale) in 80 bits."""
+    ld = np.longdouble
+    if scaling == enchip.ROPE_NTK and r > 2:
+        base = ld(base) * ld(factor) ** (ld(r) / ld(r - 2))
+    f = np.array([ld(base) ** (ld(-2 * j) / ld(r)) for j in range(r // 2)])
+    if scaling == enchip.ROPE_LINEAR:
+        return f / ld(factor), 1.0
+    if scaling == enchip.ROPE_YARN:
+        w = np.clip((ld(orig) * f / (2 * np.pi) - 1) / 31, 0, 1)
+        return f * w + f * (1 - w) / ld(factor), 0.1 * math.log(factor) + 1.0
+    return f, 1.0
+
+
+def oracle(x, pos, f, m, heads, hd, layout):
+    """(y, tolerance) for x [rows, heads*hd] in f32, in 80 bits."""
+    rows, n = x.shape[0], len(f)
+    h = x.astype(np.longdouble).reshape(rows, heads, hd)
+    y, tol = h.copy(), np.zeros(h.shape)
+    if layout == enchip.ROPE_HALF:
+        i, k = np.arange(n), n + np.arange(n)
+    else:
+        i, k = 2 * np.arange(n), 2 * np.arange(n) + 1
+    ang = pos.astype(np.longdouble)[:, None] * f
+    c, s = (np.cos(ang) * m)[:, None, :], (np.sin(ang) * m)[:, None, :]
+    y[..., i], y[..., k] = h[..., i] * c - h[..., k] * s, h[..., k] * c + h[..., i] * s
+    t = abs(m) * (np.abs(h[..., i]) + np.abs(h[..., k])) * (2.0 ** -21 + np.abs(ang)[:, None, :] * 2.0 ** -51)
+    tol[..., i] = tol[..., k] = t
+    return y.reshape(rows, -1), tol.reshape(rows, -1)
+
+
+def check(ctx, r, layout, hd, heads, nseq, L, f, m, pos=None, pos0=0, pad=0, off=0, inplace=False, stream=None, seed=0):
+    import torch
+
+    rows, W = nseq * L, heads * hd
+    g = np.random.default_rng(seed + rows * 31 + W)
+    ld = W + pad
+    x = g.standard_normal((rows, ld)).astype(np.float32)
+    base = torch.full((rows * ld + off + 8,), 5.0, device="cuda")
+    dx = base[off:off + rows * ld].view(rows, ld)  # an offset of `off` floats: alignment
+    dx.copy_(torch.from_numpy(x))
+    out = torch.full((rows * ld + off + 8,), -7.0, device="cuda")
+    dy = dx if inplace else out[off:off + rows * ld].view(rows, ld)
+    dp = None if pos is None else torch.from_numpy(np.asarray(pos, np.int32)).cuda()
+    torch.cuda.synchronize()
+    ctx.rope_rows_dev(r, layout, dx.data_ptr(), ld, dy.data_ptr(), ld, nseq, L, heads, hd, 0 if dp is None else dp.data_ptr(),
+                      pos0, 0 if stream is None else stream.cuda_stream)
+    torch.cuda.synchronize()
+    got = dy.cpu().numpy()
+    p = np.asarray(pos, np.int64) if pos is not None else np.tile(pos0 + np.arange(L), nseq)
+    want, tol = oracle(x[:, :W], p, f, m, heads, hd, layout)
+    err = np.abs(got[:, :W].astype(np.longdouble) - want)
+    assert np.all(err <= tol), f"worst {float((err - tol).max())}"
+    if pad:  # the padding of the rows is left as it was
+        assert np.array_equal(got[:, W:], x[:, W:] if inplace else np.full((rows, pad), -7.0, np.float32))
+    if not inplace:
+        assert np.array_equal(dx.cpu().numpy(), x)
+    return got
+
+
+LAYOUTS = [enchip.ROPE_HALF, enchip.ROPE_INTERLEAVED]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("hd,rot", [(64, 64), (64, 32), (32, 32), (128, 128), (128, 96), (64, 62), (64, 2), (20, 10), (2, 2),
+                                    (7, 6), (1024, 1024), (256, 40)])
+def test_shapes(ctx, layout, hd, rot):
+    r = ctx.rope(rot)
+    f, m = freqs(rot)
+    try:
+        for nseq, L, heads in ((1, 1, 1), (1, 1, 24), (3, 5, 2), (2, 77, 3), (1, 129, 4)):
+            say(f"rope layout={layout} hd={hd} rot={rot} nseq={nseq} L={L} heads={heads}")
+            check(ctx, r, layout, hd, heads, nseq, L, f, m)
+            check(ctx, r, layout, hd, heads, nseq, L, f, m, inplace=True, pad=4)
+    finally:
+        ctx.release_rope(r)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("pad,off", [(0, 1), (1, 0), (3, 2), (4, 0), (8, 4)])
+def test_pitches_and_alignment(ctx, layout, pad, off):
+    r = ctx.rope(32)
+    f, m = freqs(32)
+    try:
+        for inplace in (False, True):
+            say(f"rope pad={pad} off={off} layout={layout} inplace={inplace}")
+            check(ctx, r, layout, 64, 3, 2, 33, f, m, pad=pad, off=off, inplace=inplace)
+    finally:
+        ctx.release_rope(r)
+
+
+@pytest.mark.parametrize("scaling,factor,orig", [(enchip.ROPE_LINEAR, 4.0, 0), (enchip.ROPE_NTK, 8.0, 0),
+                                                 (enchip.ROPE_YARN, 16.0, 2048), (enchip.ROPE_YARN, 1.0, 512)])
+@pytest.mark.parametrize("rot,base", [(64, 1e4), (128, 1e6), (2, 1e4), (48, 500.0)])
+def test_scalings_at_far_positions(ctx, scaling, factor, orig, rot, base):
+    r = ctx.rope(rot, base=base, scaling=scaling, factor=factor, orig_len=orig)
+    f, m = freqs(rot, base, scaling, factor, orig)
+    g = np.random.default_rng(rot)
+    pos = np.concatenate([g.integers(-2 ** 31, 2 ** 31, size=40), [0, 1, -1, 2 ** 31 - 1, -2 ** 31, 131071, 1 << 20]])
+    try:
+        for layout in LAYOUTS:
+            say(f"rope scaling={scaling} rot={rot} base={base} layout={layout}")
+            check(ctx, r, layout, rot + 4, 2, 1, len(pos), f, m, pos=pos)
+            check(ctx, r, layout, rot + 4, 2, 2, 9, f, m, pos0=1000003)
+            check(ctx, r, layout, rot, 1, 1, 3, f, m, pos0=-2)
+    finally:
+        ctx.release_rope(r)
+
+
+def test_own_frequencies(ctx):
+    f = np.array([0.0, 1.0, -0.5, 3.0e-3, 17.0])
+    r = ctx.rope_from_freqs(f, mscale=-1.5)
+    try:
+        for layout in LAYOUTS:
+            check(ctx, r, layout, 12, 3, 2, 50, f.astype(np.longdouble), -1.5, pos0=7)
+    finally:
+        ctx.release_rope(r)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_non_finite_values_stay_in_their_pair(ctx, layout):
+    import torch
+
+    r = ctx.rope(8)
+    try:
+        x = np.ones((3, 2 * 12), np.float32)
+        x[1, 3], x[2, 12 + 9] = np.inf, np.nan  # a rotated element of head 0, a copied one of head 1
+        dx = torch.from_numpy(x).cuda()
+        dy = torch.empty_like(dx)
+        torch.cuda.synchronize()
+        ctx.rope_rows_dev(r, layout, dx.data_ptr(), 24, dy.data_ptr(), 24, 1, 3, 2, 12, pos0=5)
+        torch.cuda.synchronize()
+        y = dy.cpu().numpy()
+        bad = np.argwhere(~np.isfinite(y))
+        mate = 7 if layout == enchip.ROPE_HALF else 2
+        assert sorted(map(tuple, bad)) == sorted([(1, 3), (1, mate), (2, 21)])
+    finally:
+        ctx.release_rope(r)
+
+
+def test_query_and_key_heads_of_qkv_rows(ctx):
+    # Q and K of fused rows in one call, V left alone, a second stream, and the call in a graph
+    import torch
+
+    S, L, H, hd = 3, 50, 4, 64
+    D = H * hd
+    g = np.random.default_rng(3)
+    x = g.standard_normal((S * L, 3 * D)).astype(np.float32)
+    r = ctx.rope(hd)
+    f, m = freqs(hd)
+    want, tol = oracle(x[:, :2 * D], np.tile(np.arange(L), S), f, m, 2 * H, hd, enchip.ROPE_HALF)
+    try:
+        s = torch.cuda.Stream()
+        src = torch.from_numpy(x).cuda()
+        d = src.clone()
+        torch.cuda.synchronize()
+
+        def run():
+            ctx.rope_rows_dev(r, enchip.ROPE_HALF, d.data_ptr(), 3 * D, d.data_ptr(), 3 * D, S, L, 2 * H, hd,
+                              stream=s.cuda_stream)
+
+        run()
+        torch.cuda.synchronize()
+        eager = d.cpu().numpy()
+        assert np.all(np.abs(eager[:, :2 * D] - want) <= tol)
+        assert np.array_equal(eager[:, 2 * D:], x[:, 2 * D:])
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            run()
+        for _ in range(3):
+            d.copy_(src)
+            torch.cuda.synchronize()
+            gr.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(d.cpu().numpy(), eager)
+        del gr
+    finally:
+        ctx.release_rope(r)
+
+
+def test_many_rows(ctx):
+    # more rows than one launch takes: the rows' positions run on across launches
+    import torch
+
+    rows = (1 << 22) + 1001
+    r = ctx.rope(4)
+    try:
+        d = torch.zeros((rows, 4), device="cuda")
+        d[:, 0] = 1.0
+        torch.cuda.synchronize()
+        say(f"rope rows={rows}")
+        ctx.rope_rows_dev(r, enchip.ROPE_HALF, d.data_ptr(), 4, d.data_ptr(), 4, 1, rows, 1, 4)
+        torch.cuda.synchronize()
+        p = torch.arange(rows, device="cuda", dtype=torch.float64)
+        assert (d[:, 0].double() - torch.cos(p)).abs().max().item() <= 2.0 ** -21 + rows * 2.0 ** -50
+        assert (d[:, 2].double() - torch.sin(p)).abs().max().item() <= 2.0 ** -21 + rows * 2.0 ** -50
+        assert d[:, 1].abs().max().item() == 0 and d[:, 3].abs().max().item() == 0
+    finally:
+        ctx.release_rope(r)
+
+
+def test_refusals(ctx):
+    import torch
+
+    for bad in (dict(rot_dim=0), dict(rot_dim=3), dict(rot_dim=1026), dict(rot_dim=8, base=0.0), dict(rot_dim=8, base=np.inf),
+                dict(rot_dim=8, base=np.nan), dict(rot_dim=8, scaling=9), dict(rot_dim=8, scaling=enchip.ROPE_LINEAR, factor=0.5),
+                dict(rot_dim=8, scaling=enchip.ROPE_YARN, factor=2.0, orig_len=0)):
+        with pytest.raises(enchip.EnchipError) as e:
+            ctx.rope(**bad)
+        assert e.value.code == enchip.ERR_ARG, bad
+    for f, m in (([], 1.0), ([np.nan], 1.0), ([1.0], np.inf), ([1.0], 1e300), (np.ones(513), 1.0)):
+        with pytest.raises(enchip.EnchipError):
+            ctx.rope_from_freqs(f, m)
+    r = ctx.rope(8)
+    d = torch.zeros(64, device="cuda")
+    p = d.data_ptr()
+    ok = dict(layout=0, d_x=p, ldx=16, d_y=p, ldy=16, nseq=1, L=1, heads=1, head_dim=8)
+    for k, v in (("layout", 2), ("ldx", 7), ("ldy", 7), ("nseq", -1), ("L", -1), ("heads", -1), ("head_dim", 7), ("head_dim", 1025),
+                 ("d_x", 0), ("d_y", 0), ("ldy", 15), ("pos0", 1 << 40), ("L", 1 << 31), ("heads", 70000)):
+        with pytest.raises(enchip.EnchipError) as e:
+            ctx.rope_rows_dev(r, **{**ok, k: v})
+        assert e.value.code == enchip.ERR_ARG, (k, v)
+    for k in ("nseq", "L", "heads"):  # nothing to do
+        ctx.rope_rows_dev(r, **{**ok, k: 0, "d_x": 0, "d_y": 0})
+    ctx.release_rope(r)
+    for call in (lambda: ctx.rope_rows_dev(r, **ok), lambda: ctx.release_rope(r)):
+        with pytest.raises(enchip.EnchipError) as e:
+            call()
+        assert e.value.code == enchip.ERR_HANDLE
