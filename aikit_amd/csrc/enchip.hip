@@ -2568,14 +2568,27 @@ int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, const float
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
     const int64_t rows = nseq * L;
+    const bool inter = layout == ENCHIP_ROPE_INTERLEAVED, inplace = d_x == d_y;
+    const int64_t rot = 2 * r.n, rest = inplace ? 0 : head_dim - rot;
+    const bool vec = rot % (inter ? 4 : 8) == 0 && head_dim % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 &&
+                     (uintptr_t)d_x % 16 == 0 && (uintptr_t)d_y % 16 == 0;
+    const int64_t ipr = vec ? rot / (inter ? 4 : 8) + rest / 4 : r.n + rest;
+    auto fast_div = [](int64_t d) {
+        return enchip::FastDiv{(uint32_t)d, d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + (uint64_t)d - 1) / (uint64_t)d)};
+    };
+    // rows of a workgroup: three items a thread, while a few workgroups a CU are left
+    const int64_t by_items = std::max<int64_t>(1, 768 / (heads * ipr)), by_rows = std::max<int64_t>(1, rows / (4 * ctx->num_cus));
+    const int tr = (int)std::min({by_items, by_rows, (int64_t)enchip::ROPE_CS / r.n, (int64_t)64});
     for (int64_t r0 = 0; r0 < rows; r0 += kRowChunk) {
         const int64_t n = std::min(kRowChunk, rows - r0);
-#define ROPE_CALL(I)                                                                                                  \
-    hipLaunchKernelGGL(enchip::rope_rows<I>, dim3((unsigned)n), dim3(256), 0, s, d_x + r0 * ldx, ldx, d_y + r0 * ldy, \
-                       ldy, r.d_turns, r.mscale, d_pos ? d_pos + r0 : nullptr, pos0, r0, (int)L, n, (int)heads,       \
-                       (int)head_dim, (int)(2 * r.n))
-        if (layout == ENCHIP_ROPE_INTERLEAVED) ROPE_CALL(true);
-        else ROPE_CALL(false);
+#define ROPE_CALL(I, V)                                                                                              \
+    hipLaunchKernelGGL((enchip::rope_rows<I, V>), dim3((unsigned)((n + tr - 1) / tr)), dim3(256), 0, s, d_x + r0 * ldx, ldx, \
+                       d_y + r0 * ldy, ldy, r.d_turns, r.mscale, d_pos ? d_pos + r0 : nullptr, pos0, r0, (int)L, n, tr, \
+                       fast_div(heads), fast_div(ipr), (int)head_dim, (int)rot)
+        if (inter && vec) ROPE_CALL(true, 4);
+        else if (inter) ROPE_CALL(true, 1);
+        else if (vec) ROPE_CALL(false, 4);
+        else ROPE_CALL(false, 1);
 #undef ROPE_CALL
     }
     return check_launch(ctx, "rope_rows");

@@ -21,38 +21,107 @@
 namespace enchip {
 
 constexpr int ROPE_MAX_PAIRS = 512;  // pairs of a head (head_dim up to 1024)
+constexpr int ROPE_CS = 2048;        // angles of a workgroup's rows in LDS
+constexpr int ROPE_BATCH = 4;        // items of a thread whose loads are in flight together
 
-// One thread per element pair or passed-through element; grid.y: rows.
-template <bool INTERLEAVED>
+// x / d for x d < 2^32; m = 2^32 / d rounded up, 0 for d = 1.
+struct FastDiv {
+    uint32_t d, m;
+    __device__ __forceinline__ uint32_t div(uint32_t x) const { return m ? __umulhi(x, m) : x; }
+};
+
+template <int V>
+struct RopeVec {
+    float v[V];
+    __device__ __forceinline__ void load(const float *p) {
+        if constexpr (V == 4) {
+            const f32x4 t = *reinterpret_cast<const f32x4 *>(p);
+            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void store(float *p) const {
+        if constexpr (V == 4) {
+            *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] = v[i];
+        }
+    }
+};
+
+// A workgroup's TR rows, as items of V elements: per head first the items of the rotated part (half:
+// V elements of each half; interleaved: V elements, V / 2 pairs; V = 1: one pair), then, not in
+// place, those of the passed-through part. ipr: items per head. V = 4: r a multiple of 8 (half) or
+// 4, head_dim and pitches of 4, 16-byte aligned buffers.
+template <bool INTERLEAVED, int V>
 __global__ __launch_bounds__(256) void rope_rows(const float *__restrict__ x, int64_t ldx, float *__restrict__ y,
                                                  int64_t ldy, const double *__restrict__ turns, float mscale,
                                                  const int32_t *__restrict__ pos, int64_t pos0, int64_t row0, int L,
-                                                 int64_t rows, int heads, int hd, int r) {
-    __shared__ float2 cs[ROPE_MAX_PAIRS];
-    const int64_t row = blockIdx.x;
-    const double p = pos ? (double)pos[row] : (double)(pos0 + (row0 + row) % L);
-    for (int j = threadIdx.x; j < r / 2; j += 256) {
-        const double t = p * turns[j];
+                                                 int64_t rows, int TR, FastDiv heads, FastDiv ipr, int hd, int r) {
+    __shared__ float2 cs[ROPE_CS];
+    constexpr int PV = INTERLEAVED && V == 4 ? 2 : 1;     // an item's pairs over V
+    const int64_t first = (int64_t)blockIdx.x * TR;
+    const int tr = (int)min((int64_t)TR, rows - first), np = r / 2;
+    for (int t = threadIdx.x; t < tr * np; t += 256) {
+        const int row = t / np, j = t - row * np;
+        const double p = pos ? (double)pos[first + row] : (double)(pos0 + (row0 + first + row) % L);
+        const double a = p * turns[j];
         float s, c;
-        sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-        cs[j] = make_float2(c * mscale, s * mscale);
+        sincospif(2.0f * (float)(a - rint(a)), &s, &c);
+        cs[t] = make_float2(c * mscale, s * mscale);
     }
     __syncthreads();
-    const float *xr = x + row * ldx;
-    float *yr = y + row * ldy;
-    const int ipr = r / 2 + (hd - r);
-    for (int i = threadIdx.x; i < heads * ipr; i += 256) {
-        const int h = i / ipr, e = i % ipr;
-        if (e >= r / 2) {
-            const int at = h * hd + r + (e - r / 2);
-            yr[at] = xr[at];
-            continue;
+    const int rot = PV == 2 ? r / 4 : np / V;  // rotated items of a head
+    const uint32_t items = (uint32_t)tr * heads.d * ipr.d;
+    for (uint32_t i0 = threadIdx.x; i0 < items; i0 += 256 * ROPE_BATCH) {
+        RopeVec<V> a[ROPE_BATCH], b[ROPE_BATCH];
+        float *dst[ROPE_BATCH];
+        int at[ROPE_BATCH];  // the item's first angle, -1: passed through, -2: none
+#pragma unroll
+        for (int u = 0; u < ROPE_BATCH; ++u) {
+            const uint32_t i = i0 + 256 * u;
+            if (i >= items) {
+                at[u] = -2;
+                continue;
+            }
+            const uint32_t hr = ipr.div(i), row = heads.div(hr);
+            const int e = (int)(i - hr * ipr.d), h = (int)(hr - row * heads.d);
+            const bool turn = e < rot;
+            const int off = h * hd + (turn ? (INTERLEAVED ? (V == 4 ? 4 : 2) * e : V * e) : r + V * (e - rot));
+            const float *src = x + (first + row) * ldx + off;
+            dst[u] = y + (first + row) * ldy + off;
+            at[u] = turn ? (int)row * np + (PV == 2 ? 2 : V) * e : -1;
+            a[u].load(src);
+            if (V == 1 ? turn : (!INTERLEAVED && turn)) b[u].load(src + (INTERLEAVED ? 1 : np));
         }
-        const int a = h * hd + (INTERLEAVED ? 2 * e : e), b = a + (INTERLEAVED ? 1 : r / 2);
-        const float2 w = cs[e];
-        const float x1 = xr[a], x2 = xr[b];
-        yr[a] = x1 * w.x - x2 * w.y;
-        yr[b] = x2 * w.x + x1 * w.y;
+#pragma unroll
+        for (int u = 0; u < ROPE_BATCH; ++u) {
+            if (at[u] == -2) continue;
+            if (at[u] >= 0) {
+                if constexpr (PV == 2) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float2 w = cs[at[u] + k];
+                        const float x1 = a[u].v[2 * k], x2 = a[u].v[2 * k + 1];
+                        a[u].v[2 * k] = x1 * w.x - x2 * w.y;
+                        a[u].v[2 * k + 1] = x2 * w.x + x1 * w.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        const float2 w = cs[at[u] + k];
+                        const float x1 = a[u].v[k], x2 = b[u].v[k];
+                        a[u].v[k] = x1 * w.x - x2 * w.y;
+                        b[u].v[k] = x2 * w.x + x1 * w.y;
+                    }
+                    b[u].store(dst[u] + (INTERLEAVED ? 1 : np));
+                }
+            }
+            a[u].store(dst[u]);
+        }
     }
 }
 
