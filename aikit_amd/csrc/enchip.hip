@@ -2452,6 +2452,10 @@ int enchip_bias_act_rows_dev(enchip_ctx *ctx, float *d_x, int64_t ld, int64_t ro
 
 namespace {
 
+enchip::FastDiv fast_div(int64_t d) {
+    return {(uint32_t)d, d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + (uint64_t)d - 1) / (uint64_t)d)};
+}
+
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 
 // Copies n frequencies to the device, in turns per position, under a new handle.
@@ -2573,9 +2577,6 @@ int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, const float
     const bool vec = rot % (inter ? 4 : 8) == 0 && head_dim % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 &&
                      (uintptr_t)d_x % 16 == 0 && (uintptr_t)d_y % 16 == 0;
     const int64_t ipr = vec ? rot / (inter ? 4 : 8) + rest / 4 : r.n + rest;
-    auto fast_div = [](int64_t d) {
-        return enchip::FastDiv{(uint32_t)d, d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + (uint64_t)d - 1) / (uint64_t)d)};
-    };
     // rows of a workgroup: three items a thread, while a few workgroups a CU are left
     const int64_t by_items = std::max<int64_t>(1, 768 / (heads * ipr)), by_rows = std::max<int64_t>(1, rows / (4 * ctx->num_cus));
     const int tr = (int)std::min({by_items, by_rows, (int64_t)enchip::ROPE_CS / r.n, (int64_t)64});
@@ -2628,24 +2629,34 @@ template <int BITS, bool GATED>
 int launch_wo(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda, const float *b0, const float *b1, int act,
               float *C, int64_t ldc, int64_t M, hipStream_t s) {
     using namespace enchip;
-    const int64_t units = p.Kp / (BITS == 4 ? 32 : 16);
-    const int tilesN = (int)((p.N + 15) / 16);
-    const int mb = M == 1 ? 1 : M == 2 ? 2 : 4;
-    const bool one = units <= 4 * WO_WAVES;
-    const int64_t rows = std::max<int64_t>(mb, (((int64_t)1 << 22) / tilesN) * mb);
-    for (int64_t r0 = 0; r0 < M; r0 += rows) {
-        const int64_t n = std::min(rows, M - r0);
-        const dim3 grid((unsigned)(((n + mb - 1) / mb) * tilesN));
-#define WO_CALL(MB, PF)                                                                                              \
-    hipLaunchKernelGGL((gemv_wo<BITS, MB, GATED, PF>), grid, dim3(64 * WO_WAVES), 0, s, A + r0 * lda, lda, p.w[0], p.w[1], \
-                       b0, b1, act, C + r0 * ldc, ldc, (int)n, (int)p.N, (int)p.K, (int)p.Kp, (int)p.cpg, (int)p.G, tilesN)
-        if (mb == 1 && one) WO_CALL(1, 1);
-        else if (mb == 1) WO_CALL(1, 4);
-        else if (mb == 2) WO_CALL(2, 2);
-        else WO_CALL(4, 2);
+    const enchip::FastDiv cpg = fast_div(p.cpg);
+#define WO_CALL(KERNEL, BM, BN, THREADS)                                                                           \
+    do {                                                                                                           \
+        const int tilesN = (int)((p.N + (BN)-1) / (BN));                                                           \
+        const int64_t rows = std::max<int64_t>((BM), (((int64_t)1 << 22) / tilesN) * (BM));                        \
+        for (int64_t r0 = 0; r0 < M; r0 += rows) {                                                                 \
+            const int64_t n = std::min(rows, M - r0);                                                              \
+            hipLaunchKernelGGL((KERNEL), dim3((unsigned)((n + (BM)-1) / (BM) * tilesN)), dim3(THREADS), 0, s,      \
+                               A + r0 * lda, lda, p.w[0], p.w[1], b0, b1, act, C + r0 * ldc, ldc, (int)n, (int)p.N, \
+                               (int)p.K, (int)p.Kp, cpg, (int)p.G, tilesN);                                        \
+        }                                                                                                          \
+    } while (0)
+#define WO_TILE(TM, NT, WM, WN, KS, KC)                                                                              \
+    do {                                                                                                             \
+        if (vec) WO_CALL((gemm_wo<BITS, GATED, TM, NT, WM, WN, KS, KC, true>), 32 * TM * WM, (GATED ? 16 : 32) * NT * WN, 64 * WM * WN * KS); \
+        else WO_CALL((gemm_wo<BITS, GATED, TM, NT, WM, WN, KS, KC, false>), 32 * TM * WM, (GATED ? 16 : 32) * NT * WN, 64 * WM * WN * KS); \
+    } while (0)
+    const bool vec = p.K % 4 == 0 && lda % 4 == 0 && (uintptr_t)A % 16 == 0;
+    const bool one = p.Kp / (BITS == 4 ? 32 : 16) <= 4 * WO_WAVES;
+    if (M == 1 && one) WO_CALL((gemv_wo<BITS, 1, GATED, 1>), 1, 16, 64 * WO_WAVES);
+    else if (M == 1) WO_CALL((gemv_wo<BITS, 1, GATED, 4>), 1, 16, 64 * WO_WAVES);
+    else if (M == 2) WO_CALL((gemv_wo<BITS, 2, GATED, 2>), 2, 16, 64 * WO_WAVES);
+    else if (M <= 4) WO_CALL((gemv_wo<BITS, 4, GATED, 2>), 4, 16, 64 * WO_WAVES);
+    else if (M <= 64) WO_TILE(1, 2, 1, 1, 4, 128);
+    else WO_TILE(1, 2, 1, 4, 2, 128);
+#undef WO_TILE
 #undef WO_CALL
-    }
-    return check_launch(c, "gemv_wo");
+    return check_launch(c, "weight-only product");
 }
 
 int check_rows(enchip_ctx *c, const char *what, int64_t M, int64_t N) {

@@ -490,6 +490,12 @@ __device__ __forceinline__ int xcd_logical_tile(int pid, int nblocks) {
     return (xcd < r) ? xcd * (q + 1) + idx : r * (q + 1) + (xcd - r) * q + idx;
 }
 
+// x / d for x d < 2^32; m = 2^32 / d rounded up, 0 for d = 1.
+struct FastDiv {
+    uint32_t d, m;
+    __device__ __forceinline__ uint32_t div(uint32_t x) const { return m ? __umulhi(x, m) : x; }
+};
+
 // ----------------------------------------------------------------------------
 // Tiled GEMM. Block tile BM x BN, K stage of 64, 4 waves in a 2x2 grid, each wave a
 // (BM/2) x (BN/2) tile of 32x32x32 i8 MFMA accumulators.

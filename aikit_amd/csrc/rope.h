@@ -24,12 +24,6 @@ constexpr int ROPE_MAX_PAIRS = 512;  // pairs of a head (head_dim up to 1024)
 constexpr int ROPE_CS = 2048;        // angles of a workgroup's rows in LDS
 constexpr int ROPE_BATCH = 4;        // items of a thread whose loads are in flight together
 
-// x / d for x d < 2^32; m = 2^32 / d rounded up, 0 for d = 1.
-struct FastDiv {
-    uint32_t d, m;
-    __device__ __forceinline__ uint32_t div(uint32_t x) const { return m ? __umulhi(x, m) : x; }
-};
-
 template <int V>
 struct RopeVec {
     float v[V];

@@ -17,6 +17,7 @@
 #include <utility>
 
 #include "gated.h"
+#include "gemm_q8w.h"
 #include "kernels.h"
 
 #pragma clang fp contract(off)
@@ -78,7 +79,7 @@ template <int BITS, int MB, bool GATED, int PF>
 __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict__ A, int64_t lda, WoWeight w0, WoWeight w1,
                                                          const float *__restrict__ b0, const float *__restrict__ b1, int act,
                                                          float *__restrict__ C, int64_t ldc, int M, int N, int K, int Kp,
-                                                         int cpg, int G, int tilesN) {
+                                                         FastDiv cpg, int G, int tilesN) {
     constexpr int NWT = GATED ? 2 : 1, CK = BITS == 4 ? 32 : 16, AV = CK / 16;
     __shared__ float red[NWT][MB][WO_WAVES][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = lane >> 4, i = lane & 15;
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
                 q[p][t] = *reinterpret_cast<const uint4 *>(w[t].q + at);
                 if (BITS == 4)
                     sc[p][t] = (float)static_cast<const _Float16 *>(
-                        w[t].s)[((int64_t)(n0 >> 6) * G + min(uc / cpg, G - 1)) * 64 + (n0 & 63) + i];
+                        w[t].s)[((int64_t)(n0 >> 6) * G + min((int)cpg.div(uc), G - 1)) * 64 + (n0 & 63) + i];
             }
 #pragma unroll
             for (int m = 0; m < MB; ++m)
@@ -179,6 +180,249 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
     float v = y[0];
     if constexpr (GATED) v = gate_f32(act, b0 ? y[0] + b0[n] : y[0], b1 ? y[1] + b1[n] : y[1]);
     C[(int64_t)(m0 + m) * ldc + n] = v;
+}
+
+// 8 codes of a 4-bit image word, in k order, as bf16 values q / 16 (exact).
+__device__ __forceinline__ bf16x8 q4_widen8(uint32_t lo) {
+    uint32_t hi = lo >> 4;
+    asm("" : "+v"(hi));  // one shift for its four codes
+    auto pair = [&](int b) {
+        return q8w_pack(__float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)((lo >> (8 * b)) & 0xff))),
+                        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)((hi >> (8 * b)) & 0xff))));
+    };
+    return __builtin_bit_cast(bf16x8, (u32x4){pair(0), pair(1), pair(2), pair(3)});
+}
+
+// 8 int8 codes of a weight image, in k order, as bf16 values (exact).
+__device__ __forceinline__ bf16x8 q8_widen8(uint32_t w0, uint32_t w1) {
+    uint32_t x[4];
+    q8w_widen4(w0, x[0], x[1]);
+    q8w_widen4(w1, x[2], x[3]);
+    return __builtin_bit_cast(bf16x8, (u32x4){x[0], x[1], x[2], x[3]});
+}
+
+// Tiles on the bf16 MFMA, activations split exactly into three bf16 parts (gemm_q8w.h). A
+// workgroup computes 32 TM WM rows; each of its WM x WN x KS wavefronts TM x NT 32 x 32 tiles of
+// products over its share of every K stage: NT channel blocks of one weight, or NT / 2 of each
+// of the two, so a gate and its up projection meet in one lane. The stage's activations are split
+// by all threads into three planes in LDS (double-buffered), the weights' codes go straight into
+// registers and are widened there. A 4-bit weight's 32-deep chunk is summed from zero and added
+// scaled: 16 multiply-adds for 6 MFMAs. The KS shares meet in LDS at the end, each wavefront
+// finishing 16 / KS of the accumulator registers.
+template <int BITS, bool GATED, int TM, int NT, int WM, int WN, int KS, int KC, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_wo(const float *__restrict__ A, int64_t lda, WoWeight w0,
+                                                                WoWeight w1, const float *__restrict__ b0,
+                                                                const float *__restrict__ b1, int act, float *__restrict__ C,
+                                                                int64_t ldc, int M, int N, int K, int Kp, FastDiv cpg, int G,
+                                                                int tilesN) {
+    constexpr int NTHR = 64 * WM * WN * KS, BM = 32 * TM * WM, CPW = GATED ? 16 * NT : 32 * NT, BN = CPW * WN;
+    constexpr int KB = KC / 32 / KS;  // chunks of a wavefront per stage
+    constexpr int P = 2 * KC + 16, PL = BM * P, STAGE = 3 * PL;
+    constexpr int LPR = KC / 4, AV = BM * LPR / NTHR, ER = 16 / KS;
+    constexpr int RED = KS > 1 ? NTHR * (KS - 1) * ER * TM * NT * 4 : 0;
+    constexpr int LDS = 2 * STAGE > RED ? 2 * STAGE : RED;
+    static_assert(AV >= 1 && BM * LPR % NTHR == 0 && KB >= 1 && KC % (32 * KS) == 0 && 16 % KS == 0, "tile");
+    static_assert(!GATED || NT % 2 == 0, "a tile of each weight");
+    __shared__ __attribute__((aligned(16))) char lds[LDS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, hf = lane >> 5;
+    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x);
+    const int m0 = (logical / tilesN) * BM, n0 = (logical % tilesN) * BN;
+    const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+    const int lk = 4 * (tid % LPR), lr = tid / LPR;
+    const WoWeight w[2] = {w0, w1};
+    const float *ga[AV];
+#pragma unroll
+    for (int i = 0; i < AV; ++i) ga[i] = A + (int64_t)min(m0 + lr + (NTHR / LPR) * i, M - 1) * lda;
+    const int nk32 = Kp / 32;
+    // tile t: 32-channel block cb(t) of weight t % 2 (gated) or 0
+    const int cb0 = (n0 + wn * CPW) >> 5;
+    auto cb = [&](int t) { return cb0 + (GATED ? t >> 1 : t); };
+    const int8_t *wb[NT];
+    const _Float16 *sb[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const WoWeight &x = w[GATED ? t & 1 : 0];
+        const int c = cb(t);
+        wb[t] = x.q + (BITS == 4 ? (int64_t)(c >> 1) * nk32 * 1024 + ((c & 1) * 32 + r) * 16 + 8 * hf
+                                 : (int64_t)c * nk32 * 1024 + lane * 16);
+        sb[t] = static_cast<const _Float16 *>(x.s) + (BITS == 4 ? (int64_t)(c >> 1) * G * 64 + (c & 1) * 32 + r : 0);
+    }
+    f32x4 ra[AV];
+    uint32_t wr[KB][NT][BITS / 2];
+    _Float16 sc[KB][NT];
+    auto load_a = [&](int c) {
+        const int k = KC * c + lk;
+        if (!VEC && KC * c + KC <= K) {  // uniform: all of the stage, in unaligned 16-byte loads
+#pragma unroll
+            for (int i = 0; i < AV; ++i) ra[i] = f32x4{ga[i][k], ga[i][k + 1], ga[i][k + 2], ga[i][k + 3]};
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < AV; ++i) {
+            if (VEC) ra[i] = *reinterpret_cast<const f32x4 *>(ga[i] + min(k, K - 4));
+            else
+                ra[i] = f32x4{ga[i][min(k, K - 1)], ga[i][min(k + 1, K - 1)], ga[i][min(k + 2, K - 1)], ga[i][min(k + 3, K - 1)]};
+        }
+    };
+    auto load_w = [&](int c) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int kc = min(KC / 32 * c + KB * ks + b, nk32 - 1), g = BITS == 4 ? min((int)cpg.div(kc), G - 1) : 0;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (BITS == 4) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(wb[t] + (int64_t)kc * 1024);
+                    wr[b][t][0] = v.x, wr[b][t][1] = v.y;
+                    sc[b][t] = sb[t][(int64_t)g * 64];
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(wb[t] + (int64_t)kc * 1024);
+                    wr[b][t][0] = v.x, wr[b][t][1] = v.y, wr[b][t][2] = v.z, wr[b][t][3] = v.w;
+                }
+            }
+        }
+    };
+    auto store_a = [&](int c, char *st) {
+        const int k = KC * c + lk;
+#pragma unroll
+        for (int i = 0; i < AV; ++i) {
+            f32x4 v = ra[i];  // k past K counts as zero
+            if (VEC) {
+                if (k >= K) v = f32x4{0.f, 0.f, 0.f, 0.f};
+            } else {
+                v.x = k < K ? v.x : 0.f, v.y = k + 1 < K ? v.y : 0.f, v.z = k + 2 < K ? v.z : 0.f, v.w = k + 3 < K ? v.w : 0.f;
+            }
+            uint32_t a1[4], a2[4], a3[4];
+            q8w_split3(v.x, a1[0], a2[0], a3[0]);
+            q8w_split3(v.y, a1[1], a2[1], a3[1]);
+            q8w_split3(v.z, a1[2], a2[2], a3[2]);
+            q8w_split3(v.w, a1[3], a2[3], a3[3]);
+            char *d = st + (lr + (NTHR / LPR) * i) * P + 2 * lk;
+            *reinterpret_cast<uint2 *>(d) = make_uint2(q8w_pack(a1[0], a1[1]), q8w_pack(a1[2], a1[3]));
+            *reinterpret_cast<uint2 *>(d + PL) = make_uint2(q8w_pack(a2[0], a2[1]), q8w_pack(a2[2], a2[3]));
+            *reinterpret_cast<uint2 *>(d + 2 * PL) = make_uint2(q8w_pack(a3[0], a3[1]), q8w_pack(a3[2], a3[3]));
+        }
+    };
+    f32x16 acc[TM][NT];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][t][e] = 0.0f;
+    // Stage c + 1 is split into the other buffer behind stage c's MFMAs; past the last stage the
+    // loads re-read it and the buffer is not used.
+    const int nc = (Kp + KC - 1) / KC, last = nc - 1;
+    load_a(0);
+    load_w(0);
+    store_a(0, lds);
+    load_a(min(1, last));
+    lds_barrier();
+    for (int c = 0; c < nc; ++c) {
+        const char *cur = lds + (c & 1) * STAGE;
+        char *nxt = lds + ((c & 1) ^ 1) * STAGE;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            f32x16 part[TM][NT];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                bf16x8 p[TM][3], q[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if constexpr (BITS == 4) q[t] = q4_widen8(wr[b][t][j]);
+                    else q[t] = q8_widen8(wr[b][t][2 * j], wr[b][t][2 * j + 1]);
+                }
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int x = 0; x < 3; ++x)
+                        p[i][x] = *reinterpret_cast<const bf16x8 *>(cur + x * PL + (32 * (TM * wm + i) + r) * P +
+                                                                    64 * (KB * ks + b) + 32 * hf + 16 * j);
+#pragma unroll
+                for (int x = 2; x >= 0; --x)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            f32x16 &s = BITS == 4 ? part[i][t] : acc[i][t];
+                            if (BITS == 4 && j == 0 && x == 2) {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+                            }
+                            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[i][x], q[t], s, 0, 0, 0);
+                        }
+            }
+            if (BITS == 4) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float s = 16.0f * (float)sc[b][t];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][t][e] = __builtin_fmaf(part[i][t][e], s, acc[i][t][e]);
+                }
+            }
+        }
+        load_w(min(c + 1, last));
+        store_a(c + 1, nxt);
+        load_a(min(c + 2, last));
+        lds_barrier();
+    }
+    if constexpr (KS > 1) {
+        // share s of the registers e in [ER s, ER s + ER) goes to wavefront s of the KS
+        float *red = reinterpret_cast<float *>(lds);
+        constexpr int PER = (KS - 1) * ER * TM * NT * 64;  // floats of one receiving wavefront
+        const int mine = wave % (WM * WN);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s == ks) continue;
+            float *d = red + (mine + WM * WN * s) * PER + (ks < s ? ks : ks - 1) * (ER * TM * NT * 64) + lane;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < ER; ++e) d[((i * NT + t) * ER + e) * 64] = acc[i][t][ER * s + e];
+        }
+        lds_barrier();
+        const float *d = red + wave * PER + lane;
+        // own registers first into the low places, then the others' shares in their order
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < ER; ++e) {
+                    float v = 0.0f, o[KS];
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) o[s] = acc[i][t][ER * s + e];
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) v = ks == s ? o[s] : v;
+#pragma unroll
+                    for (int s = 0; s < KS - 1; ++s) v += d[s * (ER * TM * NT * 64) + ((i * NT + t) * ER + e) * 64];
+                    acc[i][t][e] = v;
+                }
+    }
+#pragma unroll
+    for (int u = 0; u < (GATED ? NT / 2 : NT); ++u) {
+        const int n = 32 * (cb0 + u) + r, nn = min(n, N - 1);
+        float s[2], bb[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            s[x] = BITS == 8 ? static_cast<const float *>(w[x].s)[nn] : 1.0f;
+            const float *b = x ? b1 : b0;
+            bb[x] = GATED && b ? b[nn] : kNoBias;
+        }
+        if (n >= N) continue;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < ER; ++e) {
+                const int m = m0 + 32 * (TM * wm + i) + acc_row(KS > 1 ? ER * ks + e : e, lane);
+                float v = acc[i][GATED ? 2 * u : u][e] * s[0];
+                if constexpr (GATED) v = gate_f32(act, v + bb[0], acc[i][2 * u + 1][e] * s[1] + bb[1]);
+                if (m < M) C[(int64_t)m * ldc + n] = v;
+            }
+    }
 }
 
 }  // namespace enchip
