@@ -2756,22 +2756,71 @@ int gated_wo_host(enchip_ctx *ctx, const char *what, enchip_weight gate, enchip_
     return ENCHIP_OK;
 }
 
+// The single small-M launch: quantization and both products.
+int launch_gated_q(enchip_ctx *c, const Weight &w, const float *d_a, int64_t M, const enchip::GatePair &p, int act,
+                   float *d_dst, hipStream_t s) {
+    using Kern = void (*)(const float *, enchip::GatePair, int, float *, int64_t, int, int, int, int);
+    static constexpr Kern table[7] = {enchip::gated_w8a8_q<1>, enchip::gated_w8a8_q<2>,  enchip::gated_w8a8_q<3>,
+                                      enchip::gated_w8a8_q<4>, enchip::gated_w8a8_q<8>, enchip::gated_w8a8_q<12>,
+                                      enchip::gated_w8a8_q<16>};
+    const int qch = gvq_qch(w.K);
+    const Kern fn = table[qch <= 4 ? qch - 1 : qch == 8 ? 4 : qch == 12 ? 5 : 6];
+    const size_t lds = (size_t)enchip::gated_q_lds_bytes((int)w.Kp);
+    if (lds > 64 * 1024) {
+        const std::pair<const void *, size_t> key(reinterpret_cast<const void *>(fn), lds);
+        if (std::find(c->lds_set.begin(), c->lds_set.end(), key) == c->lds_set.end()) {
+            HIP_TRY(c, hipFuncSetAttribute(key.first, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+            c->lds_set.push_back(key);
+        }
+    }
+    const dim3 grid((unsigned)((w.N + 31) / 32), (unsigned)((M + enchip::GVQ_ROWS - 1) / enchip::GVQ_ROWS));
+    hipLaunchKernelGGL(fn, grid, dim3(64 * enchip::GVQ_WAVES), lds, s, d_a, p, act, d_dst, w.N, (int)M, (int)w.N, (int)w.K,
+                       (int)w.Kp);
+    return check_launch(c, "gated_w8a8_q");
+}
+
+// The gated pair on fragment-major codes: persistent tiles, or pieces.
+template <int ACT>
+void launch_gated_frag(enchip_ctx *c, const Weight &w, const int8_t *aq, const float *as, const enchip::GatePair &p,
+                       int64_t M, float *out, hipStream_t s) {
+    using namespace enchip;
+    auto pieces = [&](int64_t cm, int64_t cn) { return ((M + cm - 1) / cm) * ((w.N + cn - 1) / cn); };
+    const bool pt = use_persistent(w, aq, w.Kp, out, w.N, M, true);
+    if (pt && pieces(32, 32) > 4 * (int64_t)c->num_cus) {
+        const int tilesN = (int)((w.N + GP_BN - 1) / GP_BN);
+        const bool small = pieces(PT_BM, GP_BN) < 2 * (int64_t)c->num_cus;
+        const int bm = small ? PT_BM_SMALL : PT_BM, tiles = (int)pieces(bm, GP_BN);
+        const dim3 grid(persistent_grid(c, tiles, small ? 3 : 2)), block(256);
+        if (small)
+            hipLaunchKernelGGL((gated_w8a8_pt<PT_BM_SMALL, ACT, 1>), grid, block, 0, s, aq, as, p, out, w.N, (int)M, (int)w.N,
+                               (int)w.Kp, tilesN, tiles);
+        else
+            hipLaunchKernelGGL((gated_w8a8_pt<PT_BM, ACT, 1>), grid, block, 0, s, aq, as, p, out, w.N, (int)M, (int)w.N,
+                               (int)w.Kp, tilesN, tiles);
+        return;
+    }
+    const int pn = (int)((w.N + 31) / 32);
+    const int64_t rows = std::max<int64_t>(32, (((int64_t)1 << 23) / pn) * 32);
+    for (int64_t r0 = 0; r0 < M; r0 += rows) {
+        const int64_t n = std::min(rows, M - r0);
+        hipLaunchKernelGGL((gated_w8a8_piece<32, 32, ACT>), dim3((unsigned)((n + 31) / 32 * pn)), dim3(256), 0, s,
+                           aq + r0 * w.Kp, as + r0, p, out + r0 * w.N, w.N, (int)n, (int)w.N, (int)w.Kp, pn);
+    }
+}
+
 // Enqueues the W8A8 gated pair on d_a [M][K] after the caller checked the arguments.
 int launch_gated_w8a8(enchip_ctx *c, const Weight &wg, const Weight &wu, const float *d_a, int64_t M, const float *bg,
                       const float *bu, int act, float *d_dst, hipStream_t s) {
     int rc;
+    const enchip::GatePair p = {{wg.d_w, wu.d_w}, {wg.d_s, wu.d_s}, {bg, bu}};
+    if (M <= c->small_m && M <= 32 && wg.K % 4 == 0 && wg.K <= enchip::GVQ_MAX_K && (uintptr_t)d_a % 16 == 0 &&
+        grid_fits((wg.N + 31) / 32, 64 * enchip::GVQ_WAVES * 4))
+        return launch_gated_q(c, wg, d_a, M, p, act, d_dst, s);
     if ((rc = ensure_act_scratch(c, M, wg.Kp))) return rc;
     if ((rc = scratch_wait(c, s))) return rc;
     if ((rc = launch_quant(c, d_a, M, wg.K, c->d_aq, wg.Kp, c->d_as, s, true))) return rc;
-    const enchip::GatePair p = {{wg.d_w, wu.d_w}, {wg.d_s, wu.d_s}, {bg, bu}};
-    const int pn = (int)((wg.N + 31) / 32);
-    const int64_t rows = std::max<int64_t>(32, (((int64_t)1 << 23) / pn) * 32);
-    for (int64_t r0 = 0; r0 < M; r0 += rows) {
-        const int64_t n = std::min(rows, M - r0);
-        hipLaunchKernelGGL((enchip::gated_w8a8_piece<32, 32, 4>), dim3((unsigned)((n + 31) / 32 * pn)), dim3(256), 0, s,
-                           c->d_aq + r0 * wg.Kp, c->d_as + r0, p, act, d_dst + r0 * wg.N, wg.N, (int)n, (int)wg.N,
-                           (int)wg.Kp, pn);
-    }
+    if (act == enchip::GATE_SILU) launch_gated_frag<enchip::GATE_SILU>(c, wg, c->d_aq, c->d_as, p, M, d_dst, s);
+    else launch_gated_frag<enchip::GATE_GELU>(c, wg, c->d_aq, c->d_as, p, M, d_dst, s);
     if ((rc = check_launch(c, "gated_w8a8"))) return rc;
     return scratch_record(c, s);
 }
