@@ -3,8 +3,6 @@
 
 #include <hip/hip_runtime.h>
 
-#include "gelu_f32.h"
-
 #pragma clang fp contract(off)
 
 namespace enchip {
@@ -24,16 +22,23 @@ __device__ __forceinline__ float silu_f32(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-// GELUF32 without branches: both sides of |u| = 1 are computed, the one that applies is taken.
-__device__ __forceinline__ float gelu_f32_select(float x) {
-    bool tail;
-    const float s = gelu_f32_series(x, tail);
-    const float t = gelu_f32_offseries(x);
-    return tail ? t : s;
+// 0.5 x erfc(-x / sqrt 2), erfc(u) = t p(t) e^(-u^2) with t = 1 / (1 + 0.3275911 u) for u >= 0
+// (Abramowitz and Stegun 7.1.26, the formula of erf_f32's tail: 1.5e-7 of 1) and 2 - erfc(-u) below:
+// one path for every x, and nothing cancels where x is far negative. GELUF32's series near 0 is a
+// little closer there; its list of tails costs more than this formula does.
+__device__ __forceinline__ float gelu_gate_f32(float x) {
+    const float u = fabsf(x) * 0.7071067811865476f;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, u, 1.0f));
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    const float q = p * t * __builtin_amdgcn_exp2f(u * u * -1.4426950408889634f);
+    return 0.5f * x * (x < 0.0f ? q : 2.0f - q);
 }
 
 __device__ __forceinline__ float gate_f32(int act, float g, float u) {  // act is uniform
-    return (act == GATE_SILU ? silu_f32(g) : gelu_f32_select(g)) * u;
+    return (act == GATE_SILU ? silu_f32(g) : gelu_gate_f32(g)) * u;
 }
 
 }  // namespace enchip

@@ -234,6 +234,7 @@ __global__ __launch_bounds__(256, 2) void gated_w8a8_piece(const int8_t *__restr
 // two accumulators meet in the wavefront that holds both. Preconditions as there (an even number of
 // 64-deep stages, 32-bit offsets, N % 4 == 0, 16-byte aligned rows of out, fragment-major A).
 constexpr int GP_BN = 128;  // output channels of a tile
+constexpr int GP_PANEL = 8;  // tile columns of a panel
 
 template <int BM, int ACT, int PRIO>
 __global__ __launch_bounds__(256, BM == PT_BM_SMALL ? 3 : 2) void gated_w8a8_pt(const int8_t *__restrict__ A,
@@ -256,10 +257,19 @@ __global__ __launch_bounds__(256, BM == PT_BM_SMALL ? 3 : 2) void gated_w8a8_pt(
     const int xcnt = q + (xcd < r ? 1 : 0);
     const int ntiles = slot < xcnt ? (xcnt - slot + per_xcd - 1) / per_xcd : 0;
     if (ntiles == 0) return;
-    auto tile_id = [&](int i) { return xbeg + slot + i * per_xcd; };
+    // Tiles are numbered panel by panel of GP_PANEL tile columns, row blocks first: what an XCD holds
+    // at once is a few row blocks times one panel, whose weights stay in its L2.
+    const int rbs = numTiles / tilesN;
+    auto tile_at = [&](int i, int &m0, int &n0) {
+        const int t = xbeg + slot + i * per_xcd, panel = t / (rbs * GP_PANEL), rest = t - panel * rbs * GP_PANEL;
+        const int width = min(GP_PANEL, tilesN - panel * GP_PANEL), rb = rest / width;
+        m0 = rb * BM;
+        n0 = (panel * GP_PANEL + rest - rb * width) * GP_BN;
+    };
     uint32_t aoff_c[FAW], aoff_x[FAW], woff_c, woff_x;  // this lane's offsets: current / next tile
     auto tile_offs = [&](int tile, uint32_t *aoff, uint32_t &woff) {
-        const int m0 = (tile / tilesN) * BM, n0 = (tile % tilesN) * GP_BN;
+        int m0, n0;
+        tile_at(tile, m0, n0);
 #pragma unroll
         for (int i = 0; i < FAW; ++i) {
             const int f = wave + NW * i;
@@ -285,8 +295,8 @@ __global__ __launch_bounds__(256, BM == PT_BM_SMALL ? 3 : 2) void gated_w8a8_pt(
             *reinterpret_cast<i32x4 *>(smem + ls * STAGE + (wave + NW * i) * 1024 + lane * 16) = areg[ring][i];
     };
     i32x16 acc[TM][2];
-    tile_offs(tile_id(0), aoff_c, woff_c);
-    tile_offs(tile_id(ntiles > 1 ? 1 : 0), aoff_x, woff_x);
+    tile_offs(0, aoff_c, woff_c);
+    tile_offs(ntiles > 1 ? 1 : 0, aoff_x, woff_x);
 #pragma unroll
     for (int d = 0; d < PW; ++d) load_stage(d, d);
     awrite(0, 0);
@@ -298,8 +308,8 @@ __global__ __launch_bounds__(256, BM == PT_BM_SMALL ? 3 : 2) void gated_w8a8_pt(
     const int as_slot = (tid & ~31) + (tid & 7) * 4 + ((tid & 31) >> 3);  // its 4 rows' scales contiguous
     int g = 0;
     for (int it = 0; it < ntiles; ++it) {
-        const int tile = tile_id(it);
-        const int m0 = (tile / tilesN) * BM, n0 = (tile % tilesN) * GP_BN;
+        int m0, n0;
+        tile_at(it, m0, n0);
         // the tile's epilogue constants, loaded before its main loop, staged in LDS after it
         const float c_as = aS[min(m0 + (tid & (BM - 1)), M - 1)];
         const int cn = min(n0 + (tid & (GP_BN - 1)), N - 1), ct = tid >> 7;
@@ -347,7 +357,7 @@ __global__ __launch_bounds__(256, BM == PT_BM_SMALL ? 3 : 2) void gated_w8a8_pt(
 #pragma unroll
         for (int i = 0; i < FAW; ++i) aoff_c[i] = aoff_x[i];
         woff_c = woff_x;
-        tile_offs(tile_id(it + 2 < ntiles ? it + 2 : ntiles - 1), aoff_x, woff_x);
+        tile_offs(it + 2 < ntiles ? it + 2 : ntiles - 1, aoff_x, woff_x);
 
         if (PRIO) __builtin_amdgcn_s_setprio(0);
         if (tid < BM) s_as[as_slot] = c_as;
