@@ -2647,13 +2647,30 @@ int launch_wo(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda, const
         else WO_CALL((gemm_wo<BITS, GATED, TM, NT, WM, WN, KS, KC, false>), 32 * TM * WM, (GATED ? 16 : 32) * NT * WN, 64 * WM * WN * KS); \
     } while (0)
     const bool vec = p.K % 4 == 0 && lda % 4 == 0 && (uintptr_t)A % 16 == 0;
-    const bool one = p.Kp / (BITS == 4 ? 32 : 16) <= 4 * WO_WAVES;
-    if (M == 1 && one) WO_CALL((gemv_wo<BITS, 1, GATED, 1>), 1, 16, 64 * WO_WAVES);
-    else if (M == 1) WO_CALL((gemv_wo<BITS, 1, GATED, 4>), 1, 16, 64 * WO_WAVES);
-    else if (M == 2) WO_CALL((gemv_wo<BITS, 2, GATED, 2>), 2, 16, 64 * WO_WAVES);
-    else if (M <= 4) WO_CALL((gemv_wo<BITS, 4, GATED, 2>), 4, 16, 64 * WO_WAVES);
+    // A few rows: a wavefront per K block while there are more blocks than wavefronts
+    const int64_t blocks = (p.Kp + (BITS == 4 ? 255 : 127)) / (BITS == 4 ? 256 : 128);
+    const int kbits = blocks >= 8 ? 3 : blocks >= 4 ? 2 : blocks >= 2 ? 1 : 0;
+#define WO_FEW(MB, NG)                                                                                               \
+    do {                                                                                                             \
+        const int chans = 8 * (NG) * (WO_WAVES >> kbits), tilesN = (int)((p.N + chans - 1) / chans);                 \
+        const int64_t rows = std::max<int64_t>((MB), (((int64_t)1 << 22) / tilesN) * (MB));                          \
+        for (int64_t r0 = 0; r0 < M; r0 += rows) {                                                                   \
+            const int64_t n = std::min(rows, M - r0);                                                                \
+            hipLaunchKernelGGL((gemv_wo<BITS, MB, NG, GATED>), dim3((unsigned)((n + (MB)-1) / (MB) * tilesN)),       \
+                               dim3(64 * WO_WAVES), 0, s, A + r0 * lda, lda, p.w[0], p.w[1], b0, b1, act, C + r0 * ldc, \
+                               ldc, (int)n, (int)p.N, (int)p.K, (int)p.Kp, cpg, (int)p.G, tilesN, kbits);            \
+        }                                                                                                            \
+    } while (0)
+    const bool wide = p.N / (16 * (WO_WAVES >> kbits)) >= 2 * (int64_t)c->num_cus;
+    if (M == 1 && wide) WO_FEW(1, 2);
+    else if (M == 1) WO_FEW(1, 1);
+    else if (M == 2 && wide) WO_FEW(2, 2);
+    else if (M == 2) WO_FEW(2, 1);
+    else if (M <= 16 && wide) WO_FEW(4, 2);
+    else if (M <= 16) WO_FEW(4, 1);
     else if (M <= 64) WO_TILE(1, 2, 1, 1, 4, 128);
     else WO_TILE(1, 2, 1, 4, 2, 128);
+#undef WO_FEW
 #undef WO_TILE
 #undef WO_CALL
     return check_launch(c, "weight-only product");

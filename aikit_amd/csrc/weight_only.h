@@ -14,8 +14,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <utility>
-
 #include "gated.h"
 #include "gemm_q8w.h"
 #include "kernels.h"
@@ -62,119 +60,165 @@ __global__ __launch_bounds__(256) void q4_scales(const uint16_t *__restrict__ s,
     out[t] = n < N ? s[n * G + g] : 0;
 }
 
-// v of lane B of each 16-lane row, in every lane of the row.
-template <int B>
-__device__ __forceinline__ float row_lane(float v) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x150 | B, 0xf, 0xf, true));
+// Sum of v over the lanes of equal lane % 8, in all of them.
+__device__ __forceinline__ float sum_units(float v) {
+    v += __uint_as_float(lane_dpp<0x128>(__float_as_uint(v)));  // lane + 8 of the 16-lane row
+    uint32_t a, b;
+    lane_swap16(__float_as_uint(v), a, b);
+    v = __uint_as_float(a) + __uint_as_float(b);
+    lane_swap32(__float_as_uint(v), a, b);
+    return __uint_as_float(a) + __uint_as_float(b);
 }
 
-// A few rows: every wavefront covers 16 channels x 4 units of k (32 k of a 4-bit weight, 16 of an
-// int8 one: 16 bytes per lane), its four 16-lane rows one unit each. A lane holds 1/16 of its
-// unit's activations, which reach the row's 16 channels as broadcasts within the row. The
-// WO_WAVES wavefronts of a workgroup split K; the sums meet in LDS and are added in one order.
-// PF: steps whose loads are in flight together.
+// A few rows. A lane takes one channel and one unit of k at a time (16 bytes of weight: 32 k of a
+// 4-bit one, 16 of an int8 one), a wavefront 8 channels x 8 units, a block of 256 or 128 k: eight
+// whole cache lines. The block's activations reach the lanes through the wavefront's own LDS and
+// stay in registers for all of its weights, so that a code costs its conversion and MB multiply-adds
+// in f32. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
+// 8 NG each. One block ahead is in flight. The lanes' and the wavefronts' sums are added in one order.
+//
+// Bound by the reading of the weights while VALU work is short of it: per 4-bit KiB 32 codes a lane,
+// 67 operations for one row and 33 more for each further one.
 constexpr int WO_WAVES = 8;
 
-template <int BITS, int MB, bool GATED, int PF>
+template <int BITS, int MB, int NG, bool GATED>
 __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict__ A, int64_t lda, WoWeight w0, WoWeight w1,
                                                          const float *__restrict__ b0, const float *__restrict__ b1, int act,
                                                          float *__restrict__ C, int64_t ldc, int M, int N, int K, int Kp,
-                                                         FastDiv cpg, int G, int tilesN) {
-    constexpr int NWT = GATED ? 2 : 1, CK = BITS == 4 ? 32 : 16, AV = CK / 16;
-    __shared__ float red[NWT][MB][WO_WAVES][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = lane >> 4, i = lane & 15;
-    const int n0 = (blockIdx.x % tilesN) * 16, m0 = (blockIdx.x / tilesN) * MB;
-    const int units = Kp / CK;
+                                                         FastDiv cpg, int G, int tilesN, int kbits) {
+    constexpr int NW = GATED ? 2 : 1, CK = BITS == 4 ? 32 : 16, BK = 8 * CK, PU = CK + 4, LV = BK / 64;
+    __shared__ __attribute__((aligned(16))) float s_a[WO_WAVES][MB][8 * PU];
+    __shared__ float red[WO_WAVES][NG * NW * MB][8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, unit = lane >> 3, ch = lane & 7;
+    const int ks = wave & ((1 << kbits) - 1), gsub = wave >> kbits, groups = NG * (WO_WAVES >> kbits);
+    const int n0 = (blockIdx.x % tilesN) * 8 * groups, m0 = (blockIdx.x / tilesN) * MB, nw = n0 + 8 * NG * gsub;
+    const int units = Kp / CK, blocks = (units + 7) / 8, step = 1 << kbits;
     const WoWeight w[2] = {w0, w1};
     const float *ar[MB];
 #pragma unroll
     for (int m = 0; m < MB; ++m) ar[m] = A + (int64_t)min(m0 + m, M - 1) * lda;
 
-    float sum[NWT][MB];
+    uint4 q[NG][NW];
+    _Float16 sc[NG][NW];
+    float av[MB][LV];
+    auto load = [&](int blk) {
+        const int u = min(8 * blk + unit, units - 1);
 #pragma unroll
-    for (int t = 0; t < NWT; ++t)
+        for (int g = 0; g < NG; ++g) {
+            const int n = nw + 8 * g;  // within Np: a multiple of 256
+            const int64_t at = BITS == 4 ? ((int64_t)(n >> 6) * units + u) * 1024 + ((n & 63) + ch) * 16
+                                         : ((int64_t)(n >> 5) * (units >> 1) + (u >> 1)) * 1024 + ((n & 31) + ch + 32 * (u & 1)) * 16;
 #pragma unroll
-        for (int m = 0; m < MB; ++m) sum[t][m] = 0.0f;
-
-    for (int s0 = 4 * wave; s0 < units; s0 += 4 * WO_WAVES * PF) {
-        uint4 q[PF][NWT];
-        float sc[PF][NWT], a[PF][MB][AV];
-#pragma unroll
-        for (int p = 0; p < PF; ++p) {
-            const int u = s0 + 4 * WO_WAVES * p + part, uc = min(u, units - 1);
-            const int64_t at = BITS == 4 ? ((int64_t)(n0 >> 6) * (Kp >> 5) + uc) * 1024 + ((n0 & 63) + i) * 16
-                                         : ((int64_t)(n0 >> 5) * (Kp >> 5) + (uc >> 1)) * 1024 + ((n0 & 31) + i + 32 * (uc & 1)) * 16;
-#pragma unroll
-            for (int t = 0; t < NWT; ++t) {
-                q[p][t] = *reinterpret_cast<const uint4 *>(w[t].q + at);
+            for (int t = 0; t < NW; ++t) {
+                q[g][t] = *reinterpret_cast<const uint4 *>(w[t].q + at);
                 if (BITS == 4)
-                    sc[p][t] = (float)static_cast<const _Float16 *>(
-                        w[t].s)[((int64_t)(n0 >> 6) * G + min((int)cpg.div(uc), G - 1)) * 64 + (n0 & 63) + i];
+                    sc[g][t] = static_cast<const _Float16 *>(
+                        w[t].s)[((int64_t)(n >> 6) * G + min((int)cpg.div(u), G - 1)) * 64 + (n & 63) + ch];
             }
-#pragma unroll
-            for (int m = 0; m < MB; ++m)
-#pragma unroll
-                for (int e = 0; e < AV; ++e) {
-                    const int k = CK * u + AV * i + e;
-                    const float v = ar[m][min(k, K - 1)];
-                    a[p][m][e] = k < K ? v : 0.0f;
-                }
         }
+        const int k = BK * blk + LV * lane;
 #pragma unroll
-        for (int p = 0; p < PF; ++p)
+        for (int m = 0; m < MB; ++m)
+            if (k + LV <= K) {
 #pragma unroll
-            for (int t = 0; t < NWT; ++t) {
-                float g[MB];  // the unit's sums, unscaled
+                for (int e = 0; e < LV; ++e) av[m][e] = ar[m][k + e];
+            } else {  // k past K counts as zero
 #pragma unroll
-                for (int m = 0; m < MB; ++m) g[m] = 0.0f;
-                const uint32_t qd[4] = {q[p][t].x, q[p][t].y, q[p][t].z, q[p][t].w};
-                auto dword = [&](auto dc) {
-                    constexpr int D = decltype(dc)::value;
-                    const uint32_t lo = qd[D];
-                    uint32_t hi = lo >> 4;
-                    if (BITS == 4) asm("" : "+v"(hi));  // one shift for its four codes
-                    auto byte = [&](auto bc) {
-                        constexpr int B = decltype(bc)::value, J = 4 * D + B;
-                        if constexpr (BITS == 4) {
-                            const float f0 = __builtin_amdgcn_cvt_off_f32_i4((int)((lo >> (8 * B)) & 0xff));  // q / 16
-                            const float f1 = __builtin_amdgcn_cvt_off_f32_i4((int)((hi >> (8 * B)) & 0xff));
+                for (int e = 0; e < LV; ++e) {
+                    const float x = ar[m][min(k + e, K - 1)];
+                    av[m][e] = k + e < K ? x : 0.0f;
+                }
+            }
+    };
+    float sum[NG][NW][MB];
 #pragma unroll
-                            for (int m = 0; m < MB; ++m) {
-                                g[m] = __builtin_fmaf(row_lane<J>(a[p][m][0]), f0, g[m]);
-                                g[m] = __builtin_fmaf(row_lane<J>(a[p][m][AV - 1]), f1, g[m]);
-                            }
-                        } else {
-                            const float f = (float)(int8_t)((lo >> (8 * B)) & 0xff);
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
-                            for (int m = 0; m < MB; ++m) g[m] = __builtin_fmaf(row_lane<J>(a[p][m][0]), f, g[m]);
+        for (int t = 0; t < NW; ++t)
+#pragma unroll
+            for (int m = 0; m < MB; ++m) sum[g][t][m] = 0.0f;
+    if (ks < blocks) load(ks);
+    for (int blk = ks; blk < blocks; blk += step) {
+        float a[MB][CK];
+        uint4 qc[NG][NW];
+        float scc[NG][NW];
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int e = 0; e < LV; ++e) s_a[wave][m][(LV * lane / CK) * PU + LV * lane % CK + e] = av[m][e];
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int t = 0; t < NW; ++t) qc[g][t] = q[g][t], scc[g][t] = BITS == 4 ? 16.0f * (float)sc[g][t] : 1.0f;
+        if (blk + step < blocks) load(blk + step);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int e = 0; e < CK; e += 4) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(&s_a[wave][m][unit * PU + e]);
+                a[m][e] = v.x, a[m][e + 1] = v.y, a[m][e + 2] = v.z, a[m][e + 3] = v.w;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int t = 0; t < NW; ++t) {
+                float y[MB];  // the unit's sums, unscaled
+#pragma unroll
+                for (int m = 0; m < MB; ++m) y[m] = 0.0f;
+                const uint32_t qd[4] = {qc[g][t].x, qc[g][t].y, qc[g][t].z, qc[g][t].w};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t lo = qd[d];
+                    if constexpr (BITS == 4) {
+                        uint32_t hi = lo >> 4;
+                        asm("" : "+v"(hi));  // one shift for its four codes
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const float f0 = __builtin_amdgcn_cvt_off_f32_i4((int)((lo >> (8 * b)) & 0xff));  // q / 16
+                            const float f1 = __builtin_amdgcn_cvt_off_f32_i4((int)((hi >> (8 * b)) & 0xff));
+#pragma unroll
+                            for (int m = 0; m < MB; ++m)
+                                y[m] = __builtin_fmaf(a[m][8 * d + 2 * b + 1], f1, __builtin_fmaf(a[m][8 * d + 2 * b], f0, y[m]));
                         }
-                    };
-                    [&]<int... B>(std::integer_sequence<int, B...>) { (byte(std::integral_constant<int, B>{}), ...); }
-                    (std::make_integer_sequence<int, 4>{});
-                };
-                [&]<int... D>(std::integer_sequence<int, D...>) { (dword(std::integral_constant<int, D>{}), ...); }
-                (std::make_integer_sequence<int, 4>{});
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const float f = (float)(int8_t)((lo >> (8 * b)) & 0xff);
+#pragma unroll
+                            for (int m = 0; m < MB; ++m) y[m] = __builtin_fmaf(a[m][4 * d + b], f, y[m]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int m = 0; m < MB; ++m)
-                    sum[t][m] = BITS == 4 ? __builtin_fmaf(g[m], 16.0f * sc[p][t], sum[t][m]) : sum[t][m] + g[m];
+                    sum[g][t][m] = BITS == 4 ? __builtin_fmaf(y[m], scc[g][t], sum[g][t][m]) : sum[g][t][m] + y[m];
             }
     }
 #pragma unroll
-    for (int t = 0; t < NWT; ++t)
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int m = 0; m < MB; ++m) red[t][m][wave][lane] = sum[t][m];
+        for (int t = 0; t < NW; ++t)
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                const float v = sum_units(sum[g][t][m]);
+                if (lane < 8) red[wave][(g * NW + t) * MB + m][lane] = v;
+            }
     __syncthreads();
-    if (tid >= 16 * MB) return;
-    const int m = tid >> 4, n = n0 + i;
-    if (m0 + m >= M || n >= N) return;
-    float y[NWT];
+    // thread: channel tid % (8 groups), row tid / (8 groups)
+    const int chans = 8 * groups, c = tid & (chans - 1), m = tid / chans, n = n0 + c;
+    if (m >= MB || m0 + m >= M || n >= N) return;
+    const int g = (c >> 3) % NG, first = (c >> 3) / NG << kbits;
+    float y[NW];
 #pragma unroll
-    for (int t = 0; t < NWT; ++t) {
+    for (int t = 0; t < NW; ++t) {
         y[t] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < WO_WAVES; ++j)
-#pragma unroll
-            for (int p = 0; p < 4; ++p) y[t] += red[t][m][j][16 * p + i];
+        for (int j = 0; j < step; ++j) y[t] += red[first + j][(g * NW + t) * MB + m][c & 7];
         if (BITS == 8) y[t] *= static_cast<const float *>(w[t].s)[n];
     }
     float v = y[0];
