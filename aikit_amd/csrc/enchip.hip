@@ -2453,7 +2453,7 @@ int enchip_bias_act_rows_dev(enchip_ctx *ctx, float *d_x, int64_t ld, int64_t ro
 namespace {
 
 enchip::FastDiv fast_div(int64_t d) {
-    return {(uint32_t)d, d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + (uint64_t)d - 1) / (uint64_t)d)};
+    return {(uint32_t)d, d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + (uint64_t)d - 1) / (uint64_t)d), d == 1 ? ~0u : 0u};
 }
 
 constexpr double kTwoPi = 6.283185307179586476925286766559;
@@ -2624,55 +2624,100 @@ WoArgs wo_args(const Weight4 &a, const Weight4 &b) {
     return {4, a.N, a.K, a.Np, a.Kp, a.group / 32, a.G, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
 }
 
+// The rows that gemv_wo takes; more are split first (split_rows) and run on the f16 MFMA.
+constexpr int64_t kFewRows = 8;
+// Bytes of split rows of one pass: more rows run in several.
+constexpr int64_t kSplitBytes = (int64_t)1 << 30;
+
+// Enqueues split_rows of M rows into the context's scratch.
+template <int CH>
+void launch_split(const float *A, int64_t lda, char *parts, float2 *scale, uint8_t *mark, int64_t M, const WoArgs &p, int nkc,
+                  bool vec, hipStream_t s) {
+    using namespace enchip;
+    const dim3 grid((unsigned)((M + SPLIT_WAVES - 1) / SPLIT_WAVES)), block(64 * SPLIT_WAVES);
+    const bool held = p.K <= 512 * CH;
+    if (held && vec) hipLaunchKernelGGL((split_rows<CH, true, true>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+    else if (held) hipLaunchKernelGGL((split_rows<CH, true, false>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+    else if (vec) hipLaunchKernelGGL((split_rows<1, false, true>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+    else hipLaunchKernelGGL((split_rows<1, false, false>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+}
+
+template <int BITS, bool GATED>
+int launch_wo_split(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda, const float *b0, const float *b1, int act,
+                    float *C, int64_t ldc, int64_t M, hipStream_t s) {
+    using namespace enchip;
+    const int nkc = (int)(round_up(p.K, 128) / 32);
+    const int64_t per_block = (int64_t)nkc * 4096, blocks = std::max<int64_t>(1, std::min((M + 31) / 32, kSplitBytes / per_block));
+    const int64_t rows = 32 * blocks, mark_bytes = blocks * (nkc / 4) * 32;
+    int rc;
+    // the parts, then (16-byte aligned) the rows' scales and the marks
+    if ((rc = ensure(c, &c->d_aq, &c->aq_cap, (size_t)(blocks * per_block + rows * 8 + mark_bytes)))) return rc;
+    if ((rc = scratch_wait(c, s))) return rc;
+    char *parts = reinterpret_cast<char *>(c->d_aq);
+    float2 *scale = reinterpret_cast<float2 *>(parts + blocks * per_block);
+    uint8_t *mark = reinterpret_cast<uint8_t *>(scale + rows);
+    const bool vec = p.K % 4 == 0 && lda % 4 == 0 && (uintptr_t)A % 16 == 0;
+    for (int64_t r0 = 0; r0 < M; r0 += rows) {
+        const int64_t n = std::min(rows, M - r0);
+        const float *a = A + r0 * lda;
+        float *out = C + r0 * ldc;
+        if (p.K <= 512) launch_split<1>(a, lda, parts, scale, mark, n, p, nkc, vec, s);
+        else if (p.K <= 1024) launch_split<2>(a, lda, parts, scale, mark, n, p, nkc, vec, s);
+        else launch_split<8>(a, lda, parts, scale, mark, n, p, nkc, vec, s);
+        const WoRows wr = {{parts, scale, mark}, a, lda, (int)n, (int)p.N, (int)p.K, (int)p.Kp, nkc, (int)p.G, fast_div(p.cpg)};
+#define WO_SPLIT(KERNEL, TM, CB, THREADS)                                                                              \
+    do {                                                                                                               \
+        const int64_t tilesN = (p.N + 32 * (CB)-1) / (32 * (CB)), tilesM = (n + 32 * (TM)-1) / (32 * (TM));            \
+        if (!grid_fits(tilesM * tilesN, THREADS))                                                                      \
+            return fail(c, ENCHIP_ERR_ARG, "weight-only product: M=%lld N=%lld needs more workgroups than one launch addresses", \
+                        (long long)M, (long long)p.N);                                                                 \
+        hipLaunchKernelGGL((KERNEL), dim3((unsigned)(tilesM * tilesN)), dim3(THREADS), 0, s, wr, p.w[0], p.w[1], b0, b1, act, \
+                           out, ldc, (int)tilesN);                                                                     \
+    } while (0)
+        const int64_t cus = c->num_cus;
+        auto tiles = [&](int64_t tm, int64_t cb) { return ((n + 32 * tm - 1) / (32 * tm)) * ((p.N + 32 * cb - 1) / (32 * cb)); };
+        constexpr int G2 = GATED ? 2 : 1;  // tiles of a wavefront for one channel block
+        const int force = getenv("WOF") ? atoi(getenv("WOF")) : -1;
+        int form = tiles(1, 1) <= 2 * cus ? 0 : tiles(2, 2 / G2) <= 2 * cus ? 1 : 2;
+        if (force >= 0) form = force;
+        if (form == 0) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, G2, 8, 4>), 1, 1, 512);
+        else if (form == 1) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, 2, 4, 3>), 1, 2 / G2, 256);
+        else if (form == 3) WO_SPLIT((gemm_wo_piece<BITS, GATED, 2, 2, 4, 2>), 2, 2 / G2, 256);
+        else if (form == 4) WO_SPLIT((gemm_wo_tile<BITS, GATED, 4, 2, 2>), 4, 8 / G2, 256);
+        else if (form == 5) WO_SPLIT((gemm_wo_tile<BITS, GATED, 1, 2, 4>), 1, 8 / G2, 256);
+        else if (form == 6) WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 2, 4>), 2, 8 / G2, 256);
+        else WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 4, 2>), 2, 16 / G2, 256);
+#undef WO_SPLIT
+        if ((rc = check_launch(c, "weight-only product"))) return rc;
+    }
+    return scratch_record(c, s);
+}
+
 // Enqueues C = A . W^T (4-bit), or the gated pair, after the caller checked the arguments.
 template <int BITS, bool GATED>
 int launch_wo(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda, const float *b0, const float *b1, int act,
               float *C, int64_t ldc, int64_t M, hipStream_t s) {
     using namespace enchip;
+    if (M > kFewRows) return launch_wo_split<BITS, GATED>(c, p, A, lda, b0, b1, act, C, ldc, M, s);
     const enchip::FastDiv cpg = fast_div(p.cpg);
-#define WO_CALL(KERNEL, BM, BN, THREADS)                                                                           \
-    do {                                                                                                           \
-        const int tilesN = (int)((p.N + (BN)-1) / (BN));                                                           \
-        const int64_t rows = std::max<int64_t>((BM), (((int64_t)1 << 22) / tilesN) * (BM));                        \
-        for (int64_t r0 = 0; r0 < M; r0 += rows) {                                                                 \
-            const int64_t n = std::min(rows, M - r0);                                                              \
-            hipLaunchKernelGGL((KERNEL), dim3((unsigned)((n + (BM)-1) / (BM) * tilesN)), dim3(THREADS), 0, s,      \
-                               A + r0 * lda, lda, p.w[0], p.w[1], b0, b1, act, C + r0 * ldc, ldc, (int)n, (int)p.N, \
-                               (int)p.K, (int)p.Kp, cpg, (int)p.G, tilesN);                                        \
-        }                                                                                                          \
-    } while (0)
-#define WO_TILE(TM, NT, WM, WN, KS, KC)                                                                              \
-    do {                                                                                                             \
-        if (vec) WO_CALL((gemm_wo<BITS, GATED, TM, NT, WM, WN, KS, KC, true>), 32 * TM * WM, (GATED ? 16 : 32) * NT * WN, 64 * WM * WN * KS); \
-        else WO_CALL((gemm_wo<BITS, GATED, TM, NT, WM, WN, KS, KC, false>), 32 * TM * WM, (GATED ? 16 : 32) * NT * WN, 64 * WM * WN * KS); \
-    } while (0)
-    const bool vec = p.K % 4 == 0 && lda % 4 == 0 && (uintptr_t)A % 16 == 0;
-    // A few rows: a wavefront per K block while there are more blocks than wavefronts
+    // a wavefront per K block while there are more blocks than wavefronts
     const int64_t blocks = (p.Kp + (BITS == 4 ? 255 : 127)) / (BITS == 4 ? 256 : 128);
     const int kbits = blocks >= 8 ? 3 : blocks >= 4 ? 2 : blocks >= 2 ? 1 : 0;
 #define WO_FEW(MB, NG)                                                                                               \
     do {                                                                                                             \
         const int chans = 8 * (NG) * (WO_WAVES >> kbits), tilesN = (int)((p.N + chans - 1) / chans);                 \
-        const int64_t rows = std::max<int64_t>((MB), (((int64_t)1 << 22) / tilesN) * (MB));                          \
-        for (int64_t r0 = 0; r0 < M; r0 += rows) {                                                                   \
-            const int64_t n = std::min(rows, M - r0);                                                                \
-            hipLaunchKernelGGL((gemv_wo<BITS, MB, NG, GATED>), dim3((unsigned)((n + (MB)-1) / (MB) * tilesN)),       \
-                               dim3(64 * WO_WAVES), 0, s, A + r0 * lda, lda, p.w[0], p.w[1], b0, b1, act, C + r0 * ldc, \
-                               ldc, (int)n, (int)p.N, (int)p.K, (int)p.Kp, cpg, (int)p.G, tilesN, kbits);            \
-        }                                                                                                            \
+        hipLaunchKernelGGL((gemv_wo<BITS, MB, NG, GATED>), dim3((unsigned)((M + (MB)-1) / (MB) * tilesN)),           \
+                           dim3(64 * WO_WAVES), 0, s, A, lda, p.w[0], p.w[1], b0, b1, act, C, ldc, (int)M, (int)p.N, \
+                           (int)p.K, (int)p.Kp, cpg, (int)p.G, tilesN, kbits);                                       \
     } while (0)
     const bool wide = p.N / (16 * (WO_WAVES >> kbits)) >= 2 * (int64_t)c->num_cus;
     if (M == 1 && wide) WO_FEW(1, 2);
     else if (M == 1) WO_FEW(1, 1);
     else if (M == 2 && wide) WO_FEW(2, 2);
     else if (M == 2) WO_FEW(2, 1);
-    else if (M <= 16 && wide) WO_FEW(4, 2);
-    else if (M <= 16) WO_FEW(4, 1);
-    else if (M <= 64) WO_TILE(1, 2, 1, 1, 4, 128);
-    else WO_TILE(1, 2, 1, 4, 2, 128);
+    else if (wide) WO_FEW(4, 2);
+    else WO_FEW(4, 1);
 #undef WO_FEW
-#undef WO_TILE
-#undef WO_CALL
     return check_launch(c, "weight-only product");
 }
 

@@ -490,10 +490,10 @@ __device__ __forceinline__ int xcd_logical_tile(int pid, int nblocks) {
     return (xcd < r) ? xcd * (q + 1) + idx : r * (q + 1) + (xcd - r) * q + idx;
 }
 
-// x / d for x d < 2^32; m = 2^32 / d rounded up, 0 for d = 1.
+// x / d for x d < 2^32: m = 2^32 / d rounded up and one = 0; for d = 1 m = 0 and one = ~0.
 struct FastDiv {
-    uint32_t d, m;
-    __device__ __forceinline__ uint32_t div(uint32_t x) const { return m ? __umulhi(x, m) : x; }
+    uint32_t d, m, one;
+    __device__ __forceinline__ uint32_t div(uint32_t x) const { return __umulhi(x, m) + (x & one); }
 };
 
 // ----------------------------------------------------------------------------

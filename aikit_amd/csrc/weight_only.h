@@ -5,17 +5,19 @@
 // y_i the product above, or for int8 weights ws[n] sum_k A[m, k] q[n, k]. The activations are
 // never quantized, sums are f32.
 //
-// 4-bit image: [Np/64][Kp/32][64][16 B], 16 bytes per channel and 32 k: two codes a byte in k
-// order, the lower k in the low half, in two's complement (the caller's c becomes q = c - 8);
-// padding channels and k are 0. Np = N rounded up to 256, Kp = K rounded up to 64. Scales f16
-// [Np/64][G][64], G = ceil(K / group). Int8 weights: the fragment-major image of kernels.h.
+// 4-bit image: [Np/64][Kp/32][64][16 B], 16 bytes per channel and 32 k, codes c = q + 8. A word holds
+// 8 k's: k 2i in bits 4i .. and k 2i + 1 in bits 16 + 4i .., so that one mask and one packed f16
+// subtraction give two neighbouring values. Padding channels and k are 0 (c = 8). Np = N rounded up
+// to 256, Kp = K rounded up to 64. Scales f16 [Np/64][G][64], G = ceil(K / group). Int8 weights: the
+// fragment-major image of kernels.h.
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "attention_f32.h"
 #include "gated.h"
-#include "gemm_q8w.h"
+#include "gemm_f32.h"
 #include "kernels.h"
 
 #pragma clang fp contract(off)
@@ -40,12 +42,11 @@ __global__ __launch_bounds__(256) void q4_image(const uint8_t *__restrict__ code
     for (int d = 0; d < 4; ++d) {
         w[d] = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int k = k0 + 8 * d + 2 * b;
-            if (n >= N || k >= K) continue;
-            uint32_t c = codes[n * kb + k / 2] ^ 0x88u;
-            if (k + 1 >= K) c &= 0x0fu;
-            w[d] |= c << (8 * b);
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + 8 * d + 2 * i;
+            uint32_t c = n < N && k < K ? codes[n * kb + k / 2] : 0x88u;
+            if (k + 1 >= K) c = (c & 0x0fu) | 0x80u;
+            w[d] |= (c & 15u) << (4 * i) | (c >> 4) << (16 + 4 * i);
         }
     }
     image[t] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -58,6 +59,27 @@ __global__ __launch_bounds__(256) void q4_scales(const uint16_t *__restrict__ s,
     if (t >= total) return;
     const int64_t n = (t >> 6) / G * 64 + (t & 63), g = (t >> 6) % G;
     out[t] = n < N ? s[n * G + g] : 0;
+}
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// 8 neighbouring codes as four pairs of f16 values, exactly: a code in the low bits of 1024 (f16's
+// step there is 1), less 1024 and the code's offset. Conversions to f32 take four times a plain
+// operation's issue; these take one each for two codes.
+__device__ __forceinline__ void widen8_q4(uint32_t w, f16x2 (&h)[4]) {
+    uint32_t mask = 0x000f000fu, base = 0x64006400u;
+    asm("" : "+s"(mask));  // kept in registers: one v_and_or each
+    asm("" : "+v"(base));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & mask) | base) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
+}
+__device__ __forceinline__ void widen8_q8(uint32_t w0, uint32_t w1, f16x2 (&h)[4]) {
+    const uint32_t w[2] = {w0 ^ 0x80808080u, w1 ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w[i >> 1], i & 1 ? 0x04030402u : 0x04010400u)) -
+               f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
 }
 
 // Sum of v over the lanes of equal lane % 8, in all of them.
@@ -73,12 +95,10 @@ __device__ __forceinline__ float sum_units(float v) {
 // A few rows. A lane takes one channel and one unit of k at a time (16 bytes of weight: 32 k of a
 // 4-bit one, 16 of an int8 one), a wavefront 8 channels x 8 units, a block of 256 or 128 k: eight
 // whole cache lines. The block's activations reach the lanes through the wavefront's own LDS and
-// stay in registers for all of its weights, so that a code costs its conversion and MB multiply-adds
-// in f32. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
+// stay in registers for all of its weights, so that a code costs its share of the widening and MB
+// mixed multiply-adds, f32 += f32 * f16. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
 // 8 NG each. One block ahead is in flight. The lanes' and the wavefronts' sums are added in one order.
 //
-// Bound by the reading of the weights while VALU work is short of it: per 4-bit KiB 32 codes a lane,
-// 67 operations for one row and 33 more for each further one.
 constexpr int WO_WAVES = 8;
 
 template <int BITS, int MB, int NG, bool GATED>
@@ -149,7 +169,7 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int t = 0; t < NW; ++t) qc[g][t] = q[g][t], scc[g][t] = BITS == 4 ? 16.0f * (float)sc[g][t] : 1.0f;
+            for (int t = 0; t < NW; ++t) qc[g][t] = q[g][t], scc[g][t] = BITS == 4 ? (float)sc[g][t] : 1.0f;
         if (blk + step < blocks) load(blk + step);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -173,27 +193,16 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
                 for (int m = 0; m < MB; ++m) y[m] = 0.0f;
                 const uint32_t qd[4] = {qc[g][t].x, qc[g][t].y, qc[g][t].z, qc[g][t].w};
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t lo = qd[d];
-                    if constexpr (BITS == 4) {
-                        uint32_t hi = lo >> 4;
-                        asm("" : "+v"(hi));  // one shift for its four codes
+                for (int d = 0; d < CK / 8; ++d) {
+                    f16x2 h[4];
+                    if constexpr (BITS == 4) widen8_q4(qd[d], h);
+                    else widen8_q8(qd[2 * d], qd[2 * d + 1], h);
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            const float f0 = __builtin_amdgcn_cvt_off_f32_i4((int)((lo >> (8 * b)) & 0xff));  // q / 16
-                            const float f1 = __builtin_amdgcn_cvt_off_f32_i4((int)((hi >> (8 * b)) & 0xff));
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int m = 0; m < MB; ++m)
-                                y[m] = __builtin_fmaf(a[m][8 * d + 2 * b + 1], f1, __builtin_fmaf(a[m][8 * d + 2 * b], f0, y[m]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            const float f = (float)(int8_t)((lo >> (8 * b)) & 0xff);
-#pragma unroll
-                            for (int m = 0; m < MB; ++m) y[m] = __builtin_fmaf(a[m][4 * d + b], f, y[m]);
-                        }
-                    }
+                        for (int m = 0; m < MB; ++m)
+                            y[m] = __builtin_fmaf(a[m][8 * d + 2 * i + 1], (float)h[i].y,
+                                                  __builtin_fmaf(a[m][8 * d + 2 * i], (float)h[i].x, y[m]));
                 }
 #pragma unroll
                 for (int m = 0; m < MB; ++m)
@@ -226,124 +235,322 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
     C[(int64_t)(m0 + m) * ldc + n] = v;
 }
 
-// 8 codes of a 4-bit image word, in k order, as bf16 values q / 16 (exact).
-__device__ __forceinline__ bf16x8 q4_widen8(uint32_t lo) {
-    uint32_t hi = lo >> 4;
-    asm("" : "+v"(hi));  // one shift for its four codes
-    auto pair = [&](int b) {
-        return q8w_pack(__float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)((lo >> (8 * b)) & 0xff))),
-                        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)((hi >> (8 * b)) & 0xff))));
+// More rows run on the f16 MFMA. split_rows scales each row of activations by the power of two that
+// brings its largest to 2^14 .. 2^15 and splits it into two f16 parts, hi by truncation, lo the rest
+// rounded: 22 bits of every activation down to 2^-18 of the row's largest, below that 2^-39 of it (lo's
+// smallest step). Codes are f16 values exactly, so products are exact and two MFMAs stand for one in
+// f32. A row's block of 128 k where more than a sixteenth of the nonzero activations lie below 2^-19 of
+// the row's largest (an outlier so large that the bits below matter) is marked: its parts are 0, and
+// the products add it on the f32 MFMA at their end.
+//
+// Parts, in the A operand's order for the weights' order of k: [M/32][Ka/32] x 4 KiB, plane x and
+// step j of chunk kc at x 2048 + j 1024, 16 bytes per lane: row lane % 32, k = 32 kc + 16 (lane / 32) + 8 j
+// .. + 7. Ka = K rounded up to 128, zero past K. Rows past M are not written (and no output is theirs).
+struct SplitRows {
+    const char *parts;
+    const float2 *scale;   // [M] the row's power of two, negative for a row with marks, and the one that takes it back
+    const uint8_t *mark;   // [M/32][Ka/128][32]
+};
+typedef float f32x2v __attribute__((ext_vector_type(2)));
+constexpr int SPLIT_WAVES = 4;
+
+// One wavefront per row. A lane holds granules of 8 k: lane + 64 i; HELD: all of the row's (K <= 512
+// CH), read once. Otherwise the row is read twice.
+template <int CH, bool HELD, bool VEC>
+__global__ __launch_bounds__(64 * SPLIT_WAVES) void split_rows(const float *__restrict__ A, int64_t lda, char *__restrict__ parts,
+                                                               float2 *__restrict__ scale, uint8_t *__restrict__ mark, int M,
+                                                               int K, int nkc) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * SPLIT_WAVES + (threadIdx.x >> 6);
+    if (row >= M) return;
+    const float *a = A + (int64_t)row * lda;
+    const int granules = 4 * nkc, rounds = (granules + 63) / 64;
+    f32x4 v[CH][2];
+    auto load = [&](int i, f32x4 (&x)[2]) {
+        const int k = 8 * (lane + 64 * i);
+        if (VEC) {
+            x[0] = *reinterpret_cast<const f32x4 *>(a + min(k, K - 4));
+            x[1] = *reinterpret_cast<const f32x4 *>(a + min(k + 4, K - 4));
+            if (k >= K) x[0] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (k + 4 >= K) x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float t = a[min(k + e, K - 1)];
+                x[e >> 2][e & 3] = k + e < K ? t : 0.0f;
+            }
+        }
     };
-    return __builtin_bit_cast(bf16x8, (u32x4){pair(0), pair(1), pair(2), pair(3)});
-}
-
-// 8 int8 codes of a weight image, in k order, as bf16 values (exact).
-__device__ __forceinline__ bf16x8 q8_widen8(uint32_t w0, uint32_t w1) {
-    uint32_t x[4];
-    q8w_widen4(w0, x[0], x[1]);
-    q8w_widen4(w1, x[2], x[3]);
-    return __builtin_bit_cast(bf16x8, (u32x4){x[0], x[1], x[2], x[3]});
-}
-
-// Tiles on the bf16 MFMA, activations split exactly into three bf16 parts (gemm_q8w.h). A
-// workgroup computes 32 TM WM rows; each of its WM x WN x KS wavefronts TM x NT 32 x 32 tiles of
-// products over its share of every K stage: NT channel blocks of one weight, or NT / 2 of each
-// of the two, so a gate and its up projection meet in one lane. The stage's activations are split
-// by all threads into three planes in LDS (double-buffered), the weights' codes go straight into
-// registers and are widened there. A 4-bit weight's 32-deep chunk is summed from zero and added
-// scaled: 16 multiply-adds for 6 MFMAs. The KS shares meet in LDS at the end, each wavefront
-// finishing 16 / KS of the accumulator registers.
-template <int BITS, bool GATED, int TM, int NT, int WM, int WN, int KS, int KC, bool VEC>
-__global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_wo(const float *__restrict__ A, int64_t lda, WoWeight w0,
-                                                                WoWeight w1, const float *__restrict__ b0,
-                                                                const float *__restrict__ b1, int act, float *__restrict__ C,
-                                                                int64_t ldc, int M, int N, int K, int Kp, FastDiv cpg, int G,
-                                                                int tilesN) {
-    constexpr int NTHR = 64 * WM * WN * KS, BM = 32 * TM * WM, CPW = GATED ? 16 * NT : 32 * NT, BN = CPW * WN;
-    constexpr int KB = KC / 32 / KS;  // chunks of a wavefront per stage
-    constexpr int P = 2 * KC + 16, PL = BM * P, STAGE = 3 * PL;
-    constexpr int LPR = KC / 4, AV = BM * LPR / NTHR, ER = 16 / KS;
-    constexpr int RED = KS > 1 ? NTHR * (KS - 1) * ER * TM * NT * 4 : 0;
-    constexpr int LDS = 2 * STAGE > RED ? 2 * STAGE : RED;
-    static_assert(AV >= 1 && BM * LPR % NTHR == 0 && KB >= 1 && KC % (32 * KS) == 0 && 16 % KS == 0, "tile");
-    static_assert(!GATED || NT % 2 == 0, "a tile of each weight");
-    __shared__ __attribute__((aligned(16))) char lds[LDS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, hf = lane >> 5;
-    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x);
-    const int m0 = (logical / tilesN) * BM, n0 = (logical % tilesN) * BN;
-    const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
-    const int lk = 4 * (tid % LPR), lr = tid / LPR;
-    const WoWeight w[2] = {w0, w1};
-    const float *ga[AV];
+    float m = 0.0f;
+    auto largest = [&](const f32x4 (&x)[2]) {  // fmaxf passes NaN over
 #pragma unroll
-    for (int i = 0; i < AV; ++i) ga[i] = A + (int64_t)min(m0 + lr + (NTHR / LPR) * i, M - 1) * lda;
-    const int nk32 = Kp / 32;
-    // tile t: 32-channel block cb(t) of weight t % 2 (gated) or 0
-    const int cb0 = (n0 + wn * CPW) >> 5;
-    auto cb = [&](int t) { return cb0 + (GATED ? t >> 1 : t); };
-    const int8_t *wb[NT];
-    const _Float16 *sb[NT];
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e >> 2][e & 3]));
+    };
+    if constexpr (HELD) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const WoWeight &x = w[GATED ? t & 1 : 0];
-        const int c = cb(t);
-        wb[t] = x.q + (BITS == 4 ? (int64_t)(c >> 1) * nk32 * 1024 + ((c & 1) * 32 + r) * 16 + 8 * hf
-                                 : (int64_t)c * nk32 * 1024 + lane * 16);
-        sb[t] = static_cast<const _Float16 *>(x.s) + (BITS == 4 ? (int64_t)(c >> 1) * G * 64 + (c & 1) * 32 + r : 0);
+        for (int i = 0; i < CH; ++i) load(i, v[i]);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) largest(v[i]);
+    } else {
+        for (int i = 0; i < rounds; ++i) {
+            load(i, v[0]);
+            largest(v[0]);
+        }
     }
-    f32x4 ra[AV];
-    uint32_t wr[KB][NT][BITS / 2];
-    _Float16 sc[KB][NT];
-    auto load_a = [&](int c) {
-        const int k = KC * c + lk;
-        if (!VEC && KC * c + KC <= K) {  // uniform: all of the stage, in unaligned 16-byte loads
+    m = wave_absmax(m);
+    // m in [2^(E-127), 2^(E-126)): times 2^(141-E), at most 2^127; an infinite m (E = 255) keeps infinities
+    // and makes the finite values beside them small
+    const int E = (int)(__float_as_uint(m) >> 23), F = min(268 - E, 254);
+    const float up = __uint_as_float((uint32_t)F << 23);
+    uint64_t marked = 0;
+    float minus1 = -1.0f;
+    asm("" : "+s"(minus1));  // keeps hi * -1 + a one mixed multiply-add
+    auto store = [&](int i, f32x4 (&x)[2]) {
+        const int g = lane + 64 * i;
+        uint32_t hi[4], lo[4];
+        int small = 0, some = 0;
 #pragma unroll
-            for (int i = 0; i < AV; ++i) ra[i] = f32x4{ga[i][k], ga[i][k + 1], ga[i][k + 2], ga[i][k + 3]};
-            return;
+        for (int e = 0; e < 4; ++e) {
+            const float p = x[e >> 1][2 * (e & 1)] * up, q = x[e >> 1][2 * (e & 1) + 1] * up;
+            const auto h = __builtin_amdgcn_cvt_pkrtz(p, q);
+            const f32x2v l = {__builtin_fmaf((float)h[0], minus1, p), __builtin_fmaf((float)h[1], minus1, q)};
+            hi[e] = __builtin_bit_cast(uint32_t, h);
+            lo[e] = E == 255 ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector(l, f16x2));  // inf - inf
+            some += (p != 0.0f) + (q != 0.0f);
+            small += (p != 0.0f && fabsf(p) < 0x1p-5f) + (q != 0.0f && fabsf(q) < 0x1p-5f);
         }
-#pragma unroll
-        for (int i = 0; i < AV; ++i) {
-            if (VEC) ra[i] = *reinterpret_cast<const f32x4 *>(ga[i] + min(k, K - 4));
-            else
-                ra[i] = f32x4{ga[i][min(k, K - 1)], ga[i][min(k + 1, K - 1)], ga[i][min(k + 2, K - 1)], ga[i][min(k + 3, K - 1)]};
-        }
+        // a block's 16 granules are a 16-lane row
+        uint32_t n = (uint32_t)(some << 16 | small);
+        n += lane_dpp<0xB1>(n);
+        n += lane_dpp<0x4E>(n);
+        n += lane_dpp<0x141>(n);
+        n += lane_dpp<0x140>(n);
+        const bool mk = E != 255 && 16 * (n & 0xffffu) > (n >> 16);
+        marked |= __builtin_amdgcn_ballot_w64(mk);
+        if (g >= granules) return;
+        char *d = parts + ((int64_t)(row >> 5) * nkc + (g >> 2)) * 4096 + (g & 1) * 1024 + ((row & 31) + 32 * ((g >> 1) & 1)) * 16;
+        *reinterpret_cast<uint4 *>(d) = mk ? make_uint4(0, 0, 0, 0) : make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(d + 2048) = mk ? make_uint4(0, 0, 0, 0) : make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if ((g & 15) == 0) mark[((int64_t)(row >> 5) * (nkc >> 2) + (g >> 4)) * 32 + (row & 31)] = mk;
     };
-    auto load_w = [&](int c) {
+    if constexpr (HELD) {
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const int kc = min(KC / 32 * c + KB * ks + b, nk32 - 1), g = BITS == 4 ? min((int)cpg.div(kc), G - 1) : 0;
+        for (int i = 0; i < CH; ++i) store(i, v[i]);
+    } else {
+        for (int i = 0; i < rounds; ++i) {
+            load(i, v[0]);
+            store(i, v[0]);
+        }
+    }
+    if (lane == 0)
+        scale[row] = make_float2(marked ? -up : up, __uint_as_float(F == 254 ? 0x400000u : (uint32_t)(254 - F) << 23));
+}
+
+// What a product of split rows reads besides the weights.
+struct WoRows {
+    SplitRows a;
+    const float *A;  // the rows as they are, for marked blocks
+    int64_t lda;
+    int M, N, K, Kp, nkc, G;
+    FastDiv cpg;
+};
+
+// TM x NT tiles' weights of one wavefront: NT channel blocks of one weight, or NT / 2 of each of the
+// two, so that a gate and its up projection meet in one lane.
+template <int BITS, bool GATED, int NT>
+struct WoTiles {
+    const int8_t *wb[NT];    // uniform: the tile's channel block, and a lane's place in a chunk of it
+    const _Float16 *sb[NT];
+    uint32_t wl, sl;
+    __device__ __forceinline__ void init(const WoWeight &w0, const WoWeight &w1, int cb0, int lane, int nk32, int G) {
+        wl = BITS == 4 ? (lane & 31) * 16 + 8 * (lane >> 5) : lane * 16;
+        sl = lane & 31;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                if constexpr (BITS == 4) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(wb[t] + (int64_t)kc * 1024);
-                    wr[b][t][0] = v.x, wr[b][t][1] = v.y;
-                    sc[b][t] = sb[t][(int64_t)g * 64];
-                } else {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(wb[t] + (int64_t)kc * 1024);
-                    wr[b][t][0] = v.x, wr[b][t][1] = v.y, wr[b][t][2] = v.z, wr[b][t][3] = v.w;
+        for (int t = 0; t < NT; ++t) {
+            const WoWeight &x = GATED && (t & 1) ? w1 : w0;
+            const int c = cb0 + (GATED ? t >> 1 : t);
+            wb[t] = x.q + (BITS == 4 ? (int64_t)(c >> 1) * nk32 * 1024 + (c & 1) * 512 : (int64_t)c * nk32 * 1024);
+            sb[t] = static_cast<const _Float16 *>(x.s) + (BITS == 4 ? (int64_t)(c >> 1) * G * 64 + (c & 1) * 32 : 0);
+        }
+    }
+    // chunk kc's codes and group scales
+    __device__ __forceinline__ void load(int kc, const FastDiv &cpg, int G, uint32_t (&w)[NT][BITS / 2], _Float16 (&sc)[NT]) const {
+        const int g = BITS == 4 ? min((int)cpg.div(kc), G - 1) : 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if constexpr (BITS == 4) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(wb[t] + (int64_t)kc * 1024 + wl);
+                w[t][0] = v.x, w[t][1] = v.y;
+                sc[t] = (sb[t] + (int64_t)g * 64)[sl];
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4 *>(wb[t] + (int64_t)kc * 1024 + wl);
+                w[t][0] = v.x, w[t][1] = v.y, w[t][2] = v.z, w[t][3] = v.w;
+            }
+        }
+    }
+    static __device__ __forceinline__ void widen(const uint32_t (&w)[BITS / 2], int j, f16x2 (&h)[4]) {
+        if constexpr (BITS == 4) widen8_q4(w[j], h);
+        else widen8_q8(w[2 * j], w[2 * j + 1], h);
+    }
+};
+
+// acc (scaled like the parts) += the products of the marked blocks first, first + step, ... on the f32
+// MFMA, the activations read again.
+template <int BITS, bool GATED, int TM, int NT>
+__device__ __forceinline__ void wo_marked(const WoRows &p, const WoTiles<BITS, GATED, NT> &tiles, int rb, int first, int step,
+                                          f32x16 (&acc)[TM][NT]) {
+    const int lane = threadIdx.x & 63, r = lane & 31, nb = p.nkc >> 2, nk32 = p.Kp >> 5;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int row = min(32 * (rb + i) + r, p.M - 1);
+        const float up = p.a.scale[row].x;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(up < 0.0f) == 0, 1)) continue;
+        const float *a = p.A + (int64_t)row * p.lda;
+        for (int b = first; b < nb; b += step) {
+            const float s = p.a.mark[((int64_t)(row >> 5) * nb + b) * 32 + (row & 31)] ? -up : 0.0f;
+            if (__builtin_amdgcn_ballot_w64(s != 0.0f) == 0) continue;
+            for (int kc = 4 * b; kc < min(4 * b + 4, nk32); ++kc) {
+                uint32_t w[NT][BITS / 2];
+                _Float16 sc[NT];
+                tiles.load(kc, p.cpg, p.G, w, sc);
+                const int k0 = 32 * kc + 16 * (lane >> 5);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    f32x16 part;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) part[e] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        f16x2 h[4];
+                        WoTiles<BITS, GATED, NT>::widen(w[t], j, h);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int k = k0 + 8 * j + e;
+                            const float x = a[min(k, p.K - 1)];
+                            part = __builtin_amdgcn_mfma_f32_32x32x2f32(k < p.K && s != 0.0f ? x * s : 0.0f,
+                                                                        (float)h[e >> 1][e & 1], part, 0, 0, 0);
+                        }
+                    }
+                    const float g = BITS == 4 ? (float)sc[t] : 1.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][t][e] = __builtin_fmaf(part[e], g, acc[i][t][e]);
                 }
             }
         }
-    };
-    auto store_a = [&](int c, char *st) {
-        const int k = KC * c + lk;
+    }
+}
+
+// The products of one chunk; read(i, x, j): row block i's part x, step j.
+template <int BITS, bool GATED, int TM, int NT, typename Read>
+__device__ __forceinline__ void wo_chunk(Read read, const uint32_t (&w)[NT][BITS / 2], const _Float16 (&sc)[NT],
+                                         f32x16 (&acc)[TM][NT]) {
+    f32x16 part[TM][NT];
 #pragma unroll
-        for (int i = 0; i < AV; ++i) {
-            f32x4 v = ra[i];  // k past K counts as zero
-            if (VEC) {
-                if (k >= K) v = f32x4{0.f, 0.f, 0.f, 0.f};
-            } else {
-                v.x = k < K ? v.x : 0.f, v.y = k + 1 < K ? v.y : 0.f, v.z = k + 2 < K ? v.z : 0.f, v.w = k + 3 < K ? v.w : 0.f;
+    for (int j = 0; j < 2; ++j) {
+        f16x8 p[TM][2], q[NT];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) p[i][x] = read(i, x, j);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            f16x2 h[4];
+            WoTiles<BITS, GATED, NT>::widen(w[t], j, h);
+            q[t] = f16x8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+        }
+#pragma unroll
+        for (int x = 1; x >= 0; --x)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (BITS == 8) {
+                        acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][x], q[t], acc[i][t], 0, 0, 0);
+                    } else {
+                        if (j == 0 && x == 1) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) part[i][t][e] = 0.0f;
+                        }
+                        part[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][x], q[t], part[i][t], 0, 0, 0);
+                    }
+                }
+    }
+    if (BITS == 4) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float s = (float)sc[t];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][t][e] = __builtin_fmaf(part[i][t][e], s, acc[i][t][e]);
+        }
+    }
+}
+
+// Stores registers e0 .. e0 + ER - 1 (held in places 0 .. ER - 1) of the tiles at row block rb, channel
+// block cb0.
+template <int BITS, bool GATED, int TM, int NT, int ER>
+__device__ __forceinline__ void wo_store(const WoRows &p, const WoWeight &w0, const WoWeight &w1, const float *b0,
+                                         const float *b1, int act, float *C, int64_t ldc, int rb, int cb0, int e0,
+                                         const f32x16 (&acc)[TM][NT]) {
+    const int lane = threadIdx.x & 63, r = lane & 31;
+    float down[TM][ER];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < ER; ++e) down[i][e] = p.a.scale[min(32 * (rb + i) + acc_row(e0 + e, lane), p.M - 1)].y;
+#pragma unroll
+    for (int u = 0; u < (GATED ? NT / 2 : NT); ++u) {
+        const int n = 32 * (cb0 + u) + r, nn = min(n, p.N - 1);
+        const float s0 = BITS == 8 ? static_cast<const float *>(w0.s)[nn] : 1.0f;
+        const float s1 = GATED && BITS == 8 ? static_cast<const float *>(w1.s)[nn] : 1.0f;
+        const float bg = GATED && b0 ? b0[nn] : kNoBias, bu = GATED && b1 ? b1[nn] : kNoBias;
+        if (n >= p.N) continue;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < ER; ++e) {
+                const int m = 32 * (rb + i) + acc_row(e0 + e, lane);
+                float v = acc[i][GATED ? 2 * u : u][e] * down[i][e] * s0;
+                if constexpr (GATED) v = gate_f32(act, v + bg, acc[i][2 * u + 1][e] * down[i][e] * s1 + bu);
+                if (m < p.M) C[(int64_t)m * ldc + n] = v;
             }
-            uint32_t a1[4], a2[4], a3[4];
-            q8w_split3(v.x, a1[0], a2[0], a3[0]);
-            q8w_split3(v.y, a1[1], a2[1], a3[1]);
-            q8w_split3(v.z, a1[2], a2[2], a3[2]);
-            q8w_split3(v.w, a1[3], a2[3], a3[3]);
-            char *d = st + (lr + (NTHR / LPR) * i) * P + 2 * lk;
-            *reinterpret_cast<uint2 *>(d) = make_uint2(q8w_pack(a1[0], a1[1]), q8w_pack(a1[2], a1[3]));
-            *reinterpret_cast<uint2 *>(d + PL) = make_uint2(q8w_pack(a2[0], a2[1]), q8w_pack(a2[2], a2[3]));
-            *reinterpret_cast<uint2 *>(d + 2 * PL) = make_uint2(q8w_pack(a3[0], a3[1]), q8w_pack(a3[2], a3[3]));
+    }
+}
+
+// Pieces: a workgroup computes 32 TM rows x NT tiles, its NW wavefronts splitting K in 64-deep stages.
+// Parts and codes go straight into registers, PW stages ahead: no LDS and no barrier in the main loop. The
+// shares meet in LDS, each wavefront finishing 16 / NW of the accumulator registers.
+template <int BITS, bool GATED, int TM, int NT, int NW, int PW>
+__global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, WoWeight w1, const float *__restrict__ b0,
+                                                         const float *__restrict__ b1, int act, float *__restrict__ C,
+                                                         int64_t ldc, int tilesN) {
+    constexpr int CB = GATED ? NT / 2 : NT, ER = 16 / NW, SH = ER * TM * NT * 64;
+    static_assert(16 % NW == 0 && (!GATED || NT % 2 == 0), "shares; a tile of each weight");
+    __shared__ float red[NW][NW - 1][SH];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x);
+    const int rb = (logical / tilesN) * TM, cb0 = (logical % tilesN) * CB;
+    const int nk32 = p.Kp >> 5, nst = p.nkc >> 1, last_rb = (p.M - 1) >> 5;
+    WoTiles<BITS, GATED, NT> tiles;
+    tiles.init(w0, w1, cb0, lane, nk32, p.G);
+    f16x8 a[PW][2][TM][2][2];
+    uint32_t w[PW][2][NT][BITS / 2];
+    _Float16 sc[PW][2][NT];
+    const char *pa[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) pa[i] = p.a.parts + (int64_t)min(rb + i, last_rb) * p.nkc * 4096;
+    auto load = [&](int slot, int s) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        a[slot][c][i][x][j] =
+                            *reinterpret_cast<const f16x8 *>(pa[i] + (int64_t)(2 * s + c) * 4096 + x * 2048 + j * 1024 + (uint32_t)(lane * 16));
+            tiles.load(min(2 * s + c, nk32 - 1), p.cpg, p.G, w[slot][c], sc[slot][c]);
         }
     };
     f32x16 acc[TM][NT];
@@ -353,120 +560,116 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_wo(const float *__r
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][t][e] = 0.0f;
-    // Stage c + 1 is split into the other buffer behind stage c's MFMAs; past the last stage the
-    // loads re-read it and the buffer is not used.
-    const int nc = (Kp + KC - 1) / KC, last = nc - 1;
-    load_a(0);
-    load_w(0);
-    store_a(0, lds);
-    load_a(min(1, last));
-    lds_barrier();
-    for (int c = 0; c < nc; ++c) {
-        const char *cur = lds + (c & 1) * STAGE;
-        char *nxt = lds + ((c & 1) ^ 1) * STAGE;
+    if (wave < nst) {
+        const int final = wave + (nst - 1 - wave) / NW * NW;  // this wavefront's last stage
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            f32x16 part[TM][NT];
+        for (int d = 0; d < PW; ++d) load(d, min(wave + d * NW, final));
+        for (int s0 = wave; s0 < nst; s0 += NW * PW) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                bf16x8 p[TM][3], q[NT];
+            for (int d = 0; d < PW; ++d) {
+                const int s = s0 + d * NW;
+                if (s >= nst) break;  // uniform
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if constexpr (BITS == 4) q[t] = q4_widen8(wr[b][t][j]);
-                    else q[t] = q8_widen8(wr[b][t][2 * j], wr[b][t][2 * j + 1]);
-                }
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int x = 0; x < 3; ++x)
-                        p[i][x] = *reinterpret_cast<const bf16x8 *>(cur + x * PL + (32 * (TM * wm + i) + r) * P +
-                                                                    64 * (KB * ks + b) + 32 * hf + 16 * j);
-#pragma unroll
-                for (int x = 2; x >= 0; --x)
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            f32x16 &s = BITS == 4 ? part[i][t] : acc[i][t];
-                            if (BITS == 4 && j == 0 && x == 2) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) s[e] = 0.0f;
-                            }
-                            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[i][x], q[t], s, 0, 0, 0);
-                        }
-            }
-            if (BITS == 4) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const float s = 16.0f * (float)sc[b][t];
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[i][t][e] = __builtin_fmaf(part[i][t][e], s, acc[i][t][e]);
-                }
+                for (int c = 0; c < 2; ++c)
+                    wo_chunk<BITS, GATED, TM, NT>([&](int i, int x, int j) { return a[d][c][i][x][j]; }, w[d][c], sc[d][c], acc);
+                load(d, min(s + PW * NW, final));
             }
         }
-        load_w(min(c + 1, last));
-        store_a(c + 1, nxt);
-        load_a(min(c + 2, last));
-        lds_barrier();
     }
-    if constexpr (KS > 1) {
-        // share s of the registers e in [ER s, ER s + ER) goes to wavefront s of the KS
-        float *red = reinterpret_cast<float *>(lds);
-        constexpr int PER = (KS - 1) * ER * TM * NT * 64;  // floats of one receiving wavefront
-        const int mine = wave % (WM * WN);
+    wo_marked<BITS, GATED, TM, NT>(p, tiles, rb, wave, NW, acc);
+    // registers [ER s, ER s + ER) are finished by wavefront s
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if (s == ks) continue;
-            float *d = red + (mine + WM * WN * s) * PER + (ks < s ? ks : ks - 1) * (ER * TM * NT * 64) + lane;
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int e = 0; e < ER; ++e) d[((i * NT + t) * ER + e) * 64] = acc[i][t][ER * s + e];
-        }
-        lds_barrier();
-        const float *d = red + wave * PER + lane;
-        // own registers first into the low places, then the others' shares in their order
+    for (int s = 0; s < NW; ++s) {
+        if (s == wave) continue;
+        float *d = red[s][wave < s ? wave : wave - 1] + lane;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int e = 0; e < ER; ++e) {
-                    float v = 0.0f, o[KS];
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) o[s] = acc[i][t][ER * s + e];
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) v = ks == s ? o[s] : v;
-#pragma unroll
-                    for (int s = 0; s < KS - 1; ++s) v += d[s * (ER * TM * NT * 64) + ((i * NT + t) * ER + e) * 64];
-                    acc[i][t][e] = v;
-                }
+                for (int e = 0; e < ER; ++e) d[((i * NT + t) * ER + e) * 64] = acc[i][t][ER * s + e];
     }
+    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < (GATED ? NT / 2 : NT); ++u) {
-        const int n = 32 * (cb0 + u) + r, nn = min(n, N - 1);
-        float s[2], bb[2];
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            s[x] = BITS == 8 ? static_cast<const float *>(w[x].s)[nn] : 1.0f;
-            const float *b = x ? b1 : b0;
-            bb[x] = GATED && b ? b[nn] : kNoBias;
-        }
-        if (n >= N) continue;
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < ER; ++e) {
-                const int m = m0 + 32 * (TM * wm + i) + acc_row(KS > 1 ? ER * ks + e : e, lane);
-                float v = acc[i][GATED ? 2 * u : u][e] * s[0];
-                if constexpr (GATED) v = gate_f32(act, v + bb[0], acc[i][2 * u + 1][e] * s[1] + bb[1]);
-                if (m < M) C[(int64_t)m * ldc + n] = v;
+                float o[NW], v = 0.0f;
+#pragma unroll
+                for (int s = 0; s < NW; ++s) o[s] = acc[i][t][ER * s + e];
+#pragma unroll
+                for (int s = 0; s < NW; ++s) v = wave == s ? o[s] : v;
+#pragma unroll
+                for (int s = 0; s < NW - 1; ++s) v += red[wave][s][((i * NT + t) * ER + e) * 64 + lane];
+                acc[i][t][e] = v;
             }
+    wo_store<BITS, GATED, TM, NT, ER>(p, w0, w1, b0, b1, act, C, ldc, rb, cb0, ER * wave, acc);
+}
+
+// Tiles for many rows: 32 TM rows x 4 wavefronts of NT tiles side by side. A chunk's parts pass through
+// LDS once for the four (double-buffered), its codes go straight into registers; PW chunks are in flight.
+template <int BITS, bool GATED, int TM, int NT, int PW>
+__global__ __launch_bounds__(256, 2) void gemm_wo_tile(WoRows p, WoWeight w0, WoWeight w1, const float *__restrict__ b0,
+                                                       const float *__restrict__ b1, int act, float *__restrict__ C,
+                                                       int64_t ldc, int tilesN) {
+    constexpr int CB = GATED ? NT / 2 : NT, STAGE = TM * 4096;
+    static_assert(PW % 2 == 0 && (!GATED || NT % 2 == 0), "LDS buffers alternate; a tile of each weight");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x);
+    const int rb = (logical / tilesN) * TM, cb0 = (logical % tilesN) * 4 * CB + wave * CB;
+    const int nk32 = p.Kp >> 5, nc = p.nkc, last = nc - 1, last_rb = (p.M - 1) >> 5;
+    WoTiles<BITS, GATED, NT> tiles;
+    tiles.init(w0, w1, cb0, lane, nk32, p.G);
+    u32x4 ra[PW][TM];  // each wavefront moves one part of every row block: plane wave / 2, step wave % 2
+    uint32_t w[PW][NT][BITS / 2];
+    _Float16 sc[PW][NT];
+    const char *pa[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) pa[i] = p.a.parts + (int64_t)min(rb + i, last_rb) * nc * 4096;
+    auto load_a = [&](int slot, int c) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) ra[slot][i] = *reinterpret_cast<const u32x4 *>(pa[i] + (int64_t)c * 4096 + (uint32_t)(tid * 16));
+    };
+    auto load_w = [&](int slot, int c) { tiles.load(min(c, nk32 - 1), p.cpg, p.G, w[slot], sc[slot]); };
+    auto store_a = [&](int slot, char *st) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) *reinterpret_cast<u32x4 *>(st + i * 4096 + tid * 16) = ra[slot][i];
+    };
+    f32x16 acc[TM][NT];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][t][e] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < PW; ++d) {
+        load_a(d, min(d, last));
+        load_w(d, min(d, last));
     }
+    store_a(0, lds);
+    load_a(0, min(PW, last));
+    lds_barrier();
+    for (int c0 = 0; c0 < nc; c0 += PW) {
+#pragma unroll
+        for (int d = 0; d < PW; ++d) {
+            const int c = c0 + d;
+            if (c >= nc) break;  // uniform
+            const char *cur = lds + (d & 1) * STAGE + lane * 16;
+            wo_chunk<BITS, GATED, TM, NT>(
+                [&](int i, int x, int j) { return *reinterpret_cast<const f16x8 *>(cur + i * 4096 + x * 2048 + j * 1024); }, w[d],
+                sc[d], acc);
+            load_w(d, min(c + PW, last));
+            store_a((d + 1) % PW, lds + ((d & 1) ^ 1) * STAGE);
+            load_a((d + 1) % PW, min(c + 1 + PW, last));
+            lds_barrier();
+        }
+    }
+    wo_marked<BITS, GATED, TM, NT>(p, tiles, rb, 0, 1, acc);
+    wo_store<BITS, GATED, TM, NT, 16>(p, w0, w1, b0, b1, act, C, ldc, rb, cb0, 0, acc);
 }
 
 }  // namespace enchip

@@ -1,8 +1,8 @@
 """Products with 4-bit weights and group scales (enchip_matmul_bt_q4) against float64.
 
 Beyond the error bound of f32 sums (weight_only_oracle.product): integer activations with
-power-of-two scales come out exact, and one-hot weights return full-significand activations bit
-for bit, so that a wrong k order, group, channel or a dropped part of a split shows."""
+power-of-two scales come out exact, and one-hot weights return single activations, so that a wrong
+k order, group, channel or a dropped part of a split shows."""
 import numpy as np
 import pytest
 
@@ -71,23 +71,47 @@ def test_exact_on_integers(ctx, M, N, K, group):
         ctx.release_weight4(h)
 
 
-@pytest.mark.parametrize("M", [1, 3, 6, 50, 300, 2100])
-def test_one_hot_selects_activations_exactly(ctx, M):
-    # one nonzero code per channel, a power of two, and power-of-two scales: the output is one
-    # activation times it, exactly, over 1e-25 .. 1e25 (a third part of 2^-16 is still normal)
+@pytest.mark.parametrize("M", [1, 3, 6, 20, 50, 300, 2100])
+@pytest.mark.parametrize("spread", [1, 8, 25])
+def test_one_hot_selects_activations(ctx, M, spread):
+    # one nonzero code per channel: the output is one activation times a power of two and a scale,
+    # to the bits that the path holds of it, whatever stands beside it (over 1e-25 .. 1e25 too)
     N, K, group = 300, 300, 32
     g = np.random.default_rng(M)
     x = g.standard_normal((M, K))
-    a = (np.where(np.abs(x) < 0.1, 0.5, x) * 10.0 ** g.integers(-25, 26, size=(M, K))).astype(np.float32)
+    a = (np.where(np.abs(x) < 0.1, 0.5, x) * 10.0 ** g.integers(-spread, spread + 1, size=(M, K))).astype(np.float32)
     at, q = g.integers(0, K, size=N), g.choice(np.array([1, -1, 2, 4, -4, -8]), size=N)
     c = np.full((N, K), 8, np.uint8)
     c[np.arange(N), at] = q + 8
     s = np.ldexp(1.0, g.integers(-4, 4, size=(N, -(-K // group)))).astype(np.float16)
     h = ctx.register_weight4(c[:, 0::2] | (c[:, 1::2] << 4), s, K, group)
     try:
-        say(f"matmul_bt_q4 one-hot M={M}")
-        want = a[:, at].astype(np.float64) * (q * s[np.arange(N), at // group].astype(np.float64))
-        assert np.array_equal(ctx.matmul_bt_q4(h, a), want.astype(np.float32))
+        say(f"matmul_bt_q4 one-hot M={M} spread={spread}")
+        got = ctx.matmul_bt_q4(h, a)
+        want, tol = product(a, values4(c, s, group))
+        assert np.all(np.abs(got - want) <= tol), f"{np.max(np.abs(got - want) / tol)} of the bound"
+        if M <= 6:  # rows few enough for f32 products
+            assert np.array_equal(got, want.astype(np.float32))
+    finally:
+        ctx.release_weight4(h)
+
+
+@pytest.mark.parametrize("M", [20, 300, 2100])
+def test_spikes_leave_their_neighbours(ctx, M):
+    # one value of 1e30 or 1e-30 among ordinary ones, and channels whose code there is 0
+    N, K, group = 200, 512, 32
+    g = np.random.default_rng(M)
+    c, s, _ = weight4(g, N, K, group)
+    codes = np.stack([c & 15, c >> 4], axis=2).reshape(N, K)
+    a = g.standard_normal((M, K)).astype(np.float32)
+    at = g.integers(0, K, size=M)
+    a[np.arange(M), at] = g.choice(np.array([1e30, -1e30, 1e-30, 1e9, 3e4], np.float32), size=M)
+    codes[::2, np.unique(at)] = 8
+    h = ctx.register_weight4(codes[:, 0::2] | (codes[:, 1::2] << 4), s, K, group)
+    try:
+        got = ctx.matmul_bt_q4(h, a)
+        want, tol = product(a, values4(codes, s, group))
+        assert np.all(np.abs(got - want) <= tol), f"{np.max(np.abs(got - want) / tol)} of the bound"
     finally:
         ctx.release_weight4(h)
 

@@ -22,11 +22,35 @@ def weight8(g, N, K):
     return q, s, q.astype(np.float64) * s.astype(np.float64)[:, None]
 
 
+def held(a):
+    """How far an activation may be from what the path holds of it. Each row is scaled by the power of
+    two that brings its largest to 2^14 .. 2^15 and split into two f16 parts: 22 bits of an
+    activation (2^-22: hi truncated, what is left rounded to 11 bits), or half of lo's smallest step,
+    2^-25 scaled, 2^-39 of the largest. Blocks of 128 with more than a sixteenth of the nonzero
+    activations under 2^-5 scaled are computed in f32, scaled: half a step of a subnormal, 2^-150
+    scaled, 2^-164 of the largest."""
+    a = np.abs(a.astype(np.float64))
+    top = a.max(axis=1, keepdims=True)
+    _, e = np.frexp(top)
+    x = np.ldexp(a, 15 - e)
+    err = np.maximum(2.0 ** -22 * a, 2.0 ** -39 * top)
+    for k in range(0, a.shape[1], 128):
+        b = x[:, k:k + 128]
+        marked = 16 * ((b != 0) & (b < 2.0 ** -5)).sum(axis=1) > (b != 0).sum(axis=1)
+        err[marked, k:k + 128] = 2.0 ** -164 * top[marked]
+    return err
+
+
 def product(a, w):
-    """(y, bound) of a . w^T: n f32 additions of exact or once rounded products, each partial sum
-    at most sum |a w|, err by (n + 2) 2^-24 sum |a w|; scaling a sum rounds once more."""
+    """(y, bound) of a . w^T. f32 sums: n additions of exact or once rounded products, each partial
+    sum at most sum |a w|, err by (n + 8) 2^-24 sum |a w|; and what is held of the activations. A
+    scaled sum that is subnormal rounds to half its step, 2^-164 of the row's largest as above, once
+    per scale group of at least 32 and twice more."""
+    h = held(a)
     a = a.astype(np.float64)
-    return a @ w.T, (a.shape[1] + 8) * U * (np.abs(a) @ np.abs(w).T)
+    K = a.shape[1]
+    tiny = (K / 32 + 3) * 2.0 ** -164 * np.abs(a).max(axis=1, keepdims=True)
+    return a @ w.T, (K + 8) * U * (np.abs(a) @ np.abs(w).T) + h @ np.abs(w).T + tiny
 
 
 def act64(name, x):
