@@ -2624,8 +2624,10 @@ WoArgs wo_args(const Weight4 &a, const Weight4 &b) {
     return {4, a.N, a.K, a.Np, a.Kp, a.group / 32, a.G, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
 }
 
-// The rows that gemv_wo takes; more are split first (split_rows) and run on the f16 MFMA.
-constexpr int64_t kFewRows = 8;
+// The rows that gemv_wo takes; more are split first (split_rows) and run on the f16 MFMA. A pass over the
+// weights takes four rows, the split a launch: K = N = 4096, 4 bits, 8 rows 11.9 us against 15.5, 16 rows
+// 19.8 and 15.9; K = 1024 8 rows 5.4, 16 rows 7.8 and 8.6.
+int64_t few_rows(int64_t weight_bytes) { return weight_bytes <= ((int64_t)4 << 20) ? 16 : 8; }
 // Bytes of split rows of one pass: more rows run in several.
 constexpr int64_t kSplitBytes = (int64_t)1 << 30;
 
@@ -2675,18 +2677,25 @@ int launch_wo_split(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda,
                            out, ldc, (int)tilesN);                                                                     \
     } while (0)
         const int64_t cus = c->num_cus;
-        auto tiles = [&](int64_t tm, int64_t cb) { return ((n + 32 * tm - 1) / (32 * tm)) * ((p.N + 32 * cb - 1) / (32 * cb)); };
+        const int64_t pieces = ((n + 31) / 32) * ((p.N + 31) / 32);
         constexpr int G2 = GATED ? 2 : 1;  // tiles of a wavefront for one channel block
-        const int force = getenv("WOF") ? atoi(getenv("WOF")) : -1;
-        int form = tiles(1, 1) <= 2 * cus ? 0 : tiles(2, 2 / G2) <= 2 * cus ? 1 : 2;
-        if (force >= 0) form = force;
-        if (form == 0) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, G2, 8, 4>), 1, 1, 512);
-        else if (form == 1) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, 2, 4, 3>), 1, 2 / G2, 256);
-        else if (form == 3) WO_SPLIT((gemm_wo_piece<BITS, GATED, 2, 2, 4, 2>), 2, 2 / G2, 256);
-        else if (form == 4) WO_SPLIT((gemm_wo_tile<BITS, GATED, 4, 2, 2>), 4, 8 / G2, 256);
-        else if (form == 5) WO_SPLIT((gemm_wo_tile<BITS, GATED, 1, 2, 4>), 1, 8 / G2, 256);
-        else if (form == 6) WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 2, 4>), 2, 8 / G2, 256);
-        else WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 4, 2>), 2, 16 / G2, 256);
+        const int fp = BITS == 8 ? 1 : p.cpg % 4 == 0 ? 4 : p.cpg % 2 == 0 ? 2 : 1;
+        // 32 x 32 pieces (of both weights): few of them split K over 8 wavefronts, more over 4; then tiles of
+        // 32 or 64 rows with K over two groups of wavefronts, and without. Measured on MI355X, us, gated
+        // int8, K = 4096, N = 4096: 128 rows 33 (4 wavefronts) against 43 (32-row tiles), 256 rows 56
+        // and 50, 512 rows 99, 88, 69 (64-row tiles, two groups) and 73 (one), 1024 rows 129 and 126;
+        // 4 bits, one weight: 256 rows 38 and 47, 512 rows 62, 52 and 74 (one group), 1024 rows 88 and 82.
+        if (pieces <= cus) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, G2, 8, 2>), 1, 1, 512);
+        else if (pieces <= (GATED ? 2 : 4) * cus) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, 2, 4, 2>), 1, 2 / G2, 256);
+        else if (pieces <= (GATED ? 4 : 15) * cus) {
+            if (fp == 1) WO_SPLIT((gemm_wo_tile<BITS, GATED, 1, 2, 2, 2, 1>), 1, 8 / G2, 512);
+            else WO_SPLIT((gemm_wo_tile<BITS, GATED, 1, 2, 2, 2, BITS == 8 ? 1 : 2>), 1, 8 / G2, 512);
+        } else if (GATED && pieces <= 10 * cus) {
+            if (fp == 1) WO_SPLIT((gemm_wo_tile<BITS, true, 2, 2, 2, 2, 1>), 2, 4, 512);
+            else WO_SPLIT((gemm_wo_tile<BITS, true, 2, 2, 2, 2, BITS == 8 ? 1 : 2>), 2, 4, 512);
+        } else if (fp == 4) WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 2, 1, BITS == 8 ? 2 : 4, BITS == 8 ? 1 : 4>), 2, 8 / G2, 256);
+        else if (fp == 2) WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 2, 1, BITS == 8 ? 2 : 4, BITS == 8 ? 1 : 2>), 2, 8 / G2, 256);
+        else WO_SPLIT((gemm_wo_tile<BITS, GATED, 2, 2, 1, 2, 1>), 2, 8 / G2, 256);
 #undef WO_SPLIT
         if ((rc = check_launch(c, "weight-only product"))) return rc;
     }
@@ -2698,7 +2707,7 @@ template <int BITS, bool GATED>
 int launch_wo(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda, const float *b0, const float *b1, int act,
               float *C, int64_t ldc, int64_t M, hipStream_t s) {
     using namespace enchip;
-    if (M > kFewRows) return launch_wo_split<BITS, GATED>(c, p, A, lda, b0, b1, act, C, ldc, M, s);
+    if (M > few_rows(p.Np * p.Kp * BITS / 8 * (GATED ? 2 : 1))) return launch_wo_split<BITS, GATED>(c, p, A, lda, b0, b1, act, C, ldc, M, s);
     const enchip::FastDiv cpg = fast_div(p.cpg);
     // a wavefront per K block while there are more blocks than wavefronts
     const int64_t blocks = (p.Kp + (BITS == 4 ? 255 : 127)) / (BITS == 4 ? 256 : 128);

@@ -95,8 +95,8 @@ __device__ __forceinline__ float sum_units(float v) {
 // A few rows. A lane takes one channel and one unit of k at a time (16 bytes of weight: 32 k of a
 // 4-bit one, 16 of an int8 one), a wavefront 8 channels x 8 units, a block of 256 or 128 k: eight
 // whole cache lines. The block's activations reach the lanes through the wavefront's own LDS and
-// stay in registers for all of its weights, so that a code costs its share of the widening and MB
-// mixed multiply-adds, f32 += f32 * f16. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
+// stay in registers for all of its weights, so that a code costs its conversion and MB multiply-adds
+// in f32. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
 // 8 NG each. One block ahead is in flight. The lanes' and the wavefronts' sums are added in one order.
 //
 constexpr int WO_WAVES = 8;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int t = 0; t < NW; ++t) qc[g][t] = q[g][t], scc[g][t] = BITS == 4 ? (float)sc[g][t] : 1.0f;
+            for (int t = 0; t < NW; ++t) qc[g][t] = q[g][t], scc[g][t] = BITS == 4 ? 16.0f * (float)sc[g][t] : 1.0f;
         if (blk + step < blocks) load(blk + step);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -193,16 +193,29 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
                 for (int m = 0; m < MB; ++m) y[m] = 0.0f;
                 const uint32_t qd[4] = {qc[g][t].x, qc[g][t].y, qc[g][t].z, qc[g][t].w};
 #pragma unroll
-                for (int d = 0; d < CK / 8; ++d) {
-                    f16x2 h[4];
-                    if constexpr (BITS == 4) widen8_q4(qd[d], h);
-                    else widen8_q8(qd[2 * d], qd[2 * d + 1], h);
+                for (int d = 0; d < 4; ++d) {
+                    if constexpr (BITS == 4) {
+                        // a byte's low and high halves, as q / 16: k 0, 4, 1, 5 and 2, 6, 3, 7 of the word's 8
+                        const uint32_t lo = qd[d] ^ 0x88888888u;
+                        uint32_t hi = lo >> 4;
+                        asm("" : "+v"(hi));  // one shift for its four codes
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                        for (int b = 0; b < 4; ++b) {
+                            const float f0 = __builtin_amdgcn_cvt_off_f32_i4((int)((lo >> (8 * b)) & 0xff));
+                            const float f1 = __builtin_amdgcn_cvt_off_f32_i4((int)((hi >> (8 * b)) & 0xff));
+                            const int k = 8 * d + (b >> 1) + 4 * (b & 1);
 #pragma unroll
-                        for (int m = 0; m < MB; ++m)
-                            y[m] = __builtin_fmaf(a[m][8 * d + 2 * i + 1], (float)h[i].y,
-                                                  __builtin_fmaf(a[m][8 * d + 2 * i], (float)h[i].x, y[m]));
+                            for (int m = 0; m < MB; ++m)
+                                y[m] = __builtin_fmaf(a[m][k + 2], f1, __builtin_fmaf(a[m][k], f0, y[m]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const float f = (float)(int8_t)((qd[d] >> (8 * b)) & 0xff);
+#pragma unroll
+                            for (int m = 0; m < MB; ++m) y[m] = __builtin_fmaf(a[m][4 * d + b], f, y[m]);
+                        }
+                    }
                 }
 #pragma unroll
                 for (int m = 0; m < MB; ++m)
@@ -608,19 +621,25 @@ __global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, 
     wo_store<BITS, GATED, TM, NT, ER>(p, w0, w1, b0, b1, act, C, ldc, rb, cb0, ER * wave, acc);
 }
 
-// Tiles for many rows: 32 TM rows x 4 wavefronts of NT tiles side by side. A chunk's parts pass through
-// LDS once for the four (double-buffered), its codes go straight into registers; PW chunks are in flight.
-template <int BITS, bool GATED, int TM, int NT, int PW>
-__global__ __launch_bounds__(256, 2) void gemm_wo_tile(WoRows p, WoWeight w0, WoWeight w1, const float *__restrict__ b0,
-                                                       const float *__restrict__ b1, int act, float *__restrict__ C,
-                                                       int64_t ldc, int tilesN) {
-    constexpr int CB = GATED ? NT / 2 : NT, STAGE = TM * 4096;
-    static_assert(PW % 2 == 0 && (!GATED || NT % 2 == 0), "LDS buffers alternate; a tile of each weight");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// Tiles: 32 TM rows x 4 wavefronts of NT tiles side by side, KS such groups of four on alternate pairs of
+// chunks. A chunk's parts pass through LDS once for its four wavefronts (double-buffered), its codes go
+// straight into registers, PW stages ahead, and are widened one stage ahead. FP: chunks of a 4-bit
+// weight that share a scale (its group is a multiple of 32 FP): their sum is added once, scaled.
+template <int BITS, bool GATED, int TM, int NT, int KS, int PW, int FP>
+__global__ __launch_bounds__(256 * KS, 2) void gemm_wo_tile(WoRows p, WoWeight w0, WoWeight w1,
+                                                                 const float *__restrict__ b0, const float *__restrict__ b1,
+                                                                 int act, float *__restrict__ C, int64_t ldc, int tilesN) {
+    constexpr int CB = GATED ? NT / 2 : NT, STAGE = KS * TM * 4096, ER = 16 / KS, SH = ER * TM * NT * 64;
+    constexpr int RED = KS > 1 ? 4 * KS * (KS - 1) * SH * 4 : 0, LDS = 2 * STAGE > RED ? 2 * STAGE : RED;
+    static_assert((PW == 2 || PW == 4) && (KS == 1 || KS == 2) && PW % FP == 0 && (KS == 1 || FP <= 2),
+                  "buffers alternate; a group's chunks lie side by side");
+    static_assert(!GATED || NT % 2 == 0, "a tile of each weight");
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ks = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
     const int logical = xcd_logical_tile(blockIdx.x, gridDim.x);
     const int rb = (logical / tilesN) * TM, cb0 = (logical % tilesN) * 4 * CB + wave * CB;
-    const int nk32 = p.Kp >> 5, nc = p.nkc, last = nc - 1, last_rb = (p.M - 1) >> 5;
+    const int nk32 = p.Kp >> 5, last = p.nkc - 1, last_rb = (p.M - 1) >> 5, nst = p.nkc / KS;
     WoTiles<BITS, GATED, NT> tiles;
     tiles.init(w0, w1, cb0, lane, nk32, p.G);
     u32x4 ra[PW][TM];  // each wavefront moves one part of every row block: plane wave / 2, step wave % 2
@@ -628,17 +647,32 @@ __global__ __launch_bounds__(256, 2) void gemm_wo_tile(WoRows p, WoWeight w0, Wo
     _Float16 sc[PW][NT];
     const char *pa[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) pa[i] = p.a.parts + (int64_t)min(rb + i, last_rb) * nc * 4096;
-    auto load_a = [&](int slot, int c) {
+    for (int i = 0; i < TM; ++i) pa[i] = p.a.parts + (int64_t)min(rb + i, last_rb) * p.nkc * 4096;
+    // two neighbouring chunks a group, in turn; past the last stage: a chunk again, not used
+    auto chunk = [&](int st) { return min(KS == 1 ? st : 4 * (st >> 1) + 2 * ks + (st & 1), last); };
+    auto load_a = [&](int slot, int st) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) ra[slot][i] = *reinterpret_cast<const u32x4 *>(pa[i] + (int64_t)c * 4096 + (uint32_t)(tid * 16));
+        for (int i = 0; i < TM; ++i)
+            ra[slot][i] = *reinterpret_cast<const u32x4 *>(pa[i] + (int64_t)chunk(st) * 4096 + (uint32_t)(tid * 16));
     };
-    auto load_w = [&](int slot, int c) { tiles.load(min(c, nk32 - 1), p.cpg, p.G, w[slot], sc[slot]); };
+    auto load_w = [&](int slot, int st) { tiles.load(min(chunk(st), nk32 - 1), p.cpg, p.G, w[slot], sc[slot]); };
     auto store_a = [&](int slot, char *st) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) *reinterpret_cast<u32x4 *>(st + i * 4096 + tid * 16) = ra[slot][i];
+        for (int i = 0; i < TM; ++i) *reinterpret_cast<u32x4 *>(st + (ks * TM + i) * 4096 + tid * 16) = ra[slot][i];
     };
-    f32x16 acc[TM][NT];
+    f16x8 q[2][NT][2];  // the widened codes of a chunk and the next
+    float s[NT], sn[NT];
+    auto widen = [&](int slot, int at) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                f16x2 h[4];
+                WoTiles<BITS, GATED, NT>::widen(w[slot][t], j, h);
+                q[at][t][j] = f16x8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+            }
+    };
+    f32x16 acc[TM][NT], part[TM][NT];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -647,29 +681,103 @@ __global__ __launch_bounds__(256, 2) void gemm_wo_tile(WoRows p, WoWeight w0, Wo
             for (int e = 0; e < 16; ++e) acc[i][t][e] = 0.0f;
 #pragma unroll
     for (int d = 0; d < PW; ++d) {
-        load_a(d, min(d, last));
-        load_w(d, min(d, last));
+        load_a(d, d);
+        load_w(d, d);
     }
     store_a(0, lds);
-    load_a(0, min(PW, last));
+    load_a(0, PW);
+    widen(0, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sn[t] = BITS == 4 ? (float)sc[0][t] : 1.0f;
+    load_w(0, PW);
     lds_barrier();
-    for (int c0 = 0; c0 < nc; c0 += PW) {
+    for (int c0 = 0; c0 < nst; c0 += PW) {
 #pragma unroll
         for (int d = 0; d < PW; ++d) {
             const int c = c0 + d;
-            if (c >= nc) break;  // uniform
-            const char *cur = lds + (d & 1) * STAGE + lane * 16;
-            wo_chunk<BITS, GATED, TM, NT>(
-                [&](int i, int x, int j) { return *reinterpret_cast<const f16x8 *>(cur + i * 4096 + x * 2048 + j * 1024); }, w[d],
-                sc[d], acc);
-            load_w(d, min(c + PW, last));
+            if (KS * PW > 4 && c >= nst) break;  // uniform
+            const char *cur = lds + (d & 1) * STAGE + ks * TM * 4096 + lane * 16;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                f16x8 a[TM][2];
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) a[i][x] = *reinterpret_cast<const f16x8 *>(cur + i * 4096 + x * 2048 + j * 1024);
+#pragma unroll
+                for (int x = 1; x >= 0; --x)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            f32x16 &y = BITS == 4 ? part[i][t] : acc[i][t];
+                            if (BITS == 4 && d % FP == 0 && j == 0 && x == 1) {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) y[e] = 0.0f;
+                            }
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][x], q[d & 1][t][j], y, 0, 0, 0);
+                        }
+            }
+            // while they run: the next chunk's codes
+            widen((d + 1) % PW, (d & 1) ^ 1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t] = sn[t], sn[t] = BITS == 4 ? (float)sc[(d + 1) % PW][t] : 1.0f;
             store_a((d + 1) % PW, lds + ((d & 1) ^ 1) * STAGE);
-            load_a((d + 1) % PW, min(c + 1 + PW, last));
+            load_a((d + 1) % PW, c + 1 + PW);
+            load_w((d + 1) % PW, c + 1 + PW);
+            if (BITS == 4 && d % FP == FP - 1) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][t][e] = __builtin_fmaf(part[i][t][e], s[t], acc[i][t][e]);
+            }
+            if (BITS == 8 && TM * NT >= 4) {
+                constexpr int MF = 4 * TM * NT;
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * TM, 0);
+#pragma unroll
+                for (int u = 0; u < MF; ++u) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, (20 * NT + MF - 1) / MF, 0);
+                    if (u == 1) __builtin_amdgcn_sched_group_barrier(0x100, 2 * TM, 0);
+                }
+            }
             lds_barrier();
         }
     }
-    wo_marked<BITS, GATED, TM, NT>(p, tiles, rb, 0, 1, acc);
-    wo_store<BITS, GATED, TM, NT, 16>(p, w0, w1, b0, b1, act, C, ldc, rb, cb0, 0, acc);
+    wo_marked<BITS, GATED, TM, NT>(p, tiles, rb, ks, KS, acc);
+    if constexpr (KS > 1) {
+        // registers [ER g, ER g + ER) are finished by group g
+        float *red = reinterpret_cast<float *>(lds);
+#pragma unroll
+        for (int g = 0; g < KS; ++g) {
+            if (g == ks) continue;
+            float *d = red + ((g * 4 + wave) * (KS - 1) + (ks < g ? ks : ks - 1)) * SH + lane;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < ER; ++e) d[((i * NT + t) * ER + e) * 64] = acc[i][t][ER * g + e];
+        }
+        lds_barrier();
+        const float *d = red + (ks * 4 + wave) * (KS - 1) * SH + lane;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < ER; ++e) {
+                    float v = acc[i][t][e];
+#pragma unroll
+                    for (int g = 1; g < KS; ++g) v = ks == g ? acc[i][t][ER * g + e] : v;
+#pragma unroll
+                    for (int g = 0; g < KS - 1; ++g) v += d[g * SH + ((i * NT + t) * ER + e) * 64];
+                    acc[i][t][e] = v;
+                }
+    }
+    wo_store<BITS, GATED, TM, NT, ER>(p, w0, w1, b0, b1, act, C, ldc, rb, cb0, ER * ks, acc);
 }
 
 }  // namespace enchip

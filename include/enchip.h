@@ -21,7 +21,7 @@
  *     encoder/model.go:214; enccuda serialises the same way,
  *     gpu/enccuda/backend.go:87,141-142). Host-pointer entry points are synchronous.
  *   - The context's device scratch (the quantized activations of the entry points
- *     that quantize themselves, the top-k candidates) is shared by all of them. Work
+ *     that quantize themselves, the split rows of the weight-only products, the top-k candidates) is shared by all of them. Work
  *     that uses it on one stream waits, on the device, for its last use on another
  *     stream (through an event of the library; the first work on a caller's stream waits
  *     for all that the context's stream holds), so host calls and
@@ -555,12 +555,15 @@ int enchip_weight4_shape(enchip_ctx *ctx, enchip_weight w, int64_t *N, int64_t *
 
 /* dst[m][n] = sum_k a[m][k] * (c[n][k] - 8) * scale[n][k / group] on host buffers, with f32
  * activations (never quantized), as enchip_matmul_bt_q8 is for int8 weights: a group's sum is
- * accumulated in f32 and scaled once, in an order of its own; the same gate against a float64
- * dot product. */
+ * accumulated in f32 and scaled once, in an order of its own (that of a row depends on how many
+ * rows there are); the same gate against a float64 dot product. */
 int enchip_matmul_bt_q4(enchip_ctx *ctx, enchip_weight w, const float *a, int64_t M, float *dst);
 
 /* Device form: d_a[M,K] with row pitch lda >= K, d_dst[M,N] with row pitch ldd >= N, on `stream`.
- * Allocates nothing. */
+ * Up to 8 rows are multiplied in f32. More (from 17 rows for small weights) go through the context's
+ * shared scratch: each row is scaled by a power of two and held in two f16 parts, 22 bits of each
+ * activation, or 2^-39 of the row's largest for the smallest ones; where an outlier leaves more than
+ * a sixteenth of a 128-wide block of the row below 2^-19 of it, the block is multiplied in f32. */
 int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, int64_t lda, int64_t M,
                             float *d_dst, int64_t ldd, void *stream);
 
@@ -574,8 +577,8 @@ int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, 
  *   gated_q4    4-bit weights, f32 activations: y as enchip_matmul_bt_q4 defines it
  *   w8a8_gated  int8 weights, activations quantized per token: y bit-identical to
  *               enchip_w8a8_linear's, one quantization shared by both projections
- * The device forms of gated_q8 and gated_q4 allocate nothing; w8a8_gated_dev uses the context's
- * shared scratch, as enchip_w8a8_linear_dev does. */
+ * The device forms use the context's shared scratch, as enchip_w8a8_linear_dev does (gated_q8 and
+ * gated_q4 as enchip_matmul_bt_q4_dev says). */
 int enchip_gated_q8(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *a, int64_t M,
                     const float *bias_gate, const float *bias_up, int act, float *dst);
 int enchip_gated_q8_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up, const float *d_a,
