@@ -2850,33 +2850,42 @@ int launch_gated_q(enchip_ctx *c, const Weight &w, const float *d_a, int64_t M, 
     return check_launch(c, "gated_w8a8_q");
 }
 
-// The gated pair on fragment-major codes: persistent tiles, or pieces.
+template <int CM, int ACT>
+void launch_gated_pieces(const Weight &w, const int8_t *aq, const float *as, const enchip::GatePair &p, int64_t M, float *out,
+                         hipStream_t s) {
+    const int pn = (int)((w.N + 31) / 32);
+    const int64_t rows = std::max<int64_t>(CM, (((int64_t)1 << 23) / pn) * CM);
+    for (int64_t r0 = 0; r0 < M; r0 += rows) {
+        const int64_t n = std::min(rows, M - r0);
+        hipLaunchKernelGGL((enchip::gated_w8a8_piece<CM, 32, ACT>), dim3((unsigned)((n + CM - 1) / CM * pn)), dim3(256), 0, s,
+                           aq + r0 * w.Kp, as + r0, p, out + r0 * w.N, w.N, (int)n, (int)w.N, (int)w.Kp, pn);
+    }
+}
+
+// The gated pair on fragment-major codes. Pieces of 32 x 32 while a CU gets one, of 64 x 32 to four 32 x 32's
+// worth and wherever the persistent tiles cannot go, else those. Measured on MI355X, us, with the
+// quantization: K = 768, N = 2304, 64 rows 7.9 (32 x 32) and 8.6 (64 x 32), 128 rows 9.8 and 8.9, 256
+// rows 12.2 and 11.3 (tiles 13.3), 512 rows 14.8 (64 x 32) and 13.6 (tiles), 4096 rows 55, 48 and 32; K =
+// 4096, N = 4096, 256 rows 46, 29 and 33, 4096 rows 584, 306 and 143.
 template <int ACT>
 void launch_gated_frag(enchip_ctx *c, const Weight &w, const int8_t *aq, const float *as, const enchip::GatePair &p,
                        int64_t M, float *out, hipStream_t s) {
     using namespace enchip;
+    const int64_t cus = c->num_cus;
     auto pieces = [&](int64_t cm, int64_t cn) { return ((M + cm - 1) / cm) * ((w.N + cn - 1) / cn); };
-    const bool pt = use_persistent(w, aq, w.Kp, out, w.N, M, true);
-    if (pt && pieces(32, 32) > 4 * (int64_t)c->num_cus) {
-        const int tilesN = (int)((w.N + GP_BN - 1) / GP_BN);
-        const bool small = pieces(PT_BM, GP_BN) < 2 * (int64_t)c->num_cus;
-        const int bm = small ? PT_BM_SMALL : PT_BM, tiles = (int)pieces(bm, GP_BN);
-        const dim3 grid(persistent_grid(c, tiles, small ? 3 : 2)), block(256);
-        if (small)
-            hipLaunchKernelGGL((gated_w8a8_pt<PT_BM_SMALL, ACT, 1>), grid, block, 0, s, aq, as, p, out, w.N, (int)M, (int)w.N,
-                               (int)w.Kp, tilesN, tiles);
-        else
-            hipLaunchKernelGGL((gated_w8a8_pt<PT_BM, ACT, 1>), grid, block, 0, s, aq, as, p, out, w.N, (int)M, (int)w.N,
-                               (int)w.Kp, tilesN, tiles);
-        return;
-    }
-    const int pn = (int)((w.N + 31) / 32);
-    const int64_t rows = std::max<int64_t>(32, (((int64_t)1 << 23) / pn) * 32);
-    for (int64_t r0 = 0; r0 < M; r0 += rows) {
-        const int64_t n = std::min(rows, M - r0);
-        hipLaunchKernelGGL((gated_w8a8_piece<32, 32, ACT>), dim3((unsigned)((n + 31) / 32 * pn)), dim3(256), 0, s,
-                           aq + r0 * w.Kp, as + r0, p, out + r0 * w.N, w.N, (int)n, (int)w.N, (int)w.Kp, pn);
-    }
+    if (pieces(32, 32) <= cus) return launch_gated_pieces<32, ACT>(w, aq, as, p, M, out, s);
+    if (pieces(32, 32) <= 4 * cus || !use_persistent(w, aq, w.Kp, out, w.N, M, true))
+        return launch_gated_pieces<64, ACT>(w, aq, as, p, M, out, s);
+    const int tilesN = (int)((w.N + GP_BN - 1) / GP_BN);
+    const bool small = pieces(PT_BM, GP_BN) < 2 * cus;
+    const int bm = small ? PT_BM_SMALL : PT_BM, tiles = (int)pieces(bm, GP_BN);
+    const dim3 grid(persistent_grid(c, tiles, small ? 3 : 2)), block(256);
+    if (small)
+        hipLaunchKernelGGL((gated_w8a8_pt<PT_BM_SMALL, ACT, 1>), grid, block, 0, s, aq, as, p, out, w.N, (int)M, (int)w.N,
+                           (int)w.Kp, tilesN, tiles);
+    else
+        hipLaunchKernelGGL((gated_w8a8_pt<PT_BM, ACT, 1>), grid, block, 0, s, aq, as, p, out, w.N, (int)M, (int)w.N, (int)w.Kp,
+                           tilesN, tiles);
 }
 
 // Enqueues the W8A8 gated pair on d_a [M][K] after the caller checked the arguments.
