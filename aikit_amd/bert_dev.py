@@ -41,34 +41,49 @@ computes that state on the device from token ids (bert.go:299-323: enchip_embed_
 then enchip_residual_layer_norm_dev with no residual). Every sequence of a batch has the
 same L.
 
+A rotary encoder passes `rope` (the query and key heads turned in place in qkv before the attention,
+enchip_rope_rows_dev), a gated one layers with an "ffn_gate" beside "ffn_up": inter = act(W8A8(h, Wg)
++ bg) * (W8A8(h, Wi) + b) in enchip_w8a8_gated_dev (encoder/forward_q8.go:264-279 swigluMLPQ8 on
+the NomicBERT forward's order, with W8A8 linears as in the rest of this module).
+
 This module holds no arithmetic of its own; torch provides device buffers and the stream.
 """
 from __future__ import annotations
 
 import math
-from typing import Dict, List, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 
 from . import enchip
 
 LN_EPS = 1e-12  # BERT's layer_norm_eps (encoder/bert.go)
+LINEARS = ("qkv", "o", "ffn_gate", "ffn_up", "ffn_down")
 
 
 class DeviceBert:
     """Weights registered once; forward() runs the layers on device tensors.
 
     layers: per layer {"qkv"|"o"|"ffn_up"|"ffn_down": (wq int8 [N,K], ws f32 [N],
-    bias f32 [N], act), "attn_ln"|"out_ln": (gain f32 [D], shift f32 [D])}.
+    bias f32 [N], act), "attn_ln"|"out_ln": (gain f32 [D], shift f32 [D])}; a gated layer
+    also has "ffn_gate", whose act (ACT_SILU or ACT_GELU) is the gate's, and its "ffn_up" has
+    ACT_NONE. rope: rotary frequencies (Context.rope) of the context, which outlive this object,
+    with rope_layout; such a model's position table (set_embeddings) is zeros.
     """
 
     def __init__(self, ctx: enchip.Context, layers: Sequence[Dict], hidden: int, heads: int, ffn: int,
-                 fused: bool = True, fuse_ln_quant: bool = True, gelu_in_quant: bool = True):
+                 fused: bool = True, fuse_ln_quant: bool = True, gelu_in_quant: bool = True,
+                 rope: Optional["enchip.Rope"] = None, rope_layout: int = enchip.ROPE_HALF):
         import torch
+
+        for lw in layers:
+            if "ffn_gate" in lw and lw["ffn_up"][3] != enchip.ACT_NONE:
+                raise ValueError("a gated layer's activation is its ffn_gate's: ffn_up must have ACT_NONE")
 
         self.fused = fused
         self.fuse_ln_quant = fuse_ln_quant
         self.gelu_in_quant = gelu_in_quant
+        self.rope, self.rope_layout = rope, rope_layout
         self.torch = torch
         self.ctx, self.D, self.H, self.I = ctx, hidden, heads, ffn
         self.hd = hidden // heads
@@ -78,7 +93,9 @@ class DeviceBert:
         dev = torch.device("cuda")
         for lw in layers:
             entry = {}
-            for name in ("qkv", "o", "ffn_up", "ffn_down"):
+            for name in LINEARS:
+                if name not in lw and name == "ffn_gate":
+                    continue
                 wq, ws, b, act = lw[name]
                 entry[name] = (ctx.register_weight(wq, ws), torch.from_numpy(np.ascontiguousarray(b)).to(dev), act)
             for name in ("attn_ln", "out_ln"):
@@ -131,8 +148,9 @@ class DeviceBert:
 
     def close(self) -> None:
         for entry in self.handles:
-            for name in ("qkv", "o", "ffn_up", "ffn_down"):
-                self.ctx.release_weight(entry[name][0])
+            for name in LINEARS:
+                if name in entry:
+                    self.ctx.release_weight(entry[name][0])
         self.handles = []
         self._bufs = {}
 
@@ -218,6 +236,9 @@ class DeviceBert:
                 c.pre_frag_dev(w, codes, pending, M, ascale, bias.data_ptr(), act, q, stream)
             else:
                 linear("qkv", w, h, bias, act, qkv)
+            if self.rope is not None:
+                self._m("rope")
+                c.rope_rows_dev(self.rope, self.rope_layout, q, 3 * D, q, 3 * D, S, L, 2 * H, hd, stream=stream)
             self._m("attention")
             if self.fused_attention(L):
                 c.attention_f32_dev(q, q + D * 4, q + 2 * D * 4, 3 * D, ctxv.data_ptr(), D, S, L, H, hd, scale, stream)
@@ -233,6 +254,17 @@ class DeviceBert:
             linear("o", w, ctxv, bias, act, out)
             g, s = e["attn_ln"]
             w, bias, act = e["ffn_up"]
+            if "ffn_gate" in e:
+                wg, bg, act = e["ffn_gate"]
+                ln_then(g, s, out, None, "attn_ln")
+                self._m("ffn_gated")
+                c.w8a8_gated_dev(wg, w, h.data_ptr(), M, bg.data_ptr(), bias.data_ptr(), act, inter.data_ptr(), stream)
+                w, bias, act = e["ffn_down"]
+                linear("ffn_down", w, inter, bias, act, ffn)
+                g, s = e["out_ln"]
+                nxt = self.handles[li + 1]["qkv"][0] if li + 1 < len(self.handles) else None
+                pending = ln_then(g, s, ffn, nxt, "out_ln")
+                continue
             gq = self.gelu_quant_route(act, e["ffn_down"][0], M)
             up_act = enchip.ACT_NONE if gq else act
             ldq = ln_then(g, s, out, w, "attn_ln")
