@@ -154,6 +154,10 @@ struct enchip_ctx {
     hipEvent_t scratch_ev = nullptr;
     hipStream_t scratch_stream = nullptr;
     bool scratch_pending = false, scratch_recorded = false, scratch_shared = false;
+    // Set once work on the scratch has been captured into a graph, which keeps its addresses: buffers
+    // that grow from then on are kept (retired) until enchip_close, not freed.
+    bool scratch_captured = false;
+    std::vector<void *> retired;
     int8_t *d_aq = nullptr;
     size_t aq_cap = 0;
     float *d_as = nullptr;
@@ -217,7 +221,18 @@ int ensure(enchip_ctx *c, T **p, size_t *cap, size_t bytes, bool scratch = true)
         return fail(c, ENCHIP_ERR_OOM, "scratch of %zu bytes exceeds the context's scratch limit of %zu", bytes,
                     c->scratch_limit);
     if (bytes <= *cap && *p) return ENCHIP_OK;
-    if (*p) {
+    size_t want = std::max<size_t>(bytes, 256);
+    if (*p && scratch && c->scratch_captured) {
+        // grows at least twofold, so that all that is kept is less than what is in use
+        want = std::max(want, c->scratch_limit ? std::min(2 * *cap, c->scratch_limit) : 2 * *cap);
+        try {
+            c->retired.push_back(*p);
+        } catch (const std::bad_alloc &) {
+            return fail(c, ENCHIP_ERR_OOM, "scratch: out of host memory");
+        }
+        *p = nullptr;
+        *cap = 0;
+    } else if (*p) {
         // the old buffer may still be read by work enqueued on another stream
         if (scratch && c->scratch_pending)
             (void)(c->scratch_recorded ? hipEventSynchronize(c->scratch_ev) : hipStreamSynchronize(c->stream));
@@ -226,8 +241,12 @@ int ensure(enchip_ctx *c, T **p, size_t *cap, size_t bytes, bool scratch = true)
         *cap = 0;
         if (e != hipSuccess) return fail(c, ENCHIP_ERR_HIP, "hipFree: %s", hipGetErrorString(e));
     }
-    size_t want = std::max<size_t>(bytes, 256);
     hipError_t e = hipMalloc((void **)p, want);
+    if (e != hipSuccess && want > std::max<size_t>(bytes, 256)) {
+        (void)hipGetLastError();
+        want = std::max<size_t>(bytes, 256);
+        e = hipMalloc((void **)p, want);
+    }
     if (e != hipSuccess) {
         *p = nullptr;
         (void)hipGetLastError();
@@ -388,7 +407,10 @@ int scratch_wait(enchip_ctx *c, hipStream_t s) {
 int scratch_record(enchip_ctx *c, hipStream_t s) {
     const bool record = s != c->stream || c->scratch_shared;
     if (record) {
-        if (s != c->stream && capturing(s)) return ENCHIP_OK;
+        if (s != c->stream && capturing(s)) {
+            c->scratch_captured = true;
+            return ENCHIP_OK;
+        }
         hipError_t e = hipEventRecord(c->scratch_ev, s);
         if (e != hipSuccess) return fail(c, ENCHIP_ERR_HIP, "hipEventRecord(scratch): %s", hipGetErrorString(e));
     }
@@ -925,6 +947,7 @@ int enchip_close(enchip_ctx *ctx) {
                         ctx->d_acc, ctx->d_fb, ctx->d_cand, ctx->d_hits};
         for (void *p : bufs)
             if (p) (void)hipFree(p);
+        for (void *p : ctx->retired) (void)hipFree(p);
         if (ctx->scratch_ev) (void)hipEventDestroy(ctx->scratch_ev);
         for (hipEvent_t e : ctx->stage_ev)
             if (e) (void)hipEventDestroy(e);
@@ -2557,7 +2580,7 @@ int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, const float
     if (layout != ENCHIP_ROPE_HALF && layout != ENCHIP_ROPE_INTERLEAVED)
         return fail(ctx, ENCHIP_ERR_ARG, "rope: bad layout %d", layout);
     if (nseq < 0 || L < 0 || heads < 0 || head_dim < 2 * r.n || head_dim > 2 * enchip::ROPE_MAX_PAIRS || heads > 65536 ||
-        nseq > INT32_MAX || L > INT32_MAX || nseq * L > INT32_MAX ||
+        heads * head_dim > ((int64_t)1 << 20) || nseq > INT32_MAX || L > INT32_MAX || nseq * L > INT32_MAX ||
         ldx < heads * head_dim || ldy < heads * head_dim)
         return fail(ctx, ENCHIP_ERR_ARG,
                     "rope: bad shape nseq=%lld L=%lld heads=%lld head_dim=%lld (%lld rotated, at most %d) ldx=%lld ldy=%lld",
@@ -2611,17 +2634,16 @@ constexpr int64_t kMaxGateN = (int64_t)1 << 24;  // output channels: one launch 
 
 // What the weight-only products take of one or two weights of one shape.
 struct WoArgs {
-    int bits;
     int64_t N, K, Np, Kp, cpg, G;  // cpg: 32-deep chunks per scale group
     enchip::WoWeight w[2];
 };
 
 WoArgs wo_args(const Weight &a, const Weight &b) {
-    return {8, a.N, a.K, a.Np, a.Kp, 1, 1, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
+    return {a.N, a.K, a.Np, a.Kp, 1, 1, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
 }
 
 WoArgs wo_args(const Weight4 &a, const Weight4 &b) {
-    return {4, a.N, a.K, a.Np, a.Kp, a.group / 32, a.G, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
+    return {a.N, a.K, a.Np, a.Kp, a.group / 32, a.G, {{a.d_w, a.d_s}, {b.d_w, b.d_s}}};
 }
 
 // The rows that gemv_wo takes; more are split first (split_rows) and run on the f16 MFMA. A pass over the

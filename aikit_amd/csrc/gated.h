@@ -9,7 +9,7 @@ namespace enchip {
 
 enum GateAct { GATE_SILU = 0, GATE_GELU = 1 };
 
-// x / (1 + e^-x) within 4 ulp: 2^z on the hardware with z = -x log2(e) and the rounding of z
+// x / (1 + e^-x) within 4 ulp while it is above 2^-100: 2^z on the hardware with z = -x log2(e) and the rounding of z
 // put back as a factor, an approximate reciprocal (1 ulp). x is bounded for the exponent only:
 // past +-150 e^-x is 0 or infinite in f32, so x = +inf gives +inf and x = -inf NaN, as the
 // formula does.

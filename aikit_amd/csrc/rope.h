@@ -51,7 +51,7 @@ struct RopeVec {
 // place, those of the passed-through part. ipr: items per head. V = 4: r a multiple of 8 (half) or
 // 4, head_dim and pitches of 4, 16-byte aligned buffers.
 template <bool INTERLEAVED, int V>
-__global__ __launch_bounds__(256) void rope_rows(const float *__restrict__ x, int64_t ldx, float *__restrict__ y,
+__global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, float *y,
                                                  int64_t ldy, const double *__restrict__ turns, float mscale,
                                                  const int32_t *__restrict__ pos, int64_t pos0, int64_t row0, int L,
                                                  int64_t rows, int TR, FastDiv heads, FastDiv ipr, int hd, int r) {

@@ -26,7 +26,9 @@
  *     stream (through an event of the library; the first work on a caller's stream waits
  *     for all that the context's stream holds), so host calls and
  *     *_dev calls on different streams may be mixed. Under HIP graph capture the
- *     library records no such event and the caller orders the streams.
+ *     library records no such event and the caller orders the streams. A graph that was
+ *     captured keeps its scratch: what later calls outgrow stays allocated until
+ *     enchip_close. (Capturing needs scratch of the size at hand: run the call once before.)
  *
  * Numerics (bit-exact against aikit's Go linalg path, default amd64 build):
  *   codes   = quantizeRowInt8Core (linalg/quant.go:43-71), activations' zero row -> scale 0
@@ -534,7 +536,7 @@ int enchip_rope_release(enchip_ctx *ctx, enchip_rope rope);
  * d_pos[row] (any int32), or pos0 + i when d_pos is NULL. d_y == d_x with ldy == ldx rotates in
  * place; otherwise the two hold no element in common. The query and key heads of fused
  * [tokens, 3D] QKV rows are one call with heads = 2D / head_dim. head_dim <= 1024, heads <=
- * 65536, nseq * L < 2^31. */
+ * 65536, heads * head_dim <= 2^20, nseq * L < 2^31. */
 int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope rope, int layout, const float *d_x, int64_t ldx,
                          float *d_y, int64_t ldy, int64_t nseq, int64_t L, int64_t heads,
                          int64_t head_dim, const int32_t *d_pos, int64_t pos0, void *stream);
@@ -563,7 +565,8 @@ int enchip_matmul_bt_q4(enchip_ctx *ctx, enchip_weight w, const float *a, int64_
  * Up to 8 rows are multiplied in f32. More (from 17 rows for small weights) go through the context's
  * shared scratch: each row is scaled by a power of two and held in two f16 parts, 22 bits of each
  * activation, or 2^-39 of the row's largest for the smallest ones; where an outlier leaves more than
- * a sixteenth of a 128-wide block of the row below 2^-19 of it, the block is multiplied in f32. */
+ * a sixteenth of a 128-wide block of the row below 2^-19 of it, the block is multiplied in f32.
+ * d_dst holds no element of d_a. */
 int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, int64_t lda, int64_t M,
                             float *d_dst, int64_t ldd, void *stream);
 
@@ -571,8 +574,9 @@ int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, 
  * The first half of a gated feed-forward block (encoder/forward_q8.go:264-279 swigluMLPQ8, up to
  * the down projection), both projections, the activation and the product in one call:
  *   dst[m][n] = act(yg[m][n]) * yu[m][n],  y = a . W^T (+ bias[n], nullable).
- * act: ENCHIP_ACT_SILU (x / (1 + e^-x)) or ENCHIP_ACT_GELU (linalg.GELUF32). Both weights have one
- * shape (and group), K > 0, N <= 2^24; the same handle may be both. dst holds no element of a.
+ * act: ENCHIP_ACT_SILU (x / (1 + e^-x)) or ENCHIP_ACT_GELU (x Phi(x), within 0.75e-7 |x| and
+ * rounding; not linalg.GELUF32's bits). Both weights have one shape (and group), K > 0, N <= 2^24;
+ * the same handle may be both. dst holds no element of a or of a bias.
  *   gated_q8    int8 weights, f32 activations: y as enchip_matmul_bt_q8 defines it
  *   gated_q4    4-bit weights, f32 activations: y as enchip_matmul_bt_q4 defines it
  *   w8a8_gated  int8 weights, activations quantized per token: y bit-identical to

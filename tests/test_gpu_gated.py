@@ -225,6 +225,81 @@ def test_same_weight_twice_and_graph(ctx, form):
         assert np.all(np.abs(one - want) <= tol)
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("M", [1, 40])
+def test_one_bias(ctx, form, M):
+    g = np.random.default_rng(6)
+    for which in (0, 1):
+        with Pair(ctx, form, g, 90, 100) as p:
+            p.b[which] = None
+            a = activations(g, M, 100)
+            want, tol = p.want(a, "silu")
+            assert np.all(np.abs(p.run(a, "silu") - want) <= tol)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_captured_call_outlives_larger_ones(form):
+    """A graph keeps the scratch it was captured with when a larger call outgrows it."""
+    import torch
+
+    with enchip.Context(0) as c:
+        g = np.random.default_rng(8)
+        M, N, K = 90, 256, 320
+        with Pair(c, form, g, N, K) as p:
+            s = torch.cuda.Stream()
+            acts = [activations(g, m, K) for m in (M, 20 * M)]
+            da = [torch.from_numpy(a).cuda() for a in acts]
+            dd = [torch.empty((len(a), N), device="cuda") for a in acts]
+            b = [torch.from_numpy(x).cuda() for x in p.b]
+            torch.cuda.synchronize()
+
+            def run(i):
+                if form == "w8a8":
+                    c.w8a8_gated_dev(p.h[0], p.h[1], da[i].data_ptr(), len(acts[i]), b[0].data_ptr(), b[1].data_ptr(),
+                                     enchip.ACT_SILU, dd[i].data_ptr(), stream=s.cuda_stream)
+                else:
+                    p.call_dev(p.h[0], p.h[1], da[i].data_ptr(), K, len(acts[i]), b[0].data_ptr(), b[1].data_ptr(),
+                               enchip.ACT_SILU, dd[i].data_ptr(), N, stream=s.cuda_stream)
+
+            run(0)
+            torch.cuda.synchronize()
+            want = dd[0].cpu().numpy()
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=s):
+                run(0)
+            run(1)
+            torch.cuda.synchronize()
+            big = dd[1].cpu().numpy()
+            filler = torch.full((64 << 20,), float("nan"), device="cuda")  # what freed memory would be given to
+            for r in range(3):
+                dd[0].zero_()
+                torch.cuda.synchronize()
+                gr.replay()
+                torch.cuda.synchronize()
+                assert np.array_equal(dd[0].cpu().numpy(), want), r
+                run(1)
+                torch.cuda.synchronize()
+                assert np.array_equal(dd[1].cpu().numpy(), big), r
+            del gr, filler
+
+
+def test_threads_share_a_context(ctx):
+    from concurrent.futures import ThreadPoolExecutor
+
+    g = np.random.default_rng(12)
+    pairs = {f: Pair(ctx, f, g, 300, 256) for f in FORMS}
+    try:
+        jobs = [(f, activations(g, M, 256)) for f in FORMS for M in (1, 30, 200, 1000)]
+        want = [pairs[f].run(a, "silu") for f, a in jobs]
+        with ThreadPoolExecutor(8) as ex:
+            for _ in range(3):
+                got = list(ex.map(lambda j: pairs[j[0]].run(j[1], "silu"), jobs))
+                assert all(np.array_equal(x, y) for x, y in zip(got, want))
+    finally:
+        for p in pairs.values():
+            p.__exit__()
+
+
 def test_refusals(ctx):
     import torch
 

@@ -84,7 +84,7 @@ LAYOUTS = [enchip.ROPE_HALF, enchip.ROPE_INTERLEAVED]
 
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("hd,rot", [(64, 64), (64, 32), (32, 32), (128, 128), (128, 96), (64, 62), (64, 2), (20, 10), (2, 2),
-                                    (7, 6), (1024, 1024), (256, 40)])
+                                    (7, 6), (1024, 1024), (256, 40), (1024, 2), (96, 42)])
 def test_shapes(ctx, layout, hd, rot):
     r = ctx.rope(rot)
     f, m = freqs(rot)
@@ -199,6 +199,19 @@ def test_query_and_key_heads_of_qkv_rows(ctx):
         ctx.release_rope(r)
 
 
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("heads,hd,rot", [(1024, 1024, 1024), (1024, 1024, 2), (65536, 16, 8), (65536, 16, 6), (65536, 7, 6)])
+def test_widest_rows(ctx, layout, heads, hd, rot):
+    r = ctx.rope(rot)
+    f, m = freqs(rot)
+    try:
+        say(f"rope heads={heads} hd={hd} rot={rot}")
+        check(ctx, r, layout, hd, heads, 1, 2, f, m)
+        check(ctx, r, layout, hd, heads, 1, 2, f, m, inplace=True, pos0=3)
+    finally:
+        ctx.release_rope(r)
+
+
 def test_many_rows(ctx):
     # more rows than one launch takes: the rows' positions run on across launches
     import torch
@@ -237,7 +250,7 @@ def test_refusals(ctx):
     p = d.data_ptr()
     ok = dict(layout=0, d_x=p, ldx=16, d_y=p, ldy=16, nseq=1, L=1, heads=1, head_dim=8)
     for k, v in (("layout", 2), ("ldx", 7), ("ldy", 7), ("nseq", -1), ("L", -1), ("heads", -1), ("head_dim", 7), ("head_dim", 1025),
-                 ("d_x", 0), ("d_y", 0), ("ldy", 15), ("pos0", 1 << 40), ("L", 1 << 31), ("heads", 70000)):
+                 ("d_x", 0), ("d_y", 0), ("ldy", 15), ("pos0", 1 << 40), ("L", 1 << 31), ("heads", 70000), ("heads", (1 << 17) + 1)):
         with pytest.raises(enchip.EnchipError) as e:
             ctx.rope_rows_dev(r, **{**ok, k: v})
         assert e.value.code == enchip.ERR_ARG, (k, v)
