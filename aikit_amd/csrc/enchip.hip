@@ -465,12 +465,20 @@ int launch_quant_rows(enchip_ctx *c, const float *d_a, int64_t M, int64_t K, int
 #undef QCASE
             default: return fail(c, ENCHIP_ERR_ARG, "quant: bad chunk count %d", ch);
         }
+    } else if (frag) {
+        // a wavefront per row up to 2048 columns, else a workgroup, which holds rows of up to 8192
+        const bool v4 = K % 4 == 0 && (uintptr_t)d_a % 16 == 0 && K > 0;
+        const dim3 grid((unsigned)(ldq <= 2048 ? (M + 3) / 4 : M)), block(256);
+#define QANY(...) hipLaunchKernelGGL((enchip::quant_rows_frag_any<__VA_ARGS__>), grid, block, 0, s, d_a, q, ldq, scale, M, K)
+        if (ldq <= 2048) QANY(1, true, false);
+        else if (ldq <= 8192 && v4) QANY(4, true, true);
+        else if (ldq <= 8192) QANY(4, true, false);
+        else if (v4) QANY(4, false, true);
+        else QANY(4, false, false);
+#undef QANY
     } else {
         const dim3 grid((unsigned)((M + 3) / 4)), block(256);
-        if (frag)
-            hipLaunchKernelGGL(enchip::quant_rows_scalar<true>, grid, block, 0, s, d_a, q, ldq, scale, M, K);
-        else
-            hipLaunchKernelGGL(enchip::quant_rows_scalar<false>, grid, block, 0, s, d_a, q, ldq, scale, M, K);
+        hipLaunchKernelGGL(enchip::quant_rows_scalar, grid, block, 0, s, d_a, q, ldq, scale, M, K);
     }
     return check_launch(c, "quant_rows");
 }
@@ -2597,22 +2605,29 @@ int enchip_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, const float
     const int64_t rows = nseq * L;
     const bool inter = layout == ENCHIP_ROPE_INTERLEAVED, inplace = d_x == d_y;
     const int64_t rot = 2 * r.n, rest = inplace ? 0 : head_dim - rot;
-    const bool vec = rot % (inter ? 4 : 8) == 0 && head_dim % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 &&
-                     (uintptr_t)d_x % 16 == 0 && (uintptr_t)d_y % 16 == 0;
-    const int64_t ipr = vec ? rot / (inter ? 4 : 8) + rest / 4 : r.n + rest;
+    // elements that an access may hold: of the rotated part (v) and of what is passed through (rv)
+    auto fits = [&](int64_t n) {
+        return head_dim % n == 0 && ldx % n == 0 && ldy % n == 0 && (uintptr_t)d_x % (4 * n) == 0 && (uintptr_t)d_y % (4 * n) == 0;
+    };
+    const int64_t unit = inter ? rot : r.n;
+    const int v = unit % 4 == 0 && fits(4) ? 4 : unit % 2 == 0 && fits(2) ? 2 : 1, rv = v > 1 ? v : fits(2) ? 2 : 1;
+    const int64_t ipr = (inter ? v > 1 ? rot / v : r.n : r.n / v) + rest / rv;
     // rows of a workgroup: three items a thread, while a few workgroups a CU are left
     const int64_t by_items = std::max<int64_t>(1, 768 / (heads * ipr)), by_rows = std::max<int64_t>(1, rows / (4 * ctx->num_cus));
     const int tr = (int)std::min({by_items, by_rows, (int64_t)enchip::ROPE_CS / r.n, (int64_t)64});
     for (int64_t r0 = 0; r0 < rows; r0 += kRowChunk) {
         const int64_t n = std::min(kRowChunk, rows - r0);
-#define ROPE_CALL(I, V)                                                                                              \
-    hipLaunchKernelGGL((enchip::rope_rows<I, V>), dim3((unsigned)((n + tr - 1) / tr)), dim3(256), 0, s, d_x + r0 * ldx, ldx, \
-                       d_y + r0 * ldy, ldy, r.d_turns, r.mscale, d_pos ? d_pos + r0 : nullptr, pos0, r0, (int)L, n, tr, \
+#define ROPE_CALL(I, V, RV)                                                                                          \
+    hipLaunchKernelGGL((enchip::rope_rows<I, V, RV>), dim3((unsigned)((n + tr - 1) / tr)), dim3(256), 0, s, d_x + r0 * ldx, \
+                       ldx, d_y + r0 * ldy, ldy, r.d_turns, r.mscale, d_pos ? d_pos + r0 : nullptr, pos0, r0, (int)L, n, tr, \
                        fast_div(heads), fast_div(ipr), (int)head_dim, (int)rot)
-        if (inter && vec) ROPE_CALL(true, 4);
-        else if (inter) ROPE_CALL(true, 1);
-        else if (vec) ROPE_CALL(false, 4);
-        else ROPE_CALL(false, 1);
+        if (inter && v == 4) ROPE_CALL(true, 4, 4);
+        else if (inter && v == 2) ROPE_CALL(true, 2, 2);
+        else if (inter) ROPE_CALL(true, 1, 1);
+        else if (v == 4) ROPE_CALL(false, 4, 4);
+        else if (v == 2) ROPE_CALL(false, 2, 2);
+        else if (rv == 2) ROPE_CALL(false, 1, 2);
+        else ROPE_CALL(false, 1, 1);
 #undef ROPE_CALL
     }
     return check_launch(ctx, "rope_rows");
@@ -2910,14 +2925,24 @@ void launch_gated_frag(enchip_ctx *c, const Weight &w, const int8_t *aq, const f
                            tilesN, tiles);
 }
 
+// Whether the one launch takes M rows of w: its workgroups (8 rows x 32 channels) all run at once, or
+// there is one group of rows. More would read their weights again, one after another. Measured on MI355X, us,
+// one launch against quantization and pieces: K = N = 4096 (one workgroup a CU) 16 rows 13.0 and 15.5, 17
+// rows 20.7 and 15.5; K = 4096, N = 11008 8 rows 25.6 and 24.9, 1 row 19.9 and 23.0, 9 rows 36.8 and
+// 24.9; K = 1024, N = 4096 (three a CU) 32 rows 7.1 and 8.6.
+bool one_launch_gated(const enchip_ctx *c, const Weight &w, int64_t M, const float *d_a) {
+    if (M > c->small_m || M > 32 || w.K % 4 != 0 || w.K > enchip::GVQ_MAX_K || (uintptr_t)d_a % 16 != 0) return false;
+    const int64_t groups = (M + enchip::GVQ_ROWS - 1) / enchip::GVQ_ROWS, cols = (w.N + 31) / 32;
+    const int64_t per_cu = 160 * 1024 / enchip::gated_q_lds_bytes((int)w.Kp);
+    return grid_fits(cols, 64 * enchip::GVQ_WAVES * 4) && (groups == 1 || groups * cols <= per_cu * c->num_cus);
+}
+
 // Enqueues the W8A8 gated pair on d_a [M][K] after the caller checked the arguments.
 int launch_gated_w8a8(enchip_ctx *c, const Weight &wg, const Weight &wu, const float *d_a, int64_t M, const float *bg,
                       const float *bu, int act, float *d_dst, hipStream_t s) {
     int rc;
     const enchip::GatePair p = {{wg.d_w, wu.d_w}, {wg.d_s, wu.d_s}, {bg, bu}};
-    if (M <= c->small_m && M <= 32 && wg.K % 4 == 0 && wg.K <= enchip::GVQ_MAX_K && (uintptr_t)d_a % 16 == 0 &&
-        grid_fits((wg.N + 31) / 32, 64 * enchip::GVQ_WAVES * 4))
-        return launch_gated_q(c, wg, d_a, M, p, act, d_dst, s);
+    if (one_launch_gated(c, wg, M, d_a)) return launch_gated_q(c, wg, d_a, M, p, act, d_dst, s);
     if ((rc = ensure_act_scratch(c, M, wg.Kp))) return rc;
     if ((rc = scratch_wait(c, s))) return rc;
     if ((rc = launch_quant(c, d_a, M, wg.K, c->d_aq, wg.Kp, c->d_as, s, true))) return rc;

@@ -1,6 +1,6 @@
 // kernels.h -- gfx950 kernels of the W8A8 linear path.
 //
-//   quant_rows_vec / quant_rows_scalar  per-token dynamic int8 quantization
+//   quant_rows_vec / quant_rows_frag / quant_rows_frag_any / quant_rows_scalar  per-token dynamic int8 quantization
 //   gemm_w8a8                           tiled int8 MFMA GEMM + fused dequant epilogue
 //   gemv_w8a8                           small-M (HBM-bound) split-K MFMA variant
 //
@@ -428,19 +428,71 @@ __global__ __launch_bounds__(512) void quant_rows_frag_gelu(const float *__restr
     }
 }
 
-// Any K and alignment: one wavefront per row, two passes over the row. FRAG as in
-// quant_rows_vec.
-template <bool FRAG>
-__global__ __launch_bounds__(256) void quant_rows_scalar(const float *__restrict__ a,
-                                                         int8_t *__restrict__ q, int64_t ldq,
-                                                         float *__restrict__ scale, int64_t M,
-                                                         int64_t K) {
+// Fragment-major codes of any K and alignment: rows that quant_rows_frag does not take. WPR wavefronts
+// per row, a thread's words of four codes NT apart (a wavefront reads 1 KiB in a row), 8 of them in flight;
+// HELD: the row (ldq <= 2048 WPR) stays in registers, else it is read twice. VEC: K % 4 == 0, 16-byte aligned rows.
+template <int WPR, bool HELD, bool VEC>
+__global__ __launch_bounds__(256) void quant_rows_frag_any(const float *__restrict__ a, int8_t *__restrict__ q, int64_t ldq,
+                                                           float *__restrict__ scale, int64_t M, int64_t K) {
+    constexpr int NT = 64 * WPR, R = 8;  // threads of a row; words a thread holds
+    static_assert(WPR == 1 || WPR == 4, "a wavefront or a workgroup per row");
+    __shared__ float s_m[4];
+    const int t = threadIdx.x & (NT - 1);
+    const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= M) return;  // WPR 1 (no barrier there)
+    const float *src = a + row * K;
+    const int64_t nk32 = ldq >> 5;
+    const int64_t words = ldq >> 2, rounds = (words + NT * R - 1) / (NT * R);
+    float4 v[R];
+    auto load = [&](int64_t w0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t k = 4 * (w0 + t + NT * i);
+            float x[4];
+            if constexpr (VEC) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(src + min(k, K - 4));
+                x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = K > 0 ? src[min(k + e, K - 1)] : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __int_as_float(__float_as_int(x[e]) & (k + e < K ? -1 : 0));
+            v[i] = make_float4(x[0], x[1], x[2], x[3]);
+        }
+    };
+    float m = 0.0f;
+    for (int64_t r = 0; r < (HELD ? 1 : rounds); ++r) {
+        load(r * NT * R);
+        m = fmaxf(m, row_absmax<R>(v));  // never NaN
+    }
+    if constexpr (WPR == 4) {
+        if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    }
+    const bool zero = m == 0.0f;
+    const float s = zero ? 0.0f : m / 127.0f;
+    const float inv = zero ? 0.0f : 1.0f / s;
+    for (int64_t r = 0; r < (HELD ? 1 : rounds); ++r) {
+        if (!HELD) load(r * NT * R);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t w = r * NT * R + t + NT * i;
+            if (w < words) *reinterpret_cast<int *>(q + frag_off(row, 4 * w, nk32)) = zero ? 0 : pack_codes(v[i], inv);
+        }
+    }
+    if (t == 0) scale[row] = s;
+}
+
+// Row-major codes of any K and alignment: one wavefront per row, two passes over the row.
+__global__ __launch_bounds__(256) void quant_rows_scalar(const float *__restrict__ a, int8_t *__restrict__ q, int64_t ldq,
+                                                         float *__restrict__ scale, int64_t M, int64_t K) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= M) return;
     const float *src = a + row * K;
-    const int64_t nk32 = ldq >> 5;
-    auto dst = [&](int64_t k) -> int8_t & { return q[FRAG ? frag_off(row, k, nk32) : row * ldq + k]; };
+    auto dst = [&](int64_t k) -> int8_t & { return q[row * ldq + k]; };
     float m = 0.0f;
     for (int64_t k = lane; k < K; k += 64) m = absmax_step(m, src[k]);
     m = wave_absmax(m);

@@ -25,38 +25,38 @@ constexpr int ROPE_CS = 2048;        // angles of a workgroup's rows in LDS
 constexpr int ROPE_BATCH = 4;        // items of a thread whose loads are in flight together
 
 template <int V>
-struct RopeVec {
-    float v[V];
-    __device__ __forceinline__ void load(const float *p) {
-        if constexpr (V == 4) {
-            const f32x4 t = *reinterpret_cast<const f32x4 *>(p);
-            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = p[i];
-        }
+__device__ __forceinline__ void rope_load(float *v, const float *p) {
+    if constexpr (V == 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4 *>(p);
+        v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+    } else if constexpr (V == 2) {
+        const float2 t = *reinterpret_cast<const float2 *>(p);
+        v[0] = t.x, v[1] = t.y;
+    } else {
+        v[0] = p[0];
     }
-    __device__ __forceinline__ void store(float *p) const {
-        if constexpr (V == 4) {
-            *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) p[i] = v[i];
-        }
-    }
-};
+}
+template <int V>
+__device__ __forceinline__ void rope_store(const float *v, float *p) {
+    if constexpr (V == 4) *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    else if constexpr (V == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+    else p[0] = v[0];
+}
 
-// A workgroup's TR rows, as items of V elements: per head first the items of the rotated part (half:
-// V elements of each half; interleaved: V elements, V / 2 pairs; V = 1: one pair), then, not in
-// place, those of the passed-through part. ipr: items per head. V = 4: r a multiple of 8 (half) or
-// 4, head_dim and pitches of 4, 16-byte aligned buffers.
-template <bool INTERLEAVED, int V>
-__global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, float *y,
-                                                 int64_t ldy, const double *__restrict__ turns, float mscale,
+// A workgroup's TR rows, as items: per head first those of the rotated part (half: V elements of each
+// half; interleaved: V elements, V / 2 pairs, or with V = 1 one pair), then, not in place, those of the
+// passed-through part, RV elements each. ipr: items per head. Every V-wide (RV-wide) access is aligned to
+// its size: the launch chooses them so.
+template <bool INTERLEAVED, int V, int RV>
+__global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, float *y, int64_t ldy,
+                                                 const double *__restrict__ turns, float mscale,
                                                  const int32_t *__restrict__ pos, int64_t pos0, int64_t row0, int L,
                                                  int64_t rows, int TR, FastDiv heads, FastDiv ipr, int hd, int r) {
     __shared__ float2 cs[ROPE_CS];
-    constexpr int PV = INTERLEAVED && V == 4 ? 2 : 1;     // an item's pairs over V
+    constexpr bool INNER = INTERLEAVED && V > 1;   // an item's pairs lie within it
+    constexpr int PI = INNER ? V / 2 : V;          // pairs of an item
+    constexpr int EI = INTERLEAVED && !INNER ? 2 : V;  // elements from one item to the next
+    constexpr int W = V > RV ? V : RV;
     const int64_t first = (int64_t)blockIdx.x * TR;
     const int tr = (int)min((int64_t)TR, rows - first), np = r / 2;
     for (int t = threadIdx.x; t < tr * np; t += 256) {
@@ -68,10 +68,11 @@ __global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, fl
         cs[t] = make_float2(c * mscale, s * mscale);
     }
     __syncthreads();
-    const int rot = PV == 2 ? r / 4 : np / V;  // rotated items of a head
+    const int rot = np / PI;                       // rotated items of a head
+    const int mate = INTERLEAVED ? 1 : np;         // from a pair's first element to its second
     const uint32_t items = (uint32_t)tr * heads.d * ipr.d;
     for (uint32_t i0 = threadIdx.x; i0 < items; i0 += 256 * ROPE_BATCH) {
-        RopeVec<V> a[ROPE_BATCH], b[ROPE_BATCH];
+        float a[ROPE_BATCH][W], b[ROPE_BATCH][V];
         float *dst[ROPE_BATCH];
         int at[ROPE_BATCH];  // the item's first angle, -1: passed through, -2: none
 #pragma unroll
@@ -84,37 +85,30 @@ __global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, fl
             const uint32_t hr = ipr.div(i), row = heads.div(hr);
             const int e = (int)(i - hr * ipr.d), h = (int)(hr - row * heads.d);
             const bool turn = e < rot;
-            const int off = h * hd + (turn ? (INTERLEAVED ? (V == 4 ? 4 : 2) * e : V * e) : r + V * (e - rot));
+            const int off = h * hd + (turn ? EI * e : r + RV * (e - rot));
             const float *src = x + (first + row) * ldx + off;
             dst[u] = y + (first + row) * ldy + off;
-            at[u] = turn ? (int)row * np + (PV == 2 ? 2 : V) * e : -1;
-            a[u].load(src);
-            if (V == 1 ? turn : (!INTERLEAVED && turn)) b[u].load(src + (INTERLEAVED ? 1 : np));
+            at[u] = turn ? (int)row * np + PI * e : -1;
+            if (V == RV || turn) rope_load<V>(a[u], src);
+            else rope_load<RV>(a[u], src);
+            if (!INNER && turn) rope_load<V>(b[u], src + mate);
         }
 #pragma unroll
         for (int u = 0; u < ROPE_BATCH; ++u) {
             if (at[u] == -2) continue;
             if (at[u] >= 0) {
-                if constexpr (PV == 2) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float2 w = cs[at[u] + k];
-                        const float x1 = a[u].v[2 * k], x2 = a[u].v[2 * k + 1];
-                        a[u].v[2 * k] = x1 * w.x - x2 * w.y;
-                        a[u].v[2 * k + 1] = x2 * w.x + x1 * w.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        const float2 w = cs[at[u] + k];
-                        const float x1 = a[u].v[k], x2 = b[u].v[k];
-                        a[u].v[k] = x1 * w.x - x2 * w.y;
-                        b[u].v[k] = x2 * w.x + x1 * w.y;
-                    }
-                    b[u].store(dst[u] + (INTERLEAVED ? 1 : np));
+                for (int k = 0; k < PI; ++k) {
+                    const float2 w = cs[at[u] + k];
+                    float &e1 = INNER ? a[u][2 * k] : a[u][k], &e2 = INNER ? a[u][2 * k + 1] : b[u][k];
+                    const float x1 = e1, x2 = e2;
+                    e1 = x1 * w.x - x2 * w.y;
+                    e2 = x2 * w.x + x1 * w.y;
                 }
+                if constexpr (!INNER) rope_store<V>(b[u], dst[u] + mate);
             }
-            a[u].store(dst[u]);
+            if (V == RV || at[u] >= 0) rope_store<V>(a[u], dst[u]);
+            else rope_store<RV>(a[u], dst[u]);
         }
     }
 }

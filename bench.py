@@ -55,8 +55,11 @@ def quant_kernel_name(K: int, frag: bool) -> str:
     Kp = (K + 63) // 64 * 64
     if frag:
         ch = (Kp + 255) // 256
-        return f"enchip::quant_rows_frag<{ch}, {2 if ch <= 2 else 1}>" if 0 < Kp <= 4096 and K % 4 == 0 else "enchip::quant_rows_scalar<true>"
-    return f"enchip::quant_rows_vec<{(K + 255) // 256}>" if 0 < K <= 4096 and K % 4 == 0 else "enchip::quant_rows_scalar<false>"
+        if 0 < Kp <= 4096 and K % 4 == 0:
+            return f"enchip::quant_rows_frag<{ch}, {2 if ch <= 2 else 1}>"
+        wpr, held, vec = (1, True, False) if Kp <= 2048 else (4, Kp <= 8192, K % 4 == 0)
+        return f"enchip::quant_rows_frag_any<{wpr}, {str(held).lower()}, {str(vec).lower()}>"
+    return f"enchip::quant_rows_vec<{(K + 255) // 256}>" if 0 < K <= 4096 and K % 4 == 0 else "enchip::quant_rows_scalar"
 
 
 def ln_cpl(D: int) -> int:

@@ -84,7 +84,8 @@ LAYOUTS = [enchip.ROPE_HALF, enchip.ROPE_INTERLEAVED]
 
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("hd,rot", [(64, 64), (64, 32), (32, 32), (128, 128), (128, 96), (64, 62), (64, 2), (20, 10), (2, 2),
-                                    (7, 6), (1024, 1024), (256, 40), (1024, 2), (96, 42)])
+                                    (7, 6), (1024, 1024), (256, 40), (1024, 2), (96, 42),
+                                    (48, 12), (80, 20), (33, 12), (6, 4)])
 def test_shapes(ctx, layout, hd, rot):
     r = ctx.rope(rot)
     f, m = freqs(rot)
@@ -106,6 +107,20 @@ def test_pitches_and_alignment(ctx, layout, pad, off):
         for inplace in (False, True):
             say(f"rope pad={pad} off={off} layout={layout} inplace={inplace}")
             check(ctx, r, layout, 64, 3, 2, 33, f, m, pad=pad, off=off, inplace=inplace)
+    finally:
+        ctx.release_rope(r)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("pad,off", [(0, 1), (1, 0), (2, 2), (6, 0)])
+@pytest.mark.parametrize("hd,rot", [(48, 20), (48, 22), (32, 32)])
+def test_narrow_accesses(ctx, layout, pad, off, hd, rot):
+    r = ctx.rope(rot)
+    f, m = freqs(rot)
+    try:
+        for inplace in (False, True):
+            say(f"rope hd={hd} rot={rot} pad={pad} off={off} layout={layout} inplace={inplace}")
+            check(ctx, r, layout, hd, 3, 2, 33, f, m, pad=pad, off=off, inplace=inplace)
     finally:
         ctx.release_rope(r)
 
