@@ -2668,17 +2668,26 @@ int64_t few_rows(int64_t weight_bytes) { return weight_bytes <= ((int64_t)4 << 2
 // Bytes of split rows of one pass: more rows run in several.
 constexpr int64_t kSplitBytes = (int64_t)1 << 30;
 
-// Enqueues split_rows of M rows into the context's scratch.
-template <int CH>
+// Enqueues split_rows of M rows into the context's scratch: a wavefront per row of up to 1024, else a workgroup,
+// which holds rows of up to 16384.
+template <int WPR, int CH, bool HELD>
+void launch_split_t(const float *A, int64_t lda, char *parts, float2 *scale, uint8_t *mark, int64_t M, const WoArgs &p, int nkc,
+                    bool vec, hipStream_t s) {
+    using namespace enchip;
+    const dim3 grid((unsigned)(WPR == 1 ? (M + SPLIT_WAVES - 1) / SPLIT_WAVES : M)), block(64 * SPLIT_WAVES);
+    if (vec) hipLaunchKernelGGL((split_rows<WPR, CH, HELD, true>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+    else hipLaunchKernelGGL((split_rows<WPR, CH, HELD, false>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+}
+
 void launch_split(const float *A, int64_t lda, char *parts, float2 *scale, uint8_t *mark, int64_t M, const WoArgs &p, int nkc,
                   bool vec, hipStream_t s) {
-    using namespace enchip;
-    const dim3 grid((unsigned)((M + SPLIT_WAVES - 1) / SPLIT_WAVES)), block(64 * SPLIT_WAVES);
-    const bool held = p.K <= 512 * CH;
-    if (held && vec) hipLaunchKernelGGL((split_rows<CH, true, true>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
-    else if (held) hipLaunchKernelGGL((split_rows<CH, true, false>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
-    else if (vec) hipLaunchKernelGGL((split_rows<1, false, true>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
-    else hipLaunchKernelGGL((split_rows<1, false, false>), grid, block, 0, s, A, lda, parts, scale, mark, (int)M, (int)p.K, nkc);
+    if (p.K <= 512) launch_split_t<1, 1, true>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
+    else if (p.K <= 1024) launch_split_t<1, 2, true>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
+    else if (p.K <= 2048) launch_split_t<4, 1, true>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
+    else if (p.K <= 4096) launch_split_t<4, 2, true>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
+    else if (p.K <= 8192) launch_split_t<4, 4, true>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
+    else if (p.K <= 16384) launch_split_t<4, 8, true>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
+    else launch_split_t<4, 4, false>(A, lda, parts, scale, mark, M, p, nkc, vec, s);
 }
 
 template <int BITS, bool GATED>
@@ -2700,9 +2709,7 @@ int launch_wo_split(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda,
         const int64_t n = std::min(rows, M - r0);
         const float *a = A + r0 * lda;
         float *out = C + r0 * ldc;
-        if (p.K <= 512) launch_split<1>(a, lda, parts, scale, mark, n, p, nkc, vec, s);
-        else if (p.K <= 1024) launch_split<2>(a, lda, parts, scale, mark, n, p, nkc, vec, s);
-        else launch_split<8>(a, lda, parts, scale, mark, n, p, nkc, vec, s);
+        launch_split(a, lda, parts, scale, mark, n, p, nkc, vec, s);
         const WoRows wr = {{parts, scale, mark}, a, lda, (int)n, (int)p.N, (int)p.K, (int)p.Kp, nkc, (int)p.G, fast_div(p.cpg)};
 #define WO_SPLIT(KERNEL, TM, CB, THREADS)                                                                              \
     do {                                                                                                               \

@@ -111,6 +111,15 @@ __device__ __forceinline__ int64_t frag_off(int64_t row, int64_t k, int64_t nk32
     return (((row >> 5) * nk32 + (k >> 5)) << 10) + ((((row & 31) + ((k >> 4) & 1) * 32)) << 4) + (k & 15);
 }
 
+// Map the hardware's round-robin XCD dispatch (block b runs on XCD b % 8) to a
+// contiguous range of logical tiles per XCD, so tiles that share an A row-block
+// run on the same XCD and share its L2.
+__device__ __forceinline__ int xcd_logical_tile(int pid, int nblocks) {
+    const int xcd = pid & 7, idx = pid >> 3;
+    const int q = nblocks >> 3, r = nblocks & 7;
+    return (xcd < r) ? xcd * (q + 1) + idx : r * (q + 1) + (xcd - r) * q + idx;
+}
+
 // One wavefront per row, 4 rows per 256-thread block. Each lane holds CH float4 of
 // the row in registers (K <= 256*CH, K % 4 == 0, rows 16-byte aligned), so the
 // row is read from HBM exactly once. The reads are nontemporal: the f32 rows are
@@ -438,7 +447,7 @@ __global__ __launch_bounds__(256) void quant_rows_frag_any(const float *__restri
     static_assert(WPR == 1 || WPR == 4, "a wavefront or a workgroup per row");
     __shared__ float s_m[4];
     const int t = threadIdx.x & (NT - 1);
-    const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int64_t b = xcd_logical_tile(blockIdx.x, gridDim.x), row = WPR == 1 ? b * 4 + (threadIdx.x >> 6) : b;
     if (row >= M) return;  // WPR 1 (no barrier there)
     const float *src = a + row * K;
     const int64_t nk32 = ldq >> 5;
@@ -531,15 +540,6 @@ __device__ __forceinline__ float epilogue(int acc, float as, float ws, float b) 
 // Row of a 32x32 i32 MFMA accumulator held by lane `lane` in register r.
 __device__ __forceinline__ int acc_row(int r, int lane) {
     return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-}
-
-// Map the hardware's round-robin XCD dispatch (block b runs on XCD b % 8) to a
-// contiguous range of logical tiles per XCD, so tiles that share an A row-block
-// run on the same XCD and share its L2.
-__device__ __forceinline__ int xcd_logical_tile(int pid, int nblocks) {
-    const int xcd = pid & 7, idx = pid >> 3;
-    const int q = nblocks >> 3, r = nblocks & 7;
-    return (xcd < r) ? xcd * (q + 1) + idx : r * (q + 1) + (xcd - r) * q + idx;
 }
 
 // x / d for x d < 2^32: m = 2^32 / d rounded up and one = 0; for d = 1 m = 0 and one = ~0.

@@ -267,19 +267,24 @@ struct SplitRows {
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 constexpr int SPLIT_WAVES = 4;
 
-// One wavefront per row. A lane holds granules of 8 k: lane + 64 i; HELD: all of the row's (K <= 512
-// CH), read once. Otherwise the row is read twice.
-template <int CH, bool HELD, bool VEC>
+// WPR wavefronts per row, thread t of them holding CH granules of 8 k at a time, 64 WPR apart. HELD: all of
+// the row's (K <= 512 WPR CH), read once. Otherwise the row is read twice.
+template <int WPR, int CH, bool HELD, bool VEC>
 __global__ __launch_bounds__(64 * SPLIT_WAVES) void split_rows(const float *__restrict__ A, int64_t lda, char *__restrict__ parts,
                                                                float2 *__restrict__ scale, uint8_t *__restrict__ mark, int M,
                                                                int K, int nkc) {
-    const int lane = threadIdx.x & 63, row = blockIdx.x * SPLIT_WAVES + (threadIdx.x >> 6);
-    if (row >= M) return;
+    constexpr int NT = 64 * WPR;
+    static_assert(WPR == 1 || WPR == SPLIT_WAVES, "a wavefront or a workgroup per row");
+    __shared__ float s_m[SPLIT_WAVES];
+    __shared__ int s_mark[SPLIT_WAVES];
+    const int t = threadIdx.x & (NT - 1), wave = threadIdx.x >> 6;
+    const int b = xcd_logical_tile(blockIdx.x, gridDim.x), row = WPR == 1 ? b * SPLIT_WAVES + wave : b;
+    if (row >= M) return;  // WPR 1 only: no barrier there
     const float *a = A + (int64_t)row * lda;
-    const int granules = 4 * nkc, rounds = (granules + 63) / 64;
+    const int granules = 4 * nkc, rounds = HELD ? 1 : (granules + NT * CH - 1) / (NT * CH);
     f32x4 v[CH][2];
     auto load = [&](int i, f32x4 (&x)[2]) {
-        const int k = 8 * (lane + 64 * i);
+        const int k = 8 * (t + NT * i);
         if (VEC) {
             x[0] = *reinterpret_cast<const f32x4 *>(a + min(k, K - 4));
             x[1] = *reinterpret_cast<const f32x4 *>(a + min(k + 4, K - 4));
@@ -298,18 +303,19 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void split_rows(const float *__re
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e >> 2][e & 3]));
     };
-    if constexpr (HELD) {
+    for (int c = 0; c < rounds; ++c) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) load(i, v[i]);
+        for (int i = 0; i < CH; ++i) load(c * CH + i, v[i]);
 #pragma unroll
         for (int i = 0; i < CH; ++i) largest(v[i]);
-    } else {
-        for (int i = 0; i < rounds; ++i) {
-            load(i, v[0]);
-            largest(v[0]);
-        }
     }
     m = wave_absmax(m);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) s_m[wave] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) m = fmaxf(m, s_m[w]);
+    }
     // m in [2^(E-127), 2^(E-126)): times 2^(141-E), at most 2^127; an infinite m (E = 255) keeps infinities
     // and makes the finite values beside them small
     const int E = (int)(__float_as_uint(m) >> 23), F = min(268 - E, 254);
@@ -318,7 +324,7 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void split_rows(const float *__re
     float minus1 = -1.0f;
     asm("" : "+s"(minus1));  // keeps hi * -1 + a one mixed multiply-add
     auto store = [&](int i, f32x4 (&x)[2]) {
-        const int g = lane + 64 * i;
+        const int g = t + NT * i;
         uint32_t hi[4], lo[4];
         int small = 0, some = 0;
 #pragma unroll
@@ -345,17 +351,23 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void split_rows(const float *__re
         *reinterpret_cast<uint4 *>(d + 2048) = mk ? make_uint4(0, 0, 0, 0) : make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if ((g & 15) == 0) mark[((int64_t)(row >> 5) * (nkc >> 2) + (g >> 4)) * 32 + (row & 31)] = mk;
     };
-    if constexpr (HELD) {
+    for (int c = 0; c < rounds; ++c) {
+        if constexpr (!HELD) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) store(i, v[i]);
-    } else {
-        for (int i = 0; i < rounds; ++i) {
-            load(i, v[0]);
-            store(i, v[0]);
+            for (int i = 0; i < CH; ++i) load(c * CH + i, v[i]);
         }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) store(c * CH + i, v[i]);
     }
-    if (lane == 0)
-        scale[row] = make_float2(marked ? -up : up, __uint_as_float(F == 254 ? 0x400000u : (uint32_t)(254 - F) << 23));
+    bool some_marked = marked != 0;
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) s_mark[wave] = some_marked;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) some_marked |= s_mark[w] != 0;
+    }
+    if (t == 0)
+        scale[row] = make_float2(some_marked ? -up : up, __uint_as_float(F == 254 ? 0x400000u : (uint32_t)(254 - F) << 23));
 }
 
 // What a product of split rows reads besides the weights.
