@@ -2882,10 +2882,15 @@ int launch_gated_q(enchip_ctx *c, const Weight &w, const float *d_a, int64_t M, 
     const Kern fn = table[qch <= 4 ? qch - 1 : qch == 8 ? 4 : qch == 12 ? 5 : 6];
     const size_t lds = (size_t)enchip::gated_q_lds_bytes((int)w.Kp);
     if (lds > 64 * 1024) {
-        const std::pair<const void *, size_t> key(reinterpret_cast<const void *>(fn), lds);
+        // once per kernel, for the longest row it takes
+        const std::pair<const void *, size_t> key(reinterpret_cast<const void *>(fn), (size_t)enchip::gated_q_lds_bytes(256 * qch));
         if (std::find(c->lds_set.begin(), c->lds_set.end(), key) == c->lds_set.end()) {
-            HIP_TRY(c, hipFuncSetAttribute(key.first, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-            c->lds_set.push_back(key);
+            HIP_TRY(c, hipFuncSetAttribute(key.first, hipFuncAttributeMaxDynamicSharedMemorySize, (int)key.second));
+            try {
+                c->lds_set.push_back(key);
+            } catch (const std::bad_alloc &) {
+                return fail(c, ENCHIP_ERR_OOM, "gated_w8a8_q: out of host memory");
+            }
         }
     }
     const dim3 grid((unsigned)((w.N + 31) / 32), (unsigned)((M + enchip::GVQ_ROWS - 1) / enchip::GVQ_ROWS));

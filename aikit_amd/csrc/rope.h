@@ -9,6 +9,12 @@
 // a frequency keeps no fraction in 32), sine and cosine of the reduced angle in 32: an error of
 // about 2^-23 of the pair's length at any position. The pairs' angles are those of every head of
 // the row, so a workgroup computes them once for its rows into LDS and then streams the rows.
+//
+// Bound by memory: 8 bytes an element. 64 x 512 tokens of 24 heads of 64 (403 MB) take 79 us on MI355X,
+// 5.1 TB/s, as a copy does (5.2); half of each of 32 heads of 64, 20011 rows, interleaved, 62 us. One item
+// in flight a thread took 109 us (four: 79), single floats in place of 16 bytes 131 us against 62. Rotated
+// parts that 16-byte accesses do not divide take 8 or 4 bytes: 32768 rows of 24 heads of 64, 42 rotated,
+// interleaved 79 us (4 bytes: 104), half 95 (100); 20 rotated, half 105 (126).
 #pragma once
 
 #include <hip/hip_runtime.h>

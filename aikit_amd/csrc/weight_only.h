@@ -99,6 +99,11 @@ __device__ __forceinline__ float sum_units(float v) {
 // in f32. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
 // 8 NG each. One block ahead is in flight. The lanes' and the wavefronts' sums are added in one order.
 //
+// MI355X, us: 4 bits, 8192 x 8192, 1 row 8.4 to 9.7 (35.7 MB, 4 TB/s; its vector instructions issue for 6),
+// 2 rows 13.0, 4 rows 17.8; K = N = 4096 1 row 5.3, 4 rows 7.8; the gated pair of K = 1024, N = 4096 4.4 (4
+// bits) and 4.8 (int8): one trip to memory and the launch. A lane on a channel's 16 bytes with its activations
+// read from LDS for every weight took 15.9 (2 rows) and 26.2 (4 rows) of 8192 x 8192. NG = 2 where it leaves
+// two workgroups a CU, so that a block's activations serve two groups of channels.
 constexpr int WO_WAVES = 8;
 
 template <int BITS, int MB, int NG, bool GATED>
@@ -259,6 +264,12 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 // Parts, in the A operand's order for the weights' order of k: [M/32][Ka/32] x 4 KiB, plane x and
 // step j of chunk kc at x 2048 + j 1024, 16 bytes per lane: row lane % 32, k = 32 kc + 16 (lane / 32) + 8 j
 // .. + 7. Ka = K rounded up to 128, zero past K. Rows past M are not written (and no output is theirs).
+//
+// Two parts take two thirds of the MFMAs of three exact bf16 parts, made in every tile that reads the row:
+// those took 57.9 us for 512 rows of K = N = 4096 in 4 bits where this takes 49, 436 where it takes 277
+// for 4096. A row costs 8 bytes an element, read and written once: MI355X 4096 x 4096 36 us (3.8 TB/s), 512 x
+// 1024 3.0 to 4.3 us and 32 x 4096 3.7 (a launch and one pass through a row). Neighbouring rows, whose 16-byte
+// pieces share lines, run on one die: 4096 x 8192 84 us, on different ones 131.
 struct SplitRows {
     const char *parts;
     const float2 *scale;   // [M] the row's power of two, negative for a row with marks, and the one that takes it back
@@ -544,7 +555,9 @@ __device__ __forceinline__ void wo_store(const WoRows &p, const WoWeight &w0, co
 
 // Pieces: a workgroup computes 32 TM rows x NT tiles, its NW wavefronts splitting K in 64-deep stages.
 // Parts and codes go straight into registers, PW stages ahead: no LDS and no barrier in the main loop. The
-// shares meet in LDS, each wavefront finishing 16 / NW of the accumulator registers.
+// shares meet in LDS, each wavefront finishing 16 / NW of the accumulator registers. Bound by what a CU
+// reads for its pieces, 128 K bytes of parts each, from L2: MI355X, K = N = 4096, 4 bits 32 rows 11 us (bf16
+// tiles 32), 128 rows 19; gated int8 14 and 27.
 template <int BITS, bool GATED, int TM, int NT, int NW, int PW>
 __global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, WoWeight w1, const float *__restrict__ b0,
                                                          const float *__restrict__ b1, int act, float *__restrict__ C,
@@ -637,6 +650,11 @@ __global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, 
 // chunks. A chunk's parts pass through LDS once for its four wavefronts (double-buffered), its codes go
 // straight into registers, PW stages ahead, and are widened one stage ahead. FP: chunks of a 4-bit
 // weight that share a scale (its group is a multiple of 32 FP): their sum is added once, scaled.
+//
+// MI355X, K = N = 4096, us: 4 bits 512 rows 44, 4096 rows 252 to 298 (275 GFLOP of f16 MFMA work, 194 at 1.42
+// PFLOP/s); gated int8 512 rows 64, 4096 rows 460 to 523 (387); gated 4 bits 4096 rows 502 to 571. Bound by
+// the MFMA together with the widening and scaling (8 vector instructions per MFMA at TM 1), which a SIMD's second
+// wavefront covers in part, and at 512 rows by few tiles a CU: 512 x 4096, K = 1024 14 us, 4 of them MFMA.
 template <int BITS, bool GATED, int TM, int NT, int KS, int PW, int FP>
 __global__ __launch_bounds__(256 * KS, 2) void gemm_wo_tile(WoRows p, WoWeight w0, WoWeight w1,
                                                                  const float *__restrict__ b0, const float *__restrict__ b1,

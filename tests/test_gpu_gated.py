@@ -225,6 +225,22 @@ def test_same_weight_twice_and_graph(ctx, form):
         assert np.all(np.abs(one - want) <= tol)
 
 
+def test_w8a8_row_lengths_in_turn(ctx):
+    # one kernel's on-chip memory grows and shrinks from call to call; one launch and codes first
+    g = np.random.default_rng(21)
+    pairs = [Pair(ctx, "w8a8", g, 96, K) for K in (2048, 1500, 4096, 1100, 3000)]
+    wide = Pair(ctx, "w8a8", g, 9000, 64)
+    try:
+        for M in (1, 8, 20, 32):
+            for p in pairs + pairs[::-1] + [wide]:
+                a = activations(g, M, p.K)
+                want, tol = p.want(a, "silu")
+                assert np.all(np.abs(p.run(a, "silu") - want) <= tol), (M, p.K)
+    finally:
+        for p in pairs + [wide]:
+            p.__exit__()
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("M", [1, 40])
 def test_one_bias(ctx, form, M):
