@@ -2662,9 +2662,13 @@ WoArgs wo_args(const Weight4 &a, const Weight4 &b) {
 }
 
 // The rows that gemv_wo takes; more are split first (split_rows) and run on the f16 MFMA. A pass over the
-// weights takes four rows, the split a launch: K = N = 4096, 4 bits, 8 rows 11.9 us against 15.5, 16 rows
-// 19.8 and 15.9; K = 1024 8 rows 5.4, 16 rows 7.8 and 8.6.
-int64_t few_rows(int64_t weight_bytes) { return weight_bytes <= ((int64_t)4 << 20) ? 16 : 8; }
+// weights takes four rows, the split a launch. Measured on MI355X, us, gemv_wo against the split: 4 bits, K =
+// 1024, N = 4096 (2 MiB) 8 rows 5.4, 16 rows 7.9 and 8.6; gated, 4 MiB, 9 rows 9.4 and 9.9, 16 rows 11.1
+// and 9.9; K = N = 4096 (8 MiB) 8 rows 11.7 and 13.3; gated, 16 MiB, 8 rows 18.1 and 17.1; 8192 x 8192 (32 MiB) 4
+// rows 18.2 (8 in two passes), the split's 5 to 16 rows 22.2.
+int64_t few_rows(int64_t weight_bytes) {
+    return weight_bytes < ((int64_t)4 << 20) ? 16 : weight_bytes < ((int64_t)16 << 20) ? 8 : 4;
+}
 // Bytes of split rows of one pass: more rows run in several.
 constexpr int64_t kSplitBytes = (int64_t)1 << 30;
 

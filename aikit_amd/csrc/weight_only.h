@@ -99,7 +99,7 @@ __device__ __forceinline__ float sum_units(float v) {
 // in f32. Of a workgroup's 8 wavefronts 1 << kbits split the blocks; the others take other channels,
 // 8 NG each. One block ahead is in flight. The lanes' and the wavefronts' sums are added in one order.
 //
-// MI355X, us: 4 bits, 8192 x 8192, 1 row 8.4 to 9.7 (35.7 MB, 4 TB/s; its vector instructions issue for 6),
+// MI355X, us: 4 bits, 8192 x 8192, 1 row 8.4 to 10 (34.6 MB, 4 TB/s; its vector instructions issue for 6),
 // 2 rows 13.0, 4 rows 17.8; K = N = 4096 1 row 5.3, 4 rows 7.8; the gated pair of K = 1024, N = 4096 4.4 (4
 // bits) and 4.8 (int8): one trip to memory and the launch. A lane on a channel's 16 bytes with its activations
 // read from LDS for every weight took 15.9 (2 rows) and 26.2 (4 rows) of 8192 x 8192. NG = 2 where it leaves

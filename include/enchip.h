@@ -562,8 +562,8 @@ int enchip_weight4_shape(enchip_ctx *ctx, enchip_weight w, int64_t *N, int64_t *
 int enchip_matmul_bt_q4(enchip_ctx *ctx, enchip_weight w, const float *a, int64_t M, float *dst);
 
 /* Device form: d_a[M,K] with row pitch lda >= K, d_dst[M,N] with row pitch ldd >= N, on `stream`.
- * Up to 8 rows are multiplied in f32. More (from 17 rows for small weights) go through the context's
- * shared scratch: each row is scaled by a power of two and held in two f16 parts, 22 bits of each
+ * Up to 4 rows (8 for weights under 16 MiB, 16 under 4 MiB) are multiplied in f32. More go through the
+ * context's shared scratch: each row is scaled by a power of two and held in two f16 parts, 22 bits of each
  * activation, or 2^-39 of the row's largest for the smallest ones; where an outlier leaves more than
  * a sixteenth of a 128-wide block of the row below 2^-19 of it, the block is multiplied in f32.
  * d_dst holds no element of d_a. */
