@@ -555,9 +555,11 @@ __device__ __forceinline__ void wo_store(const WoRows &p, const WoWeight &w0, co
 
 // Pieces: a workgroup computes 32 TM rows x NT tiles, its NW wavefronts splitting K in 64-deep stages.
 // Parts and codes go straight into registers, PW stages ahead: no LDS and no barrier in the main loop. The
-// shares meet in LDS, each wavefront finishing 16 / NW of the accumulator registers. Bound by what a CU
-// reads for its pieces, 128 K bytes of parts each, from L2: MI355X, K = N = 4096, 4 bits 32 rows 11 us (bf16
-// tiles 32), 128 rows 19; gated int8 14 and 27.
+// shares meet in LDS, each wavefront finishing 16 / NW of the accumulator registers. A piece is one CU's work
+// (K = 4096: two wavefronts of a SIMD with 16 chunks each of 128 MFMA cycles and about 50 vector instructions, 4.5
+// us) between a start and a joining end: MI355X, K = N = 4096, 4 bits 32 rows 11 us (bf16 tiles 32), 128 rows 19;
+// gated int8 14 and 27; the same at N = 1024. More stages in flight gain nothing, 16 x 32 pieces on the 16 x 16
+// MFMA neither (gated 4 bits 16 rows 17.8 -> 21.3: as many codes to widen for half of the products).
 template <int BITS, bool GATED, int TM, int NT, int NW, int PW>
 __global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, WoWeight w1, const float *__restrict__ b0,
                                                          const float *__restrict__ b1, int act, float *__restrict__ C,
