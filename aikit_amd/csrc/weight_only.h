@@ -254,20 +254,24 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 }
 
 // More rows run on the f16 MFMA. split_rows scales each row of activations by the power of two that
-// brings its largest to 2^14 .. 2^15 and splits it into two f16 parts, hi by truncation, lo the rest
-// rounded: 22 bits of every activation down to 2^-18 of the row's largest, below that 2^-39 of it (lo's
-// smallest step). Codes are f16 values exactly, so products are exact and two MFMAs stand for one in
-// f32. A row's block of 128 k where more than a sixteenth of the nonzero activations lie below 2^-19 of
-// the row's largest (an outlier so large that the bits below matter) is marked: its parts are 0, and
-// the products add it on the f32 MFMA at their end.
+// brings its largest to 2^14 .. 2^15 and splits it into two f16 parts: hi, rounded to f16's 11 bits, and lo, what
+// is left times 2^12, rounded to 11 again. What is left is at most half of hi's step, so lo errs by at most
+// 2^-23 of the activation (f32's own step; what is left is a multiple of that step, so three of four
+// activations are exact). lo at hi's own scale would run into f16's smallest step and keep 2^-39 of
+// the row's largest: nothing of an activation that far below it. Codes are f16 values exactly, and so are
+// codes / 2^12, which lo is multiplied with: products are exact and two MFMAs stand for one in f32. Where hi is
+// subnormal (under 2^-14 scaled, 2^-28 to 2^-29 of the row's largest) it has fewer bits: a row's block of 128 k
+// with such an activation is marked: its parts are 0, and the products add it on the f32 MFMA at their end. MI355X,
+// 4 bits, 4096 rows of K = N = 4096: 279 us for normal activations, 281 behind a GELU, 325 with one of 1000 a
+// thousand times larger, 2230 where every block is marked (softmax rows).
 //
 // Parts, in the A operand's order for the weights' order of k: [M/32][Ka/32] x 4 KiB, plane x and
 // step j of chunk kc at x 2048 + j 1024, 16 bytes per lane: row lane % 32, k = 32 kc + 16 (lane / 32) + 8 j
 // .. + 7. Ka = K rounded up to 128, zero past K. Rows past M are not written (and no output is theirs).
 //
 // Two parts take two thirds of the MFMAs of three exact bf16 parts, made in every tile that reads the row:
-// those took 57.9 us for 512 rows of K = N = 4096 in 4 bits where this takes 49, 436 where it takes 277
-// for 4096. A row costs 8 bytes an element, read and written once: MI355X 4096 x 4096 36 us (3.8 TB/s), 512 x
+// those took 57.9 us for 512 rows of K = N = 4096 in 4 bits where this takes 50, 436 where it takes 273
+// for 4096. lo's own codes cost 1 to 4% of that (a packed multiplication for two of them). A row costs 8 bytes an element, read and written once: MI355X 4096 x 4096 36 us (3.8 TB/s), 512 x
 // 1024 3.0 to 4.3 us and 32 x 4096 3.7 (a launch and one pass through a row). Neighbouring rows, whose 16-byte
 // pieces share lines, run on one die: 4096 x 8192 84 us, on different ones 131.
 struct SplitRows {
@@ -277,6 +281,10 @@ struct SplitRows {
 };
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 constexpr int SPLIT_WAVES = 4;
+constexpr float LO = 4096.0f;  // what lo is scaled by
+
+// The codes that lo's parts are multiplied with: q / 2^12, exact and normal in f16 for |q| from 1 to 128.
+__device__ __forceinline__ f16x8 lo_codes(const f16x8 &q) { return q * (_Float16)(1.0f / LO); }
 
 // WPR wavefronts per row, thread t of them holding CH granules of 8 k at a time, 64 WPR apart. HELD: all of
 // the row's (K <= 512 WPR CH), read once. Otherwise the row is read twice.
@@ -332,30 +340,23 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void split_rows(const float *__re
     const int E = (int)(__float_as_uint(m) >> 23), F = min(268 - E, 254);
     const float up = __uint_as_float((uint32_t)F << 23);
     uint64_t marked = 0;
-    float minus1 = -1.0f;
-    asm("" : "+s"(minus1));  // keeps hi * -1 + a one mixed multiply-add
     auto store = [&](int i, f32x4 (&x)[2]) {
         const int g = t + NT * i;
         uint32_t hi[4], lo[4];
-        int small = 0, some = 0;
+        bool small = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float p = x[e >> 1][2 * (e & 1)] * up, q = x[e >> 1][2 * (e & 1) + 1] * up;
-            const auto h = __builtin_amdgcn_cvt_pkrtz(p, q);
-            const f32x2v l = {__builtin_fmaf((float)h[0], minus1, p), __builtin_fmaf((float)h[1], minus1, q)};
+            const f16x2 h = __builtin_convertvector(f32x2v{p, q}, f16x2);
+            const f32x2v l = {__builtin_fmaf((float)h.x, -LO, p * LO), __builtin_fmaf((float)h.y, -LO, q * LO)};  // exact
             hi[e] = __builtin_bit_cast(uint32_t, h);
             lo[e] = E == 255 ? 0u : __builtin_bit_cast(uint32_t, __builtin_convertvector(l, f16x2));  // inf - inf
-            some += (p != 0.0f) + (q != 0.0f);
-            small += (p != 0.0f && fabsf(p) < 0x1p-5f) + (q != 0.0f && fabsf(q) < 0x1p-5f);
+            small |= (p != 0.0f && fabsf(p) < 0x1p-14f) || (q != 0.0f && fabsf(q) < 0x1p-14f);
         }
         // a block's 16 granules are a 16-lane row
-        uint32_t n = (uint32_t)(some << 16 | small);
-        n += lane_dpp<0xB1>(n);
-        n += lane_dpp<0x4E>(n);
-        n += lane_dpp<0x141>(n);
-        n += lane_dpp<0x140>(n);
-        const bool mk = E != 255 && 16 * (n & 0xffffu) > (n >> 16);
-        marked |= __builtin_amdgcn_ballot_w64(mk);
+        const uint64_t smalls = E == 255 ? 0 : __builtin_amdgcn_ballot_w64(small);
+        const bool mk = (smalls >> (threadIdx.x & 48) & 0xffffu) != 0;
+        marked |= smalls;
         if (g >= granules) return;
         char *d = parts + ((int64_t)(row >> 5) * nkc + (g >> 2)) * 4096 + (g & 1) * 1024 + ((row & 31) + 32 * ((g >> 1) & 1)) * 16;
         *reinterpret_cast<uint4 *>(d) = mk ? make_uint4(0, 0, 0, 0) : make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -482,7 +483,7 @@ __device__ __forceinline__ void wo_chunk(Read read, const uint32_t (&w)[NT][BITS
     f32x16 part[TM][NT];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        f16x8 p[TM][2], q[NT];
+        f16x8 p[TM][2], q[NT], ql[NT];
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -492,6 +493,7 @@ __device__ __forceinline__ void wo_chunk(Read read, const uint32_t (&w)[NT][BITS
             f16x2 h[4];
             WoTiles<BITS, GATED, NT>::widen(w[t], j, h);
             q[t] = f16x8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+            ql[t] = lo_codes(q[t]);
         }
 #pragma unroll
         for (int x = 1; x >= 0; --x)
@@ -499,14 +501,15 @@ __device__ __forceinline__ void wo_chunk(Read read, const uint32_t (&w)[NT][BITS
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
+                    const f16x8 &c = x ? ql[t] : q[t];
                     if (BITS == 8) {
-                        acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][x], q[t], acc[i][t], 0, 0, 0);
+                        acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][x], c, acc[i][t], 0, 0, 0);
                     } else {
                         if (j == 0 && x == 1) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) part[i][t][e] = 0.0f;
                         }
-                        part[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][x], q[t], part[i][t], 0, 0, 0);
+                        part[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i][x], c, part[i][t], 0, 0, 0);
                     }
                 }
     }
@@ -736,6 +739,9 @@ __global__ __launch_bounds__(256 * KS, 2) void gemm_wo_tile(WoRows p, WoWeight w
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) a[i][x] = *reinterpret_cast<const f16x8 *>(cur + i * 4096 + x * 2048 + j * 1024);
+                f16x8 ql[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) ql[t] = lo_codes(q[d & 1][t][j]);
 #pragma unroll
                 for (int x = 1; x >= 0; --x)
 #pragma unroll
@@ -747,7 +753,7 @@ __global__ __launch_bounds__(256 * KS, 2) void gemm_wo_tile(WoRows p, WoWeight w
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) y[e] = 0.0f;
                             }
-                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][x], q[d & 1][t][j], y, 0, 0, 0);
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][x], x ? ql[t] : q[d & 1][t][j], y, 0, 0, 0);
                         }
             }
             // while they run: the next chunk's codes
@@ -764,16 +770,6 @@ __global__ __launch_bounds__(256 * KS, 2) void gemm_wo_tile(WoRows p, WoWeight w
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) acc[i][t][e] = __builtin_fmaf(part[i][t][e], s[t], acc[i][t][e]);
-            }
-            if (BITS == 8 && TM * NT >= 4) {
-                constexpr int MF = 4 * TM * NT;
-                __builtin_amdgcn_sched_group_barrier(0x100, 2 * TM, 0);
-#pragma unroll
-                for (int u = 0; u < MF; ++u) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, (20 * NT + MF - 1) / MF, 0);
-                    if (u == 1) __builtin_amdgcn_sched_group_barrier(0x100, 2 * TM, 0);
-                }
             }
             lds_barrier();
         }

@@ -558,14 +558,17 @@ int enchip_weight4_shape(enchip_ctx *ctx, enchip_weight w, int64_t *N, int64_t *
 /* dst[m][n] = sum_k a[m][k] * (c[n][k] - 8) * scale[n][k / group] on host buffers, with f32
  * activations (never quantized), as enchip_matmul_bt_q8 is for int8 weights: a group's sum is
  * accumulated in f32 and scaled once, in an order of its own (that of a row depends on how many
- * rows there are); the same gate against a float64 dot product. */
+ * rows there are). Against a float64 dot product an output is off by at most ((n + 8) 2^-24 + 2^-23)
+ * sum |a w| over its channel's n nonzero weights, the second term being what is held of the
+ * activations (enchip_matmul_bt_q4_dev), whatever else the row holds. */
 int enchip_matmul_bt_q4(enchip_ctx *ctx, enchip_weight w, const float *a, int64_t M, float *dst);
 
 /* Device form: d_a[M,K] with row pitch lda >= K, d_dst[M,N] with row pitch ldd >= N, on `stream`.
  * Up to 4 rows (8 for weights under 16 MiB, 16 under 4 MiB) are multiplied in f32. More go through the
- * context's shared scratch: each row is scaled by a power of two and held in two f16 parts, 22 bits of each
- * activation, or 2^-39 of the row's largest for the smallest ones; where an outlier leaves more than
- * a sixteenth of a 128-wide block of the row below 2^-19 of it, the block is multiplied in f32.
+ * context's shared scratch: each row is scaled by a power of two and held in two f16 parts, which are
+ * within 2^-23 of each activation (one step of f32); a 128-wide block of the row with a nonzero activation
+ * smaller than the row's largest by 2^28 to 2^29 times or more is multiplied in f32 instead. Both on the scaled
+ * values: of products and sums under 2^-163 of the row's largest activation nothing need remain.
  * d_dst holds no element of d_a. */
 int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, int64_t lda, int64_t M,
                             float *d_dst, int64_t ldd, void *stream);
@@ -577,7 +580,9 @@ int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, 
  * act: ENCHIP_ACT_SILU (x / (1 + e^-x)) or ENCHIP_ACT_GELU (x Phi(x), within 0.75e-7 |x| and
  * rounding; not linalg.GELUF32's bits). Both weights have one shape (and group), K > 0, N <= 2^24;
  * the same handle may be both. dst holds no element of a or of a bias.
- *   gated_q8    int8 weights, f32 activations: y as enchip_matmul_bt_q8 defines it
+ *   gated_q8    int8 weights (no infinite scale), f32 activations: enchip_matmul_bt_q8's product, its
+ *               activations and sums held as enchip_matmul_bt_q4 says (few rows in f32, more in two f16
+ *               parts, not that call's three exact ones), and its bound
  *   gated_q4    4-bit weights, f32 activations: y as enchip_matmul_bt_q4 defines it
  *   w8a8_gated  int8 weights, activations quantized per token: y bit-identical to
  *               enchip_w8a8_linear's, one quantization shared by both projections
