@@ -57,7 +57,7 @@ struct Weight4 {
 
 // Rotary frequencies (enchip_rope_create).
 struct Rope {
-    double *d_turns = nullptr;  // [n] f_j / 2 pi
+    double2 *d_turns = nullptr;  // [n] f_j / 2 pi less whole turns, in two parts
     int64_t n = 0;              // pairs
     float mscale = 1.0f;
 };
@@ -2488,13 +2488,25 @@ enchip::FastDiv fast_div(int64_t d) {
 }
 
 constexpr double kTwoPi = 6.283185307179586476925286766559;
+constexpr double kInvTwoPi = 0x1.45f306dc9c883p-3, kInvTwoPiLow = -0x1.6b01ec5417056p-57;  // 1 / 2 pi in two parts
+constexpr double kMaxFreq = 1099511627776.0;  // 2^40
+
+// f / 2 pi less the nearest whole number, x + y, within |f| 2^-106: at whole positions whole turns change nothing.
+// Up to kMaxFreq a position of 33 bits keeps 2^-32 turns.
+double2 turns_of(double f) {
+    const double p = f * kInvTwoPi, e = std::fma(f, kInvTwoPiLow, std::fma(f, kInvTwoPi, -p));
+    const double r = p - std::rint(p), x = r + e, ee = x - r;  // r exactly; x + y = r + e exactly
+    return make_double2(x, (r - (x - ee)) + (e - ee));
+}
 
 // Copies n frequencies to the device, in turns per position, under a new handle.
 int add_rope(enchip_ctx *ctx, const double *freqs, int64_t n, double mscale, enchip_rope *out) {
-    double turns[enchip::ROPE_MAX_PAIRS];
+    double2 turns[enchip::ROPE_MAX_PAIRS];
     for (int64_t j = 0; j < n; ++j) {
         if (!std::isfinite(freqs[j])) return fail(ctx, ENCHIP_ERR_ARG, "rope: frequency %lld is not finite", (long long)j);
-        turns[j] = freqs[j] / kTwoPi;
+        if (std::fabs(freqs[j]) > kMaxFreq)
+            return fail(ctx, ENCHIP_ERR_ARG, "rope: frequency %lld is %g, past 2^40", (long long)j, freqs[j]);
+        turns[j] = turns_of(freqs[j]);
     }
     if (!std::isfinite(mscale) || !std::isfinite((float)mscale))
         return fail(ctx, ENCHIP_ERR_ARG, "rope: mscale %g is not a finite f32", mscale);
@@ -2503,8 +2515,8 @@ int add_rope(enchip_ctx *ctx, const double *freqs, int64_t n, double mscale, enc
     r.n = n;
     r.mscale = (float)mscale;
     size_t cap = 0;
-    if (int rc = ensure(ctx, &r.d_turns, &cap, (size_t)n * sizeof(double), false)) return rc;
-    const hipError_t e = hipMemcpy(r.d_turns, turns, (size_t)n * sizeof(double), hipMemcpyHostToDevice);
+    if (int rc = ensure(ctx, &r.d_turns, &cap, (size_t)n * sizeof(double2), false)) return rc;
+    const hipError_t e = hipMemcpy(r.d_turns, turns, (size_t)n * sizeof(double2), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         (void)hipFree(r.d_turns);
         return fail(ctx, ENCHIP_ERR_HIP, "rope upload: %s", hipGetErrorString(e));

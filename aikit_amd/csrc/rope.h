@@ -5,9 +5,11 @@
 // the pair being elements (j, j + r/2) of the head (half) or (2j, 2j + 1) (interleaved);
 // elements r .. head_dim pass through.
 //
-// The angle is formed in turns, p f_j / 2 pi, in 64 bits and reduced there (a far position times
-// a frequency keeps no fraction in 32), sine and cosine of the reduced angle in 32: an error of
-// about 2^-23 of the pair's length at any position. The pairs' angles are those of every head of
+// The angle is formed in turns and reduced in 64 bits (a far position times a frequency keeps no fraction in
+// 32): f_j / 2 pi less whole turns is held in two parts, and the product with p is exact (a multiplication
+// and what it rounded off) but for 2^-32 turns at the largest frequencies, 2^40. Sine and cosine of the
+// reduced angle in 32 bits: with the products' rounding under 2^-21 m (|x1| + |x2|) at any position, where f_j / 2 pi in
+// one part left 2^-51 |p f_j| more. The pairs' angles are those of every head of
 // the row, so a workgroup computes them once for its rows into LDS and then streams the rows.
 //
 // Bound by memory: 8 bytes an element. 64 x 512 tokens of 24 heads of 64 (403 MB) take 79 us on MI355X,
@@ -55,7 +57,7 @@ __device__ __forceinline__ void rope_store(const float *v, float *p) {
 // its size: the launch chooses them so.
 template <bool INTERLEAVED, int V, int RV>
 __global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, float *y, int64_t ldy,
-                                                 const double *__restrict__ turns, float mscale,
+                                                 const double2 *__restrict__ turns, float mscale,
                                                  const int32_t *__restrict__ pos, int64_t pos0, int64_t row0, int L,
                                                  int64_t rows, int TR, FastDiv heads, FastDiv ipr, int hd, int r) {
     __shared__ float2 cs[ROPE_CS];
@@ -68,9 +70,10 @@ __global__ __launch_bounds__(256) void rope_rows(const float *x, int64_t ldx, fl
     for (int t = threadIdx.x; t < tr * np; t += 256) {
         const int row = t / np, j = t - row * np;
         const double p = pos ? (double)pos[first + row] : (double)(pos0 + (row0 + first + row) % L);
-        const double a = p * turns[j];
+        const double2 f = turns[j];
+        const double a = p * f.x, e = __builtin_fma(p, f.y, __builtin_fma(p, f.x, -a));
         float s, c;
-        sincospif(2.0f * (float)(a - rint(a)), &s, &c);
+        sincospif(2.0f * (float)(a - rint(a) + e), &s, &c);
         cs[t] = make_float2(c * mscale, s * mscale);
     }
     __syncthreads();

@@ -501,8 +501,8 @@ int enchip_ann_topk_stats(enchip_ctx *ctx, int64_t *fused, int64_t *fallbacks);
  * factor mscale of the rotated values. enchip_rope_rows_dev turns pair j of every head of the
  * row at position p by the angle p f_j:
  *   y1 = mscale (x1 cos - x2 sin),  y2 = mscale (x2 cos + x1 sin).
- * The angle is formed and reduced in 64 bits, so a far position is as exact as a near one
- * (about 2^-22 of the pair's length). The reference's rotary encoders keep a table in f32
+ * The angle of the 64-bit f_j is reduced before it is rounded, so a far position is as exact as a
+ * near one: an element is within 2^-21 |mscale| (|x1| + |x2|) of the formula. The reference's rotary encoders keep a table in f32
  * (encoder's NomicBERT forward); parity with its table's last bits is not pinned. */
 typedef uint64_t enchip_rope; /* opaque handle; 0 is never a valid handle */
 
@@ -522,7 +522,8 @@ enum enchip_rope_scaling {
                                that do not turn once are divided; mscale = 0.1 ln(factor) + 1 */
 };
 
-/* rot_dim even, 2 .. 1024; base > 0; factor >= 1; orig_len >= 1 (YARN). */
+/* rot_dim even, 2 .. 1024; base > 0; factor >= 1; orig_len >= 1 (YARN). A frequency is at most 2^40 radians per
+ * position, here (a base far below 1) as in enchip_rope_create_freqs. */
 int enchip_rope_create(enchip_ctx *ctx, int64_t rot_dim, double base, int scaling, double factor,
                        int64_t orig_len, enchip_rope *out);
 
