@@ -2552,6 +2552,8 @@ int enchip_rope_create(enchip_ctx *ctx, int64_t rot_dim, double base, int scalin
     const double r = (double)rot_dim;
     double b = base, mscale = 1.0;
     if (scaling == ENCHIP_ROPE_NTK && rot_dim > 2) b = base * std::pow(factor, r / (r - 2.0));
+    if (!std::isfinite(b))
+        return fail(ctx, ENCHIP_ERR_ARG, "rope_create: base %g stretched %g times is past 64 bits", base, factor);
     if (scaling == ENCHIP_ROPE_YARN) mscale = 0.1 * std::log(factor) + 1.0;
     double f[enchip::ROPE_MAX_PAIRS];
     for (int64_t j = 0; j < rot_dim / 2; ++j) {

@@ -523,7 +523,7 @@ enum enchip_rope_scaling {
 };
 
 /* rot_dim even, 2 .. 1024; base > 0; factor >= 1; orig_len >= 1 (YARN). A frequency is at most 2^40 radians per
- * position, here (a base far below 1) as in enchip_rope_create_freqs. */
+ * position, here (a base far below 1) as in enchip_rope_create_freqs; NTK's stretched base is finite. */
 int enchip_rope_create(enchip_ctx *ctx, int64_t rot_dim, double base, int scaling, double factor,
                        int64_t orig_len, enchip_rope *out);
 

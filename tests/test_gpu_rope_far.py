@@ -100,3 +100,13 @@ def test_frequencies_past_the_range_are_refused(ctx):
     with pytest.raises(enchip.EnchipError) as e:
         ctx.rope(64, base=1e-200)  # frequencies up to 1e194
     assert e.value.code == enchip.ERR_ARG
+
+def test_stretched_bases_past_64_bits_are_refused(ctx):
+    # base factor^(r / (r - 2)) is infinite: every frequency but the first would be 0
+    with pytest.raises(enchip.EnchipError) as e:
+        ctx.rope(64, base=1e300, scaling=enchip.ROPE_NTK, factor=1e30)
+    assert e.value.code == enchip.ERR_ARG
+    with pytest.raises(enchip.EnchipError) as e:
+        ctx.rope(4, base=1e4, scaling=enchip.ROPE_NTK, factor=1e200)
+    assert e.value.code == enchip.ERR_ARG
+    ctx.release_rope(ctx.rope(64, base=1e300, scaling=enchip.ROPE_NTK, factor=1e6))
