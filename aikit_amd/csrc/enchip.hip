@@ -2677,9 +2677,9 @@ WoArgs wo_args(const Weight4 &a, const Weight4 &b) {
 
 // The rows that gemv_wo takes; more are split first (split_rows) and run on the f16 MFMA. A pass over the
 // weights takes four rows, the split a launch. Measured on MI355X, us, gemv_wo against the split: 4 bits, K =
-// 1024, N = 4096 (2 MiB) 8 rows 5.4, 16 rows 7.9 and 8.6; gated, 4 MiB, 9 rows 9.4 and 9.9, 16 rows 11.1
-// and 9.9; K = N = 4096 (8 MiB) 8 rows 11.7 and 13.3; gated, 16 MiB, 8 rows 18.1 and 17.1; 8192 x 8192 (32 MiB) 4
-// rows 18.2 (8 in two passes), the split's 5 to 16 rows 22.2.
+// 1024, N = 4096 (2 MiB) 16 rows 7.9, 17 rows 8.8 by the split; gated, 4 MiB, 9 rows 9.3 and 9.9, 16 rows 11.1
+// and 9.9; K = N = 4096 (8 MiB) 8 rows 11.8, 9 rows 15.8 and 13.7; gated, 16 MiB, 8 rows 18.3 and 18.1, 16 rows
+// 29.6 and 17.9; 8192 x 8192 (32 MiB) 4 rows 17.8, 8 rows 27.7 (two passes) and 22.7, 16 rows 51 and 22.6.
 int64_t few_rows(int64_t weight_bytes) {
     return weight_bytes < ((int64_t)4 << 20) ? 16 : weight_bytes < ((int64_t)16 << 20) ? 8 : 4;
 }
@@ -2746,7 +2746,9 @@ int launch_wo_split(enchip_ctx *c, const WoArgs &p, const float *A, int64_t lda,
         // 32 or 64 rows with K over two groups of wavefronts, and without. Measured on MI355X, us, gated
         // int8, K = 4096, N = 4096: 128 rows 33 (4 wavefronts) against 43 (32-row tiles), 256 rows 56
         // and 50, 512 rows 99, 88, 69 (64-row tiles, two groups) and 73 (one), 1024 rows 129 and 126;
-        // 4 bits, one weight: 256 rows 38 and 47, 512 rows 62, 52 and 74 (one group), 1024 rows 88 and 82.
+        // 4 bits, one weight: 256 rows 38 and 47, 512 rows 62, 52 and 74 (one group), 1024 rows 88 and 82 (the
+        // codes of lo's own, later, add 1 to 4% to each). Other N leave some rounds of workgroups partly
+        // empty: gated, 512 x 2304 runs 144 of them.
         if (pieces <= cus) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, G2, 8, 2>), 1, 1, 512);
         else if (pieces <= (GATED ? 2 : 4) * cus) WO_SPLIT((gemm_wo_piece<BITS, GATED, 1, 2, 4, 2>), 1, 2 / G2, 256);
         else if (pieces <= (GATED ? 4 : 15) * cus) {
@@ -2933,7 +2935,9 @@ void launch_gated_pieces(const Weight &w, const int8_t *aq, const float *as, con
 // worth and wherever the persistent tiles cannot go, else those. Measured on MI355X, us, with the
 // quantization: K = 768, N = 2304, 64 rows 7.9 (32 x 32) and 8.6 (64 x 32), 128 rows 9.8 and 8.9, 256
 // rows 12.2 and 11.3 (tiles 13.3), 512 rows 14.8 (64 x 32) and 13.6 (tiles), 4096 rows 55, 48 and 32; K =
-// 4096, N = 4096, 256 rows 46, 29 and 33, 4096 rows 584, 306 and 143.
+// 4096, N = 4096, 256 rows 46, 29 and 33, 4096 rows 584, 306 and 143. The tiles refuse an odd number of 64-deep
+// stages and N % 4 != 0, which costs many rows up to half of their rate: K = 1024, N = 4096 4096 rows 53 and 32768
+// rows 351, K = 1088 113 and 780, N = 4098 112 and 819.
 template <int ACT>
 void launch_gated_frag(enchip_ctx *c, const Weight &w, const int8_t *aq, const float *as, const enchip::GatePair &p,
                        int64_t M, float *out, hipStream_t s) {

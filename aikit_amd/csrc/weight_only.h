@@ -271,9 +271,10 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 //
 // Two parts take two thirds of the MFMAs of three exact bf16 parts, made in every tile that reads the row:
 // those took 57.9 us for 512 rows of K = N = 4096 in 4 bits where this takes 50, 436 where it takes 273
-// for 4096. lo's own codes cost 1 to 4% of that (a packed multiplication for two of them). A row costs 8 bytes an element, read and written once: MI355X 4096 x 4096 36 us (3.8 TB/s), 512 x
-// 1024 3.0 to 4.3 us and 32 x 4096 3.7 (a launch and one pass through a row). Neighbouring rows, whose 16-byte
-// pieces share lines, run on one die: 4096 x 8192 84 us, on different ones 131.
+// for 4096. lo's own codes cost 1 to 5% of that (a packed multiplication for two of them). A row costs 8 bytes an
+// element, read and written once: MI355X 4096 x 4096 30 to 35 us (4 TB/s), 512 x 1024 3.1 to 4.1 us and 32 x
+// 4096 3.7 (a launch and one pass through a row). Neighbouring rows, whose 16-byte pieces share lines, run on one
+// die: 4096 x 8192 84 us, on different ones 131.
 struct SplitRows {
     const char *parts;
     const float2 *scale;   // [M] the row's power of two, negative for a row with marks, and the one that takes it back
@@ -656,10 +657,11 @@ __global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, 
 // straight into registers, PW stages ahead, and are widened one stage ahead. FP: chunks of a 4-bit
 // weight that share a scale (its group is a multiple of 32 FP): their sum is added once, scaled.
 //
-// MI355X, K = N = 4096, us: 4 bits 512 rows 44, 4096 rows 252 to 298 (275 GFLOP of f16 MFMA work, 194 at 1.42
-// PFLOP/s); gated int8 512 rows 64, 4096 rows 460 to 523 (387); gated 4 bits 4096 rows 502 to 571. Bound by
-// the MFMA together with the widening and scaling (8 vector instructions per MFMA at TM 1), which a SIMD's second
-// wavefront covers in part, and at 512 rows by few tiles a CU: 512 x 4096, K = 1024 14 us, 4 of them MFMA.
+// MI355X, K = N = 4096, us, least to median: 4 bits 512 rows 45 to 46, 4096 rows 264 to 292 (275 GFLOP of f16 MFMA
+// work, 194 at 1.42 PFLOP/s); gated int8 512 rows 64 to 65, 4096 rows 479 to 530 (387); gated 4 bits 4096 rows 521
+// to 571. Bound by the MFMA together with the widening and scaling (9 vector instructions per MFMA at TM 1), which a
+// SIMD's second wavefront covers in part, and at 512 rows by few tiles a CU: 512 x 4096, K = 1024 14.6 us, 4 of them
+// MFMA.
 template <int BITS, bool GATED, int TM, int NT, int KS, int PW, int FP>
 __global__ __launch_bounds__(256 * KS, 2) void gemm_wo_tile(WoRows p, WoWeight w0, WoWeight w1,
                                                                  const float *__restrict__ b0, const float *__restrict__ b1,

@@ -468,13 +468,14 @@ class Context:
     # -- rotary positions ---------------------------------------------------------
     def rope(self, rot_dim: int, base: float = 10000.0, scaling: int = ROPE_NONE, factor: float = 1.0,
              orig_len: int = 0) -> Rope:
-        """Frequencies base^(-2j / rot_dim), stretched as enchip_rope_scaling says."""
+        """Frequencies base^(-2j / rot_dim), stretched as enchip_rope_scaling says (ROPE_YARN ramps over a
+        pair's turns within orig_len; a checkpoint trained with another ramp needs rope_from_freqs)."""
         out = _u64()
         self._check(self._lib.enchip_rope_create(self._h, rot_dim, base, scaling, factor, orig_len, ctypes.byref(out)))
         return Rope(out.value, rot_dim)
 
     def rope_from_freqs(self, freqs, mscale: float = 1.0) -> Rope:
-        """The caller's own frequencies (radians per position, one per pair)."""
+        """The caller's own frequencies (radians per position, one per pair, at most 2^40)."""
         f = np.ascontiguousarray(freqs, dtype=np.float64)
         if f.ndim != 1:
             raise ValueError(f"freqs shape {f.shape} is not one-dimensional")

@@ -519,7 +519,12 @@ enum enchip_rope_scaling {
     ENCHIP_ROPE_NTK = 2,    /* base factor^(rot_dim / (rot_dim - 2)) in place of base (rot_dim > 2) */
     ENCHIP_ROPE_YARN = 3    /* f_j (w + (1 - w) / factor), w = clamp((orig_len f_j / 2 pi - 1) / 31, 0, 1):
                                pairs that turn over 32 times within orig_len keep their frequency, those
-                               that do not turn once are divided; mscale = 0.1 ln(factor) + 1 */
+                               that do not turn once are divided; mscale = 0.1 ln(factor) + 1. The ramp
+                               is over turns. A checkpoint whose configuration asks for "yarn" may have
+                               been trained with a ramp over the pair's number between two bounds, with
+                               other bounds than 1 and 32, or another mscale: its middle frequencies
+                               differ (up to 3 times); make them as its code does and hand them to
+                               enchip_rope_create_freqs */
 };
 
 /* rot_dim even, 2 .. 1024; base > 0; factor >= 1; orig_len >= 1 (YARN). A frequency is at most 2^40 radians per
@@ -578,8 +583,9 @@ int enchip_matmul_bt_q4_dev(enchip_ctx *ctx, enchip_weight w, const float *d_a, 
  * The first half of a gated feed-forward block (encoder/forward_q8.go:264-279 swigluMLPQ8, up to
  * the down projection), both projections, the activation and the product in one call:
  *   dst[m][n] = act(yg[m][n]) * yu[m][n],  y = a . W^T (+ bias[n], nullable).
- * act: ENCHIP_ACT_SILU (x / (1 + e^-x)) or ENCHIP_ACT_GELU (x Phi(x), within 0.75e-7 |x| and
- * rounding; not linalg.GELUF32's bits). Both weights have one shape (and group), K > 0, N <= 2^24;
+ * act: ENCHIP_ACT_SILU (x / (1 + e^-x), within 4 ulp where that is above 2^-100) or ENCHIP_ACT_GELU
+ * (x Phi(x), within 0.75e-7 |x| and rounding: the far negative tail, under 1e-7, is not held to
+ * relative precision; not linalg.GELUF32's bits). x = -infinity gives NaN. Both weights have one shape (and group), K > 0, N <= 2^24;
  * the same handle may be both. dst holds no element of a or of a bias.
  *   gated_q8    int8 weights (no infinite scale), f32 activations: enchip_matmul_bt_q8's product, its
  *               activations and sums held as enchip_matmul_bt_q4 says (few rows in f32, more in two f16
