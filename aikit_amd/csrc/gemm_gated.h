@@ -234,9 +234,9 @@ __global__ __launch_bounds__(256, 2) void gated_w8a8_piece(const int8_t *__restr
 // Many rows: gemm_w8a8_pt's main loop (gemm_persistent.h) with a wavefront's two 32-channel blocks
 // taken one from each weight, so a workgroup's tile is BM rows x 128 output channels and an output's
 // two accumulators meet in the wavefront that holds both. MI355X, 32768 rows, K = 1024, N = 4096, SiLU: 320 us
-// the least and 372 to 397 the median of 24 launches (the clock gives way under it), the products
+// the least and 372 to 409 the median of 24 launches (the clock gives way under it), the products
 // (0.55 POP) and the writing of 537 MB one after the other: 1024 more of K add 235 us, and
-// without its stores it takes 100 less. K = N = 4096, 4096 rows 131 us the least (2.1 POP/s), 146 the median. Where
+// without its stores it takes 100 less. K = N = 4096, 4096 rows 129 us the least (2.1 POP/s), 136 to 146 the median. Where
 // it took 337 us, row segments of 512 bytes through LDS took 349, plain stores, 64-row tiles three a CU and
 // panels of 4 or 16 columns 354 to 361; panels of 8 in place of none took medians from 437 to 411. Preconditions as
 // there (an even number of 64-deep stages, 32-bit offsets, N % 4 == 0, 16-byte aligned rows of out,

@@ -67,12 +67,18 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // step there is 1), less 1024 and the code's offset. Conversions to f32 take four times a plain
 // operation's issue; these take one each for two codes.
 __device__ __forceinline__ void widen8_q4(uint32_t w, f16x2 (&h)[4]) {
-    uint32_t mask = 0x000f000fu, base = 0x64006400u;
-    asm("" : "+s"(mask));  // kept in registers: one v_and_or each
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, base = 0x64006400u;
+    asm("" : "+s"(low), "+s"(high));  // kept in registers: one v_and_or each
     asm("" : "+v"(base));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & mask) | base) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t v = w >> (8 * i);
+        h[2 * i] = __builtin_bit_cast(f16x2, (v & low) | base) - f16x2{(_Float16)1032.0f, (_Float16)1032.0f};
+        // four bits up a code counts 16: (1024 + 16 c) / 16 - 72, exactly, for a shift less
+        h[2 * i + 1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (v & high) | base),
+                                                 f16x2{(_Float16)0.0625f, (_Float16)0.0625f},
+                                                 f16x2{(_Float16)-72.0f, (_Float16)-72.0f});
+    }
 }
 __device__ __forceinline__ void widen8_q8(uint32_t w0, uint32_t w1, f16x2 (&h)[4]) {
     const uint32_t w[2] = {w0 ^ 0x80808080u, w1 ^ 0x80808080u};
@@ -262,7 +268,7 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 // codes / 2^12, which lo is multiplied with: products are exact and two MFMAs stand for one in f32. Where hi is
 // subnormal (under 2^-14 scaled, 2^-28 to 2^-29 of the row's largest) it has fewer bits: a row's block of 128 k
 // with such an activation is marked: its parts are 0, and the products add it on the f32 MFMA at their end. MI355X,
-// 4 bits, 4096 rows of K = N = 4096: 279 us for normal activations, 281 behind a GELU, 325 with one of 1000 a
+// 4 bits, 4096 rows of K = N = 4096: 280 us for normal activations, 281 behind a GELU, 334 with one of 1000 a
 // thousand times larger, 2230 where every block is marked (softmax rows).
 //
 // Parts, in the A operand's order for the weights' order of k: [M/32][Ka/32] x 4 KiB, plane x and
@@ -270,8 +276,8 @@ __global__ __launch_bounds__(64 * WO_WAVES) void gemv_wo(const float *__restrict
 // .. + 7. Ka = K rounded up to 128, zero past K. Rows past M are not written (and no output is theirs).
 //
 // Two parts take two thirds of the MFMAs of three exact bf16 parts, made in every tile that reads the row:
-// those took 57.9 us for 512 rows of K = N = 4096 in 4 bits where this takes 50, 436 where it takes 273
-// for 4096. lo's own codes cost 1 to 5% of that (a packed multiplication for two of them). A row costs 8 bytes an
+// those took 57.9 us for 512 rows of K = N = 4096 in 4 bits where this takes 50 to 53, 436 where it takes 272
+// to 280 for 4096. lo's own codes cost 1 to 3% of that (a packed multiplication for two of them). A row costs 8 bytes an
 // element, read and written once: MI355X 4096 x 4096 30 to 35 us (4 TB/s), 512 x 1024 3.1 to 4.1 us and 32 x
 // 4096 3.7 (a launch and one pass through a row). Neighbouring rows, whose 16-byte pieces share lines, run on one
 // die: 4096 x 8192 84 us, on different ones 131.
@@ -657,9 +663,9 @@ __global__ __launch_bounds__(64 * NW) void gemm_wo_piece(WoRows p, WoWeight w0, 
 // straight into registers, PW stages ahead, and are widened one stage ahead. FP: chunks of a 4-bit
 // weight that share a scale (its group is a multiple of 32 FP): their sum is added once, scaled.
 //
-// MI355X, K = N = 4096, us, least to median: 4 bits 512 rows 45 to 46, 4096 rows 264 to 292 (275 GFLOP of f16 MFMA
-// work, 194 at 1.42 PFLOP/s); gated int8 512 rows 64 to 65, 4096 rows 479 to 530 (387); gated 4 bits 4096 rows 521
-// to 571. Bound by the MFMA together with the widening and scaling (9 vector instructions per MFMA at TM 1), which a
+// MI355X, K = N = 4096, us, least to median: 4 bits 512 rows 45, 4096 rows 258 to 294 (275 GFLOP of f16 MFMA
+// work, 194 at 1.42 PFLOP/s); gated int8 512 rows 64 to 66, 4096 rows 472 to 543 (387); gated 4 bits 4096 rows 511
+// to 566. Bound by the MFMA together with the widening and scaling (8 vector instructions per MFMA at TM 1), which a
 // SIMD's second wavefront covers in part, and at 512 rows by few tiles a CU: 512 x 4096, K = 1024 14.6 us, 4 of them
 // MFMA.
 template <int BITS, bool GATED, int TM, int NT, int KS, int PW, int FP>
