@@ -1,7 +1,7 @@
 """Build recipe for libenchip.so (gfx950) -- used by __graft_entry__.build().
 
-One translation unit, compiled by hipcc for gfx950 only, linked as a plain C-ABI
-shared library next to this file. Flags that matter for correctness:
+Two translation units, compiled side by side by hipcc for gfx950 only and linked as a plain
+C-ABI shared library next to this file. Flags that matter for correctness:
 
 * ``-ffp-contract=off`` -- the epilogue must round after every multiply and add,
   as aikit's Go amd64 arithmetic does (no FMA contraction).
@@ -15,10 +15,11 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, "csrc", "enchip.hip")
+SRCS = [os.path.join(HERE, "csrc", n) for n in ("enchip.hip", "attention_block.hip")]
 OUT = os.path.join(HERE, "libenchip.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
@@ -27,7 +28,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-ffp-contract=off",
     "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -43,18 +43,34 @@ def hipcc() -> str:
 def build(verbose: bool = False) -> str:
     """Compile libenchip.so in-tree; returns its path. Always recompiles."""
     tmp = OUT + ".tmp"
-    cmd = [hipcc(), *HIPCC_FLAGS,
-           "-I", os.path.join(ROOT, "include"), "-I", os.path.join(HERE, "csrc"),
-           SRC, "-o", tmp, f"-Wl,-rpath,{ROCM}/lib"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    noise = "'-packed-fp32-ops' is not a recognized feature"
-    err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)
-    if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{err}")
-    if verbose and err.strip():
-        print(err)
+    inc = ["-I", os.path.join(ROOT, "include"), "-I", os.path.join(HERE, "csrc")]
+
+    def check(cmd, proc):
+        _, text = proc.communicate()
+        noise = "'-packed-fp32-ops' is not a recognized feature"
+        err = "\n".join(l for l in text.splitlines() if noise not in l)
+        if proc.returncode != 0:
+            raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{' '.join(cmd)}\n{err}")
+        if verbose and err.strip():
+            print(err)
+
+    def start(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        return cmd, subprocess.Popen(cmd, stdout=subprocess.DEVNULL, stderr=subprocess.PIPE, text=True)
+
+    with tempfile.TemporaryDirectory(prefix="enchip_build_") as d:
+        objs = [os.path.join(d, os.path.basename(src) + ".o") for src in SRCS]
+        running = [start([hipcc(), *HIPCC_FLAGS, *inc, "-c", src, "-o", o]) for src, o in zip(SRCS, objs)]
+        try:
+            for cmd, proc in running:
+                check(cmd, proc)
+        finally:
+            for _, proc in running:
+                if proc.poll() is None:
+                    proc.kill()
+                    proc.wait()
+        check(*start([hipcc(), *HIPCC_FLAGS, "-shared", *objs, "-o", tmp, f"-Wl,-rpath,{ROCM}/lib"]))
     os.replace(tmp, OUT)
     return OUT
 

@@ -1,0 +1,287 @@
+// attention_bias.h -- attention with a learned relative position bias, over spans of rows.
+//
+// For query row i and key row j of one span, head h (key head h / (heads / kv_heads)):
+//   out_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = e^(scale q_i . k_j + b[j - i][h]),
+// b by distance, clamped to reach rows either way. A span is [start, end) of the buffers' rows; rows of no
+// span are neither read nor written. A query all of whose biases are -infinity gets zeros.
+//
+// The products, the split of operands into two f16 parts and the online softmax are attention_flash.h's:
+// one workgroup takes 32 NW queries of one head and walks its keys in tiles of FA_KT, S^T = K Q^T and
+// O^T = V^T P^T on v_mfma_f32_32x32x16_f16, three products per pair. The bias joins in base 2,
+// y = fma(s, scale log2 e, b log2 e): the window of a tile's 32 NW + 63 distances is staged in LDS beside
+// its keys, and a lane reads its 16 from it (its queries are consecutive, so neighbouring lanes read
+// neighbouring words).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attention_flash.h"
+
+#pragma clang fp contract(off)
+
+namespace enchip {
+
+struct AttnBias {
+    const float *q, *k, *v;
+    float *out;
+    int64_t ldq, ldk, ldv, ldo;
+    const int2 *spans;   // [nseq] start, end of ascending spans; null: nseq sequences of L rows
+    const float *table;  // [heads][2 reach + 1], b log2 e of distance -reach .. reach; null: no bias
+    int nseq, heads, group, reach;
+    int blocks;  // with spans: query blocks of a head, L / (32 NW) + nseq
+    int L;       // rows of a sequence, or with spans those of the buffers
+    float scale;
+};
+
+template <int HD, int NW>
+struct AbLayout {
+    using Fa = FaLayout<HD>;
+    static constexpr int WINDOW = 32 * NW + FA_KT;  // distances of a tile (one to spare)
+    static constexpr int BIAS = 2 * Fa::STAGE;      // two windows behind the two stages
+    static constexpr int BYTES = BIAS + 2 * WINDOW * 4;
+};
+
+// The workgroup's rows: false where it has none. Of ascending spans, span z has the query blocks
+// start / QB + z .. of the launch, at least as many as it needs; the last span whose first block is at or
+// below b is found 64 at a time. (Spans out of order leave queries out; nothing is read past the buffers.)
+template <int QB>
+__device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int64_t &row0, int &len, int &q0) {
+    if (p.spans == nullptr) {
+        const int nqb = (p.L + QB - 1) / QB, z = b / nqb;
+        row0 = (int64_t)z * p.L, len = p.L, q0 = (b - z * nqb) * QB;
+        return true;
+    }
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = p.nseq;
+    for (;;) {
+        const int step = (n + 63) / 64, z = lo + lane * step;
+        const bool in = lane * step < n && max(p.spans[min(z, p.nseq - 1)].x, 0) / QB + z <= b;
+        const int below = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
+        if (below == 0) return false;
+        n = min(step, n - (below - 1) * step);
+        lo += (below - 1) * step;
+        if (step == 1) break;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int2 s = p.spans[lo];
+    const int start = min(max(s.x, 0), p.L), end = min(max(s.y, start), p.L);
+    const int64_t at = (int64_t)(b - (start / QB + lo)) * QB;
+    if (at < 0 || at >= end - start) return false;
+    row0 = start, len = end - start, q0 = (int)at;
+    return true;
+}
+
+// A 1-D grid of heads * query blocks, XCD-aware (a sequence's query blocks of one head on one XCD),
+// AbLayout<HD, NW>::BYTES of dynamic LDS. q, k, v 16-byte aligned, their pitches multiples of 4 and at most
+// INT32_MAX / FA_KT; VEC: ldo a multiple of 4 and out 16-byte aligned.
+template <int HD, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
+    using Fa = FaLayout<HD>;
+    using Lay = AbLayout<HD, NW>;
+    constexpr int NT = 64 * NW, QB = 32 * NW;
+    constexpr int NB = HD / 16, NOT = HD / 32;
+    constexpr int KCH = FA_KT * HD / 8, VCH = (FA_KT / 2) * HD / 4;
+    constexpr int KPT = (KCH + NT - 1) / NT, VPT = (VCH + NT - 1) / NT;
+    using Ops = SplitOps<true>;
+    using vec8 = typename Ops::vec8;
+    extern __shared__ __attribute__((aligned(16))) char ab_lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, hf = lane >> 5;
+    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_head = gridDim.x / p.heads;
+    const int head = logical / per_head;
+    int64_t row0;
+    int L, q0;
+    if (!ab_rows<QB>(p, logical - head * per_head, row0, L, q0)) return;
+    const int qw = q0 + 32 * wave;
+    const bool active = qw < L;
+    const int nt = (L + FA_KT - 1) / FA_KT;
+    const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
+    const float *vbase = p.v + row0 * p.ldv + (head / p.group) * HD;
+    const float *table = p.table ? p.table + (int64_t)head * (2 * p.reach + 1) + p.reach : nullptr;
+    const float c = p.scale * FA_LOG2E;
+
+    vec8 qh[NB], ql[NB];
+    float qt[NB][8];
+    {
+        const float *qrow = p.q + (row0 + min(qw + r, L - 1)) * p.ldq + head * HD;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) load8(qrow + 16 * b + 8 * hf, qt[b]);
+    }
+    f32x4 kr[KPT][2], vr[VPT][2];
+    float br = 0.0f;
+    const int ldk = (int)p.ldk, ldv = (int)p.ldv;
+    auto load_tile = [&](int t) {
+        const int kb0 = t * FA_KT, klast = L - 1 - kb0;
+        const float *kt = kbase + (int64_t)kb0 * ldk, *vt = vbase + (int64_t)kb0 * ldv;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int ch = tid + NT * i;
+            if (ch < KCH) {
+                const float *at = kt + (min(ch / (HD / 8), klast) * ldk + (ch % (HD / 8)) * 8);
+                kr[i][0] = *reinterpret_cast<const f32x4 *>(at);
+                kr[i][1] = *reinterpret_cast<const f32x4 *>(at + 4);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int ch = tid + NT * i;
+            if (ch < VCH) {
+                const int pr = ch / (HD / 4), col = (ch % (HD / 4)) * 4;
+                vr[i][0] = *reinterpret_cast<const f32x4 *>(vt + (min(2 * pr, klast) * ldv + col));
+                vr[i][1] = *reinterpret_cast<const f32x4 *>(vt + (min(2 * pr + 1, klast) * ldv + col));
+            }
+        }
+        // word w of the window: key kb0 + kk, query q0 + qi, w = kk - qi + QB - 1
+        if (table != nullptr && tid < Lay::WINDOW) {
+            const int d = kb0 - q0 - (QB - 1) + tid;
+            br = table[min(max(d, -p.reach), p.reach)];
+        }
+    };
+    static_assert(Lay::WINDOW <= NT, "a word of the window a thread");
+    auto store_tile = [&](int s) {
+        char *khi = ab_lds + s * Fa::STAGE, *klo = khi + Fa::KPLANE;
+        char *vhi = klo + Fa::KPLANE, *vlo = vhi + Fa::VPLANE;
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int ch = tid + NT * i;
+            if (ch < KCH) {
+                const int key = ch / (HD / 8), col = (ch % (HD / 8)) * 8;
+                const float x[8] = {kr[i][0].x, kr[i][0].y, kr[i][0].z, kr[i][0].w,
+                                    kr[i][1].x, kr[i][1].y, kr[i][1].z, kr[i][1].w};
+                vec8 h, l;
+                Ops::split8(x, h, l);
+                *reinterpret_cast<vec8 *>(khi + key * Fa::KP + 2 * col) = h;
+                *reinterpret_cast<vec8 *>(klo + key * Fa::KP + 2 * col) = l;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int ch = tid + NT * i;
+            if (ch < VCH) {
+                const int pr = ch / (HD / 4), col = (ch % (HD / 4)) * 4;
+                const int kk = 2 * pr, pos = (kk & ~15) | fa_perm16(kk & 15);
+                const float a[4] = {vr[i][0].x, vr[i][0].y, vr[i][0].z, vr[i][0].w};
+                const float b[4] = {vr[i][1].x, vr[i][1].y, vr[i][1].z, vr[i][1].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t hw, lw;
+                    Ops::pair(a[j], b[j], hw, lw);
+                    const int vo = (col + j) * Fa::VP + ((2 * pos) ^ fa_vswz(col + j));
+                    *reinterpret_cast<uint32_t *>(vhi + vo) = hw;
+                    *reinterpret_cast<uint32_t *>(vlo + vo) = lw;
+                }
+            }
+        }
+        if (tid < Lay::WINDOW) reinterpret_cast<float *>(ab_lds + Lay::BIAS)[s * Lay::WINDOW + tid] = br;
+    };
+
+    f32x16 o[NOT];
+#pragma unroll
+    for (int i = 0; i < NOT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    load_tile(0);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) Ops::split8(qt[b], qh[b], ql[b]);
+    store_tile(0);
+    lds_barrier();
+    for (int t = 0; t < nt; ++t) {
+        if (t + 1 < nt) load_tile(t + 1);
+        if (active) {
+            const char *khi = ab_lds + (t & 1) * Fa::STAGE, *klo = khi + Fa::KPLANE;
+            const char *vhi = klo + Fa::KPLANE, *vlo = vhi + Fa::VPLANE;
+            const float *window = reinterpret_cast<const float *>(ab_lds + Lay::BIAS) + (t & 1) * Lay::WINDOW;
+#pragma unroll
+            for (int s = 0; s < FA_KT / 32; ++s) {
+                const int key0 = t * FA_KT + 32 * s;
+                if (key0 >= L) break;  // uniform: no barrier inside
+                f32x16 acc;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const int off = (32 * s + r) * Fa::KP + 2 * (16 * b + 8 * hf);
+                    const vec8 kh = *reinterpret_cast<const vec8 *>(khi + off);
+                    const vec8 kl = *reinterpret_cast<const vec8 *>(klo + off);
+                    acc = mfma_split3(kh, kl, qh[b], ql[b], acc);
+                }
+                // y = c s + b in base 2; element e is key key0 + 4 hf + 8 (e / 4) + e % 4
+                const float *bw = window + (32 * s + 4 * hf - (32 * wave + r) + QB - 1);
+                float x[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(acc[e], c, bw[8 * (e >> 2) + (e & 3)]);
+                const int lim = L - key0 - 4 * hf;
+                if (__builtin_expect(key0 + 32 > L, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (8 * (e >> 2) + (e & 3) >= lim) x[e] = -INFINITY;
+                }
+                float mloc = x[0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, x[e]);
+                {
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
+                    mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+                }
+                const float m_new = fmaxf(m_run, mloc);
+                const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // nothing attended so far: every p is 0
+                const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+                float psum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - m_use);
+                    psum += x[e];
+                }
+                l_run = l_run * alpha + psum;
+                m_run = m_new;
+#pragma unroll
+                for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+                vec8 ph[2], pl[2];
+                Ops::split8(x, ph[0], pl[0]);
+                Ops::split8(x + 8, ph[1], pl[1]);
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int i = 0; i < NOT; ++i) {
+                        const int off = (32 * i + r) * Fa::VP + 64 * s + 32 * (kb ^ (i & 1)) + 16 * (hf ^ (r >> 4));
+                        const vec8 vh = *reinterpret_cast<const vec8 *>(vhi + off);
+                        const vec8 vl = *reinterpret_cast<const vec8 *>(vlo + off);
+                        o[i] = mfma_split3(vh, vl, ph[kb], pl[kb], o[i]);
+                    }
+                }
+                __builtin_amdgcn_s_setprio(0);
+            }
+        }
+        if (t + 1 < nt) store_tile((t + 1) & 1);
+        lds_barrier();
+    }
+
+    if (!active) return;
+    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+    if (qw + r >= L) return;
+    float *orow = p.out + (row0 + qw + r) * p.ldo + head * HD;
+#pragma unroll
+    for (int i = 0; i < NOT; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * i + 8 * g + 4 * hf;
+            const f32x4 val = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
+            if (VEC) {
+                *reinterpret_cast<f32x4 *>(orow + col) = val;
+            } else {
+                orow[col] = val.x;
+                orow[col + 1] = val.y;
+                orow[col + 2] = val.z;
+                orow[col + 3] = val.w;
+            }
+        }
+}
+
+}  // namespace enchip

@@ -1,0 +1,512 @@
+// attention_block.hip -- entry points of what stands in an encoder's attention block beside the linears of
+// enchip.hip: head norms with rotation, attention with a relative position bias, low-rank adapters.
+#include "context.h"
+
+#include "adapters.h"
+#include "attention_bias.h"
+#include "head_norm.h"
+
+using namespace enchip_host;
+
+extern "C" {
+
+// ---------------------------------------------------------------------------- head norms
+
+int enchip_head_norm_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, const float *d_x, int64_t ldx, float *d_y,
+                                   int64_t ldy, int64_t nseq, int64_t L, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                   const float *d_q_gain, const float *d_k_gain, double eps, const int32_t *d_pos, int64_t pos0,
+                                   void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Rope r;
+    if (h != 0) {
+        auto it = ctx->ropes.find(h);
+        if (it == ctx->ropes.end()) return fail(ctx, ENCHIP_ERR_HANDLE, "unknown rope handle %llu", (unsigned long long)h);
+        r = it->second;
+        if (layout != ENCHIP_ROPE_HALF && layout != ENCHIP_ROPE_INTERLEAVED)
+            return fail(ctx, ENCHIP_ERR_ARG, "head_norm: bad layout %d", layout);
+        if (!d_pos && (pos0 < -((int64_t)1 << 31) || pos0 > ((int64_t)1 << 31)))
+            return fail(ctx, ENCHIP_ERR_ARG, "head_norm: pos0=%lld past 32 bits", (long long)pos0);
+    } else {
+        d_pos = nullptr;
+        pos0 = 0;
+        layout = ENCHIP_ROPE_HALF;
+    }
+    const int64_t max_hd = 2 * enchip::ROPE_MAX_PAIRS;
+    if (nseq < 0 || L < 0 || q_heads < 0 || k_heads < 0 || q_heads > 65536 || k_heads > 65536 - q_heads || head_dim < 1 ||
+        head_dim < 2 * r.n || head_dim > max_hd || (q_heads + k_heads) * head_dim > ((int64_t)1 << 20) || nseq > INT32_MAX ||
+        L > INT32_MAX || nseq * L > INT32_MAX || ldx < (q_heads + k_heads) * head_dim || ldy < (q_heads + k_heads) * head_dim)
+        return fail(ctx, ENCHIP_ERR_ARG,
+                    "head_norm: bad shape nseq=%lld L=%lld q_heads=%lld k_heads=%lld head_dim=%lld (%lld rotated, at most %lld) "
+                    "ldx=%lld ldy=%lld",
+                    (long long)nseq, (long long)L, (long long)q_heads, (long long)k_heads, (long long)head_dim,
+                    (long long)(2 * r.n), (long long)max_hd, (long long)ldx, (long long)ldy);
+    if (!(eps >= 0x1p-100 && eps <= 0x1p100)) return fail(ctx, ENCHIP_ERR_ARG, "head_norm: eps %g is not from 2^-100 to 2^100", eps);
+    if (d_x == d_y && ldx != ldy)
+        return fail(ctx, ENCHIP_ERR_ARG, "head_norm: in place needs one pitch, not %lld and %lld", (long long)ldx, (long long)ldy);
+    const int64_t heads = q_heads + k_heads, rows = nseq * L;
+    if (rows == 0 || heads == 0) return ENCHIP_OK;
+    if (!d_x || !d_y || (q_heads > 0 && !d_q_gain) || (k_heads > 0 && !d_k_gain))
+        return fail(ctx, ENCHIP_ERR_ARG, "head_norm: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    const bool inter = layout == ENCHIP_ROPE_INTERLEAVED;
+    const int64_t rot = 2 * r.n;
+    // elements that an access holds: whole parts of a slot, aligned (rope.h's 16 bytes against 4: a third of the time)
+    auto fits = [&](int64_t n) {
+        return (inter ? rot % (2 * n) == 0 : r.n % n == 0) && head_dim % n == 0 && ldx % n == 0 && ldy % n == 0 &&
+               (uintptr_t)d_x % (4 * n) == 0 && (uintptr_t)d_y % (4 * n) == 0;
+    };
+    const int v = fits(4) ? 4 : fits(2) ? 2 : 1;
+    enchip::HeadNorm p;
+    p.gain_q = d_q_gain ? d_q_gain : d_k_gain;
+    p.gain_k = d_k_gain ? d_k_gain : d_q_gain;
+    p.eps = eps;
+    p.inv_hd = 1.0 / (double)head_dim;
+    p.q_heads = (int)q_heads;
+    p.hd = (int)head_dim;
+    p.r = (int)rot;
+    p.turned = (int)(r.n / v);
+    p.slots = p.turned + (int)((head_dim - rot + 2 * v - 1) / (2 * v));
+    p.lanes = 1;
+    while (p.lanes < 64 && p.lanes < p.slots) p.lanes *= 2;
+    const int need = (p.slots + p.lanes - 1) / p.lanes, it = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
+    // rows of a workgroup: three passes of its lanes, while a few workgroups a CU are left
+    const int64_t pass = 256 / p.lanes * (it >= 4 ? 1 : 4 / it);
+    const int64_t by_items = std::max<int64_t>(1, 3 * pass / heads), by_rows = std::max<int64_t>(1, rows / (4 * ctx->num_cus));
+    const int64_t by_angles = r.n ? (int64_t)enchip::ROPE_CS / r.n : 64;
+    const int tr = (int)std::min({by_items, by_rows, by_angles, (int64_t)64});
+    for (int64_t r0 = 0; r0 < rows; r0 += kRowChunk) {
+        const int64_t n = std::min(kRowChunk, rows - r0);
+#define HN_CALL(I, V, IT)                                                                                                   \
+    hipLaunchKernelGGL((enchip::head_norm_rope<I, V, IT>), dim3((unsigned)((n + tr - 1) / tr)), dim3(256), 0, s, d_x + r0 * ldx, \
+                       ldx, d_y + r0 * ldy, ldy, p, r.d_turns, r.mscale, d_pos ? d_pos + r0 : nullptr, pos0, r0, (int)L, n, tr, \
+                       fast_div(heads))
+#define HN_V(I)                                     \
+    do {                                            \
+        if (v == 4 && it == 1) HN_CALL(I, 4, 1);    \
+        else if (v == 4) HN_CALL(I, 4, 2);          \
+        else if (v == 2 && it == 1) HN_CALL(I, 2, 1); \
+        else if (v == 2 && it == 2) HN_CALL(I, 2, 2); \
+        else if (v == 2) HN_CALL(I, 2, 4);          \
+        else if (it == 1) HN_CALL(I, 1, 1);         \
+        else if (it == 2) HN_CALL(I, 1, 2);         \
+        else if (it == 4) HN_CALL(I, 1, 4);         \
+        else HN_CALL(I, 1, 8);                      \
+    } while (0)
+        if (inter) HN_V(true);
+        else HN_V(false);
+#undef HN_V
+#undef HN_CALL
+    }
+    return check_launch(ctx, "head_norm_rope");
+}
+
+// ---------------------------------------------------------------------------- relative position bias
+
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t kMaxReach = (int64_t)1 << 20;
+
+// Expands table[buckets][heads] over the distances -reach .. reach (bucket(d) within [0, buckets)) into a handle.
+template <typename F>
+int add_relpos(enchip_ctx *ctx, const float *table, int64_t buckets, int64_t heads, int64_t reach, F bucket, enchip_relpos *out) {
+    for (int64_t i = 0; i < buckets * heads; ++i)
+        if (!(table[i] <= 0x1p100f) || (table[i] < -0x1p100f && !std::isinf(table[i])))
+            return fail(ctx, ENCHIP_ERR_ARG, "relpos: value %g of bucket %lld, head %lld is neither -infinity nor within 2^100 of 0",
+                        (double)table[i], (long long)(i / heads), (long long)(i % heads));
+    const int64_t width = 2 * reach + 1;
+    std::vector<float> all;
+    try {
+        all.resize((size_t)(heads * width));
+    } catch (const std::exception &) {
+        return fail(ctx, ENCHIP_ERR_OOM, "relpos: out of host memory");
+    }
+    for (int64_t d = -reach; d <= reach; ++d) {
+        const float *row = table + bucket(d) * heads;
+        for (int64_t i = 0; i < heads; ++i) all[(size_t)(i * width + d + reach)] = (float)((double)row[i] * 1.4426950408889634074);
+    }
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    RelPos r;
+    r.heads = heads;
+    r.reach = reach;
+    size_t cap = 0;
+    if (int rc = ensure(ctx, &r.d_table, &cap, all.size() * sizeof(float), false)) return rc;
+    const hipError_t e = hipMemcpy(r.d_table, all.data(), all.size() * sizeof(float), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        (void)hipFree(r.d_table);
+        return fail(ctx, ENCHIP_ERR_HIP, "relpos upload: %s", hipGetErrorString(e));
+    }
+    try {
+        ctx->relpos[ctx->next_handle] = r;
+    } catch (const std::bad_alloc &) {
+        (void)hipFree(r.d_table);
+        return fail(ctx, ENCHIP_ERR_OOM, "relpos: out of host memory");
+    }
+    *out = ctx->next_handle++;
+    return ENCHIP_OK;
+}
+
+int check_relpos(enchip_ctx *ctx, const float *table, int64_t buckets, int64_t heads, int64_t reach, enchip_relpos *out) {
+    if (!out) return fail(ctx, ENCHIP_ERR_ARG, "relpos: out is NULL");
+    *out = 0;
+    if (buckets < 1 || buckets > ((int64_t)1 << 22) || heads < 1 || heads > 65535 || reach < 0 || reach > kMaxReach ||
+        heads * (2 * reach + 1) > ((int64_t)1 << 28))
+        return fail(ctx, ENCHIP_ERR_ARG, "relpos: bad shape buckets=%lld heads=%lld reach=%lld", (long long)buckets,
+                    (long long)heads, (long long)reach);
+    if (!table) return fail(ctx, ENCHIP_ERR_ARG, "relpos: null pointer");
+    return ENCHIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int enchip_relpos_create(enchip_ctx *ctx, const float *table, int64_t buckets, int64_t heads, int64_t max_distance,
+                         enchip_relpos *out) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (int rc = check_relpos(ctx, table, buckets, heads, max_distance, out)) return rc;
+    const int64_t half = buckets / 2, exact = half / 2;
+    if (buckets % 2 != 0 || buckets < 4 || max_distance <= exact)
+        return fail(ctx, ENCHIP_ERR_ARG, "relpos: %lld buckets (even, at least 4) up to distance %lld (past %lld)",
+                    (long long)buckets, (long long)max_distance, (long long)exact);
+    const double per = (double)(half - exact) / std::log((double)max_distance / (double)exact);
+    return add_relpos(ctx, table, buckets, heads, max_distance, [&](int64_t d) {
+        const int64_t n = d < 0 ? -d : d;
+        int64_t b = n;
+        if (n >= exact)
+            b = std::min<int64_t>(half - 1, exact + (int64_t)std::floor(std::log((double)n / (double)exact) * per + 1e-9));
+        return d > 0 ? half + b : b;
+    }, out);
+}
+
+int enchip_relpos_create_map(enchip_ctx *ctx, const float *table, int64_t buckets, int64_t heads, const int32_t *bucket_of,
+                             int64_t reach, enchip_relpos *out) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (int rc = check_relpos(ctx, table, buckets, heads, reach, out)) return rc;
+    if (!bucket_of) return fail(ctx, ENCHIP_ERR_ARG, "relpos: null pointer");
+    for (int64_t i = 0; i <= 2 * reach; ++i)
+        if (bucket_of[i] < 0 || bucket_of[i] >= buckets)
+            return fail(ctx, ENCHIP_ERR_ARG, "relpos: distance %lld has bucket %d of %lld", (long long)(i - reach), bucket_of[i],
+                        (long long)buckets);
+    return add_relpos(ctx, table, buckets, heads, reach, [&](int64_t d) { return (int64_t)bucket_of[d + reach]; }, out);
+}
+
+int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos h) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    auto it = ctx->relpos.find(h);
+    if (it == ctx->relpos.end()) return fail(ctx, ENCHIP_ERR_HANDLE, "unknown relpos handle %llu", (unsigned long long)h);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    (void)hipFree(it->second.d_table);
+    ctx->relpos.erase(it);
+    return ENCHIP_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+template <int HD, int NW, bool VEC>
+int launch_attention_bias(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
+    using Lay = enchip::AbLayout<HD, NW>;
+    constexpr int QB = 32 * NW;
+    const void *fn = reinterpret_cast<const void *>(enchip::attention_bias<HD, NW, VEC>);
+    const std::pair<const void *, size_t> key(fn, (size_t)Lay::BYTES);
+    if (std::find(ctx->lds_set.begin(), ctx->lds_set.end(), key) == ctx->lds_set.end()) {
+        HIP_TRY(ctx, hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Lay::BYTES));
+        ctx->lds_set.push_back(key);
+    }
+    // sequences of one launch: its threads are numbered in 32 bits
+    const int64_t per = p.spans ? (int64_t)p.L / QB + p.nseq : ((int64_t)p.L + QB - 1) / QB;
+    const int64_t most = (((int64_t)1 << 32) - 1) / (64 * NW) / p.heads;
+    if (per > most)
+        return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: %lld query blocks of %d heads are more than one launch holds",
+                    (long long)per, p.heads);
+    if (p.spans) {
+        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, VEC>), dim3((unsigned)(per * p.heads)), dim3(64 * NW), Lay::BYTES, s, p);
+        return check_launch(ctx, "attention_bias");
+    }
+    const int64_t chunk = most / per, nseq = p.nseq;
+    for (int64_t z0 = 0; z0 < nseq; z0 += chunk) {
+        const int64_t nz = std::min(chunk, nseq - z0);
+        enchip::AttnBias c = p;
+        c.q += z0 * p.L * p.ldq, c.k += z0 * p.L * p.ldk, c.v += z0 * p.L * p.ldv, c.out += z0 * p.L * p.ldo;
+        c.nseq = (int)nz;
+        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, VEC>), dim3((unsigned)(per * nz * p.heads)), dim3(64 * NW), Lay::BYTES, s, c);
+    }
+    return check_launch(ctx, "attention_bias");
+}
+
+}  // namespace
+
+extern "C" {
+
+int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float *d_q, int64_t ldq, const float *d_k, int64_t ldk,
+                              const float *d_v, int64_t ldv, float *d_out, int64_t ldo, const int32_t *d_spans, int64_t nseq,
+                              int64_t L, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    RelPos r;
+    if (relpos != 0) {
+        auto it = ctx->relpos.find(relpos);
+        if (it == ctx->relpos.end()) return fail(ctx, ENCHIP_ERR_HANDLE, "unknown relpos handle %llu", (unsigned long long)relpos);
+        r = it->second;
+    }
+    if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+        return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: head_dim must be 32, 64 or 128, got %lld", (long long)head_dim);
+    const int64_t max_ld = INT32_MAX / enchip::FA_KT;
+    if (nseq < 0 || L < 0 || L > ((int64_t)1 << 30) || heads < 0 || heads > 65535 || kv_heads < 0 || (heads > 0 && kv_heads < 1) ||
+        (kv_heads > 0 && heads % kv_heads != 0) || nseq > (d_spans ? (int64_t)1 << 22 : (int64_t)1 << 31) ||
+        (!d_spans && nseq * L > ((int64_t)1 << 31)) || ldq < heads * head_dim || ldo < heads * head_dim ||
+        ldk < kv_heads * head_dim || ldv < kv_heads * head_dim || ldq % 4 || ldk % 4 || ldv % 4 || ldq > max_ld || ldk > max_ld ||
+        ldv > max_ld)
+        return fail(ctx, ENCHIP_ERR_ARG,
+                    "attention_bias: bad shape nseq=%lld L=%lld heads=%lld kv_heads=%lld ldq=%lld ldk=%lld ldv=%lld ldo=%lld "
+                    "(kv_heads dividing heads; ldq, ldk, ldv multiples of 4 covering the heads, below 2^25)",
+                    (long long)nseq, (long long)L, (long long)heads, (long long)kv_heads, (long long)ldq, (long long)ldk,
+                    (long long)ldv, (long long)ldo);
+    if (relpos != 0 && r.heads != heads)
+        return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: a bias of %lld heads for %lld", (long long)r.heads, (long long)heads);
+    if (nseq == 0 || L == 0 || heads == 0) return ENCHIP_OK;
+    if (!d_q || !d_k || !d_v || !d_out) return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: null pointer");
+    if ((uintptr_t)d_q % 16 || (uintptr_t)d_k % 16 || (uintptr_t)d_v % 16 || (uintptr_t)d_spans % 8)
+        return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: q, k and v must be 16-byte aligned, spans 8-byte aligned");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    enchip::AttnBias p;
+    p.q = d_q, p.k = d_k, p.v = d_v, p.out = d_out;
+    p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldo = ldo;
+    p.spans = reinterpret_cast<const int2 *>(d_spans);
+    p.table = r.d_table;
+    p.nseq = (int)nseq, p.heads = (int)heads, p.group = (int)(heads / kv_heads), p.reach = (int)r.reach;
+    p.L = (int)L;
+    p.scale = scale;
+    const bool vec = ldo % 4 == 0 && (uintptr_t)d_out % 16 == 0;
+#define AB_CALL(HD) return vec ? launch_attention_bias<HD, 8, true>(ctx, p, s) : launch_attention_bias<HD, 8, false>(ctx, p, s)
+    if (head_dim == 32) AB_CALL(32);
+    if (head_dim == 64) AB_CALL(64);
+    AB_CALL(128);
+#undef AB_CALL
+}
+
+// ---------------------------------------------------------------------------- low-rank adapters
+
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t kMaxAdapterBytes = (int64_t)1 << 36;
+
+uint16_t bf16_of(float x) {
+    uint32_t u;
+    std::memcpy(&u, &x, 4);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+float f32_of(uint16_t b) {
+    const uint32_t u = (uint32_t)b << 16;
+    float x;
+    std::memcpy(&x, &u, 4);
+    return x;
+}
+
+// Writes x's three parts at p[0], p[plane], p[2 plane].
+void store_parts(float x, uint16_t *p, int64_t plane) {
+    for (int u = 0; u < 3; ++u) {
+        p[u * plane] = bf16_of(x);
+        x -= f32_of(p[u * plane]);
+    }
+}
+
+int find_adapters(enchip_ctx *c, enchip_adapters h, AdapterSet **out) {
+    auto it = c->adapters.find(h);
+    if (it == c->adapters.end()) return fail(c, ENCHIP_ERR_HANDLE, "unknown adapters handle %llu", (unsigned long long)h);
+    *out = &it->second;
+    return ENCHIP_OK;
+}
+
+int64_t a_bytes(const AdapterSet &s) { return s.kb * s.rt * 3 * 1024; }  // of a slot
+int64_t b_bytes(const AdapterSet &s) { return s.nb * s.rt * 3 * 1024; }
+
+// dst = act(y + adapters), chunk after chunk of rows (32-bit thread numbers of a launch). Arguments checked.
+int run_adapters(enchip_ctx *c, const AdapterSet &set, const float *d_a, int64_t lda, int64_t M, const int32_t *d_ids,
+                 const float *d_y, int64_t ldy, int act, float *d_dst, int64_t ldd, hipStream_t s) {
+    const int64_t panels = (set.N + 127) / 128;
+    const int64_t chunk = std::min(kRowChunk, std::max<int64_t>(1, ((int64_t)1 << 23) / panels) * 32);
+    const int64_t low = (std::min(M, chunk) + 31) / 32 * set.rt * 3 * 1024;
+    int rc;
+    if ((rc = ensure(c, &c->d_low, &c->low_cap, (size_t)low))) return rc;
+    if ((rc = scratch_wait(c, s))) return rc;
+    enchip::Adapters p;
+    p.a = reinterpret_cast<const enchip::bf16x8 *>(set.d_a);
+    p.b = reinterpret_cast<const enchip::bf16x8 *>(set.d_b);
+    p.t = reinterpret_cast<enchip::bf16x8 *>(c->d_low);
+    p.slots = (int)set.slots, p.kb = (int)set.kb, p.nb = (int)set.nb, p.rt = (int)set.rt;
+    const bool vec = lda % 4 == 0 && set.K % 4 == 0 && (uintptr_t)d_a % 16 == 0;
+    for (int64_t r0 = 0; r0 < M; r0 += chunk) {
+        const int64_t n = std::min(chunk, M - r0);
+        p.ids = d_ids + r0;
+        const dim3 down((unsigned)((n + enchip::AD_ROWS - 1) / enchip::AD_ROWS)), up((unsigned)((n + 31) / 32 * panels));
+        if (vec)
+            hipLaunchKernelGGL(enchip::adapter_down<true>, down, dim3(64 * enchip::AD_WAVES), 0, s, d_a + r0 * lda, lda, n, (int)set.K, p);
+        else
+            hipLaunchKernelGGL(enchip::adapter_down<false>, down, dim3(64 * enchip::AD_WAVES), 0, s, d_a + r0 * lda, lda, n, (int)set.K, p);
+        if (act == ENCHIP_ACT_GELU)
+            hipLaunchKernelGGL(enchip::adapter_up<true>, up, dim3(256), 0, s, d_y + r0 * ldy, ldy, d_dst + r0 * ldd, ldd, n, (int)set.N, p,
+                               (int)panels);
+        else
+            hipLaunchKernelGGL(enchip::adapter_up<false>, up, dim3(256), 0, s, d_y + r0 * ldy, ldy, d_dst + r0 * ldd, ldd, n, (int)set.N, p,
+                               (int)panels);
+    }
+    if ((rc = check_launch(c, "adapters"))) return rc;
+    return scratch_record(c, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int enchip_adapters_create(enchip_ctx *ctx, int64_t K, int64_t N, int64_t rank, int64_t slots, enchip_adapters *out) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (!out) return fail(ctx, ENCHIP_ERR_ARG, "adapters_create: out is NULL");
+    *out = 0;
+    if (K < 1 || K > kMaxK || N < 1 || N > ((int64_t)1 << 24) || rank < 1 || rank > 256 || slots < 1 || slots > 65536)
+        return fail(ctx, ENCHIP_ERR_ARG, "adapters_create: bad shape K=%lld N=%lld rank=%lld slots=%lld", (long long)K, (long long)N,
+                    (long long)rank, (long long)slots);
+    AdapterSet set;
+    set.K = K, set.N = N, set.rank = rank, set.slots = slots;
+    set.kb = (K + 31) / 32, set.nb = round_up(N, 256) / 32, set.rt = (rank + 15) / 16;
+    // a block of A is 32 k x 16 ranks, one of B 32 columns x 16 ranks: 1 KiB a part each
+    const int64_t na = slots * a_bytes(set), nb = slots * b_bytes(set);
+    if (na + nb > kMaxAdapterBytes)
+        return fail(ctx, ENCHIP_ERR_ARG, "adapters_create: %lld slots of K=%lld N=%lld rank=%lld are past 2^36 bytes", (long long)slots,
+                    (long long)K, (long long)N, (long long)rank);
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    size_t cap = 0;
+    if (int rc = ensure(ctx, &set.d_a, &cap, (size_t)na, false)) return rc;
+    cap = 0;
+    if (int rc = ensure(ctx, &set.d_b, &cap, (size_t)nb, false)) {
+        (void)hipFree(set.d_a);
+        return rc;
+    }
+    hipError_t e = hipMemsetAsync(set.d_a, 0, (size_t)na, ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(set.d_b, 0, (size_t)nb, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    int rc = e == hipSuccess ? ENCHIP_OK : fail(ctx, ENCHIP_ERR_HIP, "adapters_create: %s", hipGetErrorString(e));
+    if (!rc) {
+        try {
+            ctx->adapters[ctx->next_handle] = set;
+        } catch (const std::bad_alloc &) {
+            rc = fail(ctx, ENCHIP_ERR_OOM, "adapters_create: out of host memory");
+        }
+    }
+    if (rc) {
+        (void)hipFree(set.d_a);
+        (void)hipFree(set.d_b);
+        return rc;
+    }
+    *out = ctx->next_handle++;
+    return ENCHIP_OK;
+}
+
+int enchip_adapters_set(enchip_ctx *ctx, enchip_adapters h, int64_t slot, const float *A, const float *B, float scale) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    AdapterSet *set;
+    int rc = find_adapters(ctx, h, &set);
+    if (rc) return rc;
+    if (slot < 0 || slot >= set->slots) return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: slot %lld of %lld", (long long)slot, (long long)set->slots);
+    if (!A || !B) return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: null pointer");
+    const int64_t K = set->K, N = set->N, R = set->rank, rt = set->rt;
+    std::vector<uint16_t> a, b;
+    try {
+        a.resize((size_t)a_bytes(*set) / 2);
+        b.resize((size_t)b_bytes(*set) / 2);
+    } catch (const std::exception &) {
+        return fail(ctx, ENCHIP_ERR_OOM, "adapters_set: out of host memory");
+    }
+    for (int64_t j = 0; j < R; ++j)
+        for (int64_t k = 0; k < K; ++k) {
+            const float x = A[j * K + k];
+            if (!(std::fabs(x) < 0x1p127f))
+                return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: A[%lld][%lld] is %g", (long long)j, (long long)k, (double)x);
+            const int64_t block = (k / 32 * rt + j / 16) * 3, lane = j % 16 + 16 * (k % 32 / 8);
+            store_parts(x, &a[(size_t)((block * 64 + lane) * 8 + k % 8)], 512);
+        }
+    for (int64_t n = 0; n < N; ++n)
+        for (int64_t j = 0; j < R; ++j) {
+            const float x = (float)((double)scale * (double)B[n * R + j]);
+            if (!(std::fabs(x) < 0x1p127f))
+                return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: scale %g times B[%lld][%lld] is %g", (double)scale, (long long)n,
+                            (long long)j, (double)x);
+            const int64_t block = (n / 32 * rt + j / 16) * 3, lane = n % 32 + 32 * (j % 16 / 8);
+            store_parts(x, &b[(size_t)((block * 64 + lane) * 8 + j % 8)], 512);
+        }
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    HIP_TRY(ctx, hipMemcpy(set->d_a + slot * a_bytes(*set), a.data(), (size_t)a_bytes(*set), hipMemcpyHostToDevice));
+    HIP_TRY(ctx, hipMemcpy(set->d_b + slot * b_bytes(*set), b.data(), (size_t)b_bytes(*set), hipMemcpyHostToDevice));
+    return ENCHIP_OK;
+}
+
+int enchip_adapters_release(enchip_ctx *ctx, enchip_adapters h) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    AdapterSet *set;
+    int rc = find_adapters(ctx, h, &set);
+    if (rc) return rc;
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    (void)hipFree(set->d_a);
+    (void)hipFree(set->d_b);
+    ctx->adapters.erase(h);
+    return ENCHIP_OK;
+}
+
+int enchip_adapters_add_dev(enchip_ctx *ctx, enchip_adapters h, const float *d_a, int64_t lda, int64_t M, const int32_t *d_ids,
+                            const float *d_y, int64_t ldy, float *d_dst, int64_t ldd, void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    AdapterSet *set;
+    int rc = find_adapters(ctx, h, &set);
+    if (rc) return rc;
+    if (M < 0 || M > ((int64_t)1 << 30) || lda < set->K || ldy < set->N || ldd < set->N)
+        return fail(ctx, ENCHIP_ERR_ARG, "adapters_add: bad shape M=%lld lda=%lld ldy=%lld ldd=%lld for K=%lld N=%lld", (long long)M,
+                    (long long)lda, (long long)ldy, (long long)ldd, (long long)set->K, (long long)set->N);
+    if (d_y == d_dst && ldy != ldd)
+        return fail(ctx, ENCHIP_ERR_ARG, "adapters_add: in place needs one pitch, not %lld and %lld", (long long)ldy, (long long)ldd);
+    if (M == 0) return ENCHIP_OK;
+    if (!d_a || !d_ids || !d_y || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "adapters_add: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    return run_adapters(ctx, *set, d_a, lda, M, d_ids, d_y, ldy, ENCHIP_ACT_NONE, d_dst, ldd, s);
+}
+
+int enchip_w8a8_linear_adapters_dev(enchip_ctx *ctx, enchip_weight hw, enchip_adapters h, const float *d_a, int64_t M,
+                                    const int32_t *d_ids, const float *d_bias, int act, float *d_dst, void *stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Weight *w;
+    AdapterSet *set;
+    int rc = find_weight(ctx, hw, &w);
+    if (rc || (rc = find_adapters(ctx, h, &set))) return rc;
+    if (set->K != w->K || set->N != w->N)
+        return fail(ctx, ENCHIP_ERR_ARG, "linear_adapters: adapters of K=%lld N=%lld for a weight of K=%lld N=%lld", (long long)set->K,
+                    (long long)set->N, (long long)w->K, (long long)w->N);
+    if (M < 0 || M > ((int64_t)1 << 30)) return fail(ctx, ENCHIP_ERR_ARG, "linear_adapters: bad M=%lld", (long long)M);
+    if (act != ENCHIP_ACT_NONE && act != ENCHIP_ACT_GELU) return fail(ctx, ENCHIP_ERR_ARG, "linear_adapters: bad act %d", act);
+    if (M == 0) return ENCHIP_OK;
+    if (!d_a || !d_ids || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "linear_adapters: null pointer");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+    if ((rc = run_linear(ctx, *w, d_a, M, d_bias, ENCHIP_ACT_NONE, d_dst, s))) return rc;
+    return run_adapters(ctx, *set, d_a, w->K, M, d_ids, d_dst, w->N, act, d_dst, w->N, s);
+}
+
+}  // extern "C"

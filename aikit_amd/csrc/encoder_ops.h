@@ -421,11 +421,19 @@ __global__ __launch_bounds__(256) void embed_rows(const int32_t *__restrict__ id
 //   64 x 512 x 768: pooling 31 -> 15.6 us (6.4 TB/s), norm 15 -> 7.6
 constexpr int POOL_COLS = 64;
 
-__global__ __launch_bounds__(POOL_COLS) void pool_mean_cols(const float *__restrict__ h, int64_t ldh, int L, int D,
-                                                            float *__restrict__ out, int64_t ldo) {
+// spans: sequence z is rows spans[z].x .. spans[z].y - 1 of the L rows of h; null: rows z*L .. of L each.
+[[maybe_unused]] static __global__ __launch_bounds__(POOL_COLS) void pool_mean_cols(const float *__restrict__ h, int64_t ldh, int L, int D,
+                                                            const int2 *__restrict__ spans, float *__restrict__ out,
+                                                            int64_t ldo) {
     const int j = blockIdx.x * POOL_COLS + threadIdx.x;
     if (j >= D) return;
-    const float *col = h + (int64_t)blockIdx.y * L * ldh + j;
+    int64_t row0 = (int64_t)blockIdx.y * L;
+    if (spans != nullptr) {
+        const int2 s = spans[blockIdx.y];
+        row0 = min(max(s.x, 0), L);
+        L = max(min(s.y, L) - (int)row0, 0);
+    }
+    const float *col = h + row0 * ldh + j;
     double acc = 0.0;
     int i = 0;
     auto rows = [&](auto u_c, auto whole) {  // U loads in flight, then the adds in row order
@@ -446,7 +454,7 @@ __global__ __launch_bounds__(POOL_COLS) void pool_mean_cols(const float *__restr
     out[blockIdx.y * ldo + j] = L > 0 ? (float)(acc * (1.0 / (double)L)) : 0.0f;
 }
 
-__global__ __launch_bounds__(256) void l2_normalize_rows(float *__restrict__ out, int64_t ldo, int D) {
+[[maybe_unused]] static __global__ __launch_bounds__(256) void l2_normalize_rows(float *__restrict__ out, int64_t ldo, int D) {
     constexpr int U = 16;
     __shared__ __attribute__((aligned(16))) double sqs[4096 + U];
     __shared__ double norm_s;

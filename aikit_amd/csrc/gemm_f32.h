@@ -604,7 +604,7 @@ __global__ __launch_bounds__(256, 2) void gemm_f32_ksplit(const float *__restric
 }
 
 // C = 0 for a K = 0 product (the empty dot product), grid (ceil(M*N/256), inner, outer).
-__global__ __launch_bounds__(256) void fill_zero_f32(float *__restrict__ C, int64_t ldc, int64_t sc1, int64_t sc2,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void fill_zero_f32(float *__restrict__ C, int64_t ldc, int64_t sc1, int64_t sc2,
                                                      int M, int N) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)M * N) return;

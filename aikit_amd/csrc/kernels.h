@@ -498,7 +498,7 @@ __global__ __launch_bounds__(256) void quant_rows_frag_any(const float *__restri
 }
 
 // Row-major codes of any K and alignment: one wavefront per row, two passes over the row.
-__global__ __launch_bounds__(256) void quant_rows_scalar(const float *__restrict__ a, int8_t *__restrict__ q, int64_t ldq,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void quant_rows_scalar(const float *__restrict__ a, int8_t *__restrict__ q, int64_t ldq,
                                                          float *__restrict__ scale, int64_t M, int64_t K) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -927,7 +927,7 @@ __global__ __launch_bounds__(64 * GVW_WAVES) void gemv_w8a8_wide(
 // 168 us on MI355X (37 GB/s; 8 to 32 blocks alike, 64 slower).
 constexpr int COPY_OUT_BLOCKS = 16;
 
-__global__ __launch_bounds__(256) void copy_out(const char *__restrict__ src, char *__restrict__ dst, int bytes, int slice,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void copy_out(const char *__restrict__ src, char *__restrict__ dst, int bytes, int slice,
                                                 uint32_t *__restrict__ words, uint32_t epoch) {
     for (int b = 0, i = 0; b < bytes; b += slice, ++i) {
         const int e = min(b + slice, bytes), e16 = e & ~15;

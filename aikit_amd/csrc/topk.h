@@ -319,7 +319,7 @@ __device__ void top_small_k(const uint64_t (&key)[EPT], int k, uint64_t *out, ui
 // 0 for none; topk_thresh_radix), a chunk first lists its keys at or above the row's key
 // and stops there when they are at most k (they are then its only keys that can be among
 // the row's k largest), as topk_chunk_wide does.
-__global__ __launch_bounds__(256) void topk_chunk(const float *__restrict__ scores, int64_t ld, int64_t n, int k,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_chunk(const float *__restrict__ scores, int64_t ld, int64_t n, int k,
                                                   int nchunks, uint64_t *__restrict__ cand, int chunk0,
                                                   const uint64_t *__restrict__ thr) {
     constexpr int EPT = TOPK_CHUNK / 256;
@@ -402,7 +402,7 @@ __device__ __forceinline__ float topk_key_score(uint64_t key) {
     return __uint_as_float((th & 0x80000000u) ? (th & 0x7fffffffu) : ~th);
 }
 
-__global__ __launch_bounds__(256) void topk_chunk_wide(const float *__restrict__ scores, int64_t ld, int64_t n, int k,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_chunk_wide(const float *__restrict__ scores, int64_t ld, int64_t n, int k,
                                                        int nchunks, uint64_t *__restrict__ cand, int chunk0,
                                                        const uint64_t *__restrict__ thr) {
     constexpr int EPT = TOPK_WCHUNK / 256;
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(256) void topk_chunk_wide(const float *__restrict__
 // key among all their scores, a lower bound of the row's k-th largest), or 0 when those
 // chunks hold fewer than k keys. One wavefront per row; k <= TOPK_WIDE_K (the host takes
 // topk_thresh_sorted above TOPK_SORT_K).
-__global__ __launch_bounds__(256) void topk_thresh(const uint64_t *__restrict__ cand, int64_t rows, int nchunks, int k,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_thresh(const uint64_t *__restrict__ cand, int64_t rows, int nchunks, int k,
                                                    uint64_t *__restrict__ thr, unsigned *__restrict__ zero) {
     constexpr int PER_LANE = TOPK_SAMPLE_CHUNKS * TOPK_WIDE_K / 64;
     const int lane = threadIdx.x & 63;
@@ -577,7 +577,7 @@ __global__ __launch_bounds__(256) void topk_thresh(const uint64_t *__restrict__ 
 // topk_thresh for k > TOPK_SORT_K: one workgroup per row sorts the row's
 // TOPK_SAMPLE_CHUNKS * k sample keys in LDS (block_sort_desc) and takes the k-th, where k
 // dependent rounds of a wavefront maximum would cost more (k = 64: 18.8 us per 256 rows).
-__global__ __launch_bounds__(256) void topk_thresh_sorted(const uint64_t *__restrict__ cand, int nchunks, int k,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_thresh_sorted(const uint64_t *__restrict__ cand, int nchunks, int k,
                                                           uint64_t *__restrict__ thr, unsigned *__restrict__ zero) {
     __shared__ uint64_t keys[TOPK_SAMPLE_CHUNKS * TOPK_WIDE_K];
     const int64_t row = blockIdx.x;
@@ -768,7 +768,7 @@ __device__ uint64_t radix_threshold_mem(const uint64_t *__restrict__ c, int64_t 
 // The row thresholds for topk_chunk (k > TOPK_WIDE_K): the k-th largest of the keys stage 1
 // kept from each row's first TOPK_SAMPLE_CHUNKS chunks, a lower bound of the row's k-th
 // largest key, or 0 when those chunks hold at most k keys. One workgroup per row.
-__global__ __launch_bounds__(256) void topk_thresh_radix(const uint64_t *__restrict__ cand, int nchunks, int k,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_thresh_radix(const uint64_t *__restrict__ cand, int nchunks, int k,
                                                          uint64_t *__restrict__ thr) {
     __shared__ unsigned hist[256];
     __shared__ uint64_t bcast[2];
@@ -782,7 +782,7 @@ __global__ __launch_bounds__(256) void topk_thresh_radix(const uint64_t *__restr
 // power of two). The row's m = nchunks * k candidates are cand[row*m ..]. Writes
 // index[row*ldi + i] (-1 past the row's non-NaN scores) and score[row*lds_ + i] (NaN
 // there); the score is re-read from the row (scores, pitch ld) so a -0 stays -0.
-__global__ __launch_bounds__(256) void topk_merge(const uint64_t *__restrict__ cand, int64_t m, int k, int kp,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_merge(const uint64_t *__restrict__ cand, int64_t m, int k, int kp,
                                                   const float *__restrict__ scores, int64_t ld,
                                                   int32_t *__restrict__ index, int64_t ldi, float *__restrict__ score,
                                                   int64_t lds_) {
@@ -919,7 +919,7 @@ __global__ __launch_bounds__(256) void topk_merge(const uint64_t *__restrict__ c
 
 // Rows of zero scores (n == 0): index -1 and a NaN score in each of the k slots, as the
 // merge pads. Grid-stride over rows.
-__global__ __launch_bounds__(256) void topk_empty(int64_t rows, int k, int32_t *__restrict__ index, int64_t ldi,
+[[maybe_unused]] static __global__ __launch_bounds__(256) void topk_empty(int64_t rows, int k, int32_t *__restrict__ index, int64_t ldi,
                                                   float *__restrict__ score, int64_t lds_) {
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
         for (int i = threadIdx.x; i < k; i += 256) {

@@ -95,6 +95,19 @@ _SIGNATURES = {
     "enchip_gated_q4_dev": (_int, [_vp, _u64, _u64, _vp, _i64, _i64, _vp, _vp, _int, _vp, _i64, _vp]),
     "enchip_w8a8_gated": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp]),
     "enchip_w8a8_gated_dev": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp, _vp]),
+    "enchip_head_norm_rope_rows_dev": (_int, [_vp, _u64, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
+                                              _f64, _vp, _i64, _vp]),
+    "enchip_relpos_create": (_int, [_vp, _vp, _i64, _i64, _i64, ctypes.POINTER(_u64)]),
+    "enchip_relpos_create_map": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, ctypes.POINTER(_u64)]),
+    "enchip_relpos_release": (_int, [_vp, _u64]),
+    "enchip_attention_bias_dev": (_int, [_vp, _u64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                                         _i64, ctypes.c_float, _vp]),
+    "enchip_pool_mean_l2_spans_dev": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "enchip_adapters_create": (_int, [_vp, _i64, _i64, _i64, _i64, ctypes.POINTER(_u64)]),
+    "enchip_adapters_set": (_int, [_vp, _u64, _i64, _vp, _vp, ctypes.c_float]),
+    "enchip_adapters_release": (_int, [_vp, _u64]),
+    "enchip_adapters_add_dev": (_int, [_vp, _u64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "enchip_w8a8_linear_adapters_dev": (_int, [_vp, _u64, _u64, _vp, _i64, _vp, _vp, _int, _vp, _vp]),
 }
 SYMBOLS = tuple(_SIGNATURES)
 
@@ -174,6 +187,23 @@ class Rope:
     """Rotary frequencies for the first rot_dim elements of a head."""
     handle: int
     rot_dim: int
+
+
+@dataclass(frozen=True)
+class RelPos:
+    """A learned bias by relative position, for `heads` heads."""
+    handle: int
+    heads: int
+
+
+@dataclass(frozen=True)
+class Adapters:
+    """A set of low-rank adapters of linears [N, K]."""
+    handle: int
+    K: int
+    N: int
+    rank: int
+    slots: int
 
 
 class Context:
@@ -572,3 +602,84 @@ class Context:
                        d_dst: int, stream: int = 0) -> None:
         self._check(self._lib.enchip_w8a8_gated_dev(self._h, gate.handle, up.handle, d_a or None, M, d_bias_gate or None,
                                                     d_bias_up or None, act, d_dst or None, stream or None))
+
+    # -- head norms, relative position bias, low-rank adapters -------------------------
+    def head_norm_rope_rows_dev(self, r: Optional[Rope], layout: int, d_x: int, ldx: int, d_y: int, ldy: int, nseq: int, L: int,
+                                q_heads: int, k_heads: int, head_dim: int, d_q_gain: int, d_k_gain: int, eps: float,
+                                d_pos: int = 0, pos0: int = 0, stream: int = 0) -> None:
+        """RMS norms of q_heads query and k_heads key heads (d_y == d_x: in place), turned by r unless that is None."""
+        self._check(self._lib.enchip_head_norm_rope_rows_dev(self._h, 0 if r is None else r.handle, layout, d_x or None, ldx,
+                                                             d_y or None, ldy, nseq, L, q_heads, k_heads, head_dim,
+                                                             d_q_gain or None, d_k_gain or None, eps, d_pos or None, pos0,
+                                                             stream or None))
+
+    @staticmethod
+    def _bias_table(table: np.ndarray) -> np.ndarray:
+        t = np.ascontiguousarray(table, dtype=np.float32)
+        if t.ndim != 2:
+            raise ValueError(f"relative position table shape {t.shape} is not (buckets, heads)")
+        return t
+
+    def relpos(self, table: np.ndarray, max_distance: int) -> RelPos:
+        """The bias table [buckets, heads] of a bidirectional encoder, buckets by the logarithm up to max_distance."""
+        t, out = self._bias_table(table), _u64()
+        self._check(self._lib.enchip_relpos_create(self._h, _ptr(t), t.shape[0], t.shape[1], max_distance, ctypes.byref(out)))
+        return RelPos(out.value, t.shape[1])
+
+    def relpos_from_map(self, table: np.ndarray, bucket_of: np.ndarray) -> RelPos:
+        """table [buckets, heads] by the caller's own buckets of the distances -reach .. reach (2 reach + 1 of them)."""
+        t, m, out = self._bias_table(table), np.ascontiguousarray(bucket_of, dtype=np.int32), _u64()
+        if m.ndim != 1 or m.size % 2 == 0:
+            raise ValueError(f"bucket_of shape {m.shape} is not (2 reach + 1,)")
+        self._check(self._lib.enchip_relpos_create_map(self._h, _ptr(t), t.shape[0], t.shape[1], _ptr(m), m.size // 2,
+                                                       ctypes.byref(out)))
+        return RelPos(out.value, t.shape[1])
+
+    def release_relpos(self, b: RelPos) -> None:
+        self._check(self._lib.enchip_relpos_release(self._h, b.handle))
+
+    def attention_bias_dev(self, b: Optional[RelPos], d_q: int, ldq: int, d_k: int, ldk: int, d_v: int, ldv: int, d_out: int,
+                           ldo: int, nseq: int, L: int, heads: int, kv_heads: int, head_dim: int, scale: float,
+                           d_spans: int = 0, stream: int = 0) -> None:
+        """Attention with the bias b (None: none) over nseq sequences of L rows, or over the spans (int32 [nseq, 2],
+        first row and one past the last) of buffers of L rows."""
+        self._check(self._lib.enchip_attention_bias_dev(self._h, 0 if b is None else b.handle, d_q or None, ldq, d_k or None, ldk,
+                                                        d_v or None, ldv, d_out or None, ldo, d_spans or None, nseq, L, heads,
+                                                        kv_heads, head_dim, scale, stream or None))
+
+    def pool_mean_l2_spans_dev(self, d_h: int, ldh: int, rows: int, d_spans: int, nseq: int, D: int, d_out: int, ldo: int,
+                               stream: int = 0) -> None:
+        """pool_mean_l2_dev of spans of the rows."""
+        self._check(self._lib.enchip_pool_mean_l2_spans_dev(self._h, d_h or None, ldh, rows, d_spans or None, nseq, D,
+                                                            d_out or None, ldo, stream or None))
+
+    def adapters(self, K: int, N: int, rank: int, slots: int) -> Adapters:
+        """An empty set of adapters of up to `rank` for linears [N, K]."""
+        out = _u64()
+        self._check(self._lib.enchip_adapters_create(self._h, K, N, rank, slots, ctypes.byref(out)))
+        return Adapters(out.value, K, N, rank, slots)
+
+    def set_adapter(self, s: Adapters, slot: int, A: np.ndarray, B: np.ndarray, scale: float = 1.0) -> None:
+        """Slot `slot` becomes scale B A: A [r, K], B [N, r], r at most the set's rank."""
+        A, B = (np.ascontiguousarray(x, dtype=np.float32) for x in (A, B))
+        if A.ndim != 2 or not 1 <= A.shape[0] <= s.rank or A.shape[1] != s.K or B.shape != (s.N, A.shape[0]):
+            raise ValueError(f"adapter shapes {A.shape}, {B.shape} are not (r, {s.K}), ({s.N}, r) with r <= {s.rank}")
+        if A.shape[0] < s.rank:
+            A = np.concatenate([A, np.zeros((s.rank - A.shape[0], s.K), np.float32)])
+            B = np.concatenate([B, np.zeros((s.N, s.rank - B.shape[1]), np.float32)], axis=1)
+        self._check(self._lib.enchip_adapters_set(self._h, s.handle, slot, _ptr(A), _ptr(B), scale))
+
+    def release_adapters(self, s: Adapters) -> None:
+        self._check(self._lib.enchip_adapters_release(self._h, s.handle))
+
+    def adapters_add_dev(self, s: Adapters, d_a: int, lda: int, M: int, d_ids: int, d_y: int, ldy: int, d_dst: int, ldd: int,
+                         stream: int = 0) -> None:
+        """dst = y + the adapters (by row, int32 ids) of a; d_dst may be d_y."""
+        self._check(self._lib.enchip_adapters_add_dev(self._h, s.handle, d_a or None, lda, M, d_ids or None, d_y or None, ldy,
+                                                      d_dst or None, ldd, stream or None))
+
+    def linear_adapters_dev(self, w: Weight, s: Adapters, d_a: int, M: int, d_ids: int, d_bias: int, act: int, d_dst: int,
+                            stream: int = 0) -> None:
+        """linear_dev with the rows' adapters added before the activation."""
+        self._check(self._lib.enchip_w8a8_linear_adapters_dev(self._h, w.handle, s.handle, d_a or None, M, d_ids or None,
+                                                              d_bias or None, act, d_dst or None, stream or None))

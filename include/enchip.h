@@ -611,6 +611,95 @@ int enchip_w8a8_gated_dev(enchip_ctx *ctx, enchip_weight gate, enchip_weight up,
                           int64_t M, const float *d_bias_gate, const float *d_bias_up, int act,
                           float *d_dst, void *stream);
 
+/* ---- head norms ---------------------------------------------------------------------
+ * RMS norms of query and key heads, with the position rotation in the same pass. Rows and positions as
+ * enchip_rope_rows_dev has them; a row holds q_heads query heads, then k_heads key heads, of head_dim floats
+ * each (the first heads of fused [tokens, (H + 2 KV) head_dim] QKV rows). A head x becomes
+ *   n = x / sqrt(mean(x^2) + eps) * gain,  gain = d_q_gain[head_dim] or d_k_gain[head_dim],
+ * the mean over head_dim in 64 bits; then n's first rot_dim elements are turned as enchip_rope_rows_dev turns
+ * x's, and the rest stay n. rope 0: no rotation (layout, d_pos and pos0 are not read). An element is within 5 2^-23 |mscale|
+ * (|n1| + |n2|) of the formula, one that is not turned within 2^-22 |n|. A head with an infinity or a NaN has
+ * NaN there. 2^-100 <= eps <= 2^100; a gain may be NULL when its heads are 0. */
+int enchip_head_norm_rope_rows_dev(enchip_ctx *ctx, enchip_rope rope, int layout, const float *d_x, int64_t ldx,
+                                   float *d_y, int64_t ldy, int64_t nseq, int64_t L, int64_t q_heads,
+                                   int64_t k_heads, int64_t head_dim, const float *d_q_gain,
+                                   const float *d_k_gain, double eps, const int32_t *d_pos, int64_t pos0,
+                                   void *stream);
+
+/* ---- attention with a learned relative position bias ---------------------------------
+ * A bias by relative position is made once: a handle holds b[d][h] for every distance d = key row - query row
+ * and head h, from a learned table[buckets][heads] (host).
+ * enchip_relpos_create, the usual buckets of bidirectional encoders: half = buckets / 2 of them for keys at or
+ * before the query, the other half for keys after it; of a half the first exact = half / 2 buckets take one
+ * distance |d| each, and bucket exact + j takes the distances from exact (max_distance / exact)^(j / (half -
+ * exact)) on (a distance within 10^-9 of a bucket below that counts as there); the last takes all others.
+ * buckets even, at least 4; exact < max_distance <= 2^20.
+ * enchip_relpos_create_map: the caller's own, bucket_of[2 reach + 1] for d = -reach .. reach (host); distances
+ * past reach have the bucket at reach. 0 <= reach <= 2^20.
+ * A value is -infinity (such keys get no weight) or finite and at most 2^100 in magnitude.
+ * heads (2 reach + 1) <= 2^28. */
+typedef uint64_t enchip_relpos; /* opaque handle; 0 is never a valid handle */
+int enchip_relpos_create(enchip_ctx *ctx, const float *table, int64_t buckets, int64_t heads,
+                         int64_t max_distance, enchip_relpos *out);
+int enchip_relpos_create_map(enchip_ctx *ctx, const float *table, int64_t buckets, int64_t heads,
+                             const int32_t *bucket_of, int64_t reach, enchip_relpos *out);
+int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos relpos);
+
+/* out_i = softmax_j(scale q_i . k_j + b[j - i][h]) v_j over the rows j of row i's sequence, on device buffers;
+ * relpos 0: no bias. Head h of q and out are columns h*head_dim .. of a row, its keys and values the columns of
+ * head h / (heads / kv_heads) (kv_heads divides heads). Each buffer has its own pitch.
+ * d_spans NULL: nseq sequences of L rows, row i of sequence z being row z*L + i. Otherwise L is the number of
+ * rows of the buffers and d_spans[2 z], d_spans[2 z + 1] (device) are the first row of sequence z and the one
+ * past its last, ascending: no span starts before the one ahead of it ends. Spans may be empty and leave gaps (a padded batch, or
+ * documents of any lengths packed behind each other); rows of no span are not read and their output stays as
+ * it was. (Spans are cut off at 0 and L. Where they are out of order, rows stay as they were.)
+ * A query all of whose biases are -infinity gets zeros. Products as in ENCHIP_ATT_FLASH_F16, whatever
+ * enchip_set_attention_products says: q, k, v in two f16 parts (within 2^-22, and 2^-25 below 2^-3), below 65520 in magnitude (larger, infinite and NaN ones give NaN
+ * in the rows that see them), scores, weights and sums in f32. head_dim 32, 64 or 128; pitches of q, k, v
+ * multiples of 4 below 2^25, q, k, v 16-byte aligned; d_out holds no element of q, k or v; L <= 2^30,
+ * nseq <= 2^22 with d_spans. */
+int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float *d_q, int64_t ldq,
+                              const float *d_k, int64_t ldk, const float *d_v, int64_t ldv, float *d_out,
+                              int64_t ldo, const int32_t *d_spans, int64_t nseq, int64_t L, int64_t heads,
+                              int64_t kv_heads, int64_t head_dim, float scale, void *stream);
+
+/* enchip_pool_mean_l2_dev of nseq spans of the rows of d_h (d_spans as enchip_attention_bias_dev has them, in
+ * any order): the same sums in the same order. An empty span gives zeros. */
+int enchip_pool_mean_l2_spans_dev(enchip_ctx *ctx, const float *d_h, int64_t ldh, int64_t rows,
+                                  const int32_t *d_spans, int64_t nseq, int64_t D, float *d_out, int64_t ldo,
+                                  void *stream);
+
+/* ---- low-rank adapters -----------------------------------------------------------------
+ * A set holds `slots` adapters for linears of one shape: A_s[rank][K], B_s[N][rank] and a scale each (the two
+ * matrices of a low-rank update; an adapter of a smaller rank has rows of zeros in A and columns of zeros in B).
+ * enchip_adapters_set copies an adapter from the host into a slot (scale B rounded to f32 once); until then the
+ * slot adds nothing. It waits for the context's stream; on another stream no work may be in flight that
+ * reads the set. A, B, scale B finite and below 2^127 in magnitude. 1 <= rank <= 256, 1 <= slots <= 65536, K <= 131072,
+ * N <= 2^24, and 6 slots rank (K + N) bytes (rounded up to 16, 32 and 256) at most 2^36. */
+typedef uint64_t enchip_adapters; /* opaque handle; 0 is never a valid handle */
+int enchip_adapters_create(enchip_ctx *ctx, int64_t K, int64_t N, int64_t rank, int64_t slots,
+                           enchip_adapters *out);
+int enchip_adapters_set(enchip_ctx *ctx, enchip_adapters set, int64_t slot, const float *A, const float *B,
+                        float scale);
+int enchip_adapters_release(enchip_ctx *ctx, enchip_adapters set);
+
+/* dst[m][n] = y[m][n] + scale_s sum_r (sum_k a[m][k] A_s[r][k]) B_s[n][r] with s = d_ids[m], on device
+ * buffers: the adapters of M rows of many requests beside a product y of a's rows (weight-only int8 or 4-bit,
+ * f32, any). A row whose id is not in [0, slots) gets y. d_dst may be d_y (with ldd == ldy); otherwise it holds
+ * no element of y, and none of a. Sums in f32 of products that are within 2^-24 of exact (operands held in
+ * three bf16 parts, from 2^-110 up); an activation that is not finite, or 2^127 or more in magnitude, gives NaN
+ * in its row where that has an adapter. Uses the context's shared scratch. M <= 2^30. */
+int enchip_adapters_add_dev(enchip_ctx *ctx, enchip_adapters set, const float *d_a, int64_t lda, int64_t M,
+                            const int32_t *d_ids, const float *d_y, int64_t ldy, float *d_dst, int64_t ldd,
+                            void *stream);
+
+/* enchip_w8a8_linear_dev with adapters of w's shape: d_dst[M,N] = act(y + adapters), y = W8A8(a) + bias as
+ * enchip_w8a8_linear has it, the adapters' part of the unquantized activations as enchip_adapters_add_dev has
+ * it. A row without an adapter gets what enchip_w8a8_linear_dev gives it. d_dst holds no element of a. */
+int enchip_w8a8_linear_adapters_dev(enchip_ctx *ctx, enchip_weight w, enchip_adapters set, const float *d_a,
+                                    int64_t M, const int32_t *d_ids, const float *d_bias, int act,
+                                    float *d_dst, void *stream);
+
 /* Caps each growable device scratch buffer of the context at `bytes` (0, the default:
  * no cap). A call that would grow scratch past the cap declines with ENCHIP_ERR_OOM
  * before doing any work, exactly as a failed device allocation does, so a deployment
