@@ -25,13 +25,105 @@
 namespace enchip {
 
 // A set of adapters and the rows' choice. a: [slot][Kp / 32][R / 16][3][64][8] parts, lane l of a block holding
-// rank l % 16 and k 8 (l / 16) ..; b: [slot][Np / 32][R / 16][3][64][8], lane l column l % 32 and rank
+// rank l % 16 and k 4 (l / 16) .. + 3 and 16 further (so that a wavefront's 16-byte loads of rows cover whole 64
+// bytes); b: [slot][Np / 32][R / 16][3][64][8], lane l column l % 32 and rank
 // 8 (l / 32) ..; t: [rows / 32][R / 16][3][64][8], lane l row l % 32 and rank 8 (l / 32) ...
 struct Adapters {
+    static constexpr bool on = true;
     const bf16x8 *a, *b;
     bf16x8 *t;
     const int32_t *ids;
     int slots, kb, nb, rt;  // Kp / 32, Np / 32, R / 16
+
+    // The row's slot, -1 where it has none.
+    __device__ __forceinline__ int slot(int64_t row, int64_t M) const {
+        const int id = row < M ? ids[row] : -1;
+        return id >= 0 && id < slots ? id : -1;
+    }
+    __device__ __forceinline__ const bf16x8 *t_at(int64_t mb, int rs) const { return t + (mb * rt + rs) * 192; }
+    __device__ __forceinline__ const bf16x8 *b_at(int slot, int64_t n, int rs) const {
+        return b + (((int64_t)slot * nb + n) * rt + rs) * 192;
+    }
+
+    // The column blocks' operands of one slot, kept from one row block to the next.
+    template <int TN>
+    struct Held {
+        int s = -1;
+        bf16x8 w[TN][3];
+    };
+
+    // The sums of B_s t for the 32 rows of block mb (mine: the slot of row lane % 32) and the TN column blocks
+    // from n0 on, as the MFMA's accumulators have them. A row without a slot gets zeros.
+    template <int TN, class F16>
+    __device__ __forceinline__ void tiles(int mine, int64_t mb, int64_t n0, int lane, F16 (&acc)[TN], Held<TN> &held) const {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][e] = 0.0f;
+        uint32_t todo = (uint32_t)__builtin_amdgcn_ballot_w64(mine >= 0);
+        while (todo != 0) {  // uniform: the adapters among the rows, one after the other
+            const int s = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
+            todo &= ~(uint32_t)__builtin_amdgcn_ballot_w64(mine == s);
+            const u32x4 keep = (u32x4)(mine == s ? ~0u : 0u);
+            for (int rs = 0; rs < rt; ++rs) {
+                const bf16x8 *tp = t_at(mb, rs) + lane;
+                bf16x8 x[1][3];
+#pragma unroll
+                for (int u = 0; u < 3; ++u) x[0][u] = tp[64 * u];
+                if (s != held.s || rt > 1) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int u = 0; u < 3; ++u) held.w[j][u] = b_at(s, n0 + j, rs)[64 * u + lane];
+                    held.s = s;
+                }
+#pragma unroll
+                for (int u = 0; u < 3; ++u) x[0][u] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, x[0][u]) & keep);
+                f32x16 d[1][TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) d[0][j] = acc[j];
+                mfma_parts<1, TN>(x, held.w, d);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[j] = d[0][j];
+            }
+        }
+    }
+
+    // One output's sum in a thread, for few rows: the first 16 ranks' operands are loaded ahead (dot_begin), the
+    // rest in dot_end. x = h + m + l holds exactly.
+    struct Dot {
+        int s;
+        bf16x8 x[2][3], w[2][3];
+    };
+    __device__ __forceinline__ void dot_load(Dot &d, int row, int64_t n, int c, int rs) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 3; ++u) {
+                d.x[h][u] = t_at(row >> 5, rs)[64 * u + (row & 31) + 32 * h];
+                d.w[h][u] = b_at(d.s, n, rs)[64 * u + c + 32 * h];
+            }
+    }
+    __device__ __forceinline__ void dot_begin(Dot &d, int row, int64_t M, int64_t n, int c) const {
+        d.s = slot(row, M);
+        if (d.s >= 0) dot_load(d, row, n, c, 0);
+    }
+    __device__ __forceinline__ float dot_end(Dot &d, int row, int64_t M, int64_t n, int c) const {
+        float sum = 0.0f;
+        if (d.s < 0) return sum;
+        for (int rs = 0; rs < rt; ++rs) {
+            if (rs > 0) dot_load(d, row, n, c, rs);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = (float)d.x[h][0][e] + ((float)d.x[h][1][e] + (float)d.x[h][2][e]);
+                    const float w = (float)d.w[h][0][e] + ((float)d.w[h][1][e] + (float)d.w[h][2][e]);
+                    sum = __builtin_fmaf(x, w, sum);
+                }
+        }
+        return sum;
+    }
 };
 
 __device__ __forceinline__ void split3_8(const float *x, bf16x8 (&p)[3]) {
@@ -47,112 +139,179 @@ __device__ __forceinline__ void split3_8(const float *x, bf16x8 (&p)[3]) {
     for (int u = 0; u < 3; ++u) p[u] = __builtin_bit_cast(bf16x8, w[u]);
 }
 
-// The row's slot, -1 where it has none.
-__device__ __forceinline__ int adapter_of(const Adapters &p, int64_t row, int64_t M) {
-    const int id = row < M ? p.ids[row] : -1;
-    return id >= 0 && id < p.slots ? id : -1;
+// pack_codes_normal's codes (kernels.h): the conversion to whole numbers is itself the truncation, and a byte
+// permute joins two codes.
+__device__ __forceinline__ int pack4(float4 v, float inv) {
+    const float h = __uint_as_float(0x3effffffu);
+    const float a = v.x * inv, b = v.y * inv, c = v.z * inv, d = v.w * inv;
+    const uint32_t p = (uint32_t)cvt_i32_f32(a + __builtin_copysignf(h, a)), q = (uint32_t)cvt_i32_f32(b + __builtin_copysignf(h, b));
+    const uint32_t r = (uint32_t)cvt_i32_f32(c + __builtin_copysignf(h, c)), t = (uint32_t)cvt_i32_f32(d + __builtin_copysignf(h, d));
+    return (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(t, r, 0x0c0c0400u), __builtin_amdgcn_perm(q, p, 0x0c0c0400u), 0x05040100u);
 }
 
-constexpr int AD_ROWS = 16, AD_WAVES = 4;
+// Where adapter_down leaves the rows' codes for a W8A8 product: q[M][ldq] row-major or fragment-major
+// (kernels.h frag_off), columns [K, ldq) zero, and their scales.
+struct RowCodes {
+    int8_t *q;
+    float *scale;
+    int64_t ldq;
+    bool frag;
+};
 
-// VEC: 16-byte loads of a's rows (lda a multiple of 4, a 16-byte aligned, K a multiple of 4).
-template <bool VEC>
-__global__ __launch_bounds__(64 * AD_WAVES) void adapter_down(const float *__restrict__ a, int64_t lda, int64_t M, int K, Adapters p) {
-    __shared__ float red[AD_WAVES][AD_ROWS * 16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row0 = (int64_t)blockIdx.x * AD_ROWS;
-    const int mine = adapter_of(p, row0 + (lane & 15), M);
-    const float *src = a + min(row0 + (lane & 15), M - 1) * lda;
+// Grid (ceil(M / 16), y): of the set's R / 16 rank tiles a workgroup takes RTM at a time, blockIdx.y first. K is
+// split over the NW wavefronts, 32 deep blocks w, w + NW, ...; KBW of a wavefront's are in flight together, and with
+// CODES all of them (ldq <= 32 NW KBW), for the rows are quantized from those registers (by the first of the y).
+// VEC: 16-byte loads of a's rows (lda and K multiples of 4, a 16-byte aligned). The barriers order LDS alone: loads
+// and stores stay in flight.
+template <bool VEC, bool CODES, int NW, int KBW, int RTM>
+__global__ __launch_bounds__(64 * NW, 4) void adapter_down(const float *__restrict__ a, int64_t lda, int64_t M, int K, Adapters p,
+                                                           RowCodes out) {
+    __shared__ float red[NW][RTM * 256];
+    __shared__ float top[NW][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const int64_t row0 = (int64_t)blockIdx.x * 16, row = row0 + (lane & 15);
+    const int mine = p.slot(row, M);
+    const float *src = a + min(row, M - 1) * lda;
+    float x[KBW][8];
+    auto load = [&](int c) {  // the wavefront's blocks of chunk c; zeros past K
+#pragma unroll
+        for (int i = 0; i < KBW; ++i) {
+            const int k = 32 * (NW * (c * KBW + i) + wave) + 4 * g;
+            if constexpr (VEC) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 v = *reinterpret_cast<const f32x4 *>(src + min(k + 16 * h, K - 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i][4 * h + e] = v[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = src[min(k + (e & 3) + 4 * (e & 4), K - 1)];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < KBW; ++i) {
+            const int k = 32 * (NW * (c * KBW + i) + wave);
+            if (k + 32 <= K) continue;  // uniform
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + 4 * g + (e & 3) + 4 * (e & 4) >= K) x[i][e] = 0.0f;
+        }
+    };
+    load(0);
+    if (CODES && blockIdx.y == 0) {  // uniform
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KBW; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = absmax_step(m, x[i][e]);
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if (lane < 16) top[wave][lane] = m;
+        lds_barrier();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, top[w][lane & 15]);
+        const bool zero = m == 0.0f;
+        const float s = zero ? 0.0f : m / 127.0f, inv = zero ? 0.0f : 1.0f / s;
+        if (row < M) {
+            if (wave == 0 && lane < 16) out.scale[row] = s;
+#pragma unroll
+            for (int i = 0; i < KBW; ++i) {
+                const int kb = NW * i + wave, k = 32 * kb + 4 * g;
+                if (32 * kb >= out.ldq) continue;
+                const float4 lo = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]), hi = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+                int2 c = make_int2(0, 0);
+                if (s >= 0x1p-126f) c = make_int2(pack4(lo, inv), pack4(hi, inv));
+                else if (!zero) c = make_int2(pack_codes(lo, inv), pack_codes(hi, inv));
+                int8_t *to = out.q + (out.frag ? frag_off(row, k, out.ldq >> 5) : row * out.ldq + k);
+                *reinterpret_cast<int *>(to) = c.x;
+                *reinterpret_cast<int *>(to + (out.frag ? 512 : 16)) = c.y;
+            }
+        }
+    }
     uint32_t todo = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && mine >= 0);
-    while (todo != 0) {  // uniform over the workgroup
+    const int chunks = CODES ? 1 : (p.kb + NW * KBW - 1) / (NW * KBW);
+    int held = 0;  // the chunk in x
+    while (todo != 0) {  // uniform over the workgroup: the adapters among the rows, one after the other
         const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
         const uint32_t rows = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 16 && mine == slot);
         todo &= ~rows;
-        for (int rt = 0; rt < p.rt; ++rt) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int kb = wave; kb < p.kb; kb += AD_WAVES) {
-                const int k = 32 * kb + 8 * (lane >> 4);
-                float x[8];
-                if (VEC && k + 8 <= K) {
-                    load8(src + k, x);
-                } else {
+        for (int rt0 = blockIdx.y * RTM; rt0 < p.rt; rt0 += gridDim.y * RTM) {
+            f32x4 acc[RTM];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = k + i < K ? src[k + i] : 0.0f;
+            for (int j = 0; j < RTM; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 0; c < chunks; ++c) {
+                if (!CODES && c != held) load(held = c);
+#pragma unroll
+                for (int i = 0; i < KBW; ++i) {
+                    const int kb = NW * (c * KBW + i) + wave;
+                    if (kb >= p.kb) break;  // uniform
+                    bf16x8 xp[3];
+                    split3_8(x[i], xp);
+                    const bf16x8 *at = p.a + (((int64_t)slot * p.kb + kb) * p.rt + rt0) * 192 + lane;
+#pragma unroll
+                    for (int j = 0; j < RTM; ++j) {
+                        if (RTM > 1 && rt0 + j >= p.rt) break;
+                        constexpr int pi[6] = {2, 0, 1, 1, 0, 0}, qi[6] = {0, 2, 1, 0, 1, 0};
+                        bf16x8 ap[3];
+#pragma unroll
+                        for (int u = 0; u < 3; ++u) ap[u] = at[192 * j + 64 * u];
+#pragma unroll
+                        for (int u = 0; u < 6; ++u) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xp[pi[u]], ap[qi[u]], acc[j], 0, 0, 0);
+                    }
                 }
-                bf16x8 xp[3], ap[3];
-                split3_8(x, xp);
-                const bf16x8 *at = p.a + ((((int64_t)slot * p.kb + kb) * p.rt + rt) * 3) * 64 + lane;
-#pragma unroll
-                for (int u = 0; u < 3; ++u) ap[u] = at[64 * u];
-                constexpr int pi[6] = {2, 0, 1, 1, 0, 0}, qi[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-                for (int u = 0; u < 6; ++u) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xp[pi[u]], ap[qi[u]], acc, 0, 0, 0);
             }
             // register i of lane l: row 4 (l / 16) + i, rank l % 16
 #pragma unroll
-            for (int i = 0; i < 4; ++i) red[wave][(4 * (lane >> 4) + i) * 16 + (lane & 15)] = acc[i];
-            __syncthreads();
-            const int row = tid >> 4, rank = tid & 15;
-            float v = 0.0f;
+            for (int j = 0; j < RTM; ++j)
 #pragma unroll
-            for (int w = 0; w < AD_WAVES; ++w) v += red[w][tid];
-            if ((rows >> row) & 1) {
-                float big = 0.0f;
-                uint32_t q[3];
-                split3_pair(v, 0.0f, q[0], q[1], q[2], big);
-                const int64_t m = row0 + row;
-                uint16_t *to = reinterpret_cast<uint16_t *>(p.t + ((m >> 5) * p.rt + rt) * 3 * 64 + (m & 31) + 32 * (rank >> 3)) + (rank & 7);
+                for (int i = 0; i < 4; ++i) red[wave][256 * j + (4 * g + i) * 16 + (lane & 15)] = acc[j][i];
+            lds_barrier();
+            for (int o = tid; o < 256 * RTM; o += 64 * NW) {
+                const int rt = rt0 + (o >> 8), r = (o >> 4) & 15, rank = o & 15;
+                float v = 0.0f;
 #pragma unroll
-                for (int u = 0; u < 3; ++u) to[u * 64 * 8] = (uint16_t)q[u];
+                for (int w = 0; w < NW; ++w) v += red[w][o];
+                if (((rows >> r) & 1) && rt < p.rt) {
+                    float big = 0.0f;
+                    uint32_t q[3];
+                    split3_pair(v, 0.0f, q[0], q[1], q[2], big);
+                    const int64_t m = row0 + r;
+                    uint16_t *to = reinterpret_cast<uint16_t *>(p.t + ((m >> 5) * p.rt + rt) * 192 + (m & 31) + 32 * (rank >> 3)) + (rank & 7);
+#pragma unroll
+                    for (int u = 0; u < 3; ++u) to[u * 512] = (uint16_t)q[u];
+                }
             }
-            __syncthreads();
+            lds_barrier();
         }
     }
 }
 
-// The 32 x 32 sums of B_s t at row block mb, column block nb, in the MFMA's accumulator order.
-__device__ __forceinline__ f32x16 adapter_tile(const Adapters &p, int mine, int64_t mb, int64_t nb, int lane) {
-    f32x16 acc;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-    uint32_t todo = (uint32_t)__builtin_amdgcn_ballot_w64(mine >= 0);
-    while (todo != 0) {
-        const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
-        todo &= ~(uint32_t)__builtin_amdgcn_ballot_w64(mine == slot);
-        const u32x4 keep = (u32x4)(mine == slot ? ~0u : 0u);
-        for (int rt = 0; rt < p.rt; ++rt) {
-            const bf16x8 *tp = p.t + (mb * p.rt + rt) * 3 * 64 + lane;
-            const bf16x8 *bp = p.b + (((int64_t)slot * p.nb + nb) * p.rt + rt) * 3 * 64 + lane;
-            bf16x8 t[1][3], b[1][3];
-#pragma unroll
-            for (int u = 0; u < 3; ++u) {
-                t[0][u] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, tp[64 * u]) & keep);
-                b[0][u] = bp[64 * u];
-            }
-            f32x16 one[1][1] = {{acc}};
-            mfma_parts<1, 1>(t, b, one);
-            acc = one[0][0];
-        }
-    }
-    return acc;
-}
-
-// dst = act(y + B_s t): a wavefront per 32 x 32 outputs, four side by side. dst may be y.
-template <bool GELU>
-__global__ __launch_bounds__(256) void adapter_up(const float *y, int64_t ldy, float *dst, int64_t ldd, int64_t M, int N, Adapters p,
+// dst = y + B_s t: a wavefront per 32 x 32 outputs, four side by side. dst may be y.
+[[maybe_unused]] static __global__ __launch_bounds__(256) void adapter_up(const float *y, int64_t ldy, float *dst, int64_t ldd, int64_t M, int N, Adapters p,
                                                   int panels) {
     const int lane = threadIdx.x & 63, r = lane & 31;
     const int64_t mb = blockIdx.x / panels, nb = (int64_t)(blockIdx.x % panels) * 4 + (threadIdx.x >> 6);
     const int64_t col = nb * 32 + r;
     if (nb * 32 >= N) return;
-    const f32x16 d = adapter_tile(p, adapter_of(p, mb * 32 + r, M), mb, nb, lane);
+    f32x16 d[1];
+    Adapters::Held<1> held;
+    p.tiles<1>(p.slot(mb * 32 + r, M), mb, nb, lane, d, held);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const int64_t row = mb * 32 + acc_row(e, lane);
         if (row >= M || col >= N) continue;
-        const float v = y[row * ldy + col] + d[e];
-        dst[row * ldd + col] = GELU ? gelu_f32(v) : v;
+        dst[row * ldd + col] = y[row * ldy + col] + d[0][e];
     }
+}
+
+// The W8A8 product of at most 32 rows with their adapters (kernels.h's gemv_w8a8, which see).
+template <int EPI, int NB>
+__global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8a8_adapters(
+    const int8_t *__restrict__ A, int64_t lda, const int8_t *__restrict__ Wf,
+    const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
+    void *__restrict__ out, int64_t ldo, int M, int N, int Kp, Adapters p) {
+    gemv_w8a8_body<EPI, NB>(A, lda, Wf, aS, wS, bias, out, ldo, M, N, Kp, p);
 }
 
 }  // namespace enchip

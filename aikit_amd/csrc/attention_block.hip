@@ -4,6 +4,7 @@
 
 #include "adapters.h"
 #include "attention_bias.h"
+#include "gemm_pieces.h"
 #include "head_norm.h"
 
 using namespace enchip_host;
@@ -333,37 +334,145 @@ int find_adapters(enchip_ctx *c, enchip_adapters h, AdapterSet **out) {
 int64_t a_bytes(const AdapterSet &s) { return s.kb * s.rt * 3 * 1024; }  // of a slot
 int64_t b_bytes(const AdapterSet &s) { return s.nb * s.rt * 3 * 1024; }
 
-// dst = act(y + adapters), chunk after chunk of rows (32-bit thread numbers of a launch). Arguments checked.
-int run_adapters(enchip_ctx *c, const AdapterSet &set, const float *d_a, int64_t lda, int64_t M, const int32_t *d_ids,
-                 const float *d_y, int64_t ldy, int act, float *d_dst, int64_t ldd, hipStream_t s) {
-    const int64_t panels = (set.N + 127) / 128;
-    const int64_t chunk = std::min(kRowChunk, std::max<int64_t>(1, ((int64_t)1 << 23) / panels) * 32);
-    const int64_t low = (std::min(M, chunk) + 31) / 32 * set.rt * 3 * 1024;
-    int rc;
-    if ((rc = ensure(c, &c->d_low, &c->low_cap, (size_t)low))) return rc;
-    if ((rc = scratch_wait(c, s))) return rc;
+enchip::Adapters view(const enchip_ctx *c, const AdapterSet &set, const int32_t *d_ids) {
     enchip::Adapters p;
     p.a = reinterpret_cast<const enchip::bf16x8 *>(set.d_a);
     p.b = reinterpret_cast<const enchip::bf16x8 *>(set.d_b);
     p.t = reinterpret_cast<enchip::bf16x8 *>(c->d_low);
+    p.ids = d_ids;
     p.slots = (int)set.slots, p.kb = (int)set.kb, p.nb = (int)set.nb, p.rt = (int)set.rt;
-    const bool vec = lda % 4 == 0 && set.K % 4 == 0 && (uintptr_t)d_a % 16 == 0;
+    return p;
+}
+
+int ensure_low(enchip_ctx *c, const AdapterSet &set, int64_t M) {
+    return ensure(c, &c->d_low, &c->low_cap, (size_t)((M + 31) / 32 * set.rt * 3 * 1024));
+}
+
+constexpr int64_t kHeldK = 4096;  // widest rows that adapter_down quantizes
+
+// The rows' low-rank parts into scratch, and with q their codes (ldq the weight's padded K, at most kHeldK).
+// Few rows leave CUs idle: their rank tiles go to workgroups of their own.
+int launch_down(enchip_ctx *c, const enchip::Adapters &p, const float *d_a, int64_t lda, int64_t M, int64_t K, const enchip::RowCodes *q,
+                hipStream_t s) {
+    const bool vec = lda % 4 == 0 && K % 4 == 0 && (uintptr_t)d_a % 16 == 0;
+    const int64_t blocks = (M + 15) / 16, apart = std::max<int64_t>(1, 2 * c->num_cus / blocks);
+    const bool four = p.rt > 1 && apart < p.rt;  // rank tiles four at a time
+    const dim3 grid((unsigned)blocks, (unsigned)(four ? std::min<int64_t>(apart, (p.rt + 3) / 4) : p.rt));
+    const enchip::RowCodes codes = q ? *q : enchip::RowCodes{};
+#define AD_DOWN(V, C, NW, KBW)                                                                                                       \
+    do {                                                                                                                             \
+        if (four) hipLaunchKernelGGL((enchip::adapter_down<V, C, NW, KBW, 4>), grid, dim3(64 * NW), 0, s, d_a, lda, M, (int)K, p, codes); \
+        else hipLaunchKernelGGL((enchip::adapter_down<V, C, NW, KBW, 1>), grid, dim3(64 * NW), 0, s, d_a, lda, M, (int)K, p, codes); \
+    } while (0)
+#define AD_K(V)                                           \
+    do {                                                  \
+        if (!q) AD_DOWN(V, false, 8, 4);                  \
+        else if (q->ldq <= 256) AD_DOWN(V, true, 8, 1);   \
+        else if (q->ldq <= 512) AD_DOWN(V, true, 8, 2);   \
+        else if (q->ldq <= 1024) AD_DOWN(V, true, 8, 4);  \
+        else if (q->ldq <= 2048) AD_DOWN(V, true, 16, 4); \
+        else AD_DOWN(V, true, 16, 8);                     \
+    } while (0)
+    if (vec) AD_K(true);
+    else AD_K(false);
+#undef AD_K
+#undef AD_DOWN
+    return check_launch(c, "adapter_down");
+}
+
+// dst = y + adapters, chunk after chunk of rows (32-bit thread numbers of a launch). Arguments checked.
+int run_adapters(enchip_ctx *c, const AdapterSet &set, const float *d_a, int64_t lda, int64_t M, const int32_t *d_ids,
+                 const float *d_y, int64_t ldy, float *d_dst, int64_t ldd, hipStream_t s) {
+    const int64_t panels = (set.N + 127) / 128;
+    const int64_t chunk = std::min(kRowChunk, std::max<int64_t>(1, ((int64_t)1 << 23) / panels) * 32);
+    int rc;
+    if ((rc = ensure_low(c, set, std::min(M, chunk)))) return rc;
+    if ((rc = scratch_wait(c, s))) return rc;
     for (int64_t r0 = 0; r0 < M; r0 += chunk) {
         const int64_t n = std::min(chunk, M - r0);
-        p.ids = d_ids + r0;
-        const dim3 down((unsigned)((n + enchip::AD_ROWS - 1) / enchip::AD_ROWS)), up((unsigned)((n + 31) / 32 * panels));
-        if (vec)
-            hipLaunchKernelGGL(enchip::adapter_down<true>, down, dim3(64 * enchip::AD_WAVES), 0, s, d_a + r0 * lda, lda, n, (int)set.K, p);
-        else
-            hipLaunchKernelGGL(enchip::adapter_down<false>, down, dim3(64 * enchip::AD_WAVES), 0, s, d_a + r0 * lda, lda, n, (int)set.K, p);
-        if (act == ENCHIP_ACT_GELU)
-            hipLaunchKernelGGL(enchip::adapter_up<true>, up, dim3(256), 0, s, d_y + r0 * ldy, ldy, d_dst + r0 * ldd, ldd, n, (int)set.N, p,
-                               (int)panels);
-        else
-            hipLaunchKernelGGL(enchip::adapter_up<false>, up, dim3(256), 0, s, d_y + r0 * ldy, ldy, d_dst + r0 * ldd, ldd, n, (int)set.N, p,
-                               (int)panels);
+        const enchip::Adapters p = view(c, set, d_ids + r0);
+        if ((rc = launch_down(c, p, d_a + r0 * lda, lda, n, set.K, nullptr, s))) return rc;
+        hipLaunchKernelGGL(enchip::adapter_up, dim3((unsigned)((n + 31) / 32 * panels)), dim3(256), 0, s, d_y + r0 * ldy, ldy,
+                           d_dst + r0 * ldd, ldd, n, (int)set.N, p, (int)panels);
     }
-    if ((rc = check_launch(c, "adapters"))) return rc;
+    if ((rc = check_launch(c, "adapter_up"))) return rc;
+    return scratch_record(c, s);
+}
+
+// The W8A8 product of quantized rows with their adapters, on the kernels of enchip_w8a8_linear_dev (few rows:
+// row-major codes; else fragment-major, in pieces or gemm_w8a8_pt's tiles). M fits one launch.
+template <int EPI>
+void launch_linear(enchip_ctx *c, const Weight &w, const int8_t *aq, const float *as, const float *bias, float *out, int64_t M,
+                   const enchip::Adapters &p, hipStream_t s) {
+    using namespace enchip;
+    const int m = (int)M, n = (int)w.N, kp = (int)w.Kp;
+    if (M <= c->small_m) {
+        const dim3 grid((unsigned)((w.N + 31) / 32), (unsigned)((M + GV_ROWS - 1) / GV_ROWS)), block(64 * GV_WAVES);
+        const int64_t per_wave = (w.Kp / 32 + GV_WAVES - 1) / GV_WAVES;
+#define GV_LAUNCH(NB) \
+    hipLaunchKernelGGL((gemv_w8a8_adapters<EPI, NB>), grid, block, 0, s, aq, w.Kp, w.d_w, as, w.d_s, bias, out, w.N, m, n, kp, p)
+        if (per_wave <= 1) GV_LAUNCH(1);
+        else if (per_wave == 2) GV_LAUNCH(2);
+        else if (per_wave <= 4) GV_LAUNCH(4);
+        else GV_LAUNCH(8);
+#undef GV_LAUNCH
+        return;
+    }
+    const bool pt = use_persistent(w, aq, w.Kp, out, w.N, M, true);
+    const int f = piece_form(c, w, M, EPI, !pt);
+    if (pt && f < 0) {
+        // 64-row tiles at any M: with the adapters' sums 128-row ones spill (32768 x 1024, K = 1024, rank 16: 63 us
+        // against 57; without adapters 47)
+        const int tn = (int)((w.N + PT_BN - 1) / PT_BN), tiles = (int)((M + PT_BM_SMALL - 1) / PT_BM_SMALL) * tn;
+        const dim3 grid((unsigned)persistent_grid(c, tiles)), block(64 * PT_NW);
+        if (pt_prio(w, EPI))
+            hipLaunchKernelGGL((gemm_w8a8_pt_adapters<PT_BM_SMALL, PT_BN, PT_BK, PT_PW, EPI, PT_NW, 1, Adapters>), grid, block, 0, s, aq,
+                               w.Kp, w.d_w, as, w.d_s, bias, out, w.N, m, n, kp, tn, tiles, p);
+        else
+            hipLaunchKernelGGL((gemm_w8a8_pt_adapters<PT_BM_SMALL, PT_BN, PT_BK, PT_PW, EPI, PT_NW, 0, Adapters>), grid, block, 0, s, aq,
+                               w.Kp, w.d_w, as, w.d_s, bias, out, w.N, m, n, kp, tn, tiles, p);
+        return;
+    }
+#define PIECE(F, VEC)                                                                                                            \
+    do {                                                                                                                         \
+        constexpr int CM = kPieces[F].cm, CN = kPieces[F].cn;                                                                    \
+        const int64_t pn = (w.N + CN - 1) / CN;                                                                                  \
+        hipLaunchKernelGGL((gemm_w8a8_adapters<CM, CN, EPI, PT_NW, PT_PW, VEC, Adapters>), dim3((unsigned)((M + CM - 1) / CM * pn)), \
+                           dim3(64 * PT_NW), 0, s, aq, w.d_w, as, w.d_s, bias, out, w.N, m, n, kp, (int)pn, p);                  \
+    } while (0)
+    const bool vec = w.N % 4 == 0 && (uintptr_t)out % 16 == 0;
+    if (f == 0 && vec) PIECE(0, true);
+    else if (f == 0) PIECE(0, false);
+    else if (f == 1 && vec) PIECE(1, true);
+    else if (f == 1) PIECE(1, false);
+    else if (vec) PIECE(2, true);
+    else PIECE(2, false);
+#undef PIECE
+}
+
+// act(W8A8(a) + bias + adapters): the rows quantized and their low-rank parts formed in one pass over them, then
+// the product with the adapters in its epilogue. Chunk after chunk of rows, for which gemm_w8a8_pt's byte offsets
+// and a launch's thread numbers fit 32 bits. Arguments checked.
+int run_linear_adapters(enchip_ctx *c, const Weight &w, const AdapterSet &set, const float *d_a, int64_t M, const int32_t *d_ids,
+                        const float *d_bias, int act, float *d_dst, hipStream_t s) {
+    const int64_t by_codes = (((int64_t)1 << 31) - 1) / w.Kp, by_pieces = ((int64_t)1 << 34) / round_up(w.N, 32);
+    const int64_t chunk = M <= c->small_m ? M : std::max<int64_t>(128, std::min({kRowChunk, by_codes, by_pieces}) / 128 * 128);
+    int rc;
+    if ((rc = ensure_act_scratch(c, std::min(M, chunk), w.Kp))) return rc;
+    if ((rc = ensure_low(c, set, std::min(M, chunk)))) return rc;
+    if ((rc = scratch_wait(c, s))) return rc;
+    for (int64_t r0 = 0; r0 < M; r0 += chunk) {
+        const int64_t n = std::min(chunk, M - r0);
+        const enchip::Adapters p = view(c, set, d_ids + r0);
+        const float *a = d_a + r0 * w.K;
+        const bool frag = n > c->small_m;
+        const enchip::RowCodes q{c->d_aq, c->d_as, w.Kp, frag};
+        if (w.Kp > kHeldK && (rc = launch_quant(c, a, n, w.K, c->d_aq, w.Kp, c->d_as, s, frag))) return rc;
+        if ((rc = launch_down(c, p, a, w.K, n, w.K, w.Kp > kHeldK ? nullptr : &q, s))) return rc;
+        if (act == ENCHIP_ACT_GELU) launch_linear<enchip::EPI_F32_GELU>(c, w, c->d_aq, c->d_as, d_bias, d_dst + r0 * w.N, n, p, s);
+        else launch_linear<enchip::EPI_F32>(c, w, c->d_aq, c->d_as, d_bias, d_dst + r0 * w.N, n, p, s);
+        if ((rc = check_launch(c, "linear_adapters"))) return rc;
+    }
     return scratch_record(c, s);
 }
 
@@ -436,8 +545,8 @@ int enchip_adapters_set(enchip_ctx *ctx, enchip_adapters h, int64_t slot, const 
             const float x = A[j * K + k];
             if (!(std::fabs(x) < 0x1p127f))
                 return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: A[%lld][%lld] is %g", (long long)j, (long long)k, (double)x);
-            const int64_t block = (k / 32 * rt + j / 16) * 3, lane = j % 16 + 16 * (k % 32 / 8);
-            store_parts(x, &a[(size_t)((block * 64 + lane) * 8 + k % 8)], 512);
+            const int64_t block = (k / 32 * rt + j / 16) * 3, lane = j % 16 + 16 * (k % 16 / 4);
+            store_parts(x, &a[(size_t)((block * 64 + lane) * 8 + k % 32 / 16 * 4 + k % 4)], 512);
         }
     for (int64_t n = 0; n < N; ++n)
         for (int64_t j = 0; j < R; ++j) {
@@ -485,7 +594,7 @@ int enchip_adapters_add_dev(enchip_ctx *ctx, enchip_adapters h, const float *d_a
     if (!d_a || !d_ids || !d_y || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "adapters_add: null pointer");
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
-    return run_adapters(ctx, *set, d_a, lda, M, d_ids, d_y, ldy, ENCHIP_ACT_NONE, d_dst, ldd, s);
+    return run_adapters(ctx, *set, d_a, lda, M, d_ids, d_y, ldy, d_dst, ldd, s);
 }
 
 int enchip_w8a8_linear_adapters_dev(enchip_ctx *ctx, enchip_weight hw, enchip_adapters h, const float *d_a, int64_t M,
@@ -505,8 +614,7 @@ int enchip_w8a8_linear_adapters_dev(enchip_ctx *ctx, enchip_weight hw, enchip_ad
     if (!d_a || !d_ids || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "linear_adapters: null pointer");
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
-    if ((rc = run_linear(ctx, *w, d_a, M, d_bias, ENCHIP_ACT_NONE, d_dst, s))) return rc;
-    return run_adapters(ctx, *set, d_a, w->K, M, d_ids, d_dst, w->N, act, d_dst, w->N, s);
+    return run_linear_adapters(ctx, *w, *set, d_a, M, d_ids, d_bias, act, d_dst, s);
 }
 
 }  // extern "C"

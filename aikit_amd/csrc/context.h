@@ -374,8 +374,4 @@ inline enchip::FastDiv fast_div(int64_t d) {
 int launch_quant(enchip_ctx *c, const float *d_a, int64_t M, int64_t K, int8_t *q, int64_t ldq, float *scale,
                  hipStream_t s, bool frag = false);
 
-// A W8A8 linear on device buffers whose arguments have been checked, on stream s. (enchip.hip)
-int run_linear(enchip_ctx *c, const Weight &w, const float *d_a, int64_t M, const float *d_bias, int act, float *d_dst,
-               hipStream_t s);
-
 }  // namespace enchip_host

@@ -541,19 +541,6 @@ int launch_fused_small_m(enchip_ctx *c, const Weight &w, const float *d_a, int64
 
 }  // namespace
 
-int enchip_host::run_linear(enchip_ctx *c, const Weight &w, const float *d_a, int64_t M, const float *d_bias, int act,
-                            float *d_dst, hipStream_t s) {
-    if (fused_small_m(c, w, M, d_a))  // one launch, no scratch
-        return launch_fused_small_m(c, w, d_a, M, d_bias, act_code(act), d_dst, w.N, s);
-    int rc;
-    if ((rc = ensure_act_scratch(c, M, w.Kp))) return rc;
-    if ((rc = scratch_wait(c, s))) return rc;
-    const bool af = route_frag(c, w, M, act_code(act), d_dst, w.N);
-    if ((rc = launch_quant(c, d_a, M, w.K, c->d_aq, w.Kp, c->d_as, s, af))) return rc;
-    if ((rc = launch_gemm(c, w, c->d_aq, w.Kp, c->d_as, d_bias, act_code(act), d_dst, w.N, M, s, af))) return rc;
-    return scratch_record(c, s);
-}
-
 extern "C" {
 
 int enchip_abi_version(void) { return ENCHIP_ABI_VERSION; }
@@ -1122,7 +1109,15 @@ int enchip_w8a8_linear_dev(enchip_ctx *ctx, enchip_weight h, const float *d_a, i
     if ((w->K > 0 && !d_a) || !d_dst) return fail(ctx, ENCHIP_ERR_ARG, "linear: null pointer");
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
-    return run_linear(ctx, *w, d_a, M, d_bias, act, d_dst, s);
+    if (fused_small_m(ctx, *w, M, d_a))  // one launch, no scratch
+        return launch_fused_small_m(ctx, *w, d_a, M, d_bias, act_code(act), d_dst, w->N, s);
+    if ((rc = ensure_act_scratch(ctx, M, w->Kp))) return rc;
+    if ((rc = scratch_wait(ctx, s))) return rc;
+    const bool af = route_frag(ctx, *w, M, act_code(act), d_dst, w->N);
+    if ((rc = launch_quant(ctx, d_a, M, w->K, ctx->d_aq, w->Kp, ctx->d_as, s, af))) return rc;
+    if ((rc = launch_gemm(ctx, *w, ctx->d_aq, w->Kp, ctx->d_as, d_bias, act_code(act), d_dst, w->N, M, s, af)))
+        return rc;
+    return scratch_record(ctx, s);
 }
 
 int enchip_w8a8_linear_noalloc_dev(enchip_ctx *ctx, enchip_weight h, const float *d_a, int64_t M,

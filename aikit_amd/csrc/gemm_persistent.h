@@ -57,6 +57,8 @@ struct TopkSink {
     int cap = 0;
 };
 
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+
 // Tile geometry and ring depth of the persistent kernel (the host checks its
 // preconditions). PT_BM_SMALL: the 64-row tile the host picks when 128-row tiles would
 // leave workgroup slots idle (fewer tiles than 2 per CU); it runs 3 workgroups per CU.
@@ -75,11 +77,17 @@ __device__ __forceinline__ void store_nt(void *p, int4 v) {
 // wave go first when the other is in its epilogue (measured on MI355X: 4-10% faster on
 // the BERT-base and XLM-R-large bias-only shapes except BERT-base's O, 4% slower, and the
 // GELU epilogue unchanged; bit-identical either way).
-template <int BM, int BN, int BK, int PW, int EPI, bool AF, int NW, int PRIO>
-__global__ __launch_bounds__(64 * NW, BM == PT_BM_SMALL ? 3 : NW / 2) void gemm_w8a8_pt(
+// AD: what is added to the outputs before the activation (adapters.h), in f32 as the MFMA's
+// accumulators have it, so that a chunk's transpose carries finished sums.
+template <int BM, int BN, int BK, int PW, int EPI, bool AF, int NW, int PRIO, class AD>
+__device__ __forceinline__ void w8a8_pt(
     const int8_t *__restrict__ A, int64_t lda, const int8_t *__restrict__ Wf,
     const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
-    void *__restrict__ out, int64_t ldo, int M, int N, int Kp, int tilesN, int numTiles, TopkSink sink) {
+    void *__restrict__ out, int64_t ldo, int M, int N, int Kp, int tilesN, int numTiles, const TopkSink &sink, const AD &ad) {
+    auto dequant = [](int acc, float as, float ws, float b) {
+        if constexpr (AD::on) return __int_as_float(acc);  // a finished sum
+        else return enchip::dequant(acc, as, ws, b);
+    };
     constexpr int NT = 64 * NW;  // threads
     constexpr int WN = BN / NW;  // output columns per wave
     constexpr int TM = BM / 32, TN = WN / 32;
@@ -275,8 +283,23 @@ __global__ __launch_bounds__(64 * NW, BM == PT_BM_SMALL ? 3 : NW / 2) void gemm_
         const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[lcol]);
         const float wsv[4] = {ws4.x, ws4.y, ws4.z, ws4.w}, bv[4] = {b4.x, b4.y, b4.z, b4.w};
         int *scr = s_tr[wave];
+        typename AD::template Held<TN> held;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
+            if constexpr (AD::on) {
+                f32x16v low[TN];
+                ad.template tiles<TN>(ad.slot(m0 + 32 * i + (lane & 31), M), m0 / 32 + i, n0 / 32 + wave * TN, lane, low, held);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const float cw = s_ws[wave * WN + 32 * j + (lane & 31)], cb = s_b[wave * WN + 32 * j + (lane & 31)];
+#pragma unroll
+                    for (int rr = 0; rr < 16; ++rr) {
+                        const int R = acc_row(rr, lane);
+                        const float as = s_as[32 * i + (R % RPL) * KR + R / RPL];
+                        acc[i][j][rr] = __float_as_int(enchip::dequant(acc[i][j][rr], as, cw, cb) + low[j][rr]);
+                    }
+                }
+            }
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -501,6 +524,23 @@ __global__ __launch_bounds__(64 * NW, BM == PT_BM_SMALL ? 3 : NW / 2) void gemm_
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
     }
+}
+
+template <int BM, int BN, int BK, int PW, int EPI, bool AF, int NW, int PRIO>
+__global__ __launch_bounds__(64 * NW, BM == PT_BM_SMALL ? 3 : NW / 2) void gemm_w8a8_pt(
+    const int8_t *__restrict__ A, int64_t lda, const int8_t *__restrict__ Wf,
+    const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
+    void *__restrict__ out, int64_t ldo, int M, int N, int Kp, int tilesN, int numTiles, TopkSink sink) {
+    w8a8_pt<BM, BN, BK, PW, EPI, AF, NW, PRIO>(A, lda, Wf, aS, wS, bias, out, ldo, M, N, Kp, tilesN, numTiles, sink, NoAdapters{});
+}
+
+// On fragment-major codes, with the rows' adapters added (adapters.h).
+template <int BM, int BN, int BK, int PW, int EPI, int NW, int PRIO, class AD>
+__global__ __launch_bounds__(64 * NW, 2) void gemm_w8a8_pt_adapters(
+    const int8_t *__restrict__ A, int64_t lda, const int8_t *__restrict__ Wf,
+    const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
+    void *__restrict__ out, int64_t ldo, int M, int N, int Kp, int tilesN, int numTiles, AD ad) {
+    w8a8_pt<BM, BN, BK, PW, EPI, true, NW, PRIO>(A, lda, Wf, aS, wS, bias, out, ldo, M, N, Kp, tilesN, numTiles, TopkSink{}, ad);
 }
 
 }  // namespace enchip

@@ -86,11 +86,11 @@ __device__ __forceinline__ void gelu_cells(int lane, const f32x4v (&y)[NG], int 
 // The piece at rows m0.., columns n0... A is fragment-major at pitch Kp and read up to row
 // m0 + CM - 1 (its buffer holds them: CM divides 128), the weights up to column n0 + CN - 1
 // of their padded Np. VEC: N and ldo are multiples of 4 and out is 16-byte aligned.
-template <int CM, int CN, int NW, int PW, int EPI, bool VEC>
+template <int CM, int CN, int NW, int PW, int EPI, bool VEC, class AD = NoAdapters>
 __device__ __forceinline__ void w8a8_piece(const int8_t *__restrict__ A, const int8_t *__restrict__ Wf,
                                            const float *__restrict__ aS, const float *__restrict__ wS,
                                            const float *__restrict__ bias, void *__restrict__ out, int64_t ldo, int M,
-                                           int N, int Kp, int m0, int n0) {
+                                           int N, int Kp, int m0, int n0, const AD &ad = {}) {
     constexpr int TM = CM / 32, TN = CN / 32, NT = 64 * NW;
     constexpr int P = CN + 8;             // LDS row pitch in ints: rows 4 apart start 32 banks apart
     constexpr int RL = CN / 4;            // 16-byte groups per row
@@ -160,6 +160,16 @@ __device__ __forceinline__ void w8a8_piece(const int8_t *__restrict__ A, const i
             if (s + PW + d < ns) mul(d);
     }
 
+    // the adapters' sums of a 32 x 32 tile a wavefront, before the barrier too
+    f32x16v low[1];
+    const int low_i = wave / TN, low_j = wave % TN;
+    if constexpr (AD::on) {
+        static_assert(TM * TN <= NW, "a tile a wavefront");
+        typename AD::template Held<1> held;
+        if (wave < TM * TN)
+            ad.template tiles<1>(ad.slot(m0 + 32 * low_i + (lane & 31), M), m0 / 32 + low_i, n0 / 32 + low_j, lane, low, held);
+    }
+
     // this thread's outputs: group tid % RL of rows tid / RL + RP * i; their constants are
     // loaded before the barrier
     const int c4 = 4 * (tid % RL), r0 = tid / RL, col = n0 + c4;
@@ -179,11 +189,11 @@ __device__ __forceinline__ void w8a8_piece(const int8_t *__restrict__ A, const i
 #pragma unroll
             for (int r = 0; r < 16; ++r) red[wave][(32 * i + acc_row(r, lane)) * P + 32 * j + (lane & 31)] = acc[i][j][r];
     __syncthreads();
-    if (!mine) return;  // whole wavefronts
+    if (!AD::on && !mine) return;  // whole wavefronts
     int4 v[NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-        const int at = (r0 + RP * i) * P + c4;
+        const int at = (AD::on && !mine ? 0 : r0 + RP * i) * P + c4;
         int4 t = *reinterpret_cast<const int4 *>(&red[0][at]);
 #pragma unroll
         for (int k = 1; k < NW; ++k) {
@@ -192,12 +202,24 @@ __device__ __forceinline__ void w8a8_piece(const int8_t *__restrict__ A, const i
         }
         v[i] = t;
     }
+    if constexpr (AD::on) {  // the adapters' sums take the first partial sum's place
+        __syncthreads();
+        float *lds = reinterpret_cast<float *>(red[0]);
+        if (wave < TM * TN)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) lds[(32 * low_i + acc_row(r, lane)) * P + 32 * low_j + (lane & 31)] = low[0][r];
+        __syncthreads();
+        if (!mine) return;
+    }
     if constexpr (EPI != EPI_I32) {
         f32x4v y[NG];
 #pragma unroll
         for (int i = 0; i < NG; ++i)
             y[i] = f32x4v{dequant(v[i].x, as[i], ws[0], bb[0]), dequant(v[i].y, as[i], ws[1], bb[1]),
                           dequant(v[i].z, as[i], ws[2], bb[2]), dequant(v[i].w, as[i], ws[3], bb[3])};
+        if constexpr (AD::on)
+#pragma unroll
+            for (int i = 0; i < NG; ++i) y[i] += *reinterpret_cast<const f32x4v *>(&red[0][(r0 + RP * i) * P + c4]);
         if constexpr (EPI == EPI_F32_GELU) {
             // rows RP * i + wave * 64 / RL .. of the partial sums were read by this wavefront alone
             const int wrow = wave * (64 / RL);
@@ -251,6 +273,16 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm_w8a8(const int8_t *__restrict
                                                         int64_t ldo, int M, int N, int Kp, int piecesN) {
     const int l = xcd_logical_tile(blockIdx.x, gridDim.x);
     w8a8_piece<CM, CN, NW, PW, EPI, false>(A, Wf, aS, wS, bias, out, ldo, M, N, Kp, (l / piecesN) * CM, (l % piecesN) * CN);
+}
+
+// Either with the rows' adapters added (adapters.h).
+template <int CM, int CN, int EPI, int NW, int PW, bool VEC, class AD>
+__global__ __launch_bounds__(64 * NW, 2) void gemm_w8a8_adapters(const int8_t *__restrict__ A, const int8_t *__restrict__ Wf,
+                                                                 const float *__restrict__ aS, const float *__restrict__ wS,
+                                                                 const float *__restrict__ bias, void *__restrict__ out,
+                                                                 int64_t ldo, int M, int N, int Kp, int piecesN, AD ad) {
+    const int l = xcd_logical_tile(blockIdx.x, gridDim.x);
+    w8a8_piece<CM, CN, NW, PW, EPI, VEC, AD>(A, Wf, aS, wS, bias, out, ldo, M, N, Kp, (l / piecesN) * CM, (l % piecesN) * CN, ad);
 }
 
 }  // namespace enchip

@@ -704,17 +704,29 @@ __global__ __launch_bounds__(256, MINB) void gemm_w8a8(
 // N = 3072 (MI355X, graph replay over cold weights, bit-identical).
 constexpr int GV_WAVES = 8, GV_ROWS = 8;
 
-template <int EPI, int NB>
-__global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8a8(
+// What the W8A8 kernels add to their outputs before the activation: nothing, or low-rank adapters
+// (adapters.h).
+struct NoAdapters {
+    static constexpr bool on = false;
+    struct Dot {};
+    template <int TN>
+    struct Held {};
+};
+
+template <int EPI, int NB, class AD>
+__device__ __forceinline__ void gemv_w8a8_body(
     const int8_t *__restrict__ A, int64_t lda, const int8_t *__restrict__ Wf,
     const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
-    void *__restrict__ out, int64_t ldo, int M, int N, int Kp) {
+    void *__restrict__ out, int64_t ldo, int M, int N, int Kp, const AD &ad) {
     __shared__ int red[GV_WAVES * GV_ROWS * 32];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nb = blockIdx.x, rg = blockIdx.y, nk32 = Kp >> 5;
     const int q = rg & 3, r = lane & 31;  // the group's rows 8q .. 8q + 7 of the 32-row tile
     const int8_t *arow = A + (int64_t)min((r >> 3) == q ? r : 8 * q, M - 1) * lda + (lane >> 5) * 16;
     const int8_t *wfr = Wf + (int64_t)nb * nk32 * 1024 + lane * 16;
+    typename AD::Dot dot;
+    if constexpr (AD::on)  // the adapters' first operands, in flight during the main loop
+        if (tid < GV_ROWS * 32) ad.dot_begin(dot, rg * GV_ROWS + (tid >> 5), M, nb, tid & 31);
 
     i32x16 acc;
 #pragma unroll
@@ -743,15 +755,32 @@ __global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8a8(
 #pragma unroll
         for (int w = 0; w < GV_WAVES; ++w) sum += red[(w * GV_ROWS + i) * 32 + c];
         const int row = rg * GV_ROWS + i, col = nb * 32 + c;
+        float d = 0.0f;
+        if constexpr (AD::on) d = ad.dot_end(dot, row, M, nb, c);
         if (row < M && col < N) {
             if (EPI == EPI_I32) {
                 reinterpret_cast<int *>(out)[(int64_t)row * ldo + col] = sum;
             } else {
                 const float bb = bias != nullptr ? bias[col] : kNoBias;
-                reinterpret_cast<float *>(out)[(int64_t)row * ldo + col] = epilogue<EPI>(sum, aS[row], wS[col], bb);
+                float y;
+                if constexpr (AD::on) {
+                    y = dequant(sum, aS[row], wS[col], bb) + d;
+                    if (EPI == EPI_F32_GELU) y = gelu_f32(y);
+                } else {
+                    y = epilogue<EPI>(sum, aS[row], wS[col], bb);
+                }
+                reinterpret_cast<float *>(out)[(int64_t)row * ldo + col] = y;
             }
         }
     }
+}
+
+template <int EPI, int NB>
+__global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8a8(
+    const int8_t *__restrict__ A, int64_t lda, const int8_t *__restrict__ Wf,
+    const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
+    void *__restrict__ out, int64_t ldo, int M, int N, int Kp) {
+    gemv_w8a8_body<EPI, NB>(A, lda, Wf, aS, wS, bias, out, ldo, M, N, Kp, NoAdapters{});
 }
 
 // gemv_w8a8 with the per-token quantization of its (at most 32) activation rows done in
