@@ -22,6 +22,8 @@
 
 namespace enchip {
 
+constexpr float AB_LAZY = 8.0f;
+
 struct AttnBias {
     const float *q, *k, *v;
     float *out;
@@ -33,6 +35,33 @@ struct AttnBias {
     int L;       // rows of a sequence, or with spans those of the buffers
     float scale;
 };
+
+// x less the low (high) half of h, exactly: one mixed fused multiply-add in place of a conversion and a subtraction.
+__device__ __forceinline__ float ab_rest_lo(uint32_t h, float x) {
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
+    return d;
+}
+__device__ __forceinline__ float ab_rest_hi(uint32_t h, float x) {
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
+    return d;
+}
+// The parts of split_f16x8 and split_pair_f16 (attention_f32.h).
+__device__ __forceinline__ void ab_pair(float a, float b, uint32_t &hw, uint32_t &lw) {
+    hw = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+    lw = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){ab_rest_lo(hw, a), ab_rest_hi(hw, b)}, f16x2));
+}
+__device__ __forceinline__ void ab_split8(const float *x, f16x8 &hi, f16x8 &lo) {
+    u32x4 h, l;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        uint32_t hw, lw;
+        ab_pair(x[2 * s], x[2 * s + 1], hw, lw);
+        h[s] = hw, l[s] = lw;
+    }
+    hi = __builtin_bit_cast(f16x8, h), lo = __builtin_bit_cast(f16x8, l);
+}
 
 template <int HD, int NW>
 struct AbLayout {
@@ -76,7 +105,7 @@ __device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int64_t &row0,
 // AbLayout<HD, NW>::BYTES of dynamic LDS. q, k, v 16-byte aligned, their pitches multiples of 4 and at most
 // INT32_MAX / FA_KT; VEC: ldo a multiple of 4 and out 16-byte aligned.
 template <int HD, int NW, bool VEC>
-__global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
+__global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(AttnBias p) {
     using Fa = FaLayout<HD>;
     using Lay = AbLayout<HD, NW>;
     constexpr int NT = 64 * NW, QB = 32 * NW;
@@ -99,7 +128,7 @@ __global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
     const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
     const float *vbase = p.v + row0 * p.ldv + (head / p.group) * HD;
     const float *table = p.table ? p.table + (int64_t)head * (2 * p.reach + 1) + p.reach : nullptr;
-    const float c = p.scale * FA_LOG2E;
+    const float c = p.scale * FA_LOG2E;  // of the queries: scores come out in base 2
 
     vec8 qh[NB], ql[NB];
     float qt[NB][8];
@@ -150,7 +179,7 @@ __global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
                 const float x[8] = {kr[i][0].x, kr[i][0].y, kr[i][0].z, kr[i][0].w,
                                     kr[i][1].x, kr[i][1].y, kr[i][1].z, kr[i][1].w};
                 vec8 h, l;
-                Ops::split8(x, h, l);
+                ab_split8(x, h, l);
                 *reinterpret_cast<vec8 *>(khi + key * Fa::KP + 2 * col) = h;
                 *reinterpret_cast<vec8 *>(klo + key * Fa::KP + 2 * col) = l;
             }
@@ -166,7 +195,7 @@ __global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint32_t hw, lw;
-                    Ops::pair(a[j], b[j], hw, lw);
+                    ab_pair(a[j], b[j], hw, lw);
                     const int vo = (col + j) * Fa::VP + ((2 * pos) ^ fa_vswz(col + j));
                     *reinterpret_cast<uint32_t *>(vhi + vo) = hw;
                     *reinterpret_cast<uint32_t *>(vlo + vo) = lw;
@@ -185,7 +214,11 @@ __global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
 
     load_tile(0);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) Ops::split8(qt[b], qh[b], ql[b]);
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qt[b][i] *= c;
+        ab_split8(qt[b], qh[b], ql[b]);
+    }
     store_tile(0);
     lds_barrier();
     for (int t = 0; t < nt; ++t) {
@@ -198,9 +231,11 @@ __global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
             for (int s = 0; s < FA_KT / 32; ++s) {
                 const int key0 = t * FA_KT + 32 * s;
                 if (key0 >= L) break;  // uniform: no barrier inside
+                // the scores' sums start at the bias; element e is key key0 + 4 hf + 8 (e / 4) + e % 4
+                const float *bw = window + (32 * s + 4 * hf - (32 * wave + r) + QB - 1);
                 f32x16 acc;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+                for (int e = 0; e < 16; ++e) acc[e] = bw[8 * (e >> 2) + (e & 3)];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int off = (32 * s + r) * Fa::KP + 2 * (16 * b + 8 * hf);
@@ -208,42 +243,41 @@ __global__ __launch_bounds__(64 * NW) void attention_bias(AttnBias p) {
                     const vec8 kl = *reinterpret_cast<const vec8 *>(klo + off);
                     acc = mfma_split3(kh, kl, qh[b], ql[b], acc);
                 }
-                // y = c s + b in base 2; element e is key key0 + 4 hf + 8 (e / 4) + e % 4
-                const float *bw = window + (32 * s + 4 * hf - (32 * wave + r) + QB - 1);
-                float x[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(acc[e], c, bw[8 * (e >> 2) + (e & 3)]);
                 const int lim = L - key0 - 4 * hf;
                 if (__builtin_expect(key0 + 32 > L, 0)) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (8 * (e >> 2) + (e & 3) >= lim) x[e] = -INFINITY;
+                        if (8 * (e >> 2) + (e & 3) >= lim) acc[e] = -INFINITY;
                 }
-                float mloc = x[0];
+                float mloc = acc[0];
 #pragma unroll
-                for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, x[e]);
+                for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, acc[e]);
                 {
                     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
                     mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
                 }
-                const float m_new = fmaxf(m_run, mloc);
-                const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // nothing attended so far: every p is 0
-                const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-                float psum = 0.0f;
+                // The subtracted maximum follows a query's running maximum only when that is AB_LAZY above it: weights
+                // up to 2^AB_LAZY keep their precision, and after the first tiles nothing is rescaled.
+                const bool up = mloc > m_run + AB_LAZY;
+                if (__builtin_amdgcn_ballot_w64(up) != 0) {
+                    const float alpha = up ? __builtin_amdgcn_exp2f(m_run - mloc) : 1.0f;
+                    m_run = up ? mloc : m_run;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+                }
+                const float m_use = m_run == -INFINITY ? 0.0f : m_run;  // nothing attended so far: every weight is 0
+                float x[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(x[e] - m_use);
-                    psum += x[e];
+                    x[e] = __builtin_amdgcn_exp2f(acc[e] - m_use);
+                    l_run += x[e];
                 }
-                l_run = l_run * alpha + psum;
-                m_run = m_new;
-#pragma unroll
-                for (int i = 0; i < NOT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
                 vec8 ph[2], pl[2];
-                Ops::split8(x, ph[0], pl[0]);
-                Ops::split8(x + 8, ph[1], pl[1]);
+                ab_split8(x, ph[0], pl[0]);
+                ab_split8(x + 8, ph[1], pl[1]);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
