@@ -63,10 +63,10 @@ __device__ __forceinline__ void ab_split8(const float *x, f16x8 &hi, f16x8 &lo) 
     hi = __builtin_bit_cast(f16x8, h), lo = __builtin_bit_cast(f16x8, l);
 }
 
-template <int HD, int NW>
+template <int HD, int NW, int QPW>
 struct AbLayout {
     using Fa = FaLayout<HD>;
-    static constexpr int WINDOW = 32 * NW + FA_KT;  // distances of a tile (one to spare)
+    static constexpr int WINDOW = 32 * NW * QPW + FA_KT;  // distances of a tile (one to spare)
     static constexpr int BIAS = 2 * Fa::STAGE;      // two windows behind the two stages
     static constexpr int BYTES = BIAS + 2 * WINDOW * 4;
 };
@@ -101,14 +101,35 @@ __device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int64_t &row0,
     return true;
 }
 
+// acc[u] += (ah + al) (b_h(u) + b_l(u)) less al b_l, a product of every accumulator in turn.
+template <int N, class H, class Lo>
+__device__ __forceinline__ void ab_mfma3(const f16x8 &ah, const f16x8 &al, H bh, Lo bl, f32x16 (&acc)[N]) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl(u), acc[u], 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < N; ++u) acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh(u), acc[u], 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < N; ++u) acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh(u), acc[u], 0, 0, 0);
+}
+
+template <bool VEC>
+__device__ __forceinline__ void ab_store(float *to, f32x4 v) {
+    if constexpr (VEC) {
+        *reinterpret_cast<f32x4 *>(to) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = v[i];
+    }
+}
+
 // A 1-D grid of heads * query blocks, XCD-aware (a sequence's query blocks of one head on one XCD),
-// AbLayout<HD, NW>::BYTES of dynamic LDS. q, k, v 16-byte aligned, their pitches multiples of 4 and at most
+// AbLayout<HD, NW, QPW>::BYTES of dynamic LDS. q, k, v 16-byte aligned, their pitches multiples of 4 and at most
 // INT32_MAX / FA_KT; VEC: ldo a multiple of 4 and out 16-byte aligned.
-template <int HD, int NW, bool VEC>
-__global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(AttnBias p) {
+template <int HD, int NW, int QPW, bool VEC>
+__global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attention_bias(AttnBias p) {
     using Fa = FaLayout<HD>;
-    using Lay = AbLayout<HD, NW>;
-    constexpr int NT = 64 * NW, QB = 32 * NW;
+    using Lay = AbLayout<HD, NW, QPW>;
+    constexpr int NT = 64 * NW, QB = 32 * NW * QPW, WPT = (Lay::WINDOW + NT - 1) / NT;
     constexpr int NB = HD / 16, NOT = HD / 32;
     constexpr int KCH = FA_KT * HD / 8, VCH = (FA_KT / 2) * HD / 4;
     constexpr int KPT = (KCH + NT - 1) / NT, VPT = (VCH + NT - 1) / NT;
@@ -122,7 +143,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
     int64_t row0;
     int L, q0;
     if (!ab_rows<QB>(p, logical - head * per_head, row0, L, q0)) return;
-    const int qw = q0 + 32 * wave;
+    const int qw = q0 + 32 * QPW * wave;  // the wavefront's first query
     const bool active = qw < L;
     const int nt = (L + FA_KT - 1) / FA_KT;
     const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
@@ -130,15 +151,16 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
     const float *table = p.table ? p.table + (int64_t)head * (2 * p.reach + 1) + p.reach : nullptr;
     const float c = p.scale * FA_LOG2E;  // of the queries: scores come out in base 2
 
-    vec8 qh[NB], ql[NB];
-    float qt[NB][8];
-    {
-        const float *qrow = p.q + (row0 + min(qw + r, L - 1)) * p.ldq + head * HD;
+    vec8 qh[QPW][NB], ql[QPW][NB];
+    float qt[QPW][NB][8];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) load8(qrow + 16 * b + 8 * hf, qt[b]);
+    for (int u = 0; u < QPW; ++u) {
+        const float *qrow = p.q + (row0 + min(qw + 32 * u + r, L - 1)) * p.ldq + head * HD;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) load8(qrow + 16 * b + 8 * hf, qt[u][b]);
     }
     f32x4 kr[KPT][2], vr[VPT][2];
-    float br = 0.0f;
+    float br[WPT] = {};
     const int ldk = (int)p.ldk, ldv = (int)p.ldv;
     auto load_tile = [&](int t) {
         const int kb0 = t * FA_KT, klast = L - 1 - kb0;
@@ -162,12 +184,10 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
             }
         }
         // word w of the window: key kb0 + kk, query q0 + qi, w = kk - qi + QB - 1
-        if (table != nullptr && tid < Lay::WINDOW) {
-            const int d = kb0 - q0 - (QB - 1) + tid;
-            br = table[min(max(d, -p.reach), p.reach)];
-        }
+        if (table != nullptr)
+#pragma unroll
+            for (int i = 0; i < WPT; ++i) br[i] = table[min(max(kb0 - q0 - (QB - 1) + tid + NT * i, -p.reach), p.reach)];
     };
-    static_assert(Lay::WINDOW <= NT, "a word of the window a thread");
     auto store_tile = [&](int s) {
         char *khi = ab_lds + s * Fa::STAGE, *klo = khi + Fa::KPLANE;
         char *vhi = klo + Fa::KPLANE, *vlo = vhi + Fa::VPLANE;
@@ -202,23 +222,31 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
                 }
             }
         }
-        if (tid < Lay::WINDOW) reinterpret_cast<float *>(ab_lds + Lay::BIAS)[s * Lay::WINDOW + tid] = br;
+#pragma unroll
+        for (int i = 0; i < WPT; ++i)
+            if (tid + NT * i < Lay::WINDOW) reinterpret_cast<float *>(ab_lds + Lay::BIAS)[s * Lay::WINDOW + tid + NT * i] = br[i];
     };
 
-    f32x16 o[NOT];
+    f32x16 o[QPW][NOT];
+    float m_run[QPW], l_run[QPW];
 #pragma unroll
-    for (int i = 0; i < NOT; ++i)
+    for (int u = 0; u < QPW; ++u) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
+        for (int i = 0; i < NOT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[u][i][e] = 0.0f;
+        m_run[u] = -INFINITY, l_run[u] = 0.0f;
+    }
 
     load_tile(0);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
+    for (int u = 0; u < QPW; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) qt[b][i] *= c;
-        ab_split8(qt[b], qh[b], ql[b]);
-    }
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qt[u][b][i] *= c;
+            ab_split8(qt[u][b], qh[u][b], ql[u][b]);
+        }
     store_tile(0);
     lds_barrier();
     for (int t = 0; t < nt; ++t) {
@@ -232,52 +260,58 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
                 const int key0 = t * FA_KT + 32 * s;
                 if (key0 >= L) break;  // uniform: no barrier inside
                 // the scores' sums start at the bias; element e is key key0 + 4 hf + 8 (e / 4) + e % 4
-                const float *bw = window + (32 * s + 4 * hf - (32 * wave + r) + QB - 1);
-                f32x16 acc;
+                f32x16 acc[QPW];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[e] = bw[8 * (e >> 2) + (e & 3)];
+                for (int u = 0; u < QPW; ++u) {
+                    const float *bw = window + (32 * s + 4 * hf - (32 * (QPW * wave + u) + r) + QB - 1);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[u][e] = bw[8 * (e >> 2) + (e & 3)];
+                }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int off = (32 * s + r) * Fa::KP + 2 * (16 * b + 8 * hf);
                     const vec8 kh = *reinterpret_cast<const vec8 *>(khi + off);
                     const vec8 kl = *reinterpret_cast<const vec8 *>(klo + off);
-                    acc = mfma_split3(kh, kl, qh[b], ql[b], acc);
+                    ab_mfma3<QPW>(kh, kl, [&](int u) { return qh[u][b]; }, [&](int u) { return ql[u][b]; }, acc);
                 }
-                const int lim = L - key0 - 4 * hf;
-                if (__builtin_expect(key0 + 32 > L, 0)) {
+                vec8 ph[QPW][2], pl[QPW][2];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (8 * (e >> 2) + (e & 3) >= lim) acc[e] = -INFINITY;
+                for (int u = 0; u < QPW; ++u) {
+                    const int lim = L - key0 - 4 * hf;
+                    if (__builtin_expect(key0 + 32 > L, 0)) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (8 * (e >> 2) + (e & 3) >= lim) acc[u][e] = -INFINITY;
+                    }
+                    float mloc = acc[u][0];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, acc[u][e]);
+                    {
+                        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
+                        mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+                    }
+                    // The subtracted maximum follows a query's running maximum only when that is AB_LAZY above it:
+                    // weights up to 2^AB_LAZY keep their precision, and after the first tiles nothing is rescaled.
+                    const bool up = mloc > m_run[u] + AB_LAZY;
+                    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+                        const float alpha = up ? __builtin_amdgcn_exp2f(m_run[u] - mloc) : 1.0f;
+                        m_run[u] = up ? mloc : m_run[u];
+                        l_run[u] *= alpha;
+#pragma unroll
+                        for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[u][i][e] *= alpha;
+                    }
+                    const float m_use = m_run[u] == -INFINITY ? 0.0f : m_run[u];  // nothing attended so far: every weight is 0
+                    float x[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(acc[u][e] - m_use);
+                        l_run[u] += x[e];
+                    }
+                    ab_split8(x, ph[u][0], pl[u][0]);
+                    ab_split8(x + 8, ph[u][1], pl[u][1]);
                 }
-                float mloc = acc[0];
-#pragma unroll
-                for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, acc[e]);
-                {
-                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
-                    mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-                }
-                // The subtracted maximum follows a query's running maximum only when that is AB_LAZY above it: weights
-                // up to 2^AB_LAZY keep their precision, and after the first tiles nothing is rescaled.
-                const bool up = mloc > m_run + AB_LAZY;
-                if (__builtin_amdgcn_ballot_w64(up) != 0) {
-                    const float alpha = up ? __builtin_amdgcn_exp2f(m_run - mloc) : 1.0f;
-                    m_run = up ? mloc : m_run;
-                    l_run *= alpha;
-#pragma unroll
-                    for (int i = 0; i < NOT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
-                }
-                const float m_use = m_run == -INFINITY ? 0.0f : m_run;  // nothing attended so far: every weight is 0
-                float x[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(acc[e] - m_use);
-                    l_run += x[e];
-                }
-                vec8 ph[2], pl[2];
-                ab_split8(x, ph[0], pl[0]);
-                ab_split8(x + 8, ph[1], pl[1]);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
@@ -286,7 +320,12 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
                         const int off = (32 * i + r) * Fa::VP + 64 * s + 32 * (kb ^ (i & 1)) + 16 * (hf ^ (r >> 4));
                         const vec8 vh = *reinterpret_cast<const vec8 *>(vhi + off);
                         const vec8 vl = *reinterpret_cast<const vec8 *>(vlo + off);
-                        o[i] = mfma_split3(vh, vl, ph[kb], pl[kb], o[i]);
+                        f32x16 d[QPW];
+#pragma unroll
+                        for (int u = 0; u < QPW; ++u) d[u] = o[u][i];
+                        ab_mfma3<QPW>(vh, vl, [&](int u) { return ph[u][kb]; }, [&](int u) { return pl[u][kb]; }, d);
+#pragma unroll
+                        for (int u = 0; u < QPW; ++u) o[u][i] = d[u];
                     }
                 }
                 __builtin_amdgcn_s_setprio(0);
@@ -297,25 +336,22 @@ __global__ __launch_bounds__(64 * NW, HD == 128 ? 2 : 4) void attention_bias(Att
     }
 
     if (!active) return;
-    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-    if (qw + r >= L) return;
-    float *orow = p.out + (row0 + qw + r) * p.ldo + head * HD;
 #pragma unroll
-    for (int i = 0; i < NOT; ++i)
+    for (int u = 0; u < QPW; ++u) {
+        const float l_tot = l_run[u] + __shfl_xor(l_run[u], 32, 64);
+        const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+        const int query = qw + 32 * u + r;
+        if (query >= L) continue;
+        float *orow = p.out + (row0 + query) * p.ldo + head * HD;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int col = 32 * i + 8 * g + 4 * hf;
-            const f32x4 val = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
-            if (VEC) {
-                *reinterpret_cast<f32x4 *>(orow + col) = val;
-            } else {
-                orow[col] = val.x;
-                orow[col + 1] = val.y;
-                orow[col + 2] = val.z;
-                orow[col + 3] = val.w;
+        for (int i = 0; i < NOT; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x16 &a = o[u][i];
+                ab_store<VEC>(orow + 32 * i + 8 * g + 4 * hf,
+                              f32x4{a[4 * g] * inv, a[4 * g + 1] * inv, a[4 * g + 2] * inv, a[4 * g + 3] * inv});
             }
-        }
+    }
 }
 
 }  // namespace enchip

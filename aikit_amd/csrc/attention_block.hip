@@ -213,11 +213,11 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos h) {
 
 namespace {
 
-template <int HD, int NW, bool VEC>
+template <int HD, int NW, int QPW, bool VEC>
 int launch_attention_bias(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
-    using Lay = enchip::AbLayout<HD, NW>;
-    constexpr int QB = 32 * NW;
-    const void *fn = reinterpret_cast<const void *>(enchip::attention_bias<HD, NW, VEC>);
+    using Lay = enchip::AbLayout<HD, NW, QPW>;
+    constexpr int QB = 32 * NW * QPW;
+    const void *fn = reinterpret_cast<const void *>(enchip::attention_bias<HD, NW, QPW, VEC>);
     const std::pair<const void *, size_t> key(fn, (size_t)Lay::BYTES);
     if (std::find(ctx->lds_set.begin(), ctx->lds_set.end(), key) == ctx->lds_set.end()) {
         HIP_TRY(ctx, hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Lay::BYTES));
@@ -230,7 +230,7 @@ int launch_attention_bias(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
         return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: %lld query blocks of %d heads are more than one launch holds",
                     (long long)per, p.heads);
     if (p.spans) {
-        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, VEC>), dim3((unsigned)(per * p.heads)), dim3(64 * NW), Lay::BYTES, s, p);
+        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, QPW, VEC>), dim3((unsigned)(per * p.heads)), dim3(64 * NW), Lay::BYTES, s, p);
         return check_launch(ctx, "attention_bias");
     }
     const int64_t chunk = most / per, nseq = p.nseq;
@@ -239,7 +239,7 @@ int launch_attention_bias(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
         enchip::AttnBias c = p;
         c.q += z0 * p.L * p.ldq, c.k += z0 * p.L * p.ldk, c.v += z0 * p.L * p.ldv, c.out += z0 * p.L * p.ldo;
         c.nseq = (int)nz;
-        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, VEC>), dim3((unsigned)(per * nz * p.heads)), dim3(64 * NW), Lay::BYTES, s, c);
+        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, QPW, VEC>), dim3((unsigned)(per * nz * p.heads)), dim3(64 * NW), Lay::BYTES, s, c);
     }
     return check_launch(ctx, "attention_bias");
 }
@@ -289,10 +289,14 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     p.L = (int)L;
     p.scale = scale;
     const bool vec = ldo % 4 == 0 && (uintptr_t)d_out % 16 == 0;
-#define AB_CALL(HD) return vec ? launch_attention_bias<HD, 8, true>(ctx, p, s) : launch_attention_bias<HD, 8, false>(ctx, p, s)
-    if (head_dim == 32) AB_CALL(32);
-    if (head_dim == 64) AB_CALL(64);
-    AB_CALL(128);
+#ifndef ABNW
+#define ABNW 8
+#define ABQ 2
+#endif
+#define AB_CALL(HD, NW, QPW) return vec ? launch_attention_bias<HD, NW, QPW, true>(ctx, p, s) : launch_attention_bias<HD, NW, QPW, false>(ctx, p, s)
+    if (head_dim == 32) AB_CALL(32, ABNW, ABQ);
+    if (head_dim == 64) AB_CALL(64, ABNW, ABQ);
+    AB_CALL(128, 8, 1);
 #undef AB_CALL
 }
 
