@@ -31,10 +31,16 @@ struct AttnBias {
     const int2 *spans;   // [nseq] start, end of ascending spans; null: nseq sequences of L rows
     const float *table;  // [heads][2 reach + 1], b log2 e of distance -reach .. reach; null: no bias
     int nseq, heads, group, reach;
-    int blocks;  // with spans: query blocks of a head, L / (32 NW) + nseq
     int L;       // rows of a sequence, or with spans those of the buffers
+    int share;   // log2 of the heads of one key head that a workgroup takes, beside each other
+    int parts;   // workgroups that split a query's keys
+    float *part, *stat;  // parts > 1: [parts][rows][heads][hd] contexts, [parts][rows][heads][2] maxima and sums
+    int64_t rows;        // of the buffers
     float scale;
 };
+
+// Key tiles of each of a sequence's parts.
+__device__ __forceinline__ int ab_part_tiles(int nt, int parts) { return (nt + parts - 1) / parts; }
 
 // x less the low (high) half of h, exactly: one mixed fused multiply-add in place of a conversion and a subtraction.
 __device__ __forceinline__ float ab_rest_lo(uint32_t h, float x) {
@@ -66,26 +72,26 @@ __device__ __forceinline__ void ab_split8(const float *x, f16x8 &hi, f16x8 &lo) 
 template <int HD, int NW, int QPW>
 struct AbLayout {
     using Fa = FaLayout<HD>;
-    static constexpr int WINDOW = 32 * NW * QPW + FA_KT;  // distances of a tile (one to spare)
+    static constexpr int WINDOW = 32 * NW * QPW + NW * FA_KT;  // most words of a tile's windows
     static constexpr int BIAS = 2 * Fa::STAGE;      // two windows behind the two stages
     static constexpr int BYTES = BIAS + 2 * WINDOW * 4;
 };
 
-// The workgroup's rows: false where it has none. Of ascending spans, span z has the query blocks
-// start / QB + z .. of the launch, at least as many as it needs; the last span whose first block is at or
-// below b is found 64 at a time. (Spans out of order leave queries out; nothing is read past the buffers.)
-template <int QB>
-__device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int64_t &row0, int &len, int &q0) {
+// The workgroup's rows, QR = 2^qs queries from q0 on of the L from row0 on: false where it has none. Of ascending
+// spans, span z has the query blocks start / QR + z .. of the launch, at least as many as it needs; the last span
+// whose first block is at or below b is found 64 at a time. (Spans out of order leave queries out; nothing is
+// read past the buffers.)
+__device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int qs, int64_t &row0, int &len, int &q0) {
     if (p.spans == nullptr) {
-        const int nqb = (p.L + QB - 1) / QB, z = b / nqb;
-        row0 = (int64_t)z * p.L, len = p.L, q0 = (b - z * nqb) * QB;
+        const int nqb = (p.L + (1 << qs) - 1) >> qs, z = b / nqb;
+        row0 = (int64_t)z * p.L, len = p.L, q0 = (b - z * nqb) << qs;
         return true;
     }
     const int lane = threadIdx.x & 63;
     int lo = 0, n = p.nseq;
     for (;;) {
         const int step = (n + 63) / 64, z = lo + lane * step;
-        const bool in = lane * step < n && max(p.spans[min(z, p.nseq - 1)].x, 0) / QB + z <= b;
+        const bool in = lane * step < n && (max(p.spans[min(z, p.nseq - 1)].x, 0) >> qs) + z <= b;
         const int below = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
         if (below == 0) return false;
         n = min(step, n - (below - 1) * step);
@@ -95,7 +101,7 @@ __device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int64_t &row0,
     lo = __builtin_amdgcn_readfirstlane(lo);
     const int2 s = p.spans[lo];
     const int start = min(max(s.x, 0), p.L), end = min(max(s.y, start), p.L);
-    const int64_t at = (int64_t)(b - (start / QB + lo)) * QB;
+    const int64_t at = (int64_t)(b - ((start >> qs) + lo)) << qs;
     if (at < 0 || at >= end - start) return false;
     row0 = start, len = end - start, q0 = (int)at;
     return true;
@@ -122,7 +128,11 @@ __device__ __forceinline__ void ab_store(float *to, f32x4 v) {
     }
 }
 
-// A 1-D grid of heads * query blocks, XCD-aware (a sequence's query blocks of one head on one XCD),
+// A workgroup takes 32 NW QPW queries: QR = 32 NW QPW / 2^share rows of each of 2^share heads that have their keys in
+// common, so that these are split once for all of them (and short sequences fill more of a workgroup).
+// With parts > 1 the keys are split too, whole tiles to a part, and the contexts, not divided, go to scratch with their
+// maxima and sums (attention_bias_join).
+// A 1-D grid of (heads >> share) * parts * query blocks, XCD-aware (a sequence's query blocks of one head on one XCD),
 // AbLayout<HD, NW, QPW>::BYTES of dynamic LDS. q, k, v 16-byte aligned, their pitches multiples of 4 and at most
 // INT32_MAX / FA_KT; VEC: ldo a multiple of 4 and out 16-byte aligned.
 template <int HD, int NW, int QPW, bool VEC>
@@ -138,17 +148,28 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
     extern __shared__ __attribute__((aligned(16))) char ab_lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, hf = lane >> 5;
-    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_head = gridDim.x / p.heads;
-    const int head = logical / per_head;
+    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_part = gridDim.x / ((p.heads >> p.share) * p.parts);
+    const int sp = logical / per_part, set = sp / p.parts, part = sp - set * p.parts, qs = __builtin_ctz(QB) - p.share, QR = 1 << qs;
     int64_t row0;
     int L, q0;
-    if (!ab_rows<QB>(p, logical - head * per_head, row0, L, q0)) return;
-    const int qw = q0 + 32 * QPW * wave;  // the wavefront's first query
+    if (!ab_rows(p, logical - sp * per_part, qs, row0, L, q0)) return;
+    // the wavefront's head and its first query
+    const int mate = (wave * 32 * QPW) >> qs, head = (set << p.share) + mate, qr = (wave * 32 * QPW) & (QR - 1), qw = q0 + qr;
     const bool active = qw < L;
-    const int nt = (L + FA_KT - 1) / FA_KT;
+    const int tiles = (L + FA_KT - 1) / FA_KT, per = ab_part_tiles(tiles, p.parts), tbeg = part * per, nt = min(tiles, tbeg + per);
+    if (tbeg >= nt) return;
     const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
     const float *vbase = p.v + row0 * p.ldv + (head / p.group) * HD;
-    const float *table = p.table ? p.table + (int64_t)head * (2 * p.reach + 1) + p.reach : nullptr;
+    // word w of a head's window: key kb0 + kk, query q0 + qi, w = kk - qi + QR - 1. A thread's words, as distances at
+    // key 0 and places in the table.
+    const int pitch = QR + FA_KT;
+    int dist[WPT], place[WPT];
+#pragma unroll
+    for (int i = 0; i < WPT; ++i) {
+        const int w = tid + NT * i, m = min(w / pitch, (1 << p.share) - 1);
+        dist[i] = w - m * pitch - q0 - (QR - 1);
+        place[i] = ((set << p.share) + m) * (2 * p.reach + 1) + p.reach;
+    }
     const float c = p.scale * FA_LOG2E;  // of the queries: scores come out in base 2
 
     vec8 qh[QPW][NB], ql[QPW][NB];
@@ -183,10 +204,9 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
                 vr[i][1] = *reinterpret_cast<const f32x4 *>(vt + (min(2 * pr + 1, klast) * ldv + col));
             }
         }
-        // word w of the window: key kb0 + kk, query q0 + qi, w = kk - qi + QB - 1
-        if (table != nullptr)
+        if (p.table != nullptr)
 #pragma unroll
-            for (int i = 0; i < WPT; ++i) br[i] = table[min(max(kb0 - q0 - (QB - 1) + tid + NT * i, -p.reach), p.reach)];
+            for (int i = 0; i < WPT; ++i) br[i] = p.table[place[i] + min(max(kb0 + dist[i], -p.reach), p.reach)];
     };
     auto store_tile = [&](int s) {
         char *khi = ab_lds + s * Fa::STAGE, *klo = khi + Fa::KPLANE;
@@ -238,7 +258,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
         m_run[u] = -INFINITY, l_run[u] = 0.0f;
     }
 
-    load_tile(0);
+    load_tile(tbeg);
 #pragma unroll
     for (int u = 0; u < QPW; ++u)
 #pragma unroll
@@ -247,14 +267,14 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
             for (int i = 0; i < 8; ++i) qt[u][b][i] *= c;
             ab_split8(qt[u][b], qh[u][b], ql[u][b]);
         }
-    store_tile(0);
+    store_tile(tbeg & 1);
     lds_barrier();
-    for (int t = 0; t < nt; ++t) {
+    for (int t = tbeg; t < nt; ++t) {
         if (t + 1 < nt) load_tile(t + 1);
         if (active) {
             const char *khi = ab_lds + (t & 1) * Fa::STAGE, *klo = khi + Fa::KPLANE;
             const char *vhi = klo + Fa::KPLANE, *vlo = vhi + Fa::VPLANE;
-            const float *window = reinterpret_cast<const float *>(ab_lds + Lay::BIAS) + (t & 1) * Lay::WINDOW;
+            const float *window = reinterpret_cast<const float *>(ab_lds + Lay::BIAS) + (t & 1) * Lay::WINDOW + mate * pitch;
 #pragma unroll
             for (int s = 0; s < FA_KT / 32; ++s) {
                 const int key0 = t * FA_KT + 32 * s;
@@ -263,7 +283,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
                 f32x16 acc[QPW];
 #pragma unroll
                 for (int u = 0; u < QPW; ++u) {
-                    const float *bw = window + (32 * s + 4 * hf - (32 * (QPW * wave + u) + r) + QB - 1);
+                    const float *bw = window + (32 * s + 4 * hf - (qr + 32 * u + r) + QR - 1);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[u][e] = bw[8 * (e >> 2) + (e & 3)];
                 }
@@ -339,10 +359,16 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
 #pragma unroll
     for (int u = 0; u < QPW; ++u) {
         const float l_tot = l_run[u] + __shfl_xor(l_run[u], 32, 64);
-        const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+        float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
         const int query = qw + 32 * u + r;
         if (query >= L) continue;
         float *orow = p.out + (row0 + query) * p.ldo + head * HD;
+        if (p.parts > 1) {
+            const int64_t at = (part * p.rows + row0 + query) * p.heads + head;
+            orow = p.part + at * HD;
+            inv = 1.0f;
+            if (hf == 0) *reinterpret_cast<float2 *>(p.stat + 2 * at) = make_float2(m_run[u], l_tot);
+        }
 #pragma unroll
         for (int i = 0; i < NOT; ++i)
 #pragma unroll
@@ -351,6 +377,188 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
                 ab_store<VEC>(orow + 32 * i + 8 * g + 4 * hf,
                               f32x4{a[4 * g] * inv, a[4 * g + 1] * inv, a[4 * g + 2] * inv, a[4 * g + 3] * inv});
             }
+    }
+}
+
+// The parts of 32 rows of one head joined: out = sum_p o_p 2^(m_p - m) / sum_p l_p 2^(m_p - m).
+template <int HD>
+__global__ __launch_bounds__(256) void attention_bias_join(AttnBias p) {
+    const int per_head = gridDim.x / p.heads, head = blockIdx.x / per_head;
+    int64_t row0;
+    int L, q0;
+    if (!ab_rows(p, blockIdx.x - head * per_head, 5, row0, L, q0)) return;
+    const int tiles = (L + FA_KT - 1) / FA_KT, per = ab_part_tiles(tiles, p.parts), parts = (tiles + per - 1) / per;
+    for (int i = threadIdx.x; i < 32 * HD / 4; i += 256) {
+        const int query = q0 + i / (HD / 4), col = 4 * (i % (HD / 4));
+        if (query >= L) break;
+        const int64_t at = (row0 + query) * p.heads + head, step = p.rows * p.heads;
+        float m = -INFINITY, l = 0.0f;
+        for (int u = 0; u < parts; ++u) m = fmaxf(m, p.stat[2 * (at + u * step)]);
+        if (m == -INFINITY) m = 0.0f;
+        f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < parts; ++u) {
+            const float2 st = *reinterpret_cast<const float2 *>(p.stat + 2 * (at + u * step));
+            const f32x4 o = *reinterpret_cast<const f32x4 *>(p.part + (at + u * step) * HD + col);
+            const float f = __builtin_amdgcn_exp2f(st.x - m);
+            l += st.y * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] += o[e] * f;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float *to = p.out + (row0 + query) * p.ldo + head * HD + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = c[e] * inv;
+    }
+}
+
+// Few queries: a workgroup takes 32 of one head and its NW wavefronts the head's keys, 32-key blocks w, w + NW, ...
+// each with a softmax of its own; the NW maxima, sums and contexts meet in LDS. Nothing is shared before that, so
+// keys and values go from memory straight to registers in the MFMA's order (a lane's value column is 8 loads of 4
+// bytes, 32 lanes side by side), and there is no barrier in the loop: a call is a few memory round trips long.
+template <int HD, int NW>
+struct AbSplit {
+    static constexpr int PITCH = HD + 4;  // floats of a query's context: 8 of them start in distinct banks
+    static constexpr int BYTES = NW * 32 * (PITCH + 2) * 4;
+};
+
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attention_bias_split(AttnBias p) {
+    using Lay = AbSplit<HD, NW>;
+    constexpr int NB = HD / 16, NOT = HD / 32;
+    extern __shared__ __attribute__((aligned(16))) char ab_lds[];
+    float *ctx = reinterpret_cast<float *>(ab_lds), *top = ctx + NW * 32 * Lay::PITCH, *sum = top + NW * 32;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
+    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_head = gridDim.x / p.heads, head = logical / per_head;
+    int64_t row0;
+    int L, q0;
+    if (!ab_rows(p, logical - head * per_head, 5, row0, L, q0)) return;
+    const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
+    const float *vbase = p.v + row0 * p.ldv + (head / p.group) * HD;
+    const float *table = p.table ? p.table + (int64_t)head * (2 * p.reach + 1) + p.reach : nullptr;
+    const int ldk = (int)p.ldk, ldv = (int)p.ldv;
+    f16x8 qh[NB], ql[NB];
+    f32x16 o[NOT];
+#pragma unroll
+    for (int i = 0; i < NOT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+    float qt[NB][8];
+    {
+        const float *qrow = p.q + (row0 + min(q0 + r, L - 1)) * p.ldq + head * HD;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) load8(qrow + 16 * b + 8 * hf, qt[b]);
+    }
+    for (int key0 = 32 * wave, first = 1; key0 < L; key0 += 32 * NW, first = 0) {
+        const float *kt = kbase + (int64_t)key0 * ldk, *vt = vbase + (int64_t)key0 * ldv;
+        const int last = L - 1 - key0;
+        // heads of 128 load half of a key at a time, and 16 keys' values, for the registers
+        constexpr bool AHEAD = HD < 128;
+        constexpr int KN = AHEAD ? NB : NB / 2, VN = AHEAD ? 2 : 1;
+        float kx[KN][8], vx[NOT][VN][8];
+        f32x16 acc;
+        auto load_k = [&](int b0) {
+#pragma unroll
+            for (int b = 0; b < KN; ++b) load8(kt + (min(r, last) * ldk + 16 * (b0 + b) + 8 * hf), kx[b]);
+        };
+        load_k(0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int d = key0 + 4 * hf + 8 * (e >> 2) + (e & 3) - (q0 + r);
+            acc[e] = table != nullptr ? table[min(max(d, -p.reach), p.reach)] : 0.0f;
+        }
+        // value column 32 i + r: the eight keys at depth 8 hf .. of 16-key block kb
+        auto load_v = [&](int kb) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float *row = vt + (min(16 * kb + 4 * hf + (j & 3) + 2 * (j & 4), last) * ldv + r);
+#pragma unroll
+                for (int i = 0; i < NOT; ++i) vx[i][kb % VN][j] = row[32 * i];
+            }
+        };
+        if (AHEAD) load_v(0), load_v(1);
+        if (first) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) qt[b][i] *= p.scale * FA_LOG2E;
+                ab_split8(qt[b], qh[b], ql[b]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (b > 0 && b % KN == 0) load_k(b);
+            f16x8 kh, kl;
+            ab_split8(kx[b % KN], kh, kl);
+            acc = mfma_split3(kh, kl, qh[b], ql[b], acc);
+        }
+        if (!AHEAD) load_v(0);
+        if (key0 + 32 > L) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (8 * (e >> 2) + (e & 3) >= L - key0 - 4 * hf) acc[e] = -INFINITY;
+        }
+        float m = acc[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) m = fmaxf(m, acc[e]);
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        m = fmaxf(m, m_run);
+        const float m_use = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        m_run = m;
+        l_run *= alpha;
+#pragma unroll
+        for (int i = 0; i < NOT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x[e] = __builtin_amdgcn_exp2f(acc[e] - m_use);
+            l_run += x[e];
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            f16x8 ph, pl;
+            ab_split8(x + 8 * kb, ph, pl);
+            if (!AHEAD && kb > 0) load_v(kb);
+#pragma unroll
+            for (int i = 0; i < NOT; ++i) {
+                f16x8 vh, vl;
+                ab_split8(vx[i][kb % VN], vh, vl);
+                o[i] = mfma_split3(vh, vl, ph, pl, o[i]);
+            }
+        }
+    }
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (hf == 0) top[wave * 32 + r] = m_run, sum[wave * 32 + r] = l_run;
+#pragma unroll
+    for (int i = 0; i < NOT; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4 *>(ctx + (wave * 32 + r) * Lay::PITCH + 32 * i + 8 * g + 4 * hf) =
+                f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+    __syncthreads();
+    const int parts = min(NW, (L + 31) / 32);  // wavefronts that had keys
+    for (int at = tid; at < 32 * HD / 4; at += 64 * NW) {
+        const int query = at / (HD / 4), col = 4 * (at % (HD / 4));
+        if (q0 + query >= L) break;
+        float m = -INFINITY;
+        for (int w = 0; w < parts; ++w) m = fmaxf(m, top[w * 32 + query]);
+        if (m == -INFINITY) m = 0.0f;
+        float l = 0.0f;
+        f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < parts; ++w) {
+            const float f = __builtin_amdgcn_exp2f(top[w * 32 + query] - m);
+            l += sum[w * 32 + query] * f;
+            const f32x4 part = *reinterpret_cast<const f32x4 *>(ctx + (w * 32 + query) * Lay::PITCH + col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] += part[e] * f;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float *to = p.out + (row0 + q0 + query) * p.ldo + head * HD + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = c[e] * inv;
     }
 }
 

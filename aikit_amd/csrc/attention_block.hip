@@ -213,35 +213,109 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos h) {
 
 namespace {
 
-template <int HD, int NW, int QPW, bool VEC>
-int launch_attention_bias(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
-    using Lay = enchip::AbLayout<HD, NW, QPW>;
-    constexpr int QB = 32 * NW * QPW;
-    const void *fn = reinterpret_cast<const void *>(enchip::attention_bias<HD, NW, QPW, VEC>);
-    const std::pair<const void *, size_t> key(fn, (size_t)Lay::BYTES);
+// Launches fn over (query blocks of 2^qs rows) x (head sets), in chunks of sequences whose threads are numbered in 32
+// bits.
+int launch_attention_bias(enchip_ctx *ctx, void (*fn)(enchip::AttnBias), int lds, int threads, int qs, enchip::AttnBias p, hipStream_t s) {
+    const std::pair<const void *, size_t> key(reinterpret_cast<const void *>(fn), (size_t)lds);
     if (std::find(ctx->lds_set.begin(), ctx->lds_set.end(), key) == ctx->lds_set.end()) {
-        HIP_TRY(ctx, hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Lay::BYTES));
+        HIP_TRY(ctx, hipFuncSetAttribute(key.first, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         ctx->lds_set.push_back(key);
     }
-    // sequences of one launch: its threads are numbered in 32 bits
-    const int64_t per = p.spans ? (int64_t)p.L / QB + p.nseq : ((int64_t)p.L + QB - 1) / QB;
-    const int64_t most = (((int64_t)1 << 32) - 1) / (64 * NW) / p.heads;
+    const int64_t qr = (int64_t)1 << qs, sets = (int64_t)(p.heads >> p.share) * p.parts;
+    const int64_t per = p.spans ? p.L / qr + p.nseq : (p.L + qr - 1) / qr;
+    const int64_t most = (((int64_t)1 << 32) - 1) / threads / sets;
     if (per > most)
         return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: %lld query blocks of %d heads are more than one launch holds",
                     (long long)per, p.heads);
-    if (p.spans) {
-        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, QPW, VEC>), dim3((unsigned)(per * p.heads)), dim3(64 * NW), Lay::BYTES, s, p);
-        return check_launch(ctx, "attention_bias");
-    }
-    const int64_t chunk = most / per, nseq = p.nseq;
+    const int64_t chunk = p.spans ? p.nseq : most / per, nseq = p.nseq;
     for (int64_t z0 = 0; z0 < nseq; z0 += chunk) {
-        const int64_t nz = std::min(chunk, nseq - z0);
+        const int64_t nz = std::min(chunk, nseq - z0), row = z0 * p.L;  // z0 > 0 without spans only
         enchip::AttnBias c = p;
-        c.q += z0 * p.L * p.ldq, c.k += z0 * p.L * p.ldk, c.v += z0 * p.L * p.ldv, c.out += z0 * p.L * p.ldo;
+        c.q += row * p.ldq, c.k += row * p.ldk, c.v += row * p.ldv, c.out += row * p.ldo;
         c.nseq = (int)nz;
-        hipLaunchKernelGGL((enchip::attention_bias<HD, NW, QPW, VEC>), dim3((unsigned)(per * nz * p.heads)), dim3(64 * NW), Lay::BYTES, s, c);
+        hipLaunchKernelGGL(fn, dim3((unsigned)(per * (p.spans ? 1 : nz) * sets)), dim3((unsigned)threads), (size_t)lds, s, c);
     }
     return check_launch(ctx, "attention_bias");
+}
+
+// Heads of one key head that a workgroup of nw wavefronts takes beside each other: a power of two of them, its log2.
+int heads_beside(int64_t group, int nw) {
+    int share = 0;
+    while (share < 3 && (2 << share) <= nw && (group >> share) % 2 == 0) ++share;
+    return share;
+}
+
+template <int HD, int NW, int QPW>
+int attention_bias_tiles(enchip_ctx *ctx, enchip::AttnBias p, bool vec, int parts, hipStream_t s) {
+    const int qs = __builtin_ctz(32 * NW * QPW), threads = 64 * NW, lds = enchip::AbLayout<HD, NW, QPW>::BYTES;
+    p.share = heads_beside(p.group, NW);
+    if (parts == 1)
+        return launch_attention_bias(ctx, vec ? enchip::attention_bias<HD, NW, QPW, true> : enchip::attention_bias<HD, NW, QPW, false>,
+                                     lds, threads, qs - p.share, p, s);
+    int rc;
+    const size_t outputs = (size_t)parts * (size_t)p.rows * (size_t)p.heads;
+    if ((rc = ensure(ctx, &ctx->d_att, &ctx->att_cap, outputs * (HD + 2) * sizeof(float)))) return rc;
+    if ((rc = scratch_wait(ctx, s))) return rc;
+    p.parts = parts;
+    p.part = ctx->d_att;
+    p.stat = ctx->d_att + outputs * HD;
+    if ((rc = launch_attention_bias(ctx, enchip::attention_bias<HD, NW, QPW, true>, lds, threads, qs - p.share, p, s))) return rc;
+    const int64_t per = p.spans ? p.L / 32 + p.nseq : (int64_t)((p.L + 31) / 32) * p.nseq;
+    hipLaunchKernelGGL(enchip::attention_bias_join<HD>, dim3((unsigned)(per * p.heads)), dim3(256), 0, s, p);
+    if ((rc = check_launch(ctx, "attention_bias_join"))) return rc;
+    return scratch_record(ctx, s);
+}
+
+template <int HD, int NW>
+int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
+    return launch_attention_bias(ctx, enchip::attention_bias_split<HD, NW>, enchip::AbSplit<HD, NW>::BYTES, 64 * NW, 5, p, s);
+}
+
+// How an attention runs, from its sizes (spans: as if all had their mean length).
+//   split  attention_bias_split, while a workgroup per 32 queries leaves CUs for 1.5 rounds and no head has more
+//          than 512 keys. Measured on MI355X, 12 heads of 64, us, split against tiles: 1 x 512 rows 12.9 against 23,
+//          4 x 128 6.3 against 11.5; past the rule 4 x 512 34 against 31, 1 x 768 29.4 against 28.5.
+//   else by tiles, the form (heads of 64: 512 queries a workgroup, or 256 and two workgroups a CU) and the parts that
+//   the keys are split into with the least estimated time. Measured for w workgroups on a CU, us per 64-key tile:
+//          heads of 32   1.9 alone, 3.1 for two at once      heads of 64, 256 queries   3.65, 5.0
+//          heads of 128  4.6, one at once                    heads of 64, 512 queries   4.4, one at once
+//   and 8 for each round's first loads and stores; joining parts 6 + 1.5 a part, and their bytes at 4 TB/s. With it
+//   (12 heads of 64): 1 x 8192 rows 637 by 256 queries, 560 by 512, 546 in four parts; 1 x 2048 138 -> 58 in five;
+//   1 x 1024 60 -> 34; 24 x 512 95 by 512, 85 by 256; 20011 packed rows of 1 to 1024 194 by 512, 152 by 256.
+struct AttnPlan {
+    bool split, wide;
+    int parts;
+};
+
+AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_t hd) {
+    AttnPlan plan{false, false, 1};
+    const int64_t cus = ctx->num_cus, len = p.spans ? std::max<int64_t>(1, p.L / p.nseq) : p.L;
+    auto blocks = [&](int64_t rows, int64_t heads) { return (len + rows - 1) / rows * p.nseq * heads; };
+    plan.split = len <= 512 && 2 * blocks(32, p.heads) <= 3 * cus;
+    if (plan.split) return plan;
+    const int64_t tiles = (len + enchip::FA_KT - 1) / enchip::FA_KT;
+    // the join numbers its threads in 32 bits
+    const int64_t join = (p.spans ? p.L / 32 + p.nseq : (int64_t)((p.L + 31) / 32) * p.nseq) * p.heads;
+    const int most = join * 256 < ((int64_t)1 << 32) ? (int)std::min<int64_t>(8, tiles) : 1;
+    double least = 0.0;
+    for (int wide = 0; wide <= (hd == 64 ? 1 : 0); ++wide) {
+        const bool two = hd == 32 || (hd == 64 && !wide);  // workgroups at once on a CU
+        const double alone = hd == 32 ? 1.9 : hd == 128 ? 4.6 : wide ? 4.4 : 3.65, both = hd == 32 ? 3.1 : 5.0;
+        const int share = heads_beside(p.group, hd == 64 && !wide ? 4 : 8);
+        const int64_t n = blocks((wide ? 512 : 256) >> share, p.heads >> share);
+        for (int parts = 1; parts <= most; ++parts) {
+            const int64_t w = (n * parts + cus - 1) / cus, rounds = two ? (w + 1) / 2 : w;
+            const double tile = two ? (double)(w / 2) * both + (double)(w % 2) * alone : (double)w * alone;
+            double us = (double)((tiles + parts - 1) / parts) * tile + 8.0 * (double)rounds;
+            if (parts > 1) us += 6.0 + 1.5 * parts + 8.0 * parts * (double)p.rows * p.heads * (double)hd / 4e6;
+            if (least == 0.0 || us < least) {
+                least = us;
+                plan.wide = wide != 0;
+                plan.parts = parts;
+            }
+        }
+    }
+    return plan;
 }
 
 }  // namespace
@@ -288,16 +362,19 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     p.nseq = (int)nseq, p.heads = (int)heads, p.group = (int)(heads / kv_heads), p.reach = (int)r.reach;
     p.L = (int)L;
     p.scale = scale;
+    p.share = 0;
+    p.parts = 1;
+    p.part = p.stat = nullptr;
+    p.rows = d_spans ? L : nseq * L;
     const bool vec = ldo % 4 == 0 && (uintptr_t)d_out % 16 == 0;
-#ifndef ABNW
-#define ABNW 8
-#define ABQ 2
-#endif
-#define AB_CALL(HD, NW, QPW) return vec ? launch_attention_bias<HD, NW, QPW, true>(ctx, p, s) : launch_attention_bias<HD, NW, QPW, false>(ctx, p, s)
-    if (head_dim == 32) AB_CALL(32, ABNW, ABQ);
-    if (head_dim == 64) AB_CALL(64, ABNW, ABQ);
-    AB_CALL(128, 8, 1);
-#undef AB_CALL
+    const AttnPlan plan = attention_plan(ctx, p, head_dim);
+    if (plan.split && head_dim == 32) return attention_bias_split<32, 8>(ctx, p, s);
+    if (plan.split && head_dim == 64) return attention_bias_split<64, 8>(ctx, p, s);
+    if (plan.split) return attention_bias_split<128, 8>(ctx, p, s);
+    if (head_dim == 32) return attention_bias_tiles<32, 8, 1>(ctx, p, vec, plan.parts, s);
+    if (head_dim == 64 && plan.wide) return attention_bias_tiles<64, 8, 2>(ctx, p, vec, plan.parts, s);
+    if (head_dim == 64) return attention_bias_tiles<64, 4, 2>(ctx, p, vec, plan.parts, s);
+    return attention_bias_tiles<128, 8, 1>(ctx, p, vec, plan.parts, s);
 }
 
 // ---------------------------------------------------------------------------- low-rank adapters

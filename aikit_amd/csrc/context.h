@@ -124,6 +124,8 @@ struct enchip_ctx {
     size_t fb_cap = 0;
     char *d_low = nullptr;  // the rows' low-rank parts (adapters.h)
     size_t low_cap = 0;
+    float *d_att = nullptr;  // parts of an attention's contexts (attention_bias.h)
+    size_t att_cap = 0;
     uint64_t *d_cand = nullptr;  // top-k candidates
     size_t cand_cap = 0;
     // enchip_ann_topk's device results, one block so that one copy brings them back:

@@ -634,7 +634,7 @@ int enchip_close(enchip_ctx *ctx) {
         }
         ctx->adapters.clear();
         void *bufs[] = {ctx->d_aq,  ctx->d_as, ctx->d_a,     ctx->d_dst,     ctx->d_bias,
-                        ctx->d_acc, ctx->d_fb, ctx->d_cand, ctx->d_hits, ctx->d_low};
+                        ctx->d_acc, ctx->d_fb, ctx->d_cand, ctx->d_hits, ctx->d_low, ctx->d_att};
         for (void *p : bufs)
             if (p) (void)hipFree(p);
         for (void *p : ctx->retired) (void)hipFree(p);

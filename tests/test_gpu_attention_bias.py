@@ -250,7 +250,11 @@ def test_more_blocks_than_one_round(ctx):
         if b > a:
             one = Case(2, 1, 64, b - a)
             one.x, one.table = c.x[a:b].copy(), c.table
-            assert np.array_equal(one.run(ctx, nseq=1, L=b - a), got[a:b])
+            # the kernel, and with it the order of the sums, goes by the sizes: each is within 2^-17 of the formula in
+            # all (Case.check), so they are within 2^-16 of each other
+            alone = one.run(ctx, nseq=1, L=b - a)
+            assert np.linalg.norm(alone - got[a:b]) <= 2.0 ** -16 * np.linalg.norm(alone)
+            one.check(ctx, nseq=1, L=b - a)
     torch.cuda.synchronize()
 
 
