@@ -414,7 +414,8 @@ __global__ __launch_bounds__(256) void attention_bias_join(AttnBias p) {
 // Few queries: a workgroup takes 32 of one head and its NW wavefronts the head's keys, 32-key blocks w, w + NW, ...
 // each with a softmax of its own; the NW maxima, sums and contexts meet in LDS. Nothing is shared before that, so
 // keys and values go from memory straight to registers in the MFMA's order (a lane's value column is 8 loads of 4
-// bytes, 32 lanes side by side), and there is no barrier in the loop: a call is a few memory round trips long.
+// bytes, 32 lanes side by side), and there is no barrier in the loop: a call is a few memory round trips long. With
+// NW = 1 it serves short sequences, many of them: no wavefront waits for another or is left without queries.
 template <int HD, int NW>
 struct AbSplit {
     static constexpr int PITCH = HD + 4;  // floats of a query's context: 8 of them start in distinct banks

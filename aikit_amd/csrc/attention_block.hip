@@ -282,16 +282,20 @@ int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
 //   and 8 for each round's first loads and stores; joining parts 6 + 1.5 a part, and their bytes at 4 TB/s. With it
 //   (12 heads of 64): 1 x 8192 rows 637 by 256 queries, 560 by 512, 546 in four parts; 1 x 2048 138 -> 58 in five;
 //   1 x 1024 60 -> 34; 24 x 512 95 by 512, 85 by 256; 20011 packed rows of 1 to 1024 194 by 512, 152 by 256.
+//   Rows of 64 and less whose heads of 128 do not share keys four and more: attention_bias_split with a wavefront alone
+//   (1000 x 16 rows 118 -> 37, 200 x 64 41 -> 34, 5000 packed rows of 1 to 64 50 -> 22; 64 x 128 29.5 against 32).
 struct AttnPlan {
-    bool split, wide;
+    int split;  // wavefronts of attention_bias_split, 0: tiles
+    bool wide;
     int parts;
 };
 
 AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_t hd) {
-    AttnPlan plan{false, false, 1};
+    AttnPlan plan{0, false, 1};
     const int64_t cus = ctx->num_cus, len = p.spans ? std::max<int64_t>(1, p.L / p.nseq) : p.L;
     auto blocks = [&](int64_t rows, int64_t heads) { return (len + rows - 1) / rows * p.nseq * heads; };
-    plan.split = len <= 512 && 2 * blocks(32, p.heads) <= 3 * cus;
+    if (len <= 512 && 2 * blocks(32, p.heads) <= 3 * cus) plan.split = 8;
+    else if (len <= 64 && (hd < 128 || heads_beside(p.group, 8) < 2)) plan.split = 1;
     if (plan.split) return plan;
     const int64_t tiles = (len + enchip::FA_KT - 1) / enchip::FA_KT;
     // the join numbers its threads in 32 bits
@@ -368,9 +372,12 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     p.rows = d_spans ? L : nseq * L;
     const bool vec = ldo % 4 == 0 && (uintptr_t)d_out % 16 == 0;
     const AttnPlan plan = attention_plan(ctx, p, head_dim);
-    if (plan.split && head_dim == 32) return attention_bias_split<32, 8>(ctx, p, s);
-    if (plan.split && head_dim == 64) return attention_bias_split<64, 8>(ctx, p, s);
-    if (plan.split) return attention_bias_split<128, 8>(ctx, p, s);
+    if (plan.split == 8 && head_dim == 32) return attention_bias_split<32, 8>(ctx, p, s);
+    if (plan.split == 8 && head_dim == 64) return attention_bias_split<64, 8>(ctx, p, s);
+    if (plan.split == 8) return attention_bias_split<128, 8>(ctx, p, s);
+    if (plan.split == 1 && head_dim == 32) return attention_bias_split<32, 1>(ctx, p, s);
+    if (plan.split == 1 && head_dim == 64) return attention_bias_split<64, 1>(ctx, p, s);
+    if (plan.split == 1) return attention_bias_split<128, 1>(ctx, p, s);
     if (head_dim == 32) return attention_bias_tiles<32, 8, 1>(ctx, p, vec, plan.parts, s);
     if (head_dim == 64 && plan.wide) return attention_bias_tiles<64, 8, 2>(ctx, p, vec, plan.parts, s);
     if (head_dim == 64) return attention_bias_tiles<64, 4, 2>(ctx, p, vec, plan.parts, s);

@@ -150,6 +150,26 @@ def test_spans_out_of_order_stay_in_bounds(ctx):
     assert np.isfinite(got).all()
 
 
+@pytest.mark.parametrize("hd,heads,kv,nseq,L", [
+    # every form of the kernel by its sizes: a wavefront alone, tiles of 256 and 512 queries, keys in parts
+    (32, 12, 12, 70, 33), (64, 12, 12, 70, 33), (128, 12, 12, 70, 33), (128, 12, 3, 70, 33),
+    (32, 8, 8, 16, 300), (64, 8, 8, 16, 300), (128, 8, 8, 16, 300), (64, 12, 4, 43, 512), (64, 16, 16, 16, 512),
+    (32, 3, 3, 1, 1500), (64, 3, 3, 1, 1500), (128, 3, 3, 1, 1500), (64, 2, 1, 1, 3000), (32, 1, 1, 1, 4099), (64, 1, 1, 2, 2111),
+    (128, 4, 1, 1, 1300),
+])
+def test_forms(ctx, hd, heads, kv, nseq, L):
+    say(f"attention_bias form hd={hd} heads={heads} kv={kv} {nseq}x{L}")
+    Case(heads, kv, hd, nseq * L).check(ctx, nseq=nseq, L=L)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_parts_of_spans(ctx, hd):
+    # a mean length that splits keys, lengths that leave parts empty, rows between the spans
+    say(f"attention_bias parts of spans hd={hd}")
+    spans = [(0, 2000), (2000, 2001), (2050, 3300), (3300, 3300), (3301, 6000)]
+    Case(2, 1, hd, 6100).check(ctx, spans=spans, ldo=2 * hd + 3)
+
+
 def test_no_bias_and_scales(ctx):
     say("attention_bias without a bias; scales of either sign and 0")
     for scale in (0.125, -0.2, 0.0):
@@ -295,6 +315,56 @@ def test_streams_and_graph(ctx):
             torch.cuda.synchronize()
             assert torch.equal(y, e)
         del gr
+    finally:
+        ctx.release_relpos(rp)
+
+
+def test_parts_in_a_graph_and_on_two_streams(ctx):
+    import torch
+
+    heads, hd, T = 2, 64, 2500
+    W = 3 * heads * hd
+    x = torch.empty((T, W), device="cuda")
+    y, e, z = (torch.zeros((T, heads * hd), device="cuda") for _ in range(3))
+    rp = ctx.relpos(np.random.default_rng(2).standard_normal((32, heads)).astype(np.float32), 128)
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def call(out, stream):
+        p = x.data_ptr()
+        ctx.attention_bias_dev(rp, p, W, p + 4 * heads * hd, W, p + 8 * heads * hd, W, out.data_ptr(), heads * hd, 1, T, heads, heads, hd,
+                               0.125, stream=stream)
+
+    try:
+        with torch.cuda.stream(s):
+            x.normal_()
+        call(e, s.cuda_stream)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            call(y, s.cuda_stream)
+        say("attention_bias in parts captured, 3 replays; two streams on the shared scratch")
+        for _ in range(3):
+            with torch.cuda.stream(s):
+                x.normal_()
+            torch.cuda.synchronize()
+            gr.replay()
+            torch.cuda.synchronize()
+            call(e, s.cuda_stream)
+            torch.cuda.synchronize()
+            assert torch.equal(y, e)
+        del gr
+        for _ in range(6):
+            call(y, s.cuda_stream), call(z, t.cuda_stream), call(e, 0)
+        torch.cuda.synchronize()
+        assert torch.equal(y, z) and torch.equal(y, e)
+        ctx.set_scratch_limit(1000)
+        try:
+            with pytest.raises(enchip.EnchipError) as err:
+                call(y, 0)
+            assert err.value.code == enchip.ERR_OOM
+        finally:
+            ctx.set_scratch_limit(0)
     finally:
         ctx.release_relpos(rp)
 
