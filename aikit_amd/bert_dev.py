@@ -46,6 +46,12 @@ enchip_rope_rows_dev), a gated one layers with an "ffn_gate" beside "ffn_up": in
 + bg) * (W8A8(h, Wi) + b) in enchip_w8a8_gated_dev (encoder/forward_q8.go:264-279 swigluMLPQ8 on
 the NomicBERT forward's order, with W8A8 linears as in the rest of this module).
 
+Layers with "q_norm" and "k_norm" have their query and key heads RMS-normed in qkv, turned in the same pass when
+`rope` is given (enchip_head_norm_rope_rows_dev). `relpos` (a learned bias by relative position), `kv_heads` fewer
+than `heads`, heads of 128, or sequences given as spans of rows take enchip_attention_bias_dev; embed() then
+pools the spans (enchip_pool_mean_l2_spans_dev). Low-rank adapters of many requests stand beside any linear
+but a gated layer's gate and up projection (`adapters`; enchip_w8a8_linear_adapters_dev): each row's by its id.
+
 This module holds no arithmetic of its own; torch provides device buffers and the stream.
 """
 from __future__ import annotations
@@ -69,16 +75,34 @@ class DeviceBert:
     also has "ffn_gate", whose act (ACT_SILU or ACT_GELU) is the gate's, and its "ffn_up" has
     ACT_NONE. rope: rotary frequencies (Context.rope) of the context, which outlive this object,
     with rope_layout; such a model's position table (set_embeddings) is zeros.
+    A layer may have "q_norm" and "k_norm" (f32 [head_dim], both or neither): gains of RMS norms of
+    its query and key heads, with norm_eps. kv_heads: heads of keys and values, a divisor of heads; "qkv"
+    then has hidden + 2 kv_heads head_dim rows. relpos: a bias (Context.relpos) for the attention of every
+    layer. adapters: per layer a dict of Context.adapters sets by linear ("qkv", "o", "ffn_up", "ffn_down";
+    not "ffn_up" of a gated layer), used where forward() is given ids. All of these outlive this object.
     """
 
     def __init__(self, ctx: enchip.Context, layers: Sequence[Dict], hidden: int, heads: int, ffn: int,
                  fused: bool = True, fuse_ln_quant: bool = True, gelu_in_quant: bool = True,
-                 rope: Optional["enchip.Rope"] = None, rope_layout: int = enchip.ROPE_HALF):
+                 rope: Optional["enchip.Rope"] = None, rope_layout: int = enchip.ROPE_HALF,
+                 kv_heads: Optional[int] = None, norm_eps: float = 1e-6, relpos: Optional["enchip.RelPos"] = None,
+                 adapters: Optional[Sequence[Dict[str, "enchip.Adapters"]]] = None):
         import torch
 
         for lw in layers:
             if "ffn_gate" in lw and lw["ffn_up"][3] != enchip.ACT_NONE:
                 raise ValueError("a gated layer's activation is its ffn_gate's: ffn_up must have ACT_NONE")
+
+            if ("q_norm" in lw) != ("k_norm" in lw):
+                raise ValueError("a layer has both q_norm and k_norm, or neither")
+        if adapters is not None and len(adapters) != len(layers):
+            raise ValueError(f"{len(adapters)} layers of adapters for {len(layers)} layers")
+        for lw, sets in zip(layers, adapters or ()):
+            for name, a in sets.items():
+                if name not in ("qkv", "o", "ffn_up", "ffn_down") or (name == "ffn_up" and "ffn_gate" in lw):
+                    raise ValueError(f"no adapters beside {name} here")
+                if (a.N, a.K) != lw[name][0].shape:
+                    raise ValueError(f"adapters of [{a.N}, {a.K}] beside {name} {lw[name][0].shape}")
 
         self.fused = fused
         self.fuse_ln_quant = fuse_ln_quant
@@ -89,6 +113,12 @@ class DeviceBert:
         self.hd = hidden // heads
         if self.hd * heads != hidden:
             raise ValueError(f"hidden {hidden} is not a multiple of heads {heads}")
+        self.KV = heads if kv_heads is None else kv_heads
+        if self.KV < 1 or heads % self.KV:
+            raise ValueError(f"kv_heads {kv_heads} does not divide heads {heads}")
+        self.W = hidden + 2 * self.KV * self.hd  # a row of qkv
+        self.norm_eps, self.relpos = norm_eps, relpos
+        self.adapters = [dict(a) for a in adapters] if adapters is not None else None
         self.handles: List[Dict[str, Tuple]] = []
         dev = torch.device("cuda")
         for lw in layers:
@@ -98,6 +128,11 @@ class DeviceBert:
                     continue
                 wq, ws, b, act = lw[name]
                 entry[name] = (ctx.register_weight(wq, ws), torch.from_numpy(np.ascontiguousarray(b)).to(dev), act)
+            for name in ("q_norm", "k_norm"):
+                if name in lw:
+                    if np.shape(lw[name]) != (self.hd,):
+                        raise ValueError(f"{name} shape {np.shape(lw[name])} is not ({self.hd},)")
+                    entry[name] = torch.from_numpy(np.ascontiguousarray(lw[name], np.float32)).to(dev)
             for name in ("attn_ln", "out_ln"):
                 g, s = lw[name]
                 entry[name] = (torch.from_numpy(np.ascontiguousarray(g)).to(dev),
@@ -154,7 +189,13 @@ class DeviceBert:
         self.handles = []
         self._bufs = {}
 
+    def bias_attention(self, spans=None) -> bool:
+        """Whether the attention is enchip_attention_bias_dev's."""
+        return self.relpos is not None or self.KV != self.H or spans is not None or self.hd == 128
+
     def fused_attention(self, L: int) -> bool:
+        if self.bias_attention():
+            return True
         if not self.fused or self.hd not in (32, 64):
             return False
         return L <= 512 or self.ctx.attention_products in (enchip.ATT_FLASH_BF16, enchip.ATT_FLASH_F16)
@@ -174,39 +215,63 @@ class DeviceBert:
         ok, ldq = self.ctx.frag_route(down, M)
         return ldq if ok and ldq <= self.GELU_QUANT_MAX_K else 0
 
-    def _buffers(self, S: int, L: int):
+    def _buffers(self, S: int, L: int, scores: bool = True):
         key = (S, L)
-        if key not in self._bufs:
+        if key not in self._bufs or (scores and self._bufs[key]["scores"].numel() == 1 and not self.fused_attention(L)):
             t, M = self.torch, S * L
             f = dict(device="cuda", dtype=t.float32)
-            sc = (1,) if self.fused_attention(L) else (S, self.H, L, L)
+            sc = (1,) if not scores or self.fused_attention(L) else (S, self.H, L, L)
             Mp = (M + 127) // 128 * 128  # fragment-major codes are read up to a multiple of 128 rows
             kp = (max(self.D, self.I) + 63) // 64 * 64  # the widest padded K of the layer's linears
-            self._bufs = {key: dict(qkv=t.empty((M, 3 * self.D), **f), scores=t.empty(sc, **f),
-                                    ctx=t.empty((M, self.D), **f), out=t.empty((M, self.D), **f),
+            self._bufs = {key: dict(qkv=t.empty((M, self.W), **f), scores=t.empty(sc, **f),
+                                    ctx=t.zeros((M, self.D), **f), out=t.empty((M, self.D), **f),
                                     inter=t.empty((M, self.I), **f), ffn=t.empty((M, self.D), **f),
                                     codes=t.empty(Mp * kp, device="cuda", dtype=t.int8),
                                     ascale=t.empty(M, **f))}
         return self._bufs[key]
 
-    def forward(self, h, S: int, L: int, stream: int = 0) -> None:
-        """Runs every layer on h ([S*L, D] f32 on the device), in place, on `stream`."""
-        c, D, H, hd, M = self.ctx, self.D, self.H, self.hd, S * L
+    def _ints(self, name: str, t, shape) -> int:
+        if t is None:
+            return 0
+        if t.dtype != self.torch.int32 or t.device.type != "cuda" or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on the device")
+        return t.data_ptr()
+
+    def forward(self, h, S: int, L: int, stream: int = 0, spans=None, pos=None, ids=None) -> None:
+        """Runs every layer on h ([S*L, D] f32 on the device), in place, on `stream`.
+
+        spans (int32 [n, 2] on the device): the sequences are these spans of the S*L rows, first row and one past
+        the last, ascending (enchip_attention_bias_dev); what h holds in rows of none means nothing. pos (int32
+        [S*L]): the rows' positions for `rope`, else row % L. ids (int32 [S*L]): the rows' adapters."""
+        c, D, H, hd, M, W = self.ctx, self.D, self.H, self.hd, S * L, self.W
         if tuple(h.shape) != (M, D) or not h.is_contiguous():
             raise ValueError(f"h must be a contiguous [{M}, {D}] tensor")
-        b = self._buffers(S, L)
+        nspans = 0 if spans is None else spans.shape[0]
+        d_spans, d_pos = self._ints("spans", spans, (nspans, 2)), self._ints("pos", pos, (M,))
+        d_ids = self._ints("ids", ids, (M,))
+        if ids is not None and self.adapters is None:
+            raise ValueError("ids without adapters")
+        kv = self.KV * hd
+        b = self._buffers(S, L, spans is None)
         qkv, scores, ctxv, out, inter, ffn = b["qkv"], b["scores"], b["ctx"], b["out"], b["inter"], b["ffn"]
         codes, ascale = b["codes"].data_ptr(), b["ascale"].data_ptr()
         q = qkv.data_ptr()
         scale = float(np.float32(1.0 / math.sqrt(hd)))  # encoder/attention.go:86
 
-        def route(w):  # the padded K when LN + quantization can run fused before w, else 0
-            if not self.fuse_ln_quant:
+        def beside(li, name):  # the adapters of a linear, None without
+            return self.adapters[li].get(name) if d_ids else None
+
+        def route(w, low):  # the padded K when LN + quantization can run fused before w, else 0
+            if not self.fuse_ln_quant or low is not None:
                 return 0
             ok, ldq = c.frag_route(w, M)
             return ldq if ok and ldq <= D else 0
 
-        def linear(name, w, x, bias, act, dst):  # one W8A8 linear on x [M, K]
+        def linear(name, w, x, bias, act, dst, low=None):  # one W8A8 linear on x [M, K]
+            if low is not None:
+                self._m(name + "+adapters")
+                c.linear_adapters_dev(w, low, x.data_ptr(), M, d_ids, bias.data_ptr(), act, dst.data_ptr(), stream)
+                return
             ok, ldq = c.frag_route(w, M)
             if ok:  # the kernels enchip_w8a8_linear_dev launches, as two timed calls
                 self._m(name + ".quant")
@@ -217,8 +282,8 @@ class DeviceBert:
                 self._m(name)
                 c.linear_dev(w, x.data_ptr(), M, bias.data_ptr(), act, dst.data_ptr(), stream)
 
-        def ln_then(g, s_, y, nxt, label):  # h = LN(h + y); codes for weight nxt when it takes them
-            ldq = route(nxt) if nxt is not None else 0
+        def ln_then(g, s_, y, nxt, label, low=None):  # h = LN(h + y); codes for weight nxt when it takes them
+            ldq = route(nxt, low) if nxt is not None else 0
             self._m(label + ("+quant" if ldq else ""))
             if ldq:
                 c.residual_layer_norm_quant_dev(h.data_ptr(), D, y.data_ptr(), D, M, D, g.data_ptr(), s_.data_ptr(),
@@ -235,12 +300,19 @@ class DeviceBert:
                 self._m("qkv.gemm")
                 c.pre_frag_dev(w, codes, pending, M, ascale, bias.data_ptr(), act, q, stream)
             else:
-                linear("qkv", w, h, bias, act, qkv)
-            if self.rope is not None:
+                linear("qkv", w, h, bias, act, qkv, beside(li, "qkv"))
+            if "q_norm" in e:
+                self._m("head_norm")
+                c.head_norm_rope_rows_dev(self.rope, self.rope_layout, q, W, q, W, S, L, H, self.KV, hd, e["q_norm"].data_ptr(),
+                                          e["k_norm"].data_ptr(), self.norm_eps, d_pos, stream=stream)
+            elif self.rope is not None:
                 self._m("rope")
-                c.rope_rows_dev(self.rope, self.rope_layout, q, 3 * D, q, 3 * D, S, L, 2 * H, hd, stream=stream)
+                c.rope_rows_dev(self.rope, self.rope_layout, q, W, q, W, S, L, H + self.KV, hd, d_pos, stream=stream)
             self._m("attention")
-            if self.fused_attention(L):
+            if self.bias_attention(spans):
+                c.attention_bias_dev(self.relpos, q, W, q + D * 4, W, q + (D + kv) * 4, W, ctxv.data_ptr(), D,
+                                     S if spans is None else nspans, L if spans is None else M, H, self.KV, hd, scale, d_spans, stream)
+            elif self.fused_attention(L):
                 c.attention_f32_dev(q, q + D * 4, q + 2 * D * 4, 3 * D, ctxv.data_ptr(), D, S, L, H, hd, scale, stream)
             else:
                 c.matmul_bt_f32_dev(q, 3 * D, q + D * 4, 3 * D, enchip.B_NK, scores.data_ptr(), L, L, hd, L,
@@ -251,7 +323,7 @@ class DeviceBert:
                                     hd, inner=(H, L * L, hd, hd), outer=(S, H * L * L, L * 3 * D, L * D),
                                     stream=stream)
             w, bias, act = e["o"]
-            linear("o", w, ctxv, bias, act, out)
+            linear("o", w, ctxv, bias, act, out, beside(li, "o"))
             g, s = e["attn_ln"]
             w, bias, act = e["ffn_up"]
             if "ffn_gate" in e:
@@ -260,19 +332,21 @@ class DeviceBert:
                 self._m("ffn_gated")
                 c.w8a8_gated_dev(wg, w, h.data_ptr(), M, bg.data_ptr(), bias.data_ptr(), act, inter.data_ptr(), stream)
                 w, bias, act = e["ffn_down"]
-                linear("ffn_down", w, inter, bias, act, ffn)
+                linear("ffn_down", w, inter, bias, act, ffn, beside(li, "ffn_down"))
                 g, s = e["out_ln"]
                 nxt = self.handles[li + 1]["qkv"][0] if li + 1 < len(self.handles) else None
-                pending = ln_then(g, s, ffn, nxt, "out_ln")
+                pending = ln_then(g, s, ffn, nxt, "out_ln", beside(li + 1, "qkv") if nxt is not None else None)
                 continue
-            gq = self.gelu_quant_route(act, e["ffn_down"][0], M)
+            up_low, down_low = beside(li, "ffn_up"), beside(li, "ffn_down")
+            # adapters of FFN-down take the activations themselves
+            gq = self.gelu_quant_route(act, e["ffn_down"][0], M) if down_low is None else 0
             up_act = enchip.ACT_NONE if gq else act
-            ldq = ln_then(g, s, out, w, "attn_ln")
+            ldq = ln_then(g, s, out, w, "attn_ln", up_low)
             if ldq:
                 self._m("ffn_up.gemm")
                 c.pre_frag_dev(w, codes, ldq, M, ascale, bias.data_ptr(), up_act, inter.data_ptr(), stream)
             else:
-                linear("ffn_up", w, h, bias, up_act, inter)
+                linear("ffn_up", w, h, bias, up_act, inter, up_low)
             w, bias, act = e["ffn_down"]
             if gq:  # inter holds FFN-up's pre-activations: GELU them while quantizing
                 self._m("ffn_down.gelu_quant")
@@ -280,15 +354,22 @@ class DeviceBert:
                 self._m("ffn_down.gemm")
                 c.pre_frag_dev(w, codes, gq, M, ascale, bias.data_ptr(), act, ffn.data_ptr(), stream)
             else:
-                linear("ffn_down", w, inter, bias, act, ffn)
+                linear("ffn_down", w, inter, bias, act, ffn, down_low)
             g, s = e["out_ln"]
             nxt = self.handles[li + 1]["qkv"][0] if li + 1 < len(self.handles) else None
-            pending = ln_then(g, s, ffn, nxt, "out_ln")
+            pending = ln_then(g, s, ffn, nxt, "out_ln", beside(li + 1, "qkv") if nxt is not None else None)
 
-    def embed(self, h, S: int, L: int, pooled, stream: int = 0) -> None:
-        """forward(), then mean pooling + L2 normalisation of each sequence into pooled [S, D]."""
-        self.forward(h, S, L, stream)
+    def embed(self, h, S: int, L: int, pooled, stream: int = 0, spans=None, pos=None, ids=None) -> None:
+        """forward(), then mean pooling + L2 normalisation of each sequence into pooled [S, D], or of
+        each span into pooled [n, D]."""
+        self.forward(h, S, L, stream, spans, pos, ids)
         self._m("pool")
+        if spans is not None:
+            if spans.shape[0]:
+                self.ctx.pool_mean_l2_spans_dev(h.data_ptr(), self.D, S * L, spans.data_ptr(), spans.shape[0], self.D,
+                                                pooled.data_ptr(), self.D, stream)
+            self._m("end")
+            return
         self.ctx.pool_mean_l2_dev(h.data_ptr(), self.D, S, L, self.D, pooled.data_ptr(), self.D, stream)
         self._m("end")
 
