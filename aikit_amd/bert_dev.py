@@ -373,7 +373,7 @@ class DeviceBert:
         self.ctx.pool_mean_l2_dev(h.data_ptr(), self.D, S, L, self.D, pooled.data_ptr(), self.D, stream)
         self._m("end")
 
-    def rerank(self, h, S: int, L: int, pooler, classifier, logits, stream: int = 0) -> None:
+    def rerank(self, h, S: int, L: int, pooler, classifier, logits, stream: int = 0, ids=None) -> None:
         """forward(), then the cross-encoder head on each sequence's [CLS] row (row 0):
         logits [S, labels] = classifier(tanh(pooler(CLS))). pooler = (W [D, D], b [D]),
         classifier = (W [labels, D], b [labels]), f32 device tensors (PyTorch [out, in])."""
@@ -383,7 +383,7 @@ class DeviceBert:
         labels = cw.shape[0]
         if tuple(pw.shape) != (D, D) or tuple(cw.shape) != (labels, D) or tuple(logits.shape) != (S, labels):
             raise ValueError("rerank: pooler [D, D], classifier [labels, D], logits [S, labels]")
-        self.forward(h, S, L, stream)
+        self.forward(h, S, L, stream, ids=ids)
         self._m("head")
         pooled = self._bufs[(S, L)].setdefault("pooled", self.torch.empty((S, D), device="cuda"))
         # CLS rows are every L-th row of h: pitch L*D

@@ -72,9 +72,11 @@ int enchip_head_norm_rope_rows_dev(enchip_ctx *ctx, enchip_rope h, int layout, c
     p.lanes = 1;
     while (p.lanes < 64 && p.lanes < p.slots) p.lanes *= 2;
     const int need = (p.slots + p.lanes - 1) / p.lanes, it = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
-    // rows of a workgroup: three passes of its lanes, while a few workgroups a CU are left
-    const int64_t pass = 256 / p.lanes * (it >= 4 ? 1 : 4 / it);
-    const int64_t by_items = std::max<int64_t>(1, 3 * pass / heads), by_rows = std::max<int64_t>(1, rows / (4 * ctx->num_cus));
+    // rows of a workgroup: one pass of its lanes, two where the positions come from memory and the angles wait for
+    // them (64 x 512 rows of 24 heads of 64 75 us against 80 with two passes and 82 with three; 20011 rows of 20 heads
+    // of 128 with positions 93.5, 89 and 93), while a few workgroups a CU are left
+    const int64_t passes = d_pos ? 2 : 1, pass = 256 / p.lanes * (it >= 4 ? 1 : 4 / it);
+    const int64_t by_items = std::max<int64_t>(1, passes * pass / heads), by_rows = std::max<int64_t>(1, rows / (4 * ctx->num_cus));
     const int64_t by_angles = r.n ? (int64_t)enchip::ROPE_CS / r.n : 64;
     const int tr = (int)std::min({by_items, by_rows, by_angles, (int64_t)64});
     for (int64_t r0 = 0; r0 < rows; r0 += kRowChunk) {
@@ -445,6 +447,8 @@ int launch_down(enchip_ctx *c, const enchip::Adapters &p, const float *d_a, int6
     const bool vec = lda % 4 == 0 && K % 4 == 0 && (uintptr_t)d_a % 16 == 0;
     const int64_t blocks = (M + 15) / 16, apart = std::max<int64_t>(1, 2 * c->num_cus / blocks);
     const bool four = p.rt > 1 && apart < p.rt;  // rank tiles four at a time
+    // a workgroup a CU or less: 16 wavefronts, half as many steps each (1500 rows, K = 1000: 7.6 us -> 7.0)
+    const bool few = blocks <= c->num_cus;
     const dim3 grid((unsigned)blocks, (unsigned)(four ? std::min<int64_t>(apart, (p.rt + 3) / 4) : p.rt));
     const enchip::RowCodes codes = q ? *q : enchip::RowCodes{};
 #define AD_DOWN(V, C, NW, KBW)                                                                                                       \
@@ -454,8 +458,11 @@ int launch_down(enchip_ctx *c, const enchip::Adapters &p, const float *d_a, int6
     } while (0)
 #define AD_K(V)                                           \
     do {                                                  \
-        if (!q) AD_DOWN(V, false, 8, 4);                  \
+        if (!q && few) AD_DOWN(V, false, 16, 2); \
+        else if (!q) AD_DOWN(V, false, 8, 4);                  \
         else if (q->ldq <= 256) AD_DOWN(V, true, 8, 1);   \
+        else if (few && q->ldq <= 512) AD_DOWN(V, true, 16, 1); \
+        else if (few && q->ldq <= 1024) AD_DOWN(V, true, 16, 2); \
         else if (q->ldq <= 512) AD_DOWN(V, true, 8, 2);   \
         else if (q->ldq <= 1024) AD_DOWN(V, true, 8, 4);  \
         else if (q->ldq <= 2048) AD_DOWN(V, true, 16, 4); \

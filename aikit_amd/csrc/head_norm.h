@@ -44,19 +44,10 @@ __global__ __launch_bounds__(256) void head_norm_rope(const float *x, int64_t ld
     __shared__ float2 cs[ROPE_CS];
     const int64_t first = (int64_t)blockIdx.x * TR;
     const int tr = (int)min((int64_t)TR, rows - first), np = p.r / 2;
-    for (int t = threadIdx.x; t < tr * np; t += 256) {
-        const int row = t / np, j = t - row * np;
-        const double at = pos ? (double)pos[first + row] : (double)(pos0 + (row0 + first + row) % L);
-        const double2 f = turns[j];
-        const double a = at * f.x, e = __builtin_fma(at, f.y, __builtin_fma(at, f.x, -a));
-        float s, c;
-        sincospif(2.0f * (float)(a - rint(a) + e), &s, &c);
-        cs[t] = make_float2(c * mscale, s * mscale);
-    }
     const int G = p.lanes, g = threadIdx.x & (G - 1), groups = 256 / G, group = threadIdx.x / G;
+    const int units = tr * (int)heads.d;  // heads of the workgroup's rows
     // the lane's slots: offsets of their two parts, the same for every head
     int oa[IT], ob[IT];
-    float gq[IT][2 * V], gk[IT][2 * V];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int s = g + G * i;
@@ -64,23 +55,13 @@ __global__ __launch_bounds__(256) void head_norm_rope(const float *x, int64_t ld
         oa[i] = s >= p.slots ? -1 : !turn ? p.r + 2 * V * (s - p.turned) : INTERLEAVED ? 2 * V * s : V * s;
         ob[i] = oa[i] < 0 ? -1 : turn && !INTERLEAVED ? oa[i] + np : oa[i] + V;
         if (ob[i] >= p.hd) ob[i] = -1;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            gq[i][k] = oa[i] >= 0 ? p.gain_q[oa[i] + k] : 0.0f;
-            gk[i][k] = oa[i] >= 0 ? p.gain_k[oa[i] + k] : 0.0f;
-            gq[i][V + k] = ob[i] >= 0 ? p.gain_q[ob[i] + k] : 0.0f;
-            gk[i][V + k] = ob[i] >= 0 ? p.gain_k[ob[i] + k] : 0.0f;
-        }
     }
-    __syncthreads();
-    const int units = tr * (int)heads.d;  // heads of the workgroup's rows
-    for (int u0 = 0; u0 < units; u0 += groups * BATCH) {  // uniform: the exchanges need every lane
-        float v[BATCH][IT][2 * V];
-        double sum[BATCH];
+    float v[BATCH][IT][2 * V];
+    auto load = [&](int u0) {
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            const int u = u0 + group + groups * b;
-            const int row = (int)heads.div((uint32_t)min(u, units - 1)), h = min(u, units - 1) - row * (int)heads.d;
+            const int u = min(u0 + group + groups * b, units - 1);
+            const int row = (int)heads.div((uint32_t)u), h = u - row * (int)heads.d;
             const float *src = x + (first + row) * ldx + (int64_t)h * p.hd;
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
@@ -90,6 +71,33 @@ __global__ __launch_bounds__(256) void head_norm_rope(const float *x, int64_t ld
                 if (ob[i] >= 0) rope_load<V>(v[b][i] + V, src + ob[i]);
             }
         }
+    };
+    load(0);  // in flight while the angles are formed
+    for (int t = threadIdx.x; t < tr * np; t += 256) {
+        const int row = t / np, j = t - row * np;
+        const double at = pos ? (double)pos[first + row] : (double)(pos0 + (row0 + first + row) % L);
+        const double2 f = turns[j];
+        const double a = at * f.x, e = __builtin_fma(at, f.y, __builtin_fma(at, f.x, -a));
+        float s, c;
+        sincospif(2.0f * (float)(a - rint(a) + e), &s, &c);
+        cs[t] = make_float2(c * mscale, s * mscale);
+    }
+    float gq[IT][2 * V], gk[IT][2 * V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            gq[i][k] = oa[i] >= 0 ? p.gain_q[oa[i] + k] : 0.0f;
+            gk[i][k] = oa[i] >= 0 ? p.gain_k[oa[i] + k] : 0.0f;
+            gq[i][V + k] = ob[i] >= 0 ? p.gain_q[ob[i] + k] : 0.0f;
+            gk[i][V + k] = ob[i] >= 0 ? p.gain_k[ob[i] + k] : 0.0f;
+        }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    for (int u0 = 0; u0 < units; u0 += groups * BATCH) {  // uniform: the exchanges need every lane
+        if (u0 > 0) load(u0);
+        double sum[BATCH];
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
             sum[b] = 0.0;

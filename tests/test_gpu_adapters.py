@@ -86,6 +86,8 @@ def some_ids(g, M, slots, run):
     (50, 128, 60, 4, 3, 9, dict(lda=132, off=1)),              # rows that are 4-byte aligned
     (50, 128, 64, 4, 3, 9, dict(inplace=True, ldy=80)),
     (600, 64, 300, 12, 6, 100, {}),
+    (4200, 300, 130, 70, 3, 90, {}),                           # more rows than a workgroup a CU
+    (4200, 1100, 64, 16, 3, 90, dict(lda=1101)),
 ])
 def test_add(ctx, M, K, N, rank, slots, run, k):
     say(f"adapters_add M={M} K={K} N={N} rank={rank} slots={slots} run={run} {k}")
@@ -109,6 +111,10 @@ LINEAR = [
     (33, 768, 2304, 16, 4, 11), (64, 384, 384, 16, 4, 16), (70, 100, 33, 5, 3, 1), (200, 768, 768, 40, 3, 32), (513, 384, 1536, 16, 6, 100),
     (1500, 1000, 1001, 7, 3, 77), (700, 768, 3000, 20, 5, 300), (2000, 128, 1028, 8, 4, 512), (4100, 64, 2052, 16, 3, 700),
     (3000, 320, 2048, 32, 8, 1), (260, 2112, 516, 16, 3, 64), (6000, 72, 1001, 9, 3, 500),
+    # every width that adapter_down holds, in few and many rows, one and several rank tiles
+    (40, 256, 96, 70, 2, 9), (40, 512, 96, 20, 2, 9), (40, 1024, 64, 100, 2, 9), (40, 2048, 64, 20, 2, 9), (40, 4096, 64, 130, 2, 9),
+    (4113, 250, 64, 40, 2, 200), (4113, 500, 96, 16, 3, 200), (4113, 1000, 70, 40, 3, 200), (4113, 2000, 64, 16, 3, 99),
+    (4113, 2001, 64, 40, 2, 99), (4113, 4000, 64, 16, 2, 99), (4113, 4095, 64, 33, 2, 99), (4113, 5000, 64, 20, 2, 99),
 ]
 
 
