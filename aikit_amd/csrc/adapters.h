@@ -31,6 +31,7 @@ namespace enchip {
 struct Adapters {
     static constexpr bool on = true;
     const bf16x8 *a, *b;
+    const float *af;  // A as it is, [slot][R][4 ceil(K / 4)]
     bf16x8 *t;
     const int32_t *ids;
     int slots, kb, nb, rt;  // Kp / 32, Np / 32, R / 16
@@ -120,6 +121,83 @@ struct Adapters {
                     const float x = (float)d.x[h][0][e] + ((float)d.x[h][1][e] + (float)d.x[h][2][e]);
                     const float w = (float)d.w[h][0][e] + ((float)d.w[h][1][e] + (float)d.w[h][2][e]);
                     sum = __builtin_fmaf(x, w, sum);
+                }
+        }
+        return sum;
+    }
+
+    // Few rows of few products in one launch (gemv_w8a8_q, kernels.h): every workgroup forms its rows' low-rank parts
+    // itself, a row a wavefront, from the f32 A and the row that the wavefront quantizes; they meet its outputs' B
+    // in LDS.
+    static constexpr int ROW_RANKS = 32;
+    struct Row {
+        int mine, s;  // the slots of the wavefront's row and of the thread's output
+        bf16x8 w[2][3];
+    };
+    __device__ __forceinline__ static float *row_t() {
+        __shared__ float t[GVQ_ROWS][ROW_RANKS];
+        return &t[0][0];
+    }
+    __device__ __forceinline__ void b_load(Row &d, int64_t n, int c, int rs) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 3; ++u) d.w[h][u] = b_at(d.s, n, rs)[64 * u + c + 32 * h];
+    }
+    __device__ __forceinline__ void row_begin(Row &d, int row0, int wave, int M, int64_t n, int tid) const {
+        d.mine = slot(row0 + wave, M);
+        d.s = tid < GVQ_ROWS * 32 ? slot(row0 + (tid >> 5), M) : -1;
+        if (d.s >= 0) b_load(d, n, tid & 31, 0);
+    }
+    template <int QCH>
+    __device__ __forceinline__ void row_down(const Row &d, const float4 (&v)[QCH], int K4, int wave, int lane) const {
+        if (d.mine < 0) return;  // uniform
+        const float4 *at = reinterpret_cast<const float4 *>(af) + (int64_t)d.mine * 16 * rt * K4;
+        for (int j0 = 0; j0 < 16 * rt; j0 += 8) {
+            float4 x[8][QCH];
+            float sum[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < QCH; ++c)  // past K v is zero
+                    x[j][c] = at[(int64_t)(j0 + j) * K4 + min(lane + 64 * c, K4 - 1)];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum[j] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < QCH; ++c) {
+                    sum[j] = __builtin_fmaf(v[c].x, x[j][c].x, sum[j]);
+                    sum[j] = __builtin_fmaf(v[c].y, x[j][c].y, sum[j]);
+                    sum[j] = __builtin_fmaf(v[c].z, x[j][c].z, sum[j]);
+                    sum[j] = __builtin_fmaf(v[c].w, x[j][c].w, sum[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum[j] += __uint_as_float(lane_dpp<0xB1>(__float_as_uint(sum[j])));
+                sum[j] += __uint_as_float(lane_dpp<0x4E>(__float_as_uint(sum[j])));
+                sum[j] += __uint_as_float(lane_dpp<0x141>(__float_as_uint(sum[j])));
+                sum[j] += __uint_as_float(lane_dpp<0x140>(__float_as_uint(sum[j])));
+                uint32_t p, q;
+                lane_swap16(__float_as_uint(sum[j]), p, q);
+                sum[j] = __uint_as_float(p) + __uint_as_float(q);
+                lane_swap32(__float_as_uint(sum[j]), p, q);
+                sum[j] = __uint_as_float(p) + __uint_as_float(q);
+                if (lane == 0) row_t()[wave * ROW_RANKS + j0 + j] = sum[j];
+            }
+        }
+    }
+    __device__ __forceinline__ float row_up(Row &d, int i, int64_t n, int c) const {
+        float sum = 0.0f;
+        if (d.s < 0) return sum;
+        for (int rs = 0; rs < rt; ++rs) {
+            if (rs > 0) b_load(d, n, c, rs);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float w = (float)d.w[h][0][e] + ((float)d.w[h][1][e] + (float)d.w[h][2][e]);
+                    sum = __builtin_fmaf(row_t()[i * ROW_RANKS + 16 * rs + 8 * h + e], w, sum);
                 }
         }
         return sum;
@@ -288,8 +366,8 @@ __global__ __launch_bounds__(64 * NW, 4) void adapter_down(const float *__restri
 }
 
 // dst = y + B_s t: a wavefront per 32 x 32 outputs, four side by side. dst may be y.
-[[maybe_unused]] static __global__ __launch_bounds__(256) void adapter_up(const float *y, int64_t ldy, float *dst, int64_t ldd, int64_t M, int N, Adapters p,
-                                                  int panels) {
+[[maybe_unused]] static __global__ __launch_bounds__(256) void adapter_up(const float *y, int64_t ldy, float *dst,
+                                                                          int64_t ldd, int64_t M, int N, Adapters p, int panels) {
     const int lane = threadIdx.x & 63, r = lane & 31;
     const int64_t mb = blockIdx.x / panels, nb = (int64_t)(blockIdx.x % panels) * 4 + (threadIdx.x >> 6);
     const int64_t col = nb * 32 + r;
@@ -312,6 +390,49 @@ __global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8a8_adapters(
     const float *__restrict__ aS, const float *__restrict__ wS, const float *__restrict__ bias,
     void *__restrict__ out, int64_t ldo, int M, int N, int Kp, Adapters p) {
     gemv_w8a8_body<EPI, NB>(A, lda, Wf, aS, wS, bias, out, ldo, M, N, Kp, p);
+}
+
+// The same in one launch, the rows quantized and their low-rank parts formed by every workgroup (16 rows, K = 384,
+// N = 1536, rank 8: 5.9 us, where two launches take 8.3 and up to 15 for 16 different adapters).
+template <int EPI, int QCH>
+__global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q_adapters(
+    const float *__restrict__ a, const int8_t *__restrict__ Wf, const float *__restrict__ wS,
+    const float *__restrict__ bias, void *__restrict__ out, int64_t ldo, int M, int N, int K, int Kp, Adapters p) {
+    gemv_w8a8_q_body<EPI, QCH>(a, Wf, wS, bias, out, ldo, M, N, K, Kp, p);
+}
+
+// An adapter's parts from A [R][K] and B [N][R]: blocks of 256 threads, first those of A (32 kb x 16 rt values,
+// with zeros past K and R), then those of B (scale B rounded once).
+[[maybe_unused]] static __global__ __launch_bounds__(256) void adapter_pack(
+    const float *__restrict__ A, const float *__restrict__ B, double scale, int K, int N, int R, int kb, int nb, int rt,
+    bf16x8 *__restrict__ pa, bf16x8 *__restrict__ pb, float *__restrict__ fa) {
+    const int64_t na = (int64_t)kb * rt * 64, i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // 8 values a thread
+    float x[8];
+    bf16x8 p[3];
+    if (i < na) {
+        const int lane = (int)(i & 63), K4 = (K + 3) / 4;
+        const int64_t block = i >> 6;
+        const int j = 16 * (int)(block % rt) + (lane & 15), k0 = 32 * (int)(block / rt) + 4 * (lane >> 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = k0 + (e & 3) + 4 * (e & 4);  // Adapters::a's order
+            x[e] = j < R && k < K ? A[(int64_t)j * K + k] : 0.0f;
+            if (k < 4 * K4) fa[(int64_t)j * 4 * K4 + k] = x[e];
+        }
+        split3_8(x, p);
+#pragma unroll
+        for (int u = 0; u < 3; ++u) pa[(block * 3 + u) * 64 + lane] = p[u];
+    } else if (i - na < (int64_t)nb * rt * 64) {
+        const int lane = (int)((i - na) & 63);
+        const int64_t block = (i - na) >> 6;
+        const int j0 = 16 * (int)(block % rt) + 8 * (lane >> 5);
+        const int64_t n = 32 * (block / rt) + (lane & 31);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = j0 + e < R && n < N ? (float)(scale * (double)B[n * R + j0 + e]) : 0.0f;
+        split3_8(x, p);
+#pragma unroll
+        for (int u = 0; u < 3; ++u) pb[(block * 3 + u) * 64 + lane] = p[u];
+    }
 }
 
 }  // namespace enchip

@@ -394,26 +394,6 @@ namespace {
 
 constexpr int64_t kMaxAdapterBytes = (int64_t)1 << 36;
 
-uint16_t bf16_of(float x) {
-    uint32_t u;
-    std::memcpy(&u, &x, 4);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-float f32_of(uint16_t b) {
-    const uint32_t u = (uint32_t)b << 16;
-    float x;
-    std::memcpy(&x, &u, 4);
-    return x;
-}
-
-// Writes x's three parts at p[0], p[plane], p[2 plane].
-void store_parts(float x, uint16_t *p, int64_t plane) {
-    for (int u = 0; u < 3; ++u) {
-        p[u * plane] = bf16_of(x);
-        x -= f32_of(p[u * plane]);
-    }
-}
-
 int find_adapters(enchip_ctx *c, enchip_adapters h, AdapterSet **out) {
     auto it = c->adapters.find(h);
     if (it == c->adapters.end()) return fail(c, ENCHIP_ERR_HANDLE, "unknown adapters handle %llu", (unsigned long long)h);
@@ -423,11 +403,20 @@ int find_adapters(enchip_ctx *c, enchip_adapters h, AdapterSet **out) {
 
 int64_t a_bytes(const AdapterSet &s) { return s.kb * s.rt * 3 * 1024; }  // of a slot
 int64_t b_bytes(const AdapterSet &s) { return s.nb * s.rt * 3 * 1024; }
+int64_t f_floats(const AdapterSet &s) { return 16 * s.rt * round_up(s.K, 4); }
+
+void free_adapters(const AdapterSet &s) {
+    (void)hipFree(s.d_a);
+    (void)hipFree(s.d_b);
+    (void)hipFree(s.d_f);
+    (void)hipFree(s.d_up);
+}
 
 enchip::Adapters view(const enchip_ctx *c, const AdapterSet &set, const int32_t *d_ids) {
     enchip::Adapters p;
     p.a = reinterpret_cast<const enchip::bf16x8 *>(set.d_a);
     p.b = reinterpret_cast<const enchip::bf16x8 *>(set.d_b);
+    p.af = set.d_f;
     p.t = reinterpret_cast<enchip::bf16x8 *>(c->d_low);
     p.ids = d_ids;
     p.slots = (int)set.slots, p.kb = (int)set.kb, p.nb = (int)set.nb, p.rt = (int)set.rt;
@@ -456,17 +445,17 @@ int launch_down(enchip_ctx *c, const enchip::Adapters &p, const float *d_a, int6
         if (four) hipLaunchKernelGGL((enchip::adapter_down<V, C, NW, KBW, 4>), grid, dim3(64 * NW), 0, s, d_a, lda, M, (int)K, p, codes); \
         else hipLaunchKernelGGL((enchip::adapter_down<V, C, NW, KBW, 1>), grid, dim3(64 * NW), 0, s, d_a, lda, M, (int)K, p, codes); \
     } while (0)
-#define AD_K(V)                                           \
-    do {                                                  \
-        if (!q && few) AD_DOWN(V, false, 16, 2); \
-        else if (!q) AD_DOWN(V, false, 8, 4);                  \
-        else if (q->ldq <= 256) AD_DOWN(V, true, 8, 1);   \
-        else if (few && q->ldq <= 512) AD_DOWN(V, true, 16, 1); \
+#define AD_K(V)                                                  \
+    do {                                                         \
+        if (!q && few) AD_DOWN(V, false, 16, 2);                 \
+        else if (!q) AD_DOWN(V, false, 8, 4);                    \
+        else if (q->ldq <= 256) AD_DOWN(V, true, 8, 1);          \
+        else if (few && q->ldq <= 512) AD_DOWN(V, true, 16, 1);  \
         else if (few && q->ldq <= 1024) AD_DOWN(V, true, 16, 2); \
-        else if (q->ldq <= 512) AD_DOWN(V, true, 8, 2);   \
-        else if (q->ldq <= 1024) AD_DOWN(V, true, 8, 4);  \
-        else if (q->ldq <= 2048) AD_DOWN(V, true, 16, 4); \
-        else AD_DOWN(V, true, 16, 8);                     \
+        else if (q->ldq <= 512) AD_DOWN(V, true, 8, 2);          \
+        else if (q->ldq <= 1024) AD_DOWN(V, true, 8, 4);         \
+        else if (q->ldq <= 2048) AD_DOWN(V, true, 16, 4);        \
+        else AD_DOWN(V, true, 16, 8);                            \
     } while (0)
     if (vec) AD_K(true);
     else AD_K(false);
@@ -545,11 +534,45 @@ void launch_linear(enchip_ctx *c, const Weight &w, const int8_t *aq, const float
 #undef PIECE
 }
 
+// Few rows in one launch (gemv_w8a8_q_adapters): every workgroup of 32 columns quantizes its 8 rows and forms their
+// low-rank parts again, so A is small (its 16 rt rows of a slot, once a row a workgroup) and the launch about two
+// workgroups a CU at rt = 1. LDS stays under 64 KiB. One launch against two, us, rows of mixed adapters (of one):
+//   16 rows, K = 384, N = 1536, rank 8   6.2, 15.3 (10.8)    16 rows, K = 768, N = 768, rank 32   10.6, 22.7 (16.2)
+//   32 rows, K = 768, N = 2304, rank 16 (288 workgroups)  12.3, 23.5 (16.4); rank 32 19.0, 23.4 (17.1): two
+//   32 rows, K = 1024, N = 4096, rank 16 (512 workgroups)  17.0, 25.7 (17.1); rank 32 27.2, 26.2 (17.9): two
+bool one_launch(const enchip_ctx *c, const Weight &w, const AdapterSet &set, int64_t M, const float *d_a) {
+    const int64_t groups = (w.N + 31) / 32 * ((M + enchip::GVQ_ROWS - 1) / enchip::GVQ_ROWS);
+    return M <= c->small_m && M <= 32 && w.K <= 1024 && w.K % 4 == 0 && (uintptr_t)d_a % 16 == 0 &&
+           16 * set.rt <= enchip::Adapters::ROW_RANKS && groups * set.rt <= 2 * (int64_t)c->num_cus;
+}
+
+template <int EPI>
+int launch_one(enchip_ctx *c, const Weight &w, const enchip::Adapters &p, const float *d_a, int64_t M, const float *bias, float *out,
+               hipStream_t s) {
+    using namespace enchip;
+    const dim3 grid((unsigned)((w.N + 31) / 32), (unsigned)((M + GVQ_ROWS - 1) / GVQ_ROWS));
+    const size_t lds = (size_t)gvq_lds_bytes((int)w.Kp);
+#define GVQ_LAUNCH(QCH)                                                                                                     \
+    hipLaunchKernelGGL((gemv_w8a8_q_adapters<EPI, QCH>), grid, dim3(64 * GVQ_WAVES), lds, s, d_a, w.d_w, w.d_s, bias, out, w.N, (int)M, \
+                       (int)w.N, (int)w.K, (int)w.Kp, p)
+    if (w.K <= 256) GVQ_LAUNCH(1);
+    else if (w.K <= 512) GVQ_LAUNCH(2);
+    else if (w.K <= 768) GVQ_LAUNCH(3);
+    else GVQ_LAUNCH(4);
+#undef GVQ_LAUNCH
+    return check_launch(c, "gemv_w8a8_q_adapters");
+}
+
 // act(W8A8(a) + bias + adapters): the rows quantized and their low-rank parts formed in one pass over them, then
 // the product with the adapters in its epilogue. Chunk after chunk of rows, for which gemm_w8a8_pt's byte offsets
 // and a launch's thread numbers fit 32 bits. Arguments checked.
 int run_linear_adapters(enchip_ctx *c, const Weight &w, const AdapterSet &set, const float *d_a, int64_t M, const int32_t *d_ids,
                         const float *d_bias, int act, float *d_dst, hipStream_t s) {
+    if (one_launch(c, w, set, M, d_a)) {  // no scratch
+        const enchip::Adapters p = view(c, set, d_ids);
+        return act == ENCHIP_ACT_GELU ? launch_one<enchip::EPI_F32_GELU>(c, w, p, d_a, M, d_bias, d_dst, s)
+                                      : launch_one<enchip::EPI_F32>(c, w, p, d_a, M, d_bias, d_dst, s);
+    }
     const int64_t by_codes = (((int64_t)1 << 31) - 1) / w.Kp, by_pieces = ((int64_t)1 << 34) / round_up(w.N, 32);
     const int64_t chunk = M <= c->small_m ? M : std::max<int64_t>(128, std::min({kRowChunk, by_codes, by_pieces}) / 128 * 128);
     int rc;
@@ -587,22 +610,23 @@ int enchip_adapters_create(enchip_ctx *ctx, int64_t K, int64_t N, int64_t rank, 
     set.K = K, set.N = N, set.rank = rank, set.slots = slots;
     set.kb = (K + 31) / 32, set.nb = round_up(N, 256) / 32, set.rt = (rank + 15) / 16;
     // a block of A is 32 k x 16 ranks, one of B 32 columns x 16 ranks: 1 KiB a part each
-    const int64_t na = slots * a_bytes(set), nb = slots * b_bytes(set);
-    if (na + nb > kMaxAdapterBytes)
+    const int64_t bytes[4] = {slots * a_bytes(set), slots * b_bytes(set), slots * f_floats(set) * 4, rank * (K + N) * 4};
+    if (bytes[0] + bytes[1] + bytes[2] > kMaxAdapterBytes)
         return fail(ctx, ENCHIP_ERR_ARG, "adapters_create: %lld slots of K=%lld N=%lld rank=%lld are past 2^36 bytes", (long long)slots,
                     (long long)K, (long long)N, (long long)rank);
     HIP_TRY(ctx, hipSetDevice(ctx->device));
-    size_t cap = 0;
-    if (int rc = ensure(ctx, &set.d_a, &cap, (size_t)na, false)) return rc;
-    cap = 0;
-    if (int rc = ensure(ctx, &set.d_b, &cap, (size_t)nb, false)) {
-        (void)hipFree(set.d_a);
-        return rc;
+    size_t cap[4] = {};
+    int rc = ensure(ctx, &set.d_a, &cap[0], (size_t)bytes[0], false);
+    if (!rc) rc = ensure(ctx, &set.d_b, &cap[1], (size_t)bytes[1], false);
+    if (!rc) rc = ensure(ctx, &set.d_f, &cap[2], (size_t)bytes[2], false);
+    if (!rc) rc = ensure(ctx, &set.d_up, &cap[3], (size_t)bytes[3], false);
+    if (!rc) {
+        hipError_t e = hipMemsetAsync(set.d_a, 0, (size_t)bytes[0], ctx->stream);
+        if (e == hipSuccess) e = hipMemsetAsync(set.d_b, 0, (size_t)bytes[1], ctx->stream);
+        if (e == hipSuccess) e = hipMemsetAsync(set.d_f, 0, (size_t)bytes[2], ctx->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+        if (e != hipSuccess) rc = fail(ctx, ENCHIP_ERR_HIP, "adapters_create: %s", hipGetErrorString(e));
     }
-    hipError_t e = hipMemsetAsync(set.d_a, 0, (size_t)na, ctx->stream);
-    if (e == hipSuccess) e = hipMemsetAsync(set.d_b, 0, (size_t)nb, ctx->stream);
-    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
-    int rc = e == hipSuccess ? ENCHIP_OK : fail(ctx, ENCHIP_ERR_HIP, "adapters_create: %s", hipGetErrorString(e));
     if (!rc) {
         try {
             ctx->adapters[ctx->next_handle] = set;
@@ -611,8 +635,7 @@ int enchip_adapters_create(enchip_ctx *ctx, int64_t K, int64_t N, int64_t rank, 
         }
     }
     if (rc) {
-        (void)hipFree(set.d_a);
-        (void)hipFree(set.d_b);
+        free_adapters(set);
         return rc;
     }
     *out = ctx->next_handle++;
@@ -627,35 +650,25 @@ int enchip_adapters_set(enchip_ctx *ctx, enchip_adapters h, int64_t slot, const 
     if (rc) return rc;
     if (slot < 0 || slot >= set->slots) return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: slot %lld of %lld", (long long)slot, (long long)set->slots);
     if (!A || !B) return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: null pointer");
-    const int64_t K = set->K, N = set->N, R = set->rank, rt = set->rt;
-    std::vector<uint16_t> a, b;
-    try {
-        a.resize((size_t)a_bytes(*set) / 2);
-        b.resize((size_t)b_bytes(*set) / 2);
-    } catch (const std::exception &) {
-        return fail(ctx, ENCHIP_ERR_OOM, "adapters_set: out of host memory");
-    }
-    for (int64_t j = 0; j < R; ++j)
-        for (int64_t k = 0; k < K; ++k) {
-            const float x = A[j * K + k];
-            if (!(std::fabs(x) < 0x1p127f))
-                return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: A[%lld][%lld] is %g", (long long)j, (long long)k, (double)x);
-            const int64_t block = (k / 32 * rt + j / 16) * 3, lane = j % 16 + 16 * (k % 16 / 4);
-            store_parts(x, &a[(size_t)((block * 64 + lane) * 8 + k % 32 / 16 * 4 + k % 4)], 512);
-        }
-    for (int64_t n = 0; n < N; ++n)
-        for (int64_t j = 0; j < R; ++j) {
-            const float x = (float)((double)scale * (double)B[n * R + j]);
-            if (!(std::fabs(x) < 0x1p127f))
-                return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: scale %g times B[%lld][%lld] is %g", (double)scale, (long long)n,
-                            (long long)j, (double)x);
-            const int64_t block = (n / 32 * rt + j / 16) * 3, lane = n % 32 + 32 * (j % 16 / 8);
-            store_parts(x, &b[(size_t)((block * 64 + lane) * 8 + j % 8)], 512);
-        }
+    const int64_t K = set->K, N = set->N, R = set->rank;
+    for (int64_t i = 0; i < R * K; ++i)
+        if (!(std::fabs(A[i]) < 0x1p127f))
+            return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: A[%lld][%lld] is %g", (long long)(i / K), (long long)(i % K), (double)A[i]);
+    for (int64_t i = 0; i < N * R; ++i)
+        if (!(std::fabs((double)scale * (double)B[i]) < 0x1p127))
+            return fail(ctx, ENCHIP_ERR_ARG, "adapters_set: scale %g times B[%lld][%lld] is %g", (double)scale, (long long)(i / R),
+                        (long long)(i % R), (double)scale * (double)B[i]);
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
-    HIP_TRY(ctx, hipMemcpy(set->d_a + slot * a_bytes(*set), a.data(), (size_t)a_bytes(*set), hipMemcpyHostToDevice));
-    HIP_TRY(ctx, hipMemcpy(set->d_b + slot * b_bytes(*set), b.data(), (size_t)b_bytes(*set), hipMemcpyHostToDevice));
+    HIP_TRY(ctx, hipMemcpy(set->d_up, A, (size_t)(R * K) * sizeof(float), hipMemcpyHostToDevice));
+    HIP_TRY(ctx, hipMemcpy(set->d_up + R * K, B, (size_t)(N * R) * sizeof(float), hipMemcpyHostToDevice));
+    const int64_t threads = (set->kb + set->nb) * set->rt * 64;
+    hipLaunchKernelGGL(enchip::adapter_pack, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, ctx->stream, set->d_up, set->d_up + R * K,
+                       (double)scale, (int)K, (int)N, (int)R, (int)set->kb, (int)set->nb, (int)set->rt,
+                       reinterpret_cast<enchip::bf16x8 *>(set->d_a + slot * a_bytes(*set)),
+                       reinterpret_cast<enchip::bf16x8 *>(set->d_b + slot * b_bytes(*set)), set->d_f + slot * f_floats(*set));
+    if ((rc = check_launch(ctx, "adapter_pack"))) return rc;
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));  // work on any stream finds the adapter whole
     return ENCHIP_OK;
 }
 
@@ -667,8 +680,7 @@ int enchip_adapters_release(enchip_ctx *ctx, enchip_adapters h) {
     if (rc) return rc;
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
-    (void)hipFree(set->d_a);
-    (void)hipFree(set->d_b);
+    free_adapters(*set);
     ctx->adapters.erase(h);
     return ENCHIP_OK;
 }

@@ -60,6 +60,8 @@ struct RelPos {
 // Low-rank adapters of one linear's shape (enchip_adapters_create; adapters.h).
 struct AdapterSet {
     char *d_a = nullptr, *d_b = nullptr;  // the slots' parts
+    float *d_f = nullptr;                 // A as it is
+    float *d_up = nullptr;                // an adapter on its way in: A, then B
     int64_t K = 0, N = 0, rank = 0, slots = 0, kb = 0, nb = 0, rt = 0;
 };
 

@@ -631,6 +631,8 @@ int enchip_close(enchip_ctx *ctx) {
         for (auto &kv : ctx->adapters) {
             (void)hipFree(kv.second.d_a);
             (void)hipFree(kv.second.d_b);
+            (void)hipFree(kv.second.d_f);
+            (void)hipFree(kv.second.d_up);
         }
         ctx->adapters.clear();
         void *bufs[] = {ctx->d_aq,  ctx->d_as, ctx->d_a,     ctx->d_dst,     ctx->d_bias,

@@ -709,6 +709,7 @@ constexpr int GV_WAVES = 8, GV_ROWS = 8;
 struct NoAdapters {
     static constexpr bool on = false;
     struct Dot {};
+    struct Row {};
     template <int TN>
     struct Held {};
 };
@@ -813,10 +814,10 @@ constexpr int GVQ_MAX_K = 4096;
 constexpr int GVQ_ROWS = 8, GVQ_WAVES = 8;
 __host__ __device__ inline int gvq_lds_bytes(int Kp) { return Kp * 32 + GVQ_WAVES * GVQ_ROWS * 32 * 4 + 16; }
 
-template <int EPI, int QCH>
-__global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q(
+template <int EPI, int QCH, class AD>
+__device__ __forceinline__ void gemv_w8a8_q_body(
     const float *__restrict__ a, const int8_t *__restrict__ Wf, const float *__restrict__ wS,
-    const float *__restrict__ bias, void *__restrict__ out, int64_t ldo, int M, int N, int K, int Kp) {
+    const float *__restrict__ bias, void *__restrict__ out, int64_t ldo, int M, int N, int K, int Kp, const AD &ad) {
     static_assert(GVQ_ROWS == 8 && GVQ_ROWS <= GVQ_WAVES, "one row per wave, row groups of one accumulator register quad");
     extern __shared__ __attribute__((aligned(16))) int8_t gvq[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -826,6 +827,8 @@ __global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q(
     const int row = rg * GVQ_ROWS + wave;  // the row this wave quantizes (waves < GVQ_ROWS)
     const bool qwave = wave < GVQ_ROWS && row < M;
     float4 v[QCH];
+    typename AD::Row low;  // the adapters' part: of this wave's row, and of this thread's output
+    if constexpr (AD::on) ad.row_begin(low, rg * GVQ_ROWS, wave, M, nb, tid);
     if (qwave) {
         const i32x4 *src = reinterpret_cast<const i32x4 *>(a + (int64_t)row * K);
 #pragma unroll
@@ -864,6 +867,7 @@ __global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q(
                     (!zero && k4 < K4) ? pack_codes(v[c], inv) : 0;
         }
         if (lane == 0) s_as[wave] = sc;
+        if constexpr (AD::on) ad.template row_down<QCH>(low, v, K4, wave, lane);
     }
     __syncthreads();
     i32x16 acc;
@@ -892,10 +896,25 @@ __global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q(
         if (orow < M && col < N) {
             const float ws = wS[col];
             const float bb = bias != nullptr ? bias[col] : kNoBias;
-            reinterpret_cast<float *>(out)[(int64_t)orow * ldo + col] = epilogue<EPI>(sum, s_as[i], ws, bb);
+            float y;
+            if constexpr (AD::on) {
+                y = dequant(sum, s_as[i], ws, bb) + ad.row_up(low, i, nb, c);
+                if (EPI == EPI_F32_GELU) y = gelu_f32(y);
+            } else {
+                y = epilogue<EPI>(sum, s_as[i], ws, bb);
+            }
+            reinterpret_cast<float *>(out)[(int64_t)orow * ldo + col] = y;
         }
     }
 }
+
+template <int EPI, int QCH>
+__global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q(
+    const float *__restrict__ a, const int8_t *__restrict__ Wf, const float *__restrict__ wS,
+    const float *__restrict__ bias, void *__restrict__ out, int64_t ldo, int M, int N, int K, int Kp) {
+    gemv_w8a8_q_body<EPI, QCH>(a, Wf, wS, bias, out, ldo, M, N, K, Kp, NoAdapters{});
+}
+
 
 // Small-M variant for wide N (many output-channel groups, e.g. an int8 ANN index of
 // 10^5..10^6 rows): one wavefront per 32 output channels with the whole K, so no

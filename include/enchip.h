@@ -690,15 +690,16 @@ int enchip_adapters_release(enchip_ctx *ctx, enchip_adapters set);
  * buffers: the adapters of M rows of many requests beside a product y of a's rows (weight-only int8 or 4-bit,
  * f32, any). A row whose id is not in [0, slots) gets y. d_dst may be d_y (with ldd == ldy); otherwise it holds
  * no element of y, and none of a. Sums in f32 of products that are within 2^-24 of exact (operands held in
- * three bf16 parts, from 2^-110 up); an activation that is not finite, or 2^127 or more in magnitude, gives NaN
- * in its row where that has an adapter. Uses the context's shared scratch. M <= 2^30. */
+ * three bf16 parts, from 2^-110 up); an activation or a sum over k that is not finite, or 2^127 or more in
+ * magnitude, gives NaN in its row where that has an adapter. Uses the context's shared scratch. M <= 2^30. */
 int enchip_adapters_add_dev(enchip_ctx *ctx, enchip_adapters set, const float *d_a, int64_t lda, int64_t M,
                             const int32_t *d_ids, const float *d_y, int64_t ldy, float *d_dst, int64_t ldd,
                             void *stream);
 
 /* enchip_w8a8_linear_dev with adapters of w's shape: d_dst[M,N] = act(y + adapters), y = W8A8(a) + bias as
  * enchip_w8a8_linear has it, the adapters' part of the unquantized activations as enchip_adapters_add_dev has
- * it. A row without an adapter gets what enchip_w8a8_linear_dev gives it. d_dst holds no element of a. */
+ * it (2^127 or more in magnitude gives NaN or the sum). A row without an adapter gets what
+ * enchip_w8a8_linear_dev gives it. d_dst holds no element of a. */
 int enchip_w8a8_linear_adapters_dev(enchip_ctx *ctx, enchip_weight w, enchip_adapters set, const float *d_a,
                                     int64_t M, const int32_t *d_ids, const float *d_bias, int act,
                                     float *d_dst, void *stream);

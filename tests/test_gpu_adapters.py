@@ -353,3 +353,66 @@ def test_refusals(ctx):
             torch.cuda.synchronize()
     finally:
         ctx.release_weight(w)
+
+
+# One launch (a's rows 16-byte aligned, K a multiple of 4 up to 1024, ranks to 32, few workgroups) and, beside it, what
+# each of its limits leaves to two.
+@pytest.mark.parametrize("M,K,N,rank,off", [
+    (1, 4, 5, 1, 0), (7, 256, 40, 16, 0), (8, 260, 33, 17, 0), (9, 512, 64, 32, 0), (31, 516, 96, 9, 0), (32, 768, 70, 32, 0),
+    (25, 772, 32, 5, 0), (32, 1024, 1024, 32, 0), (3, 1024, 4100, 8, 0),
+    (16, 384, 96, 8, 1), (16, 386, 96, 8, 0), (16, 1028, 96, 8, 0), (16, 384, 96, 33, 0), (32, 128, 2304, 32, 0), (32, 64, 5000, 8, 0),
+])
+@pytest.mark.parametrize("act", [enchip.ACT_NONE, enchip.ACT_GELU])
+def test_few_rows(ctx, M, K, N, rank, off, act):
+    import torch
+
+    say(f"linear_adapters few rows M={M} K={K} N={N} rank={rank} off={off} act={act}")
+    g = np.random.default_rng(M * 7 + K + rank)
+    wq, ws = workloads.quantize_weights((g.standard_normal((N, K)) * 0.03).astype(np.float32))
+    b = (g.standard_normal(N) * 0.1).astype(np.float32)
+    a, slots = activations(g, M, K), 5
+    a[M // 3] *= np.float32(2.0 ** -40)
+    ids = g.integers(-1, slots + 1, M)
+    ids[M // 2] = slots - 1
+    w = ctx.register_weight(wq, ws)
+    try:
+        with Set(ctx, K, N, rank, slots) as s:
+            da = torch.empty(M * K + off, device="cuda")
+            da[off:] = torch.from_numpy(a).cuda().flatten()
+            di, db = torch.from_numpy(ids.astype(np.int32)).cuda(), torch.from_numpy(b).cuda()
+            out, plain = torch.full((M + 1, N), 4.0, device="cuda"), torch.empty((M, N), device="cuda")
+
+            def call(m, a_, i_, o_):
+                torch.cuda.synchronize()
+                ctx.linear_adapters_dev(w, s.h, a_, m, i_, db.data_ptr(), act, o_)
+                torch.cuda.synchronize()
+
+            at = da.data_ptr() + 4 * off
+            call(M, at, di.data_ptr(), out.data_ptr())
+            ctx.linear_dev(w, at, M, db.data_ptr(), act, plain.data_ptr())
+            torch.cuda.synchronize()
+            got, base = out.cpu().numpy(), plain.cpu().numpy()
+            assert (got[M] == 4.0).all()
+            part, tol = s.of(a, ids)
+            y = linear64(a, wq, ws, b)
+            tol = tol + 2.0 ** -22 * (np.abs(part) + np.abs(y) + np.abs(b))
+            want = y + part
+            if act == enchip.ACT_GELU:
+                tol = 1.13 * (tol + 2.0 ** -24 * np.abs(want)) + 2.0 ** -22 * np.abs(want) + 2.0 ** -22
+                want = oracle.gelu(want.astype(np.float32)).astype(np.float64).reshape(want.shape)
+            bad = ~(np.abs(got[:M] - want) <= tol)
+            assert not bad.any(), (np.argwhere(bad)[:3], got[:M][bad][:3], want[bad][:3], tol[bad][:3])
+            none = (ids < 0) | (ids >= slots)
+            assert np.array_equal(got[:M][none], base[none])
+            # an infinite and a NaN activation leave the other rows as they were
+            if M >= 7:
+                torch.cuda.synchronize()
+                ids[1] = ids[5] = 0
+                da[off + K + K // 2], da[off + 5 * K] = float("inf"), float("nan")
+                di.copy_(torch.from_numpy(ids.astype(np.int32)))
+                call(M, at, di.data_ptr(), out.data_ptr())
+                again = out.cpu().numpy()[:M]
+                rest = [r for r in range(M) if r not in (1, 5)]
+                assert np.isnan(again[[1, 5]]).all() and np.array_equal(again[rest], got[rest])
+    finally:
+        ctx.release_weight(w)
