@@ -48,7 +48,7 @@ the NomicBERT forward's order, with W8A8 linears as in the rest of this module).
 
 Layers with "q_norm" and "k_norm" have their query and key heads RMS-normed in qkv, turned in the same pass when
 `rope` is given (enchip_head_norm_rope_rows_dev). `relpos` (a learned bias by relative position), `kv_heads` fewer
-than `heads`, heads of 128, or sequences given as spans of rows take enchip_attention_bias_dev; embed() then
+than `heads`, or sequences given as spans of rows take enchip_attention_bias_dev (heads of 32, 64 or 128); embed() then
 pools the spans (enchip_pool_mean_l2_spans_dev). Low-rank adapters of many requests stand beside any linear
 but a gated layer's gate and up projection (`adapters`; enchip_w8a8_linear_adapters_dev): each row's by its id.
 
@@ -191,7 +191,7 @@ class DeviceBert:
 
     def bias_attention(self, spans=None) -> bool:
         """Whether the attention is enchip_attention_bias_dev's."""
-        return self.relpos is not None or self.KV != self.H or spans is not None or self.hd == 128
+        return self.relpos is not None or self.KV != self.H or spans is not None
 
     def fused_attention(self, L: int) -> bool:
         if self.bias_attention():

@@ -39,6 +39,20 @@ def test_python_shape_checks():
             c.relpos_from_map(f(8, 2), m)
 
 
+def test_which_models_take_the_biased_attention():
+    from aikit_amd.bert_dev import DeviceBert
+
+    m = DeviceBert.__new__(DeviceBert)
+    for hd in (16, 32, 64, 128):
+        m.relpos, m.H, m.KV, m.hd, m.fused = None, 4, 4, hd, False
+        assert not m.bias_attention() and not m.fused_attention(64)  # as without spans, bias and shared heads
+        assert m.bias_attention(np.zeros((1, 2)))
+        m.KV = 2
+        assert m.bias_attention()
+        m.KV, m.relpos = 4, enchip.RelPos(1, 4)
+        assert m.bias_attention()
+
+
 def test_buckets_by_whole_numbers_are_those_of_the_logarithm():
     for buckets, reach in ((32, 128), (16, 64), (64, 1000), (8, 5), (4, 2)):
         half, e = buckets // 2, buckets // 4
