@@ -9,7 +9,15 @@
 //   adapter_down  t = A_s a for 16 rows by a workgroup, K split over its wavefronts (v_mfma_f32_16x16x32_bf16);
 //                 t goes to scratch in parts, laid out for the second product
 //   adapter_up    y += B_s t for 32 x 32 outputs by a wavefront (v_mfma_f32_32x32x16_bf16)
+//   gemm_w8a8_pt_adapters, gemm_w8a8_adapters, gemv_w8a8_adapters: the second product in the epilogue of the W8A8
+//                 products, whose rows adapter_down quantizes from the registers that it multiplies
 // Rows of a block that have different adapters: each adapter among them in turn, from the lowest such row on.
+//
+// Bound by memory where rows are many: 32768 x 1024 to 1024, rank 16, rows of 8 adapters, take 97 us on MI355X, 41 in
+// adapter_down (134 MB of rows, 34 of codes: 4.1 TB/s) and 57 in the product (34 MB of codes, 134 of outputs;
+// 69 G int8 operations). A pass of its own for the codes, one for the low-rank parts and one for y took 186. 1500 x 1000
+// to 1001 with GELU 8 + 11 us, 512 x 1024 beside 4096 outputs at rank 64 4.5 + 7.4: loads' latency, a workgroup a CU
+// or less.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -372,14 +380,18 @@ __global__ __launch_bounds__(64 * NW, 4) void adapter_down(const float *__restri
     const int64_t mb = blockIdx.x / panels, nb = (int64_t)(blockIdx.x % panels) * 4 + (threadIdx.x >> 6);
     const int64_t col = nb * 32 + r;
     if (nb * 32 >= N) return;
+    const int mine = p.slot(mb * 32 + r, M);
+    float was[16];
+    const float *from = y + min(col, (int64_t)N - 1);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) was[e] = from[min(mb * 32 + acc_row(e, lane), M - 1) * ldy];
     f32x16 d[1];
     Adapters::Held<1> held;
-    p.tiles<1>(p.slot(mb * 32 + r, M), mb, nb, lane, d, held);
+    p.tiles<1>(mine, mb, nb, lane, d, held);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const int64_t row = mb * 32 + acc_row(e, lane);
-        if (row >= M || col >= N) continue;
-        dst[row * ldd + col] = y[row * ldy + col] + d[0][e];
+        if (row < M && col < N) dst[row * ldd + col] = was[e] + d[0][e];
     }
 }
 

@@ -300,9 +300,9 @@ AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_
     else if (len <= 64 && (hd < 128 || heads_beside(p.group, 8) < 2)) plan.split = 1;
     if (plan.split) return plan;
     const int64_t tiles = (len + enchip::FA_KT - 1) / enchip::FA_KT;
-    // the join numbers its threads in 32 bits
+    // with parts one launch holds all: the join's 256 threads for 32 rows, the tiles' 512 for 256 and a part
     const int64_t join = (p.spans ? p.L / 32 + p.nseq : (int64_t)((p.L + 31) / 32) * p.nseq) * p.heads;
-    const int most = join * 256 < ((int64_t)1 << 32) ? (int)std::min<int64_t>(8, tiles) : 1;
+    const int most = join * 1024 < ((int64_t)1 << 32) ? (int)std::min<int64_t>(8, tiles) : 1;
     double least = 0.0;
     for (int wide = 0; wide <= (hd == 64 ? 1 : 0); ++wide) {
         const bool two = hd == 32 || (hd == 64 && !wide);  // workgroups at once on a CU

@@ -13,7 +13,12 @@
 // G lanes hold a head: slot s of a head is two groups of V elements that belong together (the pair's two
 // halves, or neighbours), lane g has slots g, g + G, .... A sum over the head is log2 G exchanges, and every
 // element is loaded and stored once by one lane, in place or not. The angles of a workgroup's rows are
-// computed once, into LDS.
+// computed once, into LDS, while the first rows are on their way.
+//
+// Bound by memory: 8 bytes an element. 64 x 512 rows of 24 heads of 64 (403 MB) take 75 us on MI355X, 5.4 TB/s (a
+// large copy 4.9; norms and rotation in two passes of elementary operations 811); 20011 rows of 20 heads of 128 at
+// positions of their own, interleaved, 89 us, 4.6 TB/s; 16 rows 5 us, a call's latency. Rows loaded after the angles
+// took 82 and 92 us.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -667,7 +667,7 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
                               int64_t kv_heads, int64_t head_dim, float scale, void *stream);
 
 /* enchip_pool_mean_l2_dev of nseq spans of the rows of d_h (d_spans as enchip_attention_bias_dev has them, in
- * any order): the same sums in the same order. An empty span gives zeros. */
+ * any order): the same sums in the same order. An empty span gives zeros. nseq <= 65535, D <= 4096. */
 int enchip_pool_mean_l2_spans_dev(enchip_ctx *ctx, const float *d_h, int64_t ldh, int64_t rows,
                                   const int32_t *d_spans, int64_t nseq, int64_t D, float *d_out, int64_t ldo,
                                   void *stream);
@@ -678,7 +678,8 @@ int enchip_pool_mean_l2_spans_dev(enchip_ctx *ctx, const float *d_h, int64_t ldh
  * enchip_adapters_set copies an adapter from the host into a slot (scale B rounded to f32 once); until then the
  * slot adds nothing. It waits for the context's stream; on another stream no work may be in flight that
  * reads the set. A, B, scale B finite and below 2^127 in magnitude. 1 <= rank <= 256, 1 <= slots <= 65536, K <= 131072,
- * N <= 2^24, and 6 slots rank (K + N) bytes (rounded up to 16, 32 and 256) at most 2^36. */
+ * N <= 2^24, and slots rank (10 K + 6 N) bytes (K and N rounded up to 32, rank to 16) at most 2^36; the set holds
+ * one adapter as it came beside them. */
 typedef uint64_t enchip_adapters; /* opaque handle; 0 is never a valid handle */
 int enchip_adapters_create(enchip_ctx *ctx, int64_t K, int64_t N, int64_t rank, int64_t slots,
                            enchip_adapters *out);
