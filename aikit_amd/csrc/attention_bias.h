@@ -17,7 +17,7 @@
 // sums to run on and halve the loads of keys from LDS, where the registers allow it (heads of 32 and 64). On MI355X,
 // flops of the formula (4 len^2 hd) a second: 64 x 512 rows of 12 heads of 64 179 us, 288 TF; 8192 rows 547 us, 377 TF
 // (a third of a large f16 product's rate is 361); 20011 rows of documents of 1 to 1024, 16 heads of 128 that share 4 key
-// heads, 317 us, 257 TF. 1 x 512 rows take 12.3 us and 1 x 16 5.1, a call's latency.
+// heads, longest first 296 us, 275 TF (317 as they come). 1 x 512 rows take 12.3 us and 1 x 16 5.1, a call's latency.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,6 +36,7 @@ struct AttnBias {
     float *out;
     int64_t ldq, ldk, ldv, ldo;
     const int2 *spans;   // [nseq] start, end of ascending spans; null: nseq sequences of L rows
+    const int4 *order;   // attention_bias: the spans longest first (attention_bias_order); null: as they come
     const float *table;  // [heads][2 reach + 1], b log2 e of distance -reach .. reach; null: no bias
     int nseq, heads, group, reach;
     int L;       // rows of a sequence, or with spans those of the buffers
@@ -84,34 +85,97 @@ struct AbLayout {
     static constexpr int BYTES = BIAS + 2 * WINDOW * 4;
 };
 
+// The last of n things whose first(i), ascending, is at or below b, found 64 at a time by a wavefront; -1: none.
+template <class F>
+__device__ __forceinline__ int ab_last(int n, int b, F first) {
+    const int lane = threadIdx.x & 63, count = n;
+    for (int lo = 0;;) {
+        const int step = (n + 63) / 64, z = lo + lane * step;
+        const bool in = lane * step < n && first(min(z, count - 1)) <= b;
+        const int below = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
+        if (below == 0) return -1;
+        n = min(step, n - (below - 1) * step);
+        lo += (below - 1) * step;
+        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+    }
+}
+
 // The workgroup's rows, QR = 2^qs queries from q0 on of the L from row0 on: false where it has none. Of ascending
-// spans, span z has the query blocks start / QR + z .. of the launch, at least as many as it needs; the last span
-// whose first block is at or below b is found 64 at a time. (Spans out of order leave queries out; nothing is
-// read past the buffers.)
+// spans, span z has the query blocks start / QR + z .. of the launch, at least as many as it needs. (Spans out of order
+// leave queries out; nothing is read past the buffers.)
 __device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int qs, int64_t &row0, int &len, int &q0) {
     if (p.spans == nullptr) {
         const int nqb = (p.L + (1 << qs) - 1) >> qs, z = b / nqb;
         row0 = (int64_t)z * p.L, len = p.L, q0 = (b - z * nqb) << qs;
         return true;
     }
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = p.nseq;
-    for (;;) {
-        const int step = (n + 63) / 64, z = lo + lane * step;
-        const bool in = lane * step < n && (max(p.spans[min(z, p.nseq - 1)].x, 0) >> qs) + z <= b;
-        const int below = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
-        if (below == 0) return false;
-        n = min(step, n - (below - 1) * step);
-        lo += (below - 1) * step;
-        if (step == 1) break;
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int lo = ab_last(p.nseq, b, [&](int z) { return (max(p.spans[z].x, 0) >> qs) + z; });
+    if (lo < 0) return false;
     const int2 s = p.spans[lo];
     const int start = min(max(s.x, 0), p.L), end = min(max(s.y, start), p.L);
     const int64_t at = (int64_t)(b - ((start >> qs) + lo)) << qs;
     if (at < 0 || at >= end - start) return false;
     row0 = start, len = end - start, q0 = (int)at;
     return true;
+}
+
+// The same of the launch's workgroup b in p.order: sequence by sequence, each head set's query blocks behind each other.
+__device__ __forceinline__ bool ab_ordered(const AttnBias &p, int b, int qs, int &set, int64_t &row0, int &len, int &q0) {
+    const int sets = p.heads >> p.share, lo = ab_last(p.nseq, b / sets, [&](int z) { return p.order[z].x; });
+    if (lo < 0) return false;
+    const int4 s = p.order[lo];
+    const int at = b - s.x * sets, blocks = (s.z + (1 << qs) - 1) >> qs;
+    if (at >= (int64_t)blocks * sets) return false;
+    set = at / blocks;
+    row0 = s.y, len = s.z, q0 = (at - set * blocks) << qs;
+    return true;
+}
+
+// The spans by falling length, in steps of an eighth of a power of two of their key tiles, each with its first query
+// block: a workgroup's time goes by its sequence's length, and a long one that starts last leaves the others waiting.
+// Within a step the order is the atomics'; no result depends on it. One workgroup, at most AB_ORDER_MAX spans, which fill
+// order whatever they hold (overlapping ones have more query blocks than the launch; those are left out).
+constexpr int AB_ORDER_NT = 1024, AB_ORDER_MAX = 65536;
+[[maybe_unused]] static __global__ __launch_bounds__(AB_ORDER_NT) void attention_bias_order(const int2 *__restrict__ spans, int nseq, int rows,
+                                                                                           int qs, int4 *__restrict__ order) {
+    constexpr int BINS = 256;  // steps of 2^24 tiles and less
+    constexpr int COUNT = 44;  // a step's spans from bit 44 on, below them their query blocks: 2^25 of a span and less
+    __shared__ unsigned long long next[BINS];
+    const int tid = threadIdx.x;
+    if (tid < BINS) next[tid] = 0;
+    __syncthreads();
+    auto span = [&](int z, int &start, int &len) {  // its step, longest first
+        const int2 s = spans[z];
+        start = min(max(s.x, 0), rows), len = min(max(s.y, start), rows) - start;
+        const uint32_t f = __float_as_uint((float)(len / FA_KT + 1));
+        return BINS - 1 - (int)((f >> 20) - (127u << 3));
+    };
+    for (int z = tid; z < nseq; z += AB_ORDER_NT) {
+        int start, len;
+        const int bin = span(z, start, len);
+        atomicAdd(&next[bin], (1ull << COUNT) + (((unsigned)len + (1u << qs) - 1) >> qs));
+    }
+    __syncthreads();
+    if (tid < 64) {
+        unsigned long long own[BINS / 64], sum = 0;
+#pragma unroll
+        for (int i = 0; i < BINS / 64; ++i) own[i] = next[tid * (BINS / 64) + i], sum += own[i];
+        unsigned long long at = sum;
+        for (int o = 1; o < 64; o *= 2) {
+            const unsigned long long v = __shfl_up(at, o, 64);
+            if (tid >= o) at += v;
+        }
+        at -= sum;
+#pragma unroll
+        for (int i = 0; i < BINS / 64; ++i) next[tid * (BINS / 64) + i] = at, at += own[i];
+    }
+    __syncthreads();
+    for (int z = tid; z < nseq; z += AB_ORDER_NT) {
+        int start, len;
+        const int bin = span(z, start, len);
+        const unsigned long long at = atomicAdd(&next[bin], (1ull << COUNT) + (((unsigned)len + (1u << qs) - 1) >> qs));
+        order[at >> COUNT] = make_int4((int)min(at & ((1ull << COUNT) - 1), 0x7fffffffull), start, len, 0);
+    }
 }
 
 // acc[u] += (ah + al) (b_h(u) + b_l(u)) less al b_l, a product of every accumulator in turn.
@@ -155,11 +219,22 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
     extern __shared__ __attribute__((aligned(16))) char ab_lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, hf = lane >> 5;
-    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_part = gridDim.x / ((p.heads >> p.share) * p.parts);
-    const int sp = logical / per_part, set = sp / p.parts, part = sp - set * p.parts, qs = __builtin_ctz(QB) - p.share, QR = 1 << qs;
+    const int qs = __builtin_ctz(QB) - p.share, QR = 1 << qs;
+    int set, part, L, q0;
     int64_t row0;
-    int L, q0;
-    if (!ab_rows(p, logical - sp * per_part, qs, row0, L, q0)) return;
+    if (p.order != nullptr) {
+        // whole keys, the longest sequences of every head first, in runs of 4 blocks on one XCD (32768 rows of 64 equal
+        // spans, 16 heads of 128 that share 4 key heads 473 us, runs of 1 498, of 8 466; 82 documents of 1 to 4096, 8 heads
+        // 742, 757 and 754)
+        part = 0;
+        const int at = blockIdx.x;
+        if (!ab_ordered(p, (at & ~31) + (at & 7) * 4 + ((at >> 3) & 3), qs, set, row0, L, q0)) return;
+    } else {
+        const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_part = gridDim.x / ((p.heads >> p.share) * p.parts);
+        const int sp = logical / per_part;
+        set = sp / p.parts, part = sp - set * p.parts;
+        if (!ab_rows(p, logical - sp * per_part, qs, row0, L, q0)) return;
+    }
     // the wavefront's head and its first query
     const int mate = (wave * 32 * QPW) >> qs, head = (set << p.share) + mate, qr = (wave * 32 * QPW) & (QR - 1), qw = q0 + qr;
     const bool active = qw < L;

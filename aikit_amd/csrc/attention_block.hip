@@ -235,7 +235,7 @@ int launch_attention_bias(enchip_ctx *ctx, void (*fn)(enchip::AttnBias), int lds
         enchip::AttnBias c = p;
         c.q += row * p.ldq, c.k += row * p.ldk, c.v += row * p.ldv, c.out += row * p.ldo;
         c.nseq = (int)nz;
-        hipLaunchKernelGGL(fn, dim3((unsigned)(per * (p.spans ? 1 : nz) * sets)), dim3((unsigned)threads), (size_t)lds, s, c);
+        hipLaunchKernelGGL(fn, dim3((unsigned)(p.order ? round_up(per * sets, 32) : per * (p.spans ? 1 : nz) * sets)), dim3((unsigned)threads), (size_t)lds, s, c);
     }
     return check_launch(ctx, "attention_bias");
 }
@@ -248,13 +248,24 @@ int heads_beside(int64_t group, int nw) {
 }
 
 template <int HD, int NW, int QPW>
-int attention_bias_tiles(enchip_ctx *ctx, enchip::AttnBias p, bool vec, int parts, hipStream_t s) {
+int attention_bias_tiles(enchip_ctx *ctx, enchip::AttnBias p, bool vec, int parts, bool order, hipStream_t s) {
     const int qs = __builtin_ctz(32 * NW * QPW), threads = 64 * NW, lds = enchip::AbLayout<HD, NW, QPW>::BYTES;
     p.share = heads_beside(p.group, NW);
+    int rc;
+    if (order) {
+        if ((rc = ensure(ctx, &ctx->d_att, &ctx->att_cap, (size_t)p.nseq * sizeof(int4)))) return rc;
+        if ((rc = scratch_wait(ctx, s))) return rc;
+        int4 *list = reinterpret_cast<int4 *>(ctx->d_att);
+        hipLaunchKernelGGL(enchip::attention_bias_order, dim3(1), dim3(enchip::AB_ORDER_NT), 0, s, p.spans, p.nseq, p.L, qs - p.share, list);
+        p.order = list;
+        if ((rc = launch_attention_bias(ctx, vec ? enchip::attention_bias<HD, NW, QPW, true> : enchip::attention_bias<HD, NW, QPW, false>,
+                                        lds, threads, qs - p.share, p, s)))
+            return rc;
+        return scratch_record(ctx, s);
+    }
     if (parts == 1)
         return launch_attention_bias(ctx, vec ? enchip::attention_bias<HD, NW, QPW, true> : enchip::attention_bias<HD, NW, QPW, false>,
                                      lds, threads, qs - p.share, p, s);
-    int rc;
     const size_t outputs = (size_t)parts * (size_t)p.rows * (size_t)p.heads;
     if ((rc = ensure(ctx, &ctx->d_att, &ctx->att_cap, outputs * (HD + 2) * sizeof(float)))) return rc;
     if ((rc = scratch_wait(ctx, s))) return rc;
@@ -286,14 +297,19 @@ int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
 //   1 x 1024 60 -> 34; 24 x 512 95 by 512, 85 by 256; 20011 packed rows of 1 to 1024 194 by 512, 152 by 256.
 //   Rows of 64 and less whose heads of 128 do not share keys four and more: attention_bias_split with a wavefront alone
 //   (1000 x 16 rows 118 -> 37, 200 x 64 41 -> 34, 5000 packed rows of 1 to 64 50 -> 22; 64 x 128 29.5 against 32).
+//   Spans go longest first (attention_bias_order, a launch of 3 to 4 us) where a workgroup and a half a CU may come of
+//   them: 20011 rows of documents of 1 to 1024, 12 heads of 64 154 -> 130, 16 heads of 128 316 -> 295, 5000 of them 97 -> 74;
+//   64 x 512 padded rows 162 -> 75 (as they come, the padding's query blocks are a workgroup each); 64 equal spans of
+//   512 270 -> 179, 16 heads of 128 that share 4 key heads 457 -> 460. 2500 rows, under the rule, 35.8 -> 36.6.
 struct AttnPlan {
     int split;  // wavefronts of attention_bias_split, 0: tiles
     bool wide;
     int parts;
+    bool order;  // spans longest first
 };
 
 AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_t hd) {
-    AttnPlan plan{0, false, 1};
+    AttnPlan plan{0, false, 1, false};
     const int64_t cus = ctx->num_cus, len = p.spans ? std::max<int64_t>(1, p.L / p.nseq) : p.L;
     auto blocks = [&](int64_t rows, int64_t heads) { return (len + rows - 1) / rows * p.nseq * heads; };
     if (len <= 512 && 2 * blocks(32, p.heads) <= 3 * cus) plan.split = 8;
@@ -321,6 +337,9 @@ AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_
             }
         }
     }
+    const int share = heads_beside(p.group, hd == 64 && !plan.wide ? 4 : 8);
+    const int64_t n = (p.L / ((plan.wide ? 512 : 256) >> share) + p.nseq) * (p.heads >> share);
+    plan.order = p.spans != nullptr && plan.parts == 1 && p.nseq > 1 && p.nseq <= enchip::AB_ORDER_MAX && 2 * n >= 3 * cus && join * 1024 < ((int64_t)1 << 32);
     return plan;
 }
 
@@ -371,6 +390,7 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     p.share = 0;
     p.parts = 1;
     p.part = p.stat = nullptr;
+    p.order = nullptr;
     p.rows = d_spans ? L : nseq * L;
     const bool vec = ldo % 4 == 0 && (uintptr_t)d_out % 16 == 0;
     const AttnPlan plan = attention_plan(ctx, p, head_dim);
@@ -380,10 +400,10 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     if (plan.split == 1 && head_dim == 32) return attention_bias_split<32, 1>(ctx, p, s);
     if (plan.split == 1 && head_dim == 64) return attention_bias_split<64, 1>(ctx, p, s);
     if (plan.split == 1) return attention_bias_split<128, 1>(ctx, p, s);
-    if (head_dim == 32) return attention_bias_tiles<32, 8, 1>(ctx, p, vec, plan.parts, s);
-    if (head_dim == 64 && plan.wide) return attention_bias_tiles<64, 8, 2>(ctx, p, vec, plan.parts, s);
-    if (head_dim == 64) return attention_bias_tiles<64, 4, 2>(ctx, p, vec, plan.parts, s);
-    return attention_bias_tiles<128, 8, 1>(ctx, p, vec, plan.parts, s);
+    if (head_dim == 32) return attention_bias_tiles<32, 8, 1>(ctx, p, vec, plan.parts, plan.order, s);
+    if (head_dim == 64 && plan.wide) return attention_bias_tiles<64, 8, 2>(ctx, p, vec, plan.parts, plan.order, s);
+    if (head_dim == 64) return attention_bias_tiles<64, 4, 2>(ctx, p, vec, plan.parts, plan.order, s);
+    return attention_bias_tiles<128, 8, 1>(ctx, p, vec, plan.parts, plan.order, s);
 }
 
 // ---------------------------------------------------------------------------- low-rank adapters

@@ -22,7 +22,7 @@
  *     gpu/enccuda/backend.go:87,141-142). Host-pointer entry points are synchronous.
  *   - The context's device scratch (the quantized activations of the entry points
  *     that quantize themselves, the split rows of the weight-only products, the top-k candidates, the low-rank
- *     rows of adapters, the parts of an attention with a bias) is shared by all of them. Work
+ *     rows of adapters, the parts or the order of an attention with a bias) is shared by all of them. Work
  *     that uses it on one stream waits, on the device, for its last use on another
  *     stream (through an event of the library; the first work on a caller's stream waits
  *     for all that the context's stream holds), so host calls and
@@ -653,14 +653,14 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos relpos);
  * rows of the buffers and d_spans[2 z], d_spans[2 z + 1] (device) are the first row of sequence z and the one
  * past its last, ascending: no span starts before the one ahead of it ends. Spans may be empty and leave gaps (a padded batch, or
  * documents of any lengths packed behind each other); rows of no span are not read and their output stays as
- * it was. (Spans are cut off at 0 and L. Where they are out of order, rows stay as they were.)
+ * it was. (Spans are cut off at 0 and L. Where they are out of order, rows may stay as they were.)
  * A query all of whose biases are -infinity gets zeros. Products as in ENCHIP_ATT_FLASH_F16, whatever
  * enchip_set_attention_products says: scale q log2 e, k and v in two f16 parts each (within 2^-22, and 2^-25 below
  * 2^-3), below 65520 in magnitude (larger, infinite and NaN ones give NaN in the rows that see them); scores, weights
  * and sums in f32, in an order that goes by the sizes (by L / nseq with d_spans). head_dim 32, 64 or 128; pitches of
  * q, k, v multiples of 4 below 2^25, q, k, v 16-byte aligned, d_spans 8-byte; d_out holds no element of q, k or v;
- * L <= 2^30, nseq L <= 2^31, nseq <= 2^22 with d_spans. Few queries of many keys are split over workgroups through the
- * context's shared scratch. */
+ * L <= 2^30, nseq L <= 2^31, nseq <= 2^22 with d_spans. Few queries of many keys are split over workgroups, and
+ * many spans taken longest first, through the context's shared scratch. */
 int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float *d_q, int64_t ldq,
                               const float *d_k, int64_t ldk, const float *d_v, int64_t ldv, float *d_out,
                               int64_t ldo, const int32_t *d_spans, int64_t nseq, int64_t L, int64_t heads,

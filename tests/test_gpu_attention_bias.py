@@ -435,3 +435,93 @@ def test_pool_spans(ctx):
             ctx.pool_mean_l2_spans_dev(h.data_ptr(), k.get("ld", 96), 400, k.get("spans", sp.data_ptr()), k.get("nseq", 7), 96,
                                        out.data_ptr(), 96)
     torch.cuda.synchronize()
+
+
+def ragged(T, n, seed):
+    """n ascending spans of T rows: some empty, some of a row or two, one long, gaps."""
+    g = np.random.default_rng(seed)
+    size = g.lognormal(0, 1.2, n)
+    size[g.random(n) < 0.1] = 0
+    size[n // 3] = size.sum() * 0.3
+    size = np.floor(size / size.sum() * T * 0.9).astype(int)
+    spans, at = [], 0
+    for z in size:
+        at += int(g.integers(0, 2)) * int(g.integers(0, T // n // 10))
+        spans.append((at, min(at + int(z), T)))
+        at = spans[-1][1]
+    return spans
+
+
+@pytest.mark.parametrize("heads,kv,hd,T,n", [(32, 32, 32, 3000, 30), (16, 16, 64, 5000, 40), (64, 16, 64, 2600, 33), (16, 2, 64, 9000, 70),
+                                             (32, 8, 128, 3000, 30), (10, 10, 128, 5000, 55)])
+@pytest.mark.parametrize("ldo", [0, 3])
+def test_longest_first(ctx, heads, kv, hd, T, n, ldo):
+    say(f"attention_bias spans longest first heads={heads} kv={kv} hd={hd} T={T} n={n} ldo+{ldo}")
+    spans = ragged(T, n, T + n + hd)
+    c = Case(heads, kv, hd, T, reach=100, buckets=32)
+    inside = np.zeros(T, bool)
+    for a, b in spans:
+        inside[a:b] = True
+    assert not inside.all()
+    c.x[~inside] = np.nan
+    q = c.x[inside]
+    assert np.isfinite(q).all()
+    c.check(ctx, spans=spans, ldo=heads * hd + ldo)
+
+
+def test_longest_first_in_a_graph_and_on_two_streams(ctx):
+    import torch
+
+    heads, hd, T, n = 24, 64, 4000, 40
+    W = 3 * heads * hd
+    x = torch.empty((T, W), device="cuda")
+    y, e, z = (torch.zeros((T, heads * hd), device="cuda") for _ in range(3))
+    lists = [torch.tensor(ragged(T, n, i), dtype=torch.int32, device="cuda") for i in range(4)]
+    spans = lists[3].clone()
+    rp = ctx.relpos(np.random.default_rng(2).standard_normal((32, heads)).astype(np.float32), 128)
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def call(out, stream):
+        p = x.data_ptr()
+        ctx.attention_bias_dev(rp, p, W, p + 4 * heads * hd, W, p + 8 * heads * hd, W, out.data_ptr(), heads * hd, n, T, heads, heads, hd,
+                               0.125, spans.data_ptr(), stream)
+
+    try:
+        with torch.cuda.stream(s):
+            x.normal_()
+        call(e, s.cuda_stream)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            call(y, s.cuda_stream)
+        say("attention_bias longest first captured, 3 replays with other spans; two streams on the shared scratch")
+        for i in range(3):
+            with torch.cuda.stream(s):
+                x.normal_()
+                spans.copy_(lists[i])
+                y.zero_(), e.zero_()
+            torch.cuda.synchronize()
+            gr.replay()
+            torch.cuda.synchronize()
+            call(e, s.cuda_stream)
+            torch.cuda.synchronize()
+            assert torch.equal(y, e)
+        del gr
+        for u in (y, z, e):
+            u.zero_()
+        torch.cuda.synchronize()
+        for _ in range(6):
+            call(y, s.cuda_stream), call(z, t.cuda_stream), call(e, 0)
+        torch.cuda.synchronize()
+        assert torch.equal(y, z) and torch.equal(y, e)
+    finally:
+        ctx.release_relpos(rp)
+
+
+def test_many_spans_out_of_order_stay_in_bounds(ctx):
+    # not a valid call: rows may stay as they were or be another span's, and nothing outside the buffers is touched
+    say("attention_bias many spans out of order")
+    c = Case(24, 24, 64, 3000)
+    far = [(-2 ** 31, 2 ** 31 - 1)] * 10 + [(2900 - 100 * i, 3000 - 100 * i) for i in range(29)] + [(2 ** 31 - 1, -2 ** 31)]
+    assert np.isfinite(c.run(ctx, spans=far)).all()
