@@ -297,7 +297,7 @@ int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
 //   1 x 1024 60 -> 34; 24 x 512 95 by 512, 85 by 256; 20011 packed rows of 1 to 1024 194 by 512, 152 by 256.
 //   Rows of 64 and less whose heads of 128 do not share keys four and more: attention_bias_split with a wavefront alone
 //   (1000 x 16 rows 118 -> 37, 200 x 64 41 -> 34, 5000 packed rows of 1 to 64 50 -> 22; 64 x 128 29.5 against 32).
-//   Spans go longest first (attention_bias_order, a launch of 3 to 4 us) where a workgroup and a half a CU may come of
+//   Spans go longest first (attention_bias_order, a launch of 5 us) where a workgroup and a half a CU may come of
 //   them: 20011 rows of documents of 1 to 1024, 12 heads of 64 154 -> 130, 16 heads of 128 316 -> 295, 5000 of them 97 -> 74;
 //   64 x 512 padded rows 162 -> 75 (as they come, the padding's query blocks are a workgroup each); 64 equal spans of
 //   512 270 -> 179, 16 heads of 128 that share 4 key heads 457 -> 460. 2500 rows, under the rule, 35.8 -> 36.6.
