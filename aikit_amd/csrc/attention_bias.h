@@ -36,7 +36,7 @@ struct AttnBias {
     float *out;
     int64_t ldq, ldk, ldv, ldo;
     const int2 *spans;   // [nseq] start, end of ascending spans; null: nseq sequences of L rows
-    const int4 *order;   // attention_bias: the spans longest first (attention_bias_order); null: as they come
+    const int4 *order;   // the spans longest first (attention_bias_order); null: as they come
     const float *table;  // [heads][2 reach + 1], b log2 e of distance -reach .. reach; null: no bias
     int nseq, heads, group, reach;
     int L;       // rows of a sequence, or with spans those of the buffers
@@ -512,10 +512,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_bias_split(AttnBias p) {
     float *ctx = reinterpret_cast<float *>(ab_lds), *top = ctx + NW * 32 * Lay::PITCH, *sum = top + NW * 32;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
-    const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_head = gridDim.x / p.heads, head = logical / per_head;
+    int head, L, q0;
     int64_t row0;
-    int L, q0;
-    if (!ab_rows(p, logical - head * per_head, 5, row0, L, q0)) return;
+    if (NW == 1 && p.order != nullptr) {
+        const int at = blockIdx.x;
+        if (!ab_ordered(p, (at & ~31) + (at & 7) * 4 + ((at >> 3) & 3), 5, head, row0, L, q0)) return;
+    } else {
+        const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_head = gridDim.x / p.heads;
+        head = logical / per_head;
+        if (!ab_rows(p, logical - head * per_head, 5, row0, L, q0)) return;
+    }
     const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
     const float *vbase = p.v + row0 * p.ldv + (head / p.group) * HD;
     const float *table = p.table ? p.table + (int64_t)head * (2 * p.reach + 1) + p.reach : nullptr;

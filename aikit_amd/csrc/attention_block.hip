@@ -247,17 +247,24 @@ int heads_beside(int64_t group, int nw) {
     return share;
 }
 
+// p's spans longest first, in scratch, for query blocks of 2^qs rows.
+int order_spans(enchip_ctx *ctx, enchip::AttnBias &p, int qs, hipStream_t s) {
+    int rc;
+    if ((rc = ensure(ctx, &ctx->d_att, &ctx->att_cap, (size_t)p.nseq * sizeof(int4)))) return rc;
+    if ((rc = scratch_wait(ctx, s))) return rc;
+    int4 *list = reinterpret_cast<int4 *>(ctx->d_att);
+    hipLaunchKernelGGL(enchip::attention_bias_order, dim3(1), dim3(enchip::AB_ORDER_NT), 0, s, p.spans, p.nseq, p.L, qs, list);
+    p.order = list;
+    return check_launch(ctx, "attention_bias_order");
+}
+
 template <int HD, int NW, int QPW>
 int attention_bias_tiles(enchip_ctx *ctx, enchip::AttnBias p, bool vec, int parts, bool order, hipStream_t s) {
     const int qs = __builtin_ctz(32 * NW * QPW), threads = 64 * NW, lds = enchip::AbLayout<HD, NW, QPW>::BYTES;
     p.share = heads_beside(p.group, NW);
     int rc;
     if (order) {
-        if ((rc = ensure(ctx, &ctx->d_att, &ctx->att_cap, (size_t)p.nseq * sizeof(int4)))) return rc;
-        if ((rc = scratch_wait(ctx, s))) return rc;
-        int4 *list = reinterpret_cast<int4 *>(ctx->d_att);
-        hipLaunchKernelGGL(enchip::attention_bias_order, dim3(1), dim3(enchip::AB_ORDER_NT), 0, s, p.spans, p.nseq, p.L, qs - p.share, list);
-        p.order = list;
+        if ((rc = order_spans(ctx, p, qs - p.share, s))) return rc;
         if ((rc = launch_attention_bias(ctx, vec ? enchip::attention_bias<HD, NW, QPW, true> : enchip::attention_bias<HD, NW, QPW, false>,
                                         lds, threads, qs - p.share, p, s)))
             return rc;
@@ -280,8 +287,12 @@ int attention_bias_tiles(enchip_ctx *ctx, enchip::AttnBias p, bool vec, int part
 }
 
 template <int HD, int NW>
-int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
-    return launch_attention_bias(ctx, enchip::attention_bias_split<HD, NW>, enchip::AbSplit<HD, NW>::BYTES, 64 * NW, 5, p, s);
+int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, bool order, hipStream_t s) {
+    if (!order) return launch_attention_bias(ctx, enchip::attention_bias_split<HD, NW>, enchip::AbSplit<HD, NW>::BYTES, 64 * NW, 5, p, s);
+    int rc;
+    if ((rc = order_spans(ctx, p, 5, s))) return rc;
+    if ((rc = launch_attention_bias(ctx, enchip::attention_bias_split<HD, NW>, enchip::AbSplit<HD, NW>::BYTES, 64 * NW, 5, p, s))) return rc;
+    return scratch_record(ctx, s);
 }
 
 // How an attention runs, from its sizes (spans: as if all had their mean length).
@@ -301,6 +312,8 @@ int attention_bias_split(enchip_ctx *ctx, enchip::AttnBias p, hipStream_t s) {
 //   them: 20011 rows of documents of 1 to 1024, 12 heads of 64 154 -> 130, 16 heads of 128 316 -> 295, 5000 of them 97 -> 74;
 //   64 x 512 padded rows 162 -> 75 (as they come, the padding's query blocks are a workgroup each); 64 equal spans of
 //   512 270 -> 179, 16 heads of 128 that share 4 key heads 457 -> 460. 2500 rows, under the rule, 35.8 -> 36.6.
+//   For a wavefront alone where the mean is past 32 rows and 8 wavefronts a CU may come of them: 20011 rows of 1 to 400 12
+//   heads of 64 109 -> 100, 8 heads of 128 179 -> 147, of 1 to 200 77 -> 76 and 126 -> 115; 5000 rows of 1 to 64 21.6 -> 24.
 struct AttnPlan {
     int split;  // wavefronts of attention_bias_split, 0: tiles
     bool wide;
@@ -314,11 +327,14 @@ AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_
     auto blocks = [&](int64_t rows, int64_t heads) { return (len + rows - 1) / rows * p.nseq * heads; };
     if (len <= 512 && 2 * blocks(32, p.heads) <= 3 * cus) plan.split = 8;
     else if (len <= 64 && (hd < 128 || heads_beside(p.group, 8) < 2)) plan.split = 1;
+    // blocks of 32 rows, of all heads; below single any form's rounded grid is one launch
+    const int64_t join = (p.spans ? p.L / 32 + p.nseq : (int64_t)((p.L + 31) / 32) * p.nseq) * p.heads, single = (int64_t)1 << 22;
+    const bool sorts = p.spans != nullptr && p.nseq > 1 && p.nseq <= enchip::AB_ORDER_MAX && join < single;
+    if (plan.split == 1) plan.order = sorts && len > 32 && join >= 8 * cus;
     if (plan.split) return plan;
     const int64_t tiles = (len + enchip::FA_KT - 1) / enchip::FA_KT;
-    // with parts one launch holds all: the join's 256 threads for 32 rows, the tiles' 512 for 256 and a part
-    const int64_t join = (p.spans ? p.L / 32 + p.nseq : (int64_t)((p.L + 31) / 32) * p.nseq) * p.heads;
-    const int most = join * 1024 < ((int64_t)1 << 32) ? (int)std::min<int64_t>(8, tiles) : 1;
+    // with parts one launch holds all: the join's 256 threads for 32 rows, the tiles' 512 for 256 and each of 8 parts
+    const int most = join < single ? (int)std::min<int64_t>(8, tiles) : 1;
     double least = 0.0;
     for (int wide = 0; wide <= (hd == 64 ? 1 : 0); ++wide) {
         const bool two = hd == 32 || (hd == 64 && !wide);  // workgroups at once on a CU
@@ -339,7 +355,7 @@ AttnPlan attention_plan(const enchip_ctx *ctx, const enchip::AttnBias &p, int64_
     }
     const int share = heads_beside(p.group, hd == 64 && !plan.wide ? 4 : 8);
     const int64_t n = (p.L / ((plan.wide ? 512 : 256) >> share) + p.nseq) * (p.heads >> share);
-    plan.order = p.spans != nullptr && plan.parts == 1 && p.nseq > 1 && p.nseq <= enchip::AB_ORDER_MAX && 2 * n >= 3 * cus && join * 1024 < ((int64_t)1 << 32);
+    plan.order = sorts && plan.parts == 1 && 2 * n >= 3 * cus;
     return plan;
 }
 
@@ -394,12 +410,12 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     p.rows = d_spans ? L : nseq * L;
     const bool vec = ldo % 4 == 0 && (uintptr_t)d_out % 16 == 0;
     const AttnPlan plan = attention_plan(ctx, p, head_dim);
-    if (plan.split == 8 && head_dim == 32) return attention_bias_split<32, 8>(ctx, p, s);
-    if (plan.split == 8 && head_dim == 64) return attention_bias_split<64, 8>(ctx, p, s);
-    if (plan.split == 8) return attention_bias_split<128, 8>(ctx, p, s);
-    if (plan.split == 1 && head_dim == 32) return attention_bias_split<32, 1>(ctx, p, s);
-    if (plan.split == 1 && head_dim == 64) return attention_bias_split<64, 1>(ctx, p, s);
-    if (plan.split == 1) return attention_bias_split<128, 1>(ctx, p, s);
+    if (plan.split == 8 && head_dim == 32) return attention_bias_split<32, 8>(ctx, p, plan.order, s);
+    if (plan.split == 8 && head_dim == 64) return attention_bias_split<64, 8>(ctx, p, plan.order, s);
+    if (plan.split == 8) return attention_bias_split<128, 8>(ctx, p, plan.order, s);
+    if (plan.split == 1 && head_dim == 32) return attention_bias_split<32, 1>(ctx, p, plan.order, s);
+    if (plan.split == 1 && head_dim == 64) return attention_bias_split<64, 1>(ctx, p, plan.order, s);
+    if (plan.split == 1) return attention_bias_split<128, 1>(ctx, p, plan.order, s);
     if (head_dim == 32) return attention_bias_tiles<32, 8, 1>(ctx, p, vec, plan.parts, plan.order, s);
     if (head_dim == 64 && plan.wide) return attention_bias_tiles<64, 8, 2>(ctx, p, vec, plan.parts, plan.order, s);
     if (head_dim == 64) return attention_bias_tiles<64, 4, 2>(ctx, p, vec, plan.parts, plan.order, s);

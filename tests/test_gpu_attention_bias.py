@@ -453,7 +453,9 @@ def ragged(T, n, seed):
 
 
 @pytest.mark.parametrize("heads,kv,hd,T,n", [(32, 32, 32, 3000, 30), (16, 16, 64, 5000, 40), (64, 16, 64, 2600, 33), (16, 2, 64, 9000, 70),
-                                             (32, 8, 128, 3000, 30), (10, 10, 128, 5000, 55)])
+                                             (32, 8, 128, 3000, 30), (10, 10, 128, 5000, 55),
+                                             # a wavefront alone: means of 33 to 64 rows
+                                             (16, 4, 32, 3700, 110), (24, 24, 64, 3000, 60), (12, 12, 128, 5100, 90)])
 @pytest.mark.parametrize("ldo", [0, 3])
 def test_longest_first(ctx, heads, kv, hd, T, n, ldo):
     say(f"attention_bias spans longest first heads={heads} kv={kv} hd={hd} T={T} n={n} ldo+{ldo}")
