@@ -237,6 +237,14 @@ class DeviceBert:
             raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on the device")
         return t.data_ptr()
 
+    def _floats(self, name: str, t, rows: int, more: bool = False) -> None:
+        """Refuses what is no contiguous f32 [rows, D] device tensor; more: further rows may follow."""
+        shape = tuple(t.shape)
+        if len(shape) != 2 or shape[1] != self.D or not (shape[0] == rows or (more and shape[0] > rows)) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{rows}, {self.D}] tensor, not {list(shape)}")
+        if t.dtype != self.torch.float32 or t.device.type != "cuda":
+            raise ValueError(f"{name} must be f32 on the device, not {t.dtype} on {t.device}")
+
     def forward(self, h, S: int, L: int, stream: int = 0, spans=None, pos=None, ids=None) -> None:
         """Runs every layer on h ([S*L, D] f32 on the device), in place, on `stream`.
 
@@ -244,8 +252,7 @@ class DeviceBert:
         the last, ascending (enchip_attention_bias_dev); what h holds in rows of none means nothing. pos (int32
         [S*L]): the rows' positions for `rope`, else row % L. ids (int32 [S*L]): the rows' adapters."""
         c, D, H, hd, M, W = self.ctx, self.D, self.H, self.hd, S * L, self.W
-        if tuple(h.shape) != (M, D) or not h.is_contiguous():
-            raise ValueError(f"h must be a contiguous [{M}, {D}] tensor")
+        self._floats("h", h, M)
         nspans = 0 if spans is None else spans.shape[0]
         d_spans, d_pos = self._ints("spans", spans, (nspans, 2)), self._ints("pos", pos, (M,))
         d_ids = self._ints("ids", ids, (M,))
@@ -361,7 +368,8 @@ class DeviceBert:
 
     def embed(self, h, S: int, L: int, pooled, stream: int = 0, spans=None, pos=None, ids=None) -> None:
         """forward(), then mean pooling + L2 normalisation of each sequence into pooled [S, D], or of
-        each span into pooled [n, D]."""
+        each span into pooled [n, D] (rows of pooled past those stay as they were)."""
+        self._floats("pooled", pooled, S if spans is None else spans.shape[0], more=True)
         self.forward(h, S, L, stream, spans, pos, ids)
         self._m("pool")
         if spans is not None:
