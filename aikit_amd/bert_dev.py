@@ -215,7 +215,14 @@ class DeviceBert:
         ok, ldq = self.ctx.frag_route(down, M)
         return ldq if ok and ldq <= self.GELU_QUANT_MAX_K else 0
 
-    def _buffers(self, S: int, L: int, scores: bool = True):
+    def _on(self, stream: int):
+        """What is allocated within belongs to `stream`, on which the layers run: torch's allocator gives it to
+        another tensor only there, behind the work that is queued on it (not to the caller's tensors, whose work on
+        torch's own stream nothing orders after this object's)."""
+        return self.torch.cuda.stream(self.torch.cuda.ExternalStream(stream or self.ctx.stream()))
+
+    def _buffers(self, S: int, L: int, stream: int, scores: bool = True):
+        """The activations of S * L rows. Nothing is filled: rows are independent, and rows of no span mean nothing."""
         key = (S, L)
         if key not in self._bufs or (scores and self._bufs[key]["scores"].numel() == 1 and not self.fused_attention(L)):
             t, M = self.torch, S * L
@@ -223,11 +230,12 @@ class DeviceBert:
             sc = (1,) if not scores or self.fused_attention(L) else (S, self.H, L, L)
             Mp = (M + 127) // 128 * 128  # fragment-major codes are read up to a multiple of 128 rows
             kp = (max(self.D, self.I) + 63) // 64 * 64  # the widest padded K of the layer's linears
-            self._bufs = {key: dict(qkv=t.empty((M, self.W), **f), scores=t.empty(sc, **f),
-                                    ctx=t.zeros((M, self.D), **f), out=t.empty((M, self.D), **f),
-                                    inter=t.empty((M, self.I), **f), ffn=t.empty((M, self.D), **f),
-                                    codes=t.empty(Mp * kp, device="cuda", dtype=t.int8),
-                                    ascale=t.empty(M, **f))}
+            with self._on(stream):
+                self._bufs = {key: dict(qkv=t.empty((M, self.W), **f), scores=t.empty(sc, **f),
+                                        ctx=t.empty((M, self.D), **f), out=t.empty((M, self.D), **f),
+                                        inter=t.empty((M, self.I), **f), ffn=t.empty((M, self.D), **f),
+                                        codes=t.empty(Mp * kp, device="cuda", dtype=t.int8),
+                                        ascale=t.empty(M, **f))}
         return self._bufs[key]
 
     def _ints(self, name: str, t, shape) -> int:
@@ -246,7 +254,8 @@ class DeviceBert:
             raise ValueError(f"{name} must be f32 on the device, not {t.dtype} on {t.device}")
 
     def forward(self, h, S: int, L: int, stream: int = 0, spans=None, pos=None, ids=None) -> None:
-        """Runs every layer on h ([S*L, D] f32 on the device), in place, on `stream`.
+        """Runs every layer on h ([S*L, D] f32 on the device), in place, on `stream`. One shape's activations are
+        kept: a call on another stream is ordered behind the last one's by the caller.
 
         spans (int32 [n, 2] on the device): the sequences are these spans of the S*L rows, first row and one past
         the last, ascending (enchip_attention_bias_dev); what h holds in rows of none means nothing. pos (int32
@@ -259,7 +268,7 @@ class DeviceBert:
         if ids is not None and self.adapters is None:
             raise ValueError("ids without adapters")
         kv = self.KV * hd
-        b = self._buffers(S, L, spans is None)
+        b = self._buffers(S, L, stream, spans is None)
         qkv, scores, ctxv, out, inter, ffn = b["qkv"], b["scores"], b["ctx"], b["out"], b["inter"], b["ffn"]
         codes, ascale = b["codes"].data_ptr(), b["ascale"].data_ptr()
         q = qkv.data_ptr()
@@ -393,7 +402,11 @@ class DeviceBert:
             raise ValueError("rerank: pooler [D, D], classifier [labels, D], logits [S, labels]")
         self.forward(h, S, L, stream, ids=ids)
         self._m("head")
-        pooled = self._bufs[(S, L)].setdefault("pooled", self.torch.empty((S, D), device="cuda"))
+        b = self._bufs[(S, L)]
+        if "pooled" not in b:
+            with self._on(stream):
+                b["pooled"] = self.torch.empty((S, D), device="cuda")
+        pooled = b["pooled"]
         # CLS rows are every L-th row of h: pitch L*D
         c.matmul_bt_f32_dev(h.data_ptr(), L * D, pw.data_ptr(), D, enchip.B_NK, pooled.data_ptr(), D, S, D, D,
                             stream=stream)

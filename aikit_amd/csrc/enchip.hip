@@ -661,6 +661,14 @@ int enchip_device_info(enchip_ctx *ctx, int *num_cus, int *clock_khz, char *name
     return ENCHIP_OK;
 }
 
+int enchip_stream(enchip_ctx *ctx, void **stream) {
+    if (!ctx) return ENCHIP_ERR_ARG;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (!stream) return fail(ctx, ENCHIP_ERR_ARG, "stream: null pointer");
+    *stream = ctx->stream;
+    return ENCHIP_OK;
+}
+
 int enchip_gemm_kernel_name(enchip_ctx *ctx, enchip_weight h, int64_t M, int act, char *buf, int len) {
     if (!ctx) return ENCHIP_ERR_ARG;
     std::lock_guard<std::mutex> g(ctx->mu);

@@ -39,6 +39,7 @@ _SIGNATURES = {
     "enchip_close": (_int, [_vp]),
     "enchip_last_error": (ctypes.c_char_p, [_vp]),
     "enchip_device_info": (_int, [_vp, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.c_char_p, _int]),
+    "enchip_stream": (_int, [_vp, ctypes.POINTER(_vp)]),
     "enchip_quant_rows": (_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "enchip_weight_register": (_int, [_vp, _vp, _vp, _i64, _i64, ctypes.POINTER(ctypes.c_uint64)]),
     "enchip_weight_release": (_int, [_vp, ctypes.c_uint64]),
@@ -250,6 +251,12 @@ class Context:
         name = ctypes.create_string_buffer(64)
         self._check(self._lib.enchip_device_info(self._h, ctypes.byref(cus), ctypes.byref(clk), name, 64))
         return {"num_cus": cus.value, "clock_khz": clk.value, "arch": name.value.decode()}
+
+    def stream(self) -> int:
+        """The context's own stream (hipStream_t), where device calls with stream 0 run."""
+        s = _vp()
+        self._check(self._lib.enchip_stream(self._h, ctypes.byref(s)))
+        return s.value
 
     def gemm_kernel_name(self, w: Weight, M: int, act: int) -> str:
         buf = ctypes.create_string_buffer(128)

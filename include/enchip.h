@@ -103,6 +103,10 @@ const char *enchip_last_error(const enchip_ctx *ctx);
 int enchip_device_info(enchip_ctx *ctx, int *num_cus, int *clock_khz, char *name,
                        int name_len);
 
+/* The context's own stream (a hipStream_t) into *stream: where the *_dev entry points run that are given
+ * none. For callers whose allocator or events go by stream. It lives until enchip_close. */
+int enchip_stream(enchip_ctx *ctx, void **stream);
+
 /* Per-row dynamic symmetric int8 quantization of a[M,K] into aq[M,K] and
  * ascale[M], on the device, host buffers in and out. Replaces
  * linalg.QuantizeActivationsInto (linalg/quant.go:206-213; all-zero row ->

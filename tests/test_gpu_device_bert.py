@@ -1,0 +1,103 @@
+"""DeviceBert's own buffers: which stream they belong to, and what a change of shape or of attention leaves of them."""
+import numpy as np
+import pytest
+
+from aikit_amd import enchip
+from aikit_amd.bert_dev import DeviceBert
+from test_gpu_attention_block import layers_of
+
+pytestmark = pytest.mark.gpu
+
+D, H, I, HD = 128, 4, 256, 32
+SHAPES = [(4, 64), (2, 96), (4, 63)]  # the third's buffers fit where the first's were
+
+
+def say(msg):
+    print(f"[case] {msg}", flush=True)
+
+
+@pytest.fixture
+def model(ctx):
+    m = DeviceBert(ctx, layers_of(np.random.default_rng(5), 2, D, 3 * D, I, HD, False, False), D, H, I)
+    yield m
+    m.close()
+
+
+def hidden(torch, S, L):
+    return torch.from_numpy(np.random.default_rng(S * L).standard_normal((S * L, D)).astype(np.float32)).cuda()
+
+
+def sleep(torch, stream=None):  # about 50 ms of the shader clock
+    with torch.cuda.stream(stream or torch.cuda.current_stream()):
+        torch.cuda._sleep(100_000_000)
+
+
+def alone(torch, model, stream=0):
+    out = []
+    for S, L in SHAPES:
+        h, p = hidden(torch, S, L), torch.zeros((S, D), device="cuda")
+        torch.cuda.synchronize()
+        model.embed(h, S, L, p, stream)
+        torch.cuda.synchronize()
+        out.append((h.cpu().numpy(), p.cpu().numpy()))
+    return out
+
+
+def test_the_contexts_stream(ctx):
+    import torch
+
+    s = ctx.stream()
+    assert s and s == ctx.stream()
+    x = torch.full((4, 8), 2.0, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.ExternalStream(s)):
+        x.mul_(3.0)
+        x.add_(1.0)
+    torch.cuda.synchronize()
+    assert (x == 7.0).all()
+    assert enchip.load().enchip_stream(ctx.handle, None) == enchip.ERR_ARG
+
+
+@pytest.mark.parametrize("own", [True, False])
+def test_shapes_queued_behind_each_other(ctx, model, own):
+    import torch
+
+    say(f"three shapes queued behind each other, on the context's stream: {own}")
+    want = alone(torch, model)
+    for busy in (True, False):  # torch's stream far behind the layers' stream, or far ahead of it
+        st = torch.cuda.Stream()
+        sp = ctx.stream() if own else st.cuda_stream
+        model._bufs = {}
+        hs = [hidden(torch, *k) for k in SHAPES]
+        ps = [torch.zeros((S, D), device="cuda") for S, _ in SHAPES]
+        torch.cuda.synchronize()
+        sleep(torch, None if busy else torch.cuda.ExternalStream(sp))
+        for (S, L), h, p in zip(SHAPES, hs, ps):
+            model.embed(h, S, L, p, 0 if own else sp)
+        # tensors of the caller's, of the dropped buffers' sizes, while the first shapes may still be queued
+        mine = [torch.full((S * L, w), 7.0, device="cuda") for S, L in SHAPES for w in (3 * D, D, I, D, D)]
+        torch.cuda.synchronize()
+        for (h, p), a, b in zip(want, hs, ps):
+            assert np.array_equal(a.cpu().numpy(), h) and np.array_equal(b.cpu().numpy(), p), busy
+        for t in mine:
+            assert (t == 7.0).all(), busy
+
+
+def test_nothing_of_torchs_stream_lands_between_the_layers(ctx, model):
+    # everything torch has queued lands after the attention and before the linear that reads its output
+    import torch
+
+    say("a new shape behind a busy torch stream")
+    want = alone(torch, model)
+    for i, (S, L) in enumerate(SHAPES):
+        h, p = hidden(torch, S, L), torch.zeros((S, D), device="cuda")
+        torch.cuda.synchronize()
+        model._bufs = {}
+        sleep(torch)
+        model.mark = lambda label: torch.cuda.synchronize() if label.startswith("o") else None
+        try:
+            model.embed(h, S, L, p)
+            torch.cuda.synchronize()
+        finally:
+            model.mark = None
+        assert np.array_equal(h.cpu().numpy(), want[i][0]) and np.array_equal(p.cpu().numpy(), want[i][1])
