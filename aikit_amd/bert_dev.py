@@ -224,19 +224,23 @@ class DeviceBert:
     def _buffers(self, S: int, L: int, stream: int, scores: bool = True):
         """The activations of S * L rows. Nothing is filled: rows are independent, and rows of no span mean nothing."""
         key = (S, L)
-        if key not in self._bufs or (scores and self._bufs[key]["scores"].numel() == 1 and not self.fused_attention(L)):
-            t, M = self.torch, S * L
-            f = dict(device="cuda", dtype=t.float32)
-            sc = (1,) if not scores or self.fused_attention(L) else (S, self.H, L, L)
+        t, M = self.torch, S * L
+        f = dict(device="cuda", dtype=t.float32)
+        scores = scores and not self.fused_attention(L)
+        if key not in self._bufs:
             Mp = (M + 127) // 128 * 128  # fragment-major codes are read up to a multiple of 128 rows
             kp = (max(self.D, self.I) + 63) // 64 * 64  # the widest padded K of the layer's linears
             with self._on(stream):
-                self._bufs = {key: dict(qkv=t.empty((M, self.W), **f), scores=t.empty(sc, **f),
+                self._bufs = {key: dict(qkv=t.empty((M, self.W), **f), scores=t.empty(1, **f),
                                         ctx=t.empty((M, self.D), **f), out=t.empty((M, self.D), **f),
                                         inter=t.empty((M, self.I), **f), ffn=t.empty((M, self.D), **f),
                                         codes=t.empty(Mp * kp, device="cuda", dtype=t.int8),
                                         ascale=t.empty(M, **f))}
-        return self._bufs[key]
+        b = self._bufs[key]
+        if scores and b["scores"].numel() < S * self.H * L * L:  # beside the others, whose addresses a graph may hold
+            with self._on(stream):
+                b["scores"] = t.empty((S, self.H, L, L), **f)
+        return b
 
     def _ints(self, name: str, t, shape) -> int:
         if t is None:

@@ -101,3 +101,44 @@ def test_nothing_of_torchs_stream_lands_between_the_layers(ctx, model):
         finally:
             model.mark = None
         assert np.array_equal(h.cpu().numpy(), want[i][0]) and np.array_equal(p.cpu().numpy(), want[i][1])
+
+
+@pytest.mark.parametrize("L", [70, 1])
+def test_buffers_of_a_shape_stay_where_a_graph_has_them(ctx, L):
+    # heads without a fused attention keep scores, which spans do not need: the shape's other buffers stay
+    import torch
+
+    S = 2
+    g = np.random.default_rng(8)
+    m = DeviceBert(ctx, layers_of(g, 1, D, 3 * D, I, HD, False, False), D, H, I, fused=False)
+    say(f"a captured forward over spans, then one without them, {S} x {L}")
+    try:
+        st = torch.cuda.Stream()
+        x = hidden(torch, S, L)
+        spans = torch.tensor([[0, L], [L, 2 * L]], dtype=torch.int32, device="cuda")
+        h, p, q = x.clone(), torch.zeros((S, D), device="cuda"), torch.zeros((S, D), device="cuda")
+        torch.cuda.synchronize()
+        m.embed(h, S, L, p, st.cuda_stream, spans=spans)
+        torch.cuda.synchronize()
+        want = p.cpu().numpy()
+        held = {k: (t, t.data_ptr()) for k, t in m._bufs[(S, L)].items() if k != "scores"}
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            m.embed(h, S, L, p, st.cuda_stream, spans=spans)
+        for _ in range(3):
+            h.copy_(x)
+            torch.cuda.synchronize()
+            m.embed(h, S, L, q, st.cuda_stream)  # its scores in a buffer of its own
+            torch.cuda.synchronize()
+            assert all(m._bufs[(S, L)][k] is t and t.data_ptr() == at for k, (t, at) in held.items())
+            # unit vectors whose cosine is at least the encoders' bar of 0.9999
+            assert (np.linalg.norm(q.cpu().numpy() - want, axis=1) <= (2e-4) ** 0.5).all()
+            h.copy_(x)
+            p.zero_()
+            torch.cuda.synchronize()
+            gr.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(p.cpu().numpy(), want)
+        del gr
+    finally:
+        m.close()
