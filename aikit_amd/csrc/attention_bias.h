@@ -29,7 +29,16 @@
 
 namespace enchip {
 
-constexpr float AB_LAZY = 8.0f;
+// Weights are 2^(score - u) with a u below the running maximum, so that those far below it keep bits in f16's range: up
+// to 2^AB_ABOVE when u is set, 2^15 at most (f16 ends at 65504), and off by 2^-25, f16's last place. A weight is held
+// within 2^-22 of itself and 2^-36 (with AB_ABOVE) of the row's largest. u cancels in the division.
+constexpr float AB_LAZY = 4.0f, AB_ABOVE = 15.0f - AB_LAZY;
+
+// The u of a maximum m. Where m is so large that m - above is rounded to 16 below it, m itself.
+__device__ __forceinline__ float ab_under(float m, float above) {
+    const float u = m - above;
+    return m - u > 15.5f ? m : u;
+}
 
 struct AttnBias {
     const float *q, *k, *v;
@@ -392,12 +401,12 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
                         const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
                         mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
                     }
-                    // The subtracted maximum follows a query's running maximum only when that is AB_LAZY above it:
-                    // weights up to 2^AB_LAZY keep their precision, and after the first tiles nothing is rescaled.
-                    const bool up = mloc > m_run[u] + AB_LAZY;
+                    // What is subtracted follows a query's running maximum only when that is AB_LAZY past where it was
+                    // set: after the first tiles nothing is rescaled. (The difference of two numbers so near is exact.)
+                    const bool up = mloc - m_run[u] > AB_ABOVE + AB_LAZY;
                     if (__builtin_amdgcn_ballot_w64(up) != 0) {
-                        const float alpha = up ? __builtin_amdgcn_exp2f(m_run[u] - mloc) : 1.0f;
-                        m_run[u] = up ? mloc : m_run[u];
+                        const float next = ab_under(mloc, AB_ABOVE), alpha = up ? __builtin_amdgcn_exp2f(m_run[u] - next) : 1.0f;
+                        m_run[u] = up ? next : m_run[u];
                         l_run[u] *= alpha;
 #pragma unroll
                         for (int i = 0; i < NOT; ++i)
@@ -594,7 +603,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_bias_split(AttnBias p) {
 #pragma unroll
         for (int e = 1; e < 16; ++e) m = fmaxf(m, acc[e]);
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        m = fmaxf(m, m_run);
+        m = fmaxf(ab_under(m, 15.0f), m_run);  // followed at once: within 2^-40 of the row's largest weight
         const float m_use = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(m_run - m_use);
         m_run = m;
         l_run *= alpha;

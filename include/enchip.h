@@ -660,8 +660,10 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos relpos);
  * it was. (Spans are cut off at 0 and L. Where they are out of order, rows may stay as they were.)
  * A query all of whose biases are -infinity gets zeros. Products as in ENCHIP_ATT_FLASH_F16, whatever
  * enchip_set_attention_products says: scale q log2 e, k and v in two f16 parts each (within 2^-22, and 2^-25 below
- * 2^-3), below 65520 in magnitude (larger, infinite and NaN ones give NaN in the rows that see them); scores, weights
- * and sums in f32, in an order that goes by the sizes (by L / nseq with d_spans). head_dim 32, 64 or 128; pitches of
+ * 2^-3), below 65520 in magnitude (larger, infinite and NaN ones give NaN in the rows of their sequence that see them,
+ * as they do in keys and values of weight 0); scores and sums in f32, in an order that goes by the sizes (by L / nseq with
+ * d_spans); weights in two f16 parts too, within 2^-22 of themselves and 2^-36 of the row's largest (2^-25 where scores
+ * pass 10^7). head_dim 32, 64 or 128; pitches of
  * q, k, v multiples of 4 below 2^25, q, k, v 16-byte aligned, d_spans 8-byte; d_out holds no element of q, k or v;
  * L <= 2^30, nseq L <= 2^31, nseq <= 2^22 with d_spans. Few queries of many keys are split over workgroups, and
  * many spans taken longest first, through the context's shared scratch. */

@@ -1,0 +1,82 @@
+"""Weights and sums of attention with a relative position bias where a bound by the largest value says little: one key far
+above many others that hold all that comes out, and long rows of equal weights.
+
+Per output, with e a key's weight relative to the row's largest, the kernel's sums S' of weights and N' of weights times
+values are off from the exact S and N by
+  2 delta + 2^-21 of each weight, delta the score's error: (hd 2^-24 + 3 2^-22) sum |q k| scale + 2^-22 |y| as the products
+      have it and the operands' floor hd 2^-24 scale (max|q| + max|k|), doubled for 2^x,
+  2^-36 a key that its two f16 parts lose below the largest, which N' alone sees, and 3 2^-22 of the second product,
+  one rounding of 2^-24 for each addition."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+# how the sizes choose the kernel: 8 wavefronts to 32 queries, one, tiles whole, tiles in parts, tiles in order of length
+FORMS = {
+    "8 wavefronts": dict(heads=1, before=299, after=0),
+    "1 wavefront": dict(heads=4, before=150, after=149),
+    "parts": dict(heads=2, before=0, after=0),
+    "whole": dict(heads=32, before=0, after=0),
+    "ordered": dict(heads=32, before=1, after=2),
+}
+
+
+def say(msg):
+    print(f"[case] {msg}", flush=True)
+
+
+def run(ctx, x, heads, hd, scale, before, after, n):
+    """n rows among spans of no rows, every head the same columns of x [n, 3 hd]."""
+    import torch
+
+    W = heads * hd
+    q, k, v = (np.tile(x[:, i * hd:(i + 1) * hd], (1, heads)) for i in range(3))
+    d = torch.from_numpy(np.concatenate([q, k, v], axis=1)).cuda()
+    out = torch.full((n, W), 3.0, device="cuda")
+    spans = [(0, 0)] * before + [(0, n)] + [(n, n)] * after
+    sp = torch.tensor(spans, dtype=torch.int32, device="cuda") if before + after else None
+    p = d.data_ptr()
+    torch.cuda.synchronize()
+    ctx.attention_bias_dev(None, p, 3 * W, p + 4 * W, 3 * W, p + 8 * W, 3 * W, out.data_ptr(), W, len(spans), n, heads, heads, hd, scale,
+                           0 if sp is None else sp.data_ptr())
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(n, heads, hd)
+    assert (got == got[:, :1]).all()  # no head differs from another
+    return got[:, 0]
+
+
+def exact(x, hd, scale, rows):
+    q, k, v = (x[:, i * hd:(i + 1) * hd].astype(np.float64) for i in range(3))
+    y = scale * (q[rows] @ k.T)
+    e = np.exp(y - y.max(axis=1, keepdims=True))
+    mass = abs(scale) * (np.abs(q[rows]) @ np.abs(k).T)
+    delta = (hd * 2.0 ** -24 + 3 * 2.0 ** -22) * mass + 2.0 ** -22 * np.abs(y) + \
+        abs(scale) * hd * 2.0 ** -24 * (np.abs(q[rows]).max() + np.abs(k).max())
+    return e, v, (2 * delta + 2.0 ** -21).max(axis=1, keepdims=True)
+
+
+@pytest.mark.parametrize("gap", [17.0, 18.5, 20.0])
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_keys_far_below_the_largest(ctx, hd, form, gap):
+    n, scale, sink = 8192 + 37, hd ** -0.5, 4000
+    say(f"attention_bias one key {gap} above {n - 1} others, hd={hd}, {form}")
+    g = np.random.default_rng(hd)
+    x = np.zeros((n, 3 * hd), np.float32)
+    x[:, 0] = 8.0
+    x[:, 1:hd] = g.standard_normal((n, hd - 1)) * 0.05
+    x[:, hd] = -gap / (8.0 * scale)
+    x[sink, hd] = 0.0
+    x[:, hd + 1:2 * hd] = g.standard_normal((n, hd - 1)) * 0.05
+    x[:, 2 * hd:] = 1.0 + 0.1 * g.standard_normal((n, hd))
+    x[sink, 2 * hd:] = 0.0
+    got = run(ctx, x, hd=hd, scale=scale, n=n, **FORMS[form])
+    rows = np.concatenate([np.arange(0, n, 211), [sink, n - 1]])
+    e, v, rel = exact(x, hd, scale, rows)
+    S, N, A = e.sum(axis=1, keepdims=True), e @ v, e @ np.abs(v)
+    adds = (n / 8 + 64) * 2.0 ** -24  # of 16 keys each at least, in two parts each
+    tol = ((2 * rel + 3 * 2.0 ** -22 + 2 * adds) * A + n * 2.0 ** -36 * np.abs(v).max()) / S
+    assert (tol < 0.02 * N / S).all()  # far from what all of them weigh
+    bad = ~(np.abs(got[rows] - N / S) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:3], got[rows][bad][:3], (N / S)[bad][:3], tol[bad][:3])
