@@ -40,6 +40,22 @@ __device__ __forceinline__ float ab_under(float m, float above) {
     return m - u > 15.5f ? m : u;
 }
 
+// Sums of long rows: the 16 weights of a lane's 32-key block are added in pairs, and what AB_FOLD keys gave is set aside
+// (in the outputs' place, or LDS) and a new sum begun, so that roundings grow with AB_FOLD and not with the row. One sum
+// over 131077 equal weights came out 8 10^-4 off, now 6 10^-6. 32768 rows of 12 heads of 64 8.86 ms, 8.77 in one sum; 8192 as before.
+constexpr int AB_FOLD = 4096;
+
+__device__ __forceinline__ float ab_sum16(const float (&x)[16]) {
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = x[e] + x[e + 8];
+#pragma unroll
+    for (int n = 4; n > 0; n /= 2)
+#pragma unroll
+        for (int e = 0; e < n; ++e) s[e] += s[e + n];
+    return s[0];
+}
+
 struct AttnBias {
     const float *q, *k, *v;
     float *out;
@@ -91,7 +107,8 @@ struct AbLayout {
     using Fa = FaLayout<HD>;
     static constexpr int WINDOW = 32 * NW * QPW + NW * FA_KT;  // most words of a tile's windows
     static constexpr int BIAS = 2 * Fa::STAGE;      // two windows behind the two stages
-    static constexpr int BYTES = BIAS + 2 * WINDOW * 4;
+    static constexpr int STAT = BIAS + 2 * WINDOW * 4;  // a float2 a query, of what is set aside
+    static constexpr int BYTES = STAT + 32 * NW * QPW * 8;
 };
 
 // The last of n things whose first(i), ascending, is at or below b, found 64 at a time by a wavefront; -1: none.
@@ -227,7 +244,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
     using vec8 = typename Ops::vec8;
     extern __shared__ __attribute__((aligned(16))) char ab_lds[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, hf = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
     const int qs = __builtin_ctz(QB) - p.share, QR = 1 << qs;
     int set, part, L, q0;
     int64_t row0;
@@ -360,114 +377,142 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
         }
     store_tile(tbeg & 1);
     lds_barrier();
-    for (int t = tbeg; t < nt; ++t) {
-        if (t + 1 < nt) load_tile(t + 1);
-        if (active) {
-            const char *khi = ab_lds + (t & 1) * Fa::STAGE, *klo = khi + Fa::KPLANE;
-            const char *vhi = klo + Fa::KPLANE, *vlo = vhi + Fa::VPLANE;
-            const float *window = reinterpret_cast<const float *>(ab_lds + Lay::BIAS) + (t & 1) * Lay::WINDOW + mate * pitch;
+    constexpr int FOLD = AB_FOLD / FA_KT;
+    for (int t0 = tbeg;; t0 += FOLD) {
+        for (int t = t0; t < min(nt, t0 + FOLD); ++t) {
+            if (t + 1 < nt) load_tile(t + 1);
+            if (active) {
+                const char *khi = ab_lds + (t & 1) * Fa::STAGE, *klo = khi + Fa::KPLANE;
+                const char *vhi = klo + Fa::KPLANE, *vlo = vhi + Fa::VPLANE;
+                const float *window = reinterpret_cast<const float *>(ab_lds + Lay::BIAS) + (t & 1) * Lay::WINDOW + mate * pitch;
 #pragma unroll
-            for (int s = 0; s < FA_KT / 32; ++s) {
-                const int key0 = t * FA_KT + 32 * s;
-                if (key0 >= L) break;  // uniform: no barrier inside
-                // the scores' sums start at the bias; element e is key key0 + 4 hf + 8 (e / 4) + e % 4
-                f32x16 acc[QPW];
+                for (int s = 0; s < FA_KT / 32; ++s) {
+                    const int key0 = t * FA_KT + 32 * s;
+                    if (key0 >= L) break;  // uniform: no barrier inside
+                    // the scores' sums start at the bias; element e is key key0 + 4 hf + 8 (e / 4) + e % 4
+                    f32x16 acc[QPW];
 #pragma unroll
-                for (int u = 0; u < QPW; ++u) {
-                    const float *bw = window + (32 * s + 4 * hf - (qr + 32 * u + r) + QR - 1);
+                    for (int u = 0; u < QPW; ++u) {
+                        const float *bw = window + (32 * s + 4 * hf - (qr + 32 * u + r) + QR - 1);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[u][e] = bw[8 * (e >> 2) + (e & 3)];
+                        for (int e = 0; e < 16; ++e) acc[u][e] = bw[8 * (e >> 2) + (e & 3)];
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int off = (32 * s + r) * Fa::KP + 2 * (16 * b + 8 * hf);
+                        const vec8 kh = *reinterpret_cast<const vec8 *>(khi + off);
+                        const vec8 kl = *reinterpret_cast<const vec8 *>(klo + off);
+                        ab_mfma3<QPW>(kh, kl, [&](int u) { return qh[u][b]; }, [&](int u) { return ql[u][b]; }, acc);
+                    }
+                    vec8 ph[QPW][2], pl[QPW][2];
+#pragma unroll
+                    for (int u = 0; u < QPW; ++u) {
+                        const int lim = L - key0 - 4 * hf;
+                        if (__builtin_expect(key0 + 32 > L, 0)) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (8 * (e >> 2) + (e & 3) >= lim) acc[u][e] = -INFINITY;
+                        }
+                        float mloc = acc[u][0];
+#pragma unroll
+                        for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, acc[u][e]);
+                        {
+                            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
+                            mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+                        }
+                        // What is subtracted follows a query's running maximum only when that is AB_LAZY past where it was
+                        // set: after the first tiles nothing is rescaled. (The difference of two numbers so near is exact.)
+                        const bool up = mloc - m_run[u] > AB_ABOVE + AB_LAZY;
+                        if (__builtin_amdgcn_ballot_w64(up) != 0) {
+                            const float next = ab_under(mloc, AB_ABOVE), alpha = up ? __builtin_amdgcn_exp2f(m_run[u] - next) : 1.0f;
+                            m_run[u] = up ? next : m_run[u];
+                            l_run[u] *= alpha;
+#pragma unroll
+                            for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[u][i][e] *= alpha;
+                        }
+                        const float m_use = m_run[u] == -INFINITY ? 0.0f : m_run[u];  // nothing attended so far: every weight is 0
+                        float x[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(acc[u][e] - m_use);
+                        l_run[u] += ab_sum16(x);
+                        ab_split8(x, ph[u][0], pl[u][0]);
+                        ab_split8(x + 8, ph[u][1], pl[u][1]);
+                    }
+                    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                        for (int i = 0; i < NOT; ++i) {
+                            const int off = (32 * i + r) * Fa::VP + 64 * s + 32 * (kb ^ (i & 1)) + 16 * (hf ^ (r >> 4));
+                            const vec8 vh = *reinterpret_cast<const vec8 *>(vhi + off);
+                            const vec8 vl = *reinterpret_cast<const vec8 *>(vlo + off);
+                            f32x16 d[QPW];
+#pragma unroll
+                            for (int u = 0; u < QPW; ++u) d[u] = o[u][i];
+                            ab_mfma3<QPW>(vh, vl, [&](int u) { return ph[u][kb]; }, [&](int u) { return pl[u][kb]; }, d);
+#pragma unroll
+                            for (int u = 0; u < QPW; ++u) o[u][i] = d[u];
+                        }
+                    }
+                    __builtin_amdgcn_s_setprio(0);
                 }
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const int off = (32 * s + r) * Fa::KP + 2 * (16 * b + 8 * hf);
-                    const vec8 kh = *reinterpret_cast<const vec8 *>(khi + off);
-                    const vec8 kl = *reinterpret_cast<const vec8 *>(klo + off);
-                    ab_mfma3<QPW>(kh, kl, [&](int u) { return qh[u][b]; }, [&](int u) { return ql[u][b]; }, acc);
-                }
-                vec8 ph[QPW][2], pl[QPW][2];
-#pragma unroll
-                for (int u = 0; u < QPW; ++u) {
-                    const int lim = L - key0 - 4 * hf;
-                    if (__builtin_expect(key0 + 32 > L, 0)) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (8 * (e >> 2) + (e & 3) >= lim) acc[u][e] = -INFINITY;
-                    }
-                    float mloc = acc[u][0];
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) mloc = fmaxf(mloc, acc[u][e]);
-                    {
-                        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
-                        mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-                    }
-                    // What is subtracted follows a query's running maximum only when that is AB_LAZY past where it was
-                    // set: after the first tiles nothing is rescaled. (The difference of two numbers so near is exact.)
-                    const bool up = mloc - m_run[u] > AB_ABOVE + AB_LAZY;
-                    if (__builtin_amdgcn_ballot_w64(up) != 0) {
-                        const float next = ab_under(mloc, AB_ABOVE), alpha = up ? __builtin_amdgcn_exp2f(m_run[u] - next) : 1.0f;
-                        m_run[u] = up ? next : m_run[u];
-                        l_run[u] *= alpha;
-#pragma unroll
-                        for (int i = 0; i < NOT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[u][i][e] *= alpha;
-                    }
-                    const float m_use = m_run[u] == -INFINITY ? 0.0f : m_run[u];  // nothing attended so far: every weight is 0
-                    float x[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        x[e] = __builtin_amdgcn_exp2f(acc[u][e] - m_use);
-                        l_run[u] += x[e];
-                    }
-                    ab_split8(x, ph[u][0], pl[u][0]);
-                    ab_split8(x + 8, ph[u][1], pl[u][1]);
-                }
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                    for (int i = 0; i < NOT; ++i) {
-                        const int off = (32 * i + r) * Fa::VP + 64 * s + 32 * (kb ^ (i & 1)) + 16 * (hf ^ (r >> 4));
-                        const vec8 vh = *reinterpret_cast<const vec8 *>(vhi + off);
-                        const vec8 vl = *reinterpret_cast<const vec8 *>(vlo + off);
-                        f32x16 d[QPW];
-#pragma unroll
-                        for (int u = 0; u < QPW; ++u) d[u] = o[u][i];
-                        ab_mfma3<QPW>(vh, vl, [&](int u) { return ph[u][kb]; }, [&](int u) { return pl[u][kb]; }, d);
-#pragma unroll
-                        for (int u = 0; u < QPW; ++u) o[u][i] = d[u];
-                    }
-                }
-                __builtin_amdgcn_s_setprio(0);
             }
+            if (t + 1 < nt) store_tile((t + 1) & 1);
+            lds_barrier();
         }
-        if (t + 1 < nt) store_tile((t + 1) & 1);
-        lds_barrier();
-    }
-
-    if (!active) return;
-#pragma unroll
-    for (int u = 0; u < QPW; ++u) {
-        const float l_tot = l_run[u] + __shfl_xor(l_run[u], 32, 64);
-        float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-        const int query = qw + 32 * u + r;
-        if (query >= L) continue;
-        float *orow = p.out + (row0 + query) * p.ldo + head * HD;
-        if (p.parts > 1) {
-            const int64_t at = (part * p.rows + row0 + query) * p.heads + head;
-            orow = p.part + at * HD;
-            inv = 1.0f;
-            if (hf == 0) *reinterpret_cast<float2 *>(p.stat + 2 * at) = make_float2(m_run[u], l_tot);
+        if (!active) {
+            if (t0 + FOLD >= nt) return;
+            continue;
         }
+        const bool begun = t0 > tbeg, last = t0 + FOLD >= nt;
+        int rr = r;
+        asm volatile("" : "+v"(rr));  // the outputs' addresses are formed here, not held (and spilled) all along
+        // the chunk's sums on top of what is set aside, which is in the outputs' place; divided after the last
 #pragma unroll
-        for (int i = 0; i < NOT; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x16 &a = o[u][i];
-                ab_store<VEC>(orow + 32 * i + 8 * g + 4 * hf,
-                              f32x4{a[4 * g] * inv, a[4 * g + 1] * inv, a[4 * g + 2] * inv, a[4 * g + 3] * inv});
+        for (int u = 0; u < QPW; ++u) {
+            const int query = qw + 32 * u + rr;
+            float l_tot = l_run[u] + __shfl_xor(l_run[u], 32, 64), was = 0.0f;
+            float2 *stat = reinterpret_cast<float2 *>(ab_lds + Lay::STAT) + (wave * QPW + u) * 32 + rr;
+            if (begun) {
+                was = __builtin_amdgcn_exp2f(stat->x - (m_run[u] == -INFINITY ? 0.0f : m_run[u]));
+                l_tot += stat->y * was;
             }
+            if (!last) *stat = make_float2(m_run[u], l_tot);  // by both halves of the lanes, the same
+            if (query >= L) continue;
+            float *orow = p.out + (row0 + query) * p.ldo + head * HD;
+            float by = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+            if (p.parts > 1) {
+                const int64_t at = (part * p.rows + row0 + query) * p.heads + head;
+                orow = p.part + at * HD;
+                if (last && hf == 0) *reinterpret_cast<float2 *>(p.stat + 2 * at) = make_float2(m_run[u], l_tot);
+            }
+            if (!last || p.parts > 1) by = 1.0f;
+            if (begun) {
+#pragma unroll
+                for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[u][i][e] += orow[32 * i + 8 * (e >> 2) + 4 * hf + (e & 3)] * was;
+            }
+#pragma unroll
+            for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16 &a = o[u][i];
+                    ab_store<VEC>(orow + 32 * i + 8 * g + 4 * hf,
+                                  f32x4{a[4 * g] * by, a[4 * g + 1] * by, a[4 * g + 2] * by, a[4 * g + 3] * by});
+                }
+        }
+        if (last) return;
+#pragma unroll
+        for (int u = 0; u < QPW; ++u) {
+            l_run[u] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[u][i][e] = 0.0f;
+        }
     }
 }
 
@@ -559,85 +604,103 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_bias_split(AttnBias p) {
         }
     };
     if (!AHEAD) split_q();  // behind the first loads it would spill (551 documents of 1 to 200: 156 us for 126)
-    for (int key0 = 32 * wave, first = 1; key0 < L; key0 += 32 * NW, first = 0) {
-        const float *kt = kbase + (int64_t)key0 * ldk, *vt = vbase + (int64_t)key0 * ldv;
-        const int last = L - 1 - key0;
-        constexpr int KN = AHEAD ? NB : NB / 2, VN = AHEAD ? 2 : 1;
-        float kx[KN][8], vx[NOT][VN][8];
-        f32x16 acc;
-        auto load_k = [&](int b0) {
+    int key0 = 32 * wave;
+    for (bool begun = false;; begun = true) {
+        const int stop = min(L, key0 + AB_FOLD * NW);
+        for (; key0 < stop; key0 += 32 * NW) {
+            const float *kt = kbase + (int64_t)key0 * ldk, *vt = vbase + (int64_t)key0 * ldv;
+            const int last = L - 1 - key0;
+            constexpr int KN = AHEAD ? NB : NB / 2, VN = AHEAD ? 2 : 1;
+            float kx[KN][8], vx[NOT][VN][8];
+            f32x16 acc;
+            auto load_k = [&](int b0) {
 #pragma unroll
-            for (int b = 0; b < KN; ++b) load8(kt + (min(r, last) * ldk + 16 * (b0 + b) + 8 * hf), kx[b]);
-        };
-        load_k(0);
+                for (int b = 0; b < KN; ++b) load8(kt + (min(r, last) * ldk + 16 * (b0 + b) + 8 * hf), kx[b]);
+            };
+            load_k(0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int d = key0 + 4 * hf + 8 * (e >> 2) + (e & 3) - (q0 + r);
-            acc[e] = table != nullptr ? table[min(max(d, -p.reach), p.reach)] : 0.0f;
-        }
-        // value column 32 i + r: the eight keys at depth 8 hf .. of 16-key block kb
-        auto load_v = [&](int kb) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float *row = vt + (min(16 * kb + 4 * hf + (j & 3) + 2 * (j & 4), last) * ldv + r);
-#pragma unroll
-                for (int i = 0; i < NOT; ++i) vx[i][kb % VN][j] = row[32 * i];
+            for (int e = 0; e < 16; ++e) {
+                const int d = key0 + 4 * hf + 8 * (e >> 2) + (e & 3) - (q0 + r);
+                acc[e] = table != nullptr ? table[min(max(d, -p.reach), p.reach)] : 0.0f;
             }
-        };
-        if (AHEAD) load_v(0), load_v(1);
-        if (AHEAD && first) split_q();
+            // value column 32 i + r: the eight keys at depth 8 hf .. of 16-key block kb
+            auto load_v = [&](int kb) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (b > 0 && b % KN == 0) load_k(b);
-            f16x8 kh, kl;
-            ab_split8(kx[b % KN], kh, kl);
-            acc = mfma_split3(kh, kl, qh[b], ql[b], acc);
+                for (int j = 0; j < 8; ++j) {
+                    const float *row = vt + (min(16 * kb + 4 * hf + (j & 3) + 2 * (j & 4), last) * ldv + r);
+#pragma unroll
+                    for (int i = 0; i < NOT; ++i) vx[i][kb % VN][j] = row[32 * i];
+                }
+            };
+            if (AHEAD) load_v(0), load_v(1);
+            if (AHEAD && key0 == 32 * wave) split_q();
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (b > 0 && b % KN == 0) load_k(b);
+                f16x8 kh, kl;
+                ab_split8(kx[b % KN], kh, kl);
+                acc = mfma_split3(kh, kl, qh[b], ql[b], acc);
+            }
+            if (!AHEAD) load_v(0);
+            if (key0 + 32 > L) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (8 * (e >> 2) + (e & 3) >= L - key0 - 4 * hf) acc[e] = -INFINITY;
+            }
+            float m = acc[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) m = fmaxf(m, acc[e]);
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            m = fmaxf(ab_under(m, 15.0f), m_run);  // followed at once: within 2^-40 of the row's largest weight
+            const float m_use = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+            m_run = m;
+            l_run *= alpha;
+#pragma unroll
+            for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(acc[e] - m_use);
+            l_run += ab_sum16(x);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                f16x8 ph, pl;
+                ab_split8(x + 8 * kb, ph, pl);
+                if (!AHEAD && kb > 0) load_v(kb);
+#pragma unroll
+                for (int i = 0; i < NOT; ++i) {
+                    f16x8 vh, vl;
+                    ab_split8(vx[i][kb % VN], vh, vl);
+                    o[i] = mfma_split3(vh, vl, ph, pl, o[i]);
+                }
+            }
         }
-        if (!AHEAD) load_v(0);
-        if (key0 + 32 > L) {
+        l_run += __shfl_xor(l_run, 32, 64);
+        // on top of what is set aside in LDS
+        if (begun) {
+            const float was = __builtin_amdgcn_exp2f(top[wave * 32 + r] - (m_run == -INFINITY ? 0.0f : m_run));
+            l_run += sum[wave * 32 + r] * was;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (8 * (e >> 2) + (e & 3) >= L - key0 - 4 * hf) acc[e] = -INFINITY;
+            for (int i = 0; i < NOT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    o[i][e] += ctx[(wave * 32 + r) * Lay::PITCH + 32 * i + 8 * (e >> 2) + 4 * hf + (e & 3)] * was;
         }
-        float m = acc[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) m = fmaxf(m, acc[e]);
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        m = fmaxf(ab_under(m, 15.0f), m_run);  // followed at once: within 2^-40 of the row's largest weight
-        const float m_use = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-        m_run = m;
-        l_run *= alpha;
+        top[wave * 32 + r] = m_run, sum[wave * 32 + r] = l_run;  // by both halves of the lanes, the same
 #pragma unroll
         for (int i = 0; i < NOT; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
-        float x[16];
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4 *>(ctx + (wave * 32 + r) * Lay::PITCH + 32 * i + 8 * g + 4 * hf) =
+                    f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+        if (key0 >= L) break;
+        l_run = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            x[e] = __builtin_amdgcn_exp2f(acc[e] - m_use);
-            l_run += x[e];
-        }
+        for (int i = 0; i < NOT; ++i)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            f16x8 ph, pl;
-            ab_split8(x + 8 * kb, ph, pl);
-            if (!AHEAD && kb > 0) load_v(kb);
-#pragma unroll
-            for (int i = 0; i < NOT; ++i) {
-                f16x8 vh, vl;
-                ab_split8(vx[i][kb % VN], vh, vl);
-                o[i] = mfma_split3(vh, vl, ph, pl, o[i]);
-            }
-        }
+            for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
     }
-    l_run += __shfl_xor(l_run, 32, 64);
-    if (hf == 0) top[wave * 32 + r] = m_run, sum[wave * 32 + r] = l_run;
-#pragma unroll
-    for (int i = 0; i < NOT; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<f32x4 *>(ctx + (wave * 32 + r) * Lay::PITCH + 32 * i + 8 * g + 4 * hf) =
-                f32x4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
     __syncthreads();
     const int parts = min(NW, (L + 31) / 32);  // wavefronts that had keys
     for (int at = tid; at < 32 * HD / 4; at += 64 * NW) {

@@ -661,7 +661,7 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos relpos);
  * A query all of whose biases are -infinity gets zeros. Products as in ENCHIP_ATT_FLASH_F16, whatever
  * enchip_set_attention_products says: scale q log2 e, k and v in two f16 parts each (within 2^-22, and 2^-25 below
  * 2^-3), below 65520 in magnitude (larger, infinite and NaN ones give NaN in the rows of their sequence that see them,
- * as they do in keys and values of weight 0); scores and sums in f32, in an order that goes by the sizes (by L / nseq with
+ * as they do in keys and values of weight 0); scores and sums in f32, 4096 keys at a time, in an order that goes by the sizes (by L / nseq with
  * d_spans); weights in two f16 parts too, within 2^-22 of themselves and 2^-36 of the row's largest (2^-25 where scores
  * pass 10^7). head_dim 32, 64 or 128; pitches of
  * q, k, v multiples of 4 below 2^25, q, k, v 16-byte aligned, d_spans 8-byte; d_out holds no element of q, k or v;

@@ -31,8 +31,8 @@ def run(ctx, x, heads, hd, scale, before, after, n):
     import torch
 
     W = heads * hd
-    q, k, v = (np.tile(x[:, i * hd:(i + 1) * hd], (1, heads)) for i in range(3))
-    d = torch.from_numpy(np.concatenate([q, k, v], axis=1)).cuda()
+    one = torch.from_numpy(x).cuda()
+    d = torch.cat([one[:, i * hd:(i + 1) * hd].repeat(1, heads) for i in range(3)], dim=1).contiguous()
     out = torch.full((n, W), 3.0, device="cuda")
     spans = [(0, 0)] * before + [(0, n)] + [(n, n)] * after
     sp = torch.tensor(spans, dtype=torch.int32, device="cuda") if before + after else None
@@ -41,9 +41,9 @@ def run(ctx, x, heads, hd, scale, before, after, n):
     ctx.attention_bias_dev(None, p, 3 * W, p + 4 * W, 3 * W, p + 8 * W, 3 * W, out.data_ptr(), W, len(spans), n, heads, heads, hd, scale,
                            0 if sp is None else sp.data_ptr())
     torch.cuda.synchronize()
-    got = out.cpu().numpy().reshape(n, heads, hd)
+    got = out.reshape(n, heads, hd)
     assert (got == got[:, :1]).all()  # no head differs from another
-    return got[:, 0]
+    return got[:, 0].cpu().numpy()
 
 
 def exact(x, hd, scale, rows):
@@ -80,3 +80,30 @@ def test_keys_far_below_the_largest(ctx, hd, form, gap):
     assert (tol < 0.02 * N / S).all()  # far from what all of them weigh
     bad = ~(np.abs(got[rows] - N / S) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:3], got[rows][bad][:3], (N / S)[bad][:3], tol[bad][:3])
+
+
+@pytest.mark.parametrize("weight", [0.7, 0.93])
+@pytest.mark.parametrize("n", [8192 + 37, 2 ** 17 + 5])
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_long_rows_of_equal_weights(ctx, hd, form, n, weight):
+    # every addition of equal numbers is rounded the same way: an error that grows with the row, if anything's does
+    f, scale = FORMS[form], hd ** -0.5
+    if n > 2 ** 17 and hd > 32 and f["heads"] > 4:
+        f = dict(f, heads=max(12, f["heads"] * 32 // hd))
+    say(f"attention_bias {n} keys of weight {weight}, hd={hd}, {form}")
+    x = np.zeros((n, 3 * hd), np.float32)
+    x[:, 0] = 8.0
+    x[0, hd] = -np.log(weight) / (8.0 * scale)
+    x[:, 2 * hd:] = 1.0
+    x[:, 2 * hd + 1] = np.arange(n) % 3
+    x[:, 2 * hd + 2] = np.arange(n) % 64 < 32
+    x[:, 2 * hd + 3] = np.linspace(0.5, 1.5, n)
+    got = run(ctx, x, hd=hd, scale=scale, n=n, **f)
+    e, v, rel = exact(x, hd, scale, np.arange(1))
+    want = e @ v / e.sum()
+    # roundings in a sum: six for each 32 of the keys that are summed before they are set aside, three for each of those sums
+    adds = (4096 / 32 * 6 + 64 + 3 * n / 4096) * 2.0 ** -24
+    tol = (2 * rel + 3 * 2.0 ** -22 + 2 * adds) * want
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:3], np.abs(got / want - 1).max(), (tol / want).max())
