@@ -17,8 +17,12 @@
 //     query's softmax state is the lane's own (plus one exchange between the two lane
 //     halves);
 //   * online softmax per query in base 2: with c = |scale| log2 e (Q negated when scale
-//     < 0), m' = max(m, c max s), p = 2^(fma(s, c, -m')), l' = l 2^(m - m') + sum p, and
-//     the context accumulator rescaled by the same factor;
+//     < 0), m' = max(m, c max s - above), p = 2^(fma(s, c, -m')), l' = l 2^(m - m') + sum p,
+//     and the context accumulator rescaled by the same factor. F16: above = 7, which cancels in
+//     the division, so that weights are at most 2^7 and their two parts, off by up to 2^-25, hold
+//     keys far below the largest (2^-32 of it): with one key 17 above 8191 others whose value is 0
+//     the outputs came out 45% small without it. A rounded m' moves it by less than another 2^8
+//     while scores stay below 2^28. bfloat16 parts have f32's range: above = 0;
 //   * O^T = V^T P^T on the same MFMA: P^T is the B operand straight from the score
 //     accumulator registers (its keys in the accumulator's order), V^T the A operand read
 //     from LDS, where V is stored transposed with each 16-key block permuted into that
@@ -211,6 +215,7 @@ __global__ __launch_bounds__(64 * NW) void attention_flash(
     for (int i = 0; i < NOT; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    constexpr float above = F16 ? 7.0f : 0.0f;
     float m_run = -INFINITY, l_run = 0.0f;
 
     load_tile(0);
@@ -269,7 +274,7 @@ __global__ __launch_bounds__(64 * NW) void attention_flash(
                     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
                     mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
                 }
-                const float m_new = fmaxf(m_run, mloc * c);      // c >= 0: max of c s = c max s
+                const float m_new = fmaxf(m_run, __builtin_fmaf(mloc, c, -above));  // c >= 0: max of c s = c max s
                 const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);  // 0 on the first tile
                 float x[16];
                 float psum = 0.0f;

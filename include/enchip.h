@@ -447,7 +447,8 @@ int enchip_attention_f32_dev(enchip_ctx *ctx, const float *d_q, const float *d_k
  *                         the maximum grows, divided by the sum at the end), both products
  *                         on the f16 MFMA over operands split into two IEEE half parts
  *                         (x.y ~ hi.hi' + hi.lo' + lo.hi', each product within ~3 * 2^-22
- *                         of exact, summed in f32), K and V staged through on-chip memory
+ *                         of exact, operands below 2^-3 and weights below 2^-10 of the row's
+ *                         largest within 2^-25 and 2^-32 of it, summed in f32), K and V staged through on-chip memory
  *                         once per 256 queries. Any L. Within the f32 MatmulBT gate on
  *                         inputs of standard deviation up to 4 (tested). Operands must be
  *                         below 65520 in magnitude: larger ones give NaN.

@@ -56,12 +56,8 @@ def exact(x, hd, scale, rows):
     return e, v, (2 * delta + 2.0 ** -21).max(axis=1, keepdims=True)
 
 
-@pytest.mark.parametrize("gap", [17.0, 18.5, 20.0])
-@pytest.mark.parametrize("form", sorted(FORMS))
-@pytest.mark.parametrize("hd", [32, 64, 128])
-def test_keys_far_below_the_largest(ctx, hd, form, gap):
-    n, scale, sink = 8192 + 37, hd ** -0.5, 4000
-    say(f"attention_bias one key {gap} above {n - 1} others, hd={hd}, {form}")
+def one_above(n, hd, scale, sink, gap):
+    """q, k and v of n rows: key `sink`, of value 0, has scores about `gap` above all others'."""
     g = np.random.default_rng(hd)
     x = np.zeros((n, 3 * hd), np.float32)
     x[:, 0] = 8.0
@@ -71,15 +67,28 @@ def test_keys_far_below_the_largest(ctx, hd, form, gap):
     x[:, hd + 1:2 * hd] = g.standard_normal((n, hd - 1)) * 0.05
     x[:, 2 * hd:] = 1.0 + 0.1 * g.standard_normal((n, hd))
     x[sink, 2 * hd:] = 0.0
-    got = run(ctx, x, hd=hd, scale=scale, n=n, **FORMS[form])
+    return x
+
+
+def held(got, x, n, hd, scale, sink, floor):
     rows = np.concatenate([np.arange(0, n, 211), [sink, n - 1]])
     e, v, rel = exact(x, hd, scale, rows)
     S, N, A = e.sum(axis=1, keepdims=True), e @ v, e @ np.abs(v)
     adds = (n / 8 + 64) * 2.0 ** -24  # of 16 keys each at least, in two parts each
-    tol = ((2 * rel + 3 * 2.0 ** -22 + 2 * adds) * A + n * 2.0 ** -36 * np.abs(v).max()) / S
+    tol = ((2 * rel + 3 * 2.0 ** -22 + 2 * adds) * A + n * floor * np.abs(v).max()) / S
     assert (tol < 0.02 * N / S).all()  # far from what all of them weigh
     bad = ~(np.abs(got[rows] - N / S) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:3], got[rows][bad][:3], (N / S)[bad][:3], tol[bad][:3])
+
+
+@pytest.mark.parametrize("gap", [17.0, 18.5, 20.0])
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_keys_far_below_the_largest(ctx, hd, form, gap):
+    n, scale, sink = 8192 + 37, hd ** -0.5, 4000
+    say(f"attention_bias one key {gap} above {n - 1} others, hd={hd}, {form}")
+    x = one_above(n, hd, scale, sink, gap)
+    held(run(ctx, x, hd=hd, scale=scale, n=n, **FORMS[form]), x, n, hd, scale, sink, 2.0 ** -36)
 
 
 @pytest.mark.parametrize("weight", [0.7, 0.93])
@@ -107,3 +116,27 @@ def test_long_rows_of_equal_weights(ctx, hd, form, n, weight):
     tol = (2 * rel + 3 * 2.0 ** -22 + 2 * adds) * want
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:3], np.abs(got / want - 1).max(), (tol / want).max())
+
+
+@pytest.mark.parametrize("gap", [16.0, 17.0])
+@pytest.mark.parametrize("heads", [1, 24])  # workgroups of 8 and of 16 wavefronts
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_the_fused_attention_without_a_bias(ctx, hd, heads, gap, sign):
+    import torch
+
+    n, scale, sink = 8192 + 37, hd ** -0.5, 4000
+    say(f"attention_f32 one key {gap} above {n - 1} others, hd={hd}, {heads} heads, scale {sign * scale}")
+    x = one_above(n, hd, scale, sink, gap)
+    one = torch.from_numpy(x).cuda()
+    one[:, :hd] *= sign
+    W = heads * hd
+    d = torch.cat([one[:, i * hd:(i + 1) * hd].repeat(1, heads) for i in range(3)], dim=1).contiguous()
+    out = torch.full((n, W), 3.0, device="cuda")
+    p = d.data_ptr()
+    torch.cuda.synchronize()
+    ctx.attention_f32_dev(p, p + 4 * W, p + 8 * W, 3 * W, out.data_ptr(), W, 1, n, heads, hd, sign * scale)
+    torch.cuda.synchronize()
+    got = out.reshape(n, heads, hd)
+    assert (got == got[:, :1]).all()
+    held(got[:, 0].cpu().numpy(), x, n, hd, scale, sink, 2.0 ** -32)
