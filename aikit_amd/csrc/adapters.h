@@ -12,6 +12,7 @@
 //   gemm_w8a8_pt_adapters, gemm_w8a8_adapters, gemv_w8a8_adapters: the second product in the epilogue of the W8A8
 //                 products, whose rows adapter_down quantizes from the registers that it multiplies
 // Rows of a block that have different adapters: each adapter among them in turn, from the lowest such row on.
+// What is added to a row without one is -0, the number that leaves every sum as it was: +0 makes a -0 of y's a +0.
 //
 // Bound by memory where rows are many: 32768 x 1024 to 1024, rank 16, rows of 8 adapters, take 97 us on MI355X, 41 in
 // adapter_down (134 MB of rows, 34 of codes: 4.1 TB/s) and 57 in the product (34 MB of codes, 134 of outputs;
@@ -62,14 +63,15 @@ struct Adapters {
     };
 
     // The sums of B_s t for the 32 rows of block mb (mine: the slot of row lane % 32) and the TN column blocks
-    // from n0 on, as the MFMA's accumulators have them. A row without a slot gets zeros.
+    // from n0 on, as the MFMA's accumulators have them. A row without a slot gets -0.
     template <int TN, class F16>
     __device__ __forceinline__ void tiles(int mine, int64_t mb, int64_t n0, int lane, F16 (&acc)[TN], Held<TN> &held) const {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[j][e] = 0.0f;
-        uint32_t todo = (uint32_t)__builtin_amdgcn_ballot_w64(mine >= 0);
+            for (int e = 0; e < 16; ++e) acc[j][e] = -0.0f;
+        const uint32_t some = (uint32_t)__builtin_amdgcn_ballot_w64(mine >= 0);
+        uint32_t todo = some;
         while (todo != 0) {  // uniform: the adapters among the rows, one after the other
             const int s = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
             todo &= ~(uint32_t)__builtin_amdgcn_ballot_w64(mine == s);
@@ -96,6 +98,14 @@ struct Adapters {
                 for (int j = 0; j < TN; ++j) acc[j] = d[0][j];
             }
         }
+        if (some != 0 && some != ~0u) {  // the others' zeros became +0 in the products
+            const uint32_t none = ~some >> acc_row(0, lane);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[j][e] = __uint_as_float(__float_as_uint(acc[j][e]) | ((none << (31 - acc_row(e, 0))) & 0x80000000u));
+        }
     }
 
     // One output's sum in a thread, for few rows: the first 16 ranks' operands are loaded ahead (dot_begin), the
@@ -119,7 +129,7 @@ struct Adapters {
     }
     __device__ __forceinline__ float dot_end(Dot &d, int row, int64_t M, int64_t n, int c) const {
         float sum = 0.0f;
-        if (d.s < 0) return sum;
+        if (d.s < 0) return -0.0f;
         for (int rs = 0; rs < rt; ++rs) {
             if (rs > 0) dot_load(d, row, n, c, rs);
 #pragma unroll
@@ -197,7 +207,7 @@ struct Adapters {
     }
     __device__ __forceinline__ float row_up(Row &d, int i, int64_t n, int c) const {
         float sum = 0.0f;
-        if (d.s < 0) return sum;
+        if (d.s < 0) return -0.0f;
         for (int rs = 0; rs < rt; ++rs) {
             if (rs > 0) b_load(d, n, c, rs);
 #pragma unroll

@@ -756,7 +756,7 @@ __device__ __forceinline__ void gemv_w8a8_body(
 #pragma unroll
         for (int w = 0; w < GV_WAVES; ++w) sum += red[(w * GV_ROWS + i) * 32 + c];
         const int row = rg * GV_ROWS + i, col = nb * 32 + c;
-        float d = 0.0f;
+        float d = -0.0f;
         if constexpr (AD::on) d = ad.dot_end(dot, row, M, nb, c);
         if (row < M && col < N) {
             if (EPI == EPI_I32) {
