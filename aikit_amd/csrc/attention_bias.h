@@ -64,6 +64,7 @@ struct AttnBias {
     const int4 *order;   // the spans longest first (attention_bias_order); null: as they come
     const float *table;  // [heads][2 reach + 1], b log2 e of distance -reach .. reach; null: no bias
     int nseq, heads, group, reach;
+    int block0;  // with spans, the first of the launch's query blocks
     int L;       // rows of a sequence, or with spans those of the buffers
     int share;   // log2 of the heads of one key head that a workgroup takes, beside each other
     int parts;   // workgroups that split a query's keys
@@ -127,7 +128,7 @@ __device__ __forceinline__ int ab_last(int n, int b, F first) {
 }
 
 // The workgroup's rows, QR = 2^qs queries from q0 on of the L from row0 on: false where it has none. Of ascending
-// spans, span z has the query blocks start / QR + z .. of the launch, at least as many as it needs. (Spans out of order
+// spans, span z has the query blocks start / QR + z .. of the call, at least as many as it needs. (Spans out of order
 // leave queries out; nothing is read past the buffers.)
 __device__ __forceinline__ bool ab_rows(const AttnBias &p, int b, int qs, int64_t &row0, int &len, int &q0) {
     if (p.spans == nullptr) {
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 || QPW == 2 ? 2 : 4) void attent
         const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_part = gridDim.x / ((p.heads >> p.share) * p.parts);
         const int sp = logical / per_part;
         set = sp / p.parts, part = sp - set * p.parts;
-        if (!ab_rows(p, logical - sp * per_part, qs, row0, L, q0)) return;
+        if (!ab_rows(p, logical - sp * per_part + p.block0, qs, row0, L, q0)) return;
     }
     // the wavefront's head and its first query
     const int mate = (wave * 32 * QPW) >> qs, head = (set << p.share) + mate, qr = (wave * 32 * QPW) & (QR - 1), qw = q0 + qr;
@@ -574,7 +575,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_bias_split(AttnBias p) {
     } else {
         const int logical = xcd_logical_tile(blockIdx.x, gridDim.x), per_head = gridDim.x / p.heads;
         head = logical / per_head;
-        if (!ab_rows(p, logical - head * per_head, 5, row0, L, q0)) return;
+        if (!ab_rows(p, logical - head * per_head + p.block0, 5, row0, L, q0)) return;
     }
     const float *kbase = p.k + row0 * p.ldk + (head / p.group) * HD;
     const float *vbase = p.v + row0 * p.ldv + (head / p.group) * HD;

@@ -215,8 +215,8 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos h) {
 
 namespace {
 
-// Launches fn over (query blocks of 2^qs rows) x (head sets), in chunks of sequences whose threads are numbered in 32
-// bits.
+// Launches fn over (query blocks of 2^qs rows) x (head sets), in chunks of sequences, or with spans of query blocks, whose
+// threads are numbered in 32 bits. p.order, and parts, are one launch (attention_plan).
 int launch_attention_bias(enchip_ctx *ctx, void (*fn)(enchip::AttnBias), int lds, int threads, int qs, enchip::AttnBias p, hipStream_t s) {
     const std::pair<const void *, size_t> key(reinterpret_cast<const void *>(fn), (size_t)lds);
     if (std::find(ctx->lds_set.begin(), ctx->lds_set.end(), key) == ctx->lds_set.end()) {
@@ -226,16 +226,27 @@ int launch_attention_bias(enchip_ctx *ctx, void (*fn)(enchip::AttnBias), int lds
     const int64_t qr = (int64_t)1 << qs, sets = (int64_t)(p.heads >> p.share) * p.parts;
     const int64_t per = p.spans ? p.L / qr + p.nseq : (p.L + qr - 1) / qr;
     const int64_t most = (((int64_t)1 << 32) - 1) / threads / sets;
+    if (p.order) {
+        hipLaunchKernelGGL(fn, dim3((unsigned)round_up(per * sets, 32)), dim3((unsigned)threads), (size_t)lds, s, p);
+        return check_launch(ctx, "attention_bias");
+    }
+    if (p.spans) {
+        for (int64_t b0 = 0; b0 < per; b0 += most) {
+            p.block0 = (int)b0;
+            hipLaunchKernelGGL(fn, dim3((unsigned)(std::min(most, per - b0) * sets)), dim3((unsigned)threads), (size_t)lds, s, p);
+        }
+        return check_launch(ctx, "attention_bias");
+    }
     if (per > most)
         return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: %lld query blocks of %d heads are more than one launch holds",
                     (long long)per, p.heads);
-    const int64_t chunk = p.spans ? p.nseq : most / per, nseq = p.nseq;
+    const int64_t chunk = most / per, nseq = p.nseq;
     for (int64_t z0 = 0; z0 < nseq; z0 += chunk) {
-        const int64_t nz = std::min(chunk, nseq - z0), row = z0 * p.L;  // z0 > 0 without spans only
+        const int64_t nz = std::min(chunk, nseq - z0), row = z0 * p.L;
         enchip::AttnBias c = p;
         c.q += row * p.ldq, c.k += row * p.ldk, c.v += row * p.ldv, c.out += row * p.ldo;
         c.nseq = (int)nz;
-        hipLaunchKernelGGL(fn, dim3((unsigned)(p.order ? round_up(per * sets, 32) : per * (p.spans ? 1 : nz) * sets)), dim3((unsigned)threads), (size_t)lds, s, c);
+        hipLaunchKernelGGL(fn, dim3((unsigned)(per * nz * sets)), dim3((unsigned)threads), (size_t)lds, s, c);
     }
     return check_launch(ctx, "attention_bias");
 }
@@ -404,6 +415,7 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
     p.L = (int)L;
     p.scale = scale;
     p.share = 0;
+    p.block0 = 0;
     p.parts = 1;
     p.part = p.stat = nullptr;
     p.order = nullptr;
