@@ -389,7 +389,7 @@ int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float
         return fail(ctx, ENCHIP_ERR_ARG, "attention_bias: head_dim must be 32, 64 or 128, got %lld", (long long)head_dim);
     const int64_t max_ld = INT32_MAX / enchip::FA_KT;
     if (nseq < 0 || L < 0 || L > ((int64_t)1 << 30) || heads < 0 || heads > 65535 || kv_heads < 0 || (heads > 0 && kv_heads < 1) ||
-        (kv_heads > 0 && heads % kv_heads != 0) || nseq > (d_spans ? (int64_t)1 << 22 : (int64_t)1 << 31) ||
+        (kv_heads > 0 && heads % kv_heads != 0) || nseq > (d_spans ? (int64_t)1 << 22 : (int64_t)INT32_MAX) ||
         (!d_spans && nseq * L > ((int64_t)1 << 31)) || ldq < heads * head_dim || ldo < heads * head_dim ||
         ldk < kv_heads * head_dim || ldv < kv_heads * head_dim || ldq % 4 || ldk % 4 || ldv % 4 || ldq > max_ld || ldk > max_ld ||
         ldv > max_ld)

@@ -658,7 +658,8 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos relpos);
  * rows of the buffers and d_spans[2 z], d_spans[2 z + 1] (device) are the first row of sequence z and the one
  * past its last, ascending: no span starts before the one ahead of it ends. Spans may be empty and leave gaps (a padded batch, or
  * documents of any lengths packed behind each other); rows of no span are not read and their output stays as
- * it was. (Spans are cut off at 0 and L. Where they are out of order, rows may stay as they were.)
+ * it was. (Spans are cut off at 0 and L. Where they are out of order, rows may stay as they were: a list of a fixed
+ * number of spans is filled up with L, L.)
  * A query all of whose biases are -infinity gets zeros. Products as in ENCHIP_ATT_FLASH_F16, whatever
  * enchip_set_attention_products says: scale q log2 e, k and v in two f16 parts each (within 2^-22, and 2^-25 below
  * 2^-3), below 65520 in magnitude (larger, infinite and NaN ones give NaN in the rows of their sequence that see them,
@@ -666,7 +667,7 @@ int enchip_relpos_release(enchip_ctx *ctx, enchip_relpos relpos);
  * d_spans); weights in two f16 parts too, within 2^-22 of themselves and 2^-36 of the row's largest (2^-25 where scores
  * pass 10^7). head_dim 32, 64 or 128; pitches of
  * q, k, v multiples of 4 below 2^25, q, k, v 16-byte aligned, d_spans 8-byte; d_out holds no element of q, k or v;
- * L <= 2^30, nseq L <= 2^31, nseq <= 2^22 with d_spans. Few queries of many keys are split over workgroups, and
+ * L <= 2^30, nseq L <= 2^31, nseq < 2^31, nseq <= 2^22 with d_spans. Few queries of many keys are split over workgroups, and
  * many spans taken longest first, through the context's shared scratch. */
 int enchip_attention_bias_dev(enchip_ctx *ctx, enchip_relpos relpos, const float *d_q, int64_t ldq,
                               const float *d_k, int64_t ldk, const float *d_v, int64_t ldv, float *d_out,

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from aikit_amd import enchip
 from block_oracle import attention
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +47,38 @@ def test_attention_in_ranges_of_query_blocks(ctx, hd, heads, kv, nseq):
     delta = (hd * 2.0 ** -24 + 4 * 2.0 ** -22) * mass
     assert np.abs(got - want).max() <= (2 * delta + (200 + 64) * 2.0 ** -24) * np.abs(v).max()
     assert np.linalg.norm(got - want) <= 2.0 ** -17 * np.linalg.norm(want)
+
+
+def test_a_number_of_sequences_past_32_bits_is_refused(ctx):
+    # nothing ran, and the call said it had
+    import torch
+
+    x = torch.zeros(4096, device="cuda")
+    p = x.data_ptr()
+    for nseq in (2 ** 31, 2 ** 31 + 5, 2 ** 40):
+        with pytest.raises(enchip.EnchipError) as err:
+            ctx.attention_bias_dev(None, p, 32, p, 32, p, 32, p + 8192, 32, nseq, 1, 1, 1, 32, 1.0)
+        assert err.value.code == enchip.ERR_ARG
+    torch.cuda.synchronize()
+    assert (x == 0).all()
+
+
+def test_a_list_of_spans_filled_up_with_the_end(ctx):
+    import torch
+
+    say("attention_bias spans filled up with L, L")
+    L, heads, hd = 300, 2, 64
+    x = torch.from_numpy(np.random.default_rng(3).standard_normal((L, 3 * heads * hd)).astype(np.float32)).cuda()
+    outs = []
+    for spans in ([(0, 100), (100, 101), (110, 290)], [(0, 100), (100, 101), (110, 290)] + [(L, L)] * 50):
+        out = torch.full((L, heads * hd), 3.0, device="cuda")
+        sp = torch.tensor(spans, dtype=torch.int32, device="cuda")
+        p, W = x.data_ptr(), heads * hd
+        torch.cuda.synchronize()
+        ctx.attention_bias_dev(None, p, 3 * W, p + 4 * W, 3 * W, p + 8 * W, 3 * W, out.data_ptr(), W, len(spans), L, heads, heads, hd, 0.125,
+                               sp.data_ptr())
+        torch.cuda.synchronize()
+        outs.append(out.cpu().numpy())
+    # the order of the sums goes by L / nseq
+    assert np.linalg.norm(outs[0] - outs[1]) <= 2.0 ** -16 * np.linalg.norm(outs[0])
+    assert (outs[1][101:110] == 3.0).all() and (outs[1][290:] == 3.0).all()
