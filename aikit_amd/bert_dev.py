@@ -379,6 +379,8 @@ class DeviceBert:
             nxt = self.handles[li + 1]["qkv"][0] if li + 1 < len(self.handles) else None
             pending = ln_then(g, s, ffn, nxt, "out_ln", beside(li + 1, "qkv") if nxt is not None else None)
 
+    POOL_SPANS = 65535  # the most that one call pools
+
     def embed(self, h, S: int, L: int, pooled, stream: int = 0, spans=None, pos=None, ids=None) -> None:
         """forward(), then mean pooling + L2 normalisation of each sequence into pooled [S, D], or of
         each span into pooled [n, D] (rows of pooled past those stay as they were)."""
@@ -386,9 +388,10 @@ class DeviceBert:
         self.forward(h, S, L, stream, spans, pos, ids)
         self._m("pool")
         if spans is not None:
-            if spans.shape[0]:
-                self.ctx.pool_mean_l2_spans_dev(h.data_ptr(), self.D, S * L, spans.data_ptr(), spans.shape[0], self.D,
-                                                pooled.data_ptr(), self.D, stream)
+            n = spans.shape[0]
+            for z in range(0, n, self.POOL_SPANS):
+                self.ctx.pool_mean_l2_spans_dev(h.data_ptr(), self.D, S * L, spans.data_ptr() + 8 * z, min(self.POOL_SPANS, n - z),
+                                                self.D, pooled.data_ptr() + 4 * self.D * z, self.D, stream)
             self._m("end")
             return
         self.ctx.pool_mean_l2_dev(h.data_ptr(), self.D, S, L, self.D, pooled.data_ptr(), self.D, stream)

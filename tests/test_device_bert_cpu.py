@@ -45,3 +45,21 @@ def test_forward_refuses_hidden_rows_that_are_not_f32_on_the_device():
     for bad in (Tensor(19, 64), Tensor(21, 64), Tensor(20, 64, dtype="f64"), Tensor(20, 64, device="cpu"), Tensor(20, 64, contiguous=False)):
         with pytest.raises(ValueError, match="h must"):
             m.forward(bad, 2, 10)
+
+
+@pytest.mark.parametrize("n", [0, 1, 65535, 65536, 200000])
+def test_any_number_of_spans_is_pooled(n):
+    m, calls = model(), []
+    m.forward, m.mark = (lambda *a, **k: None), None
+    m.ctx = SimpleNamespace(pool_mean_l2_spans_dev=lambda *a: calls.append(a))
+    at = {}
+    for name, t in (("h", Tensor(20, 64)), ("spans", Tensor(n, 2, dtype="i32")), ("pooled", Tensor(n, 64))):
+        at[name] = t
+        t.data_ptr = lambda base=len(at) << 40: base
+    m.embed(at["h"], 2, 10, at["pooled"], 7, spans=at["spans"])
+    done = 0
+    for h, ldh, rows, spans, k, D, out, ldo, stream in calls:
+        assert (h, ldh, rows, D, ldo, stream) == (1 << 40, 64, 20, 64, 64, 7) and 1 <= k <= 65535
+        assert spans == (2 << 40) + 8 * done and out == (3 << 40) + 4 * 64 * done
+        done += k
+    assert done == n

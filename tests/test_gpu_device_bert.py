@@ -142,3 +142,33 @@ def test_buffers_of_a_shape_stay_where_a_graph_has_them(ctx, L):
         del gr
     finally:
         m.close()
+
+
+def test_more_spans_than_one_call_pools(ctx, model):
+    import torch
+
+    n, L = 70000, 66000
+    say(f"embed {n} spans, most of them empty")
+    g = np.random.default_rng(12)
+    size = np.zeros(n, np.int64)
+    some = np.sort(g.choice(n, 600, replace=False))
+    some[-1] = n - 1
+    size[some] = g.integers(1, 100, 600)
+    end = np.cumsum(size)
+    assert end[-1] <= L
+    spans = np.stack([end - size, end], axis=1).astype(np.int32)
+    x = torch.from_numpy(g.standard_normal((L, D)).astype(np.float32)).cuda()
+    out = []
+    for keep in (np.arange(n), some):
+        h, p = x.clone(), torch.full((len(keep) + 1, D), 5.0, device="cuda")
+        sp = torch.from_numpy(spans[keep]).cuda()
+        torch.cuda.synchronize()
+        model.embed(h, 1, L, p, spans=sp)
+        torch.cuda.synchronize()
+        out.append(p.cpu().numpy())
+    many, few = out
+    empty = np.ones(n, bool)
+    empty[some] = False
+    assert (many[-1] == 5.0).all() and (many[:n][empty] == 0).all()
+    # the order of the attention's sums goes by L / n: codes on a rounding border, the encoders' bar of 0.9999
+    assert (np.linalg.norm(many[some] - few[:-1], axis=1) <= (2e-4) ** 0.5).all()
