@@ -48,7 +48,8 @@ the NomicBERT forward's order, with W8A8 linears as in the rest of this module).
 
 Layers with "q_norm" and "k_norm" have their query and key heads RMS-normed in qkv, turned in the same pass when
 `rope` is given (enchip_head_norm_rope_rows_dev). `relpos` (a learned bias by relative position), `kv_heads` fewer
-than `heads`, or sequences given as spans of rows take enchip_attention_bias_dev (heads of 32, 64 or 128); embed() then
+than `heads`, or sequences given as spans of rows take enchip_attention_bias_dev (heads of 32, 64 or 128; its products are
+ATT_FLASH_F16's, whatever Context.set_attention_products says); embed() then
 pools the spans (enchip_pool_mean_l2_spans_dev). Low-rank adapters of many requests stand beside any linear
 but a gated layer's gate and up projection (`adapters`; enchip_w8a8_linear_adapters_dev): each row's by its id.
 
@@ -262,7 +263,7 @@ class DeviceBert:
         kept: a call on another stream is ordered behind the last one's by the caller.
 
         spans (int32 [n, 2] on the device): the sequences are these spans of the S*L rows, first row and one past
-        the last, ascending (enchip_attention_bias_dev); what h holds in rows of none means nothing. pos (int32
+        the last, ascending (enchip_attention_bias_dev; a list of a fixed number of them is filled up with S*L, S*L); what h holds in rows of none means nothing. pos (int32
         [S*L]): the rows' positions for `rope`, else row % L. ids (int32 [S*L]): the rows' adapters."""
         c, D, H, hd, M, W = self.ctx, self.D, self.H, self.hd, S * L, self.W
         self._floats("h", h, M)

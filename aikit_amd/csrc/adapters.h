@@ -14,7 +14,7 @@
 // Rows of a block that have different adapters: each adapter among them in turn, from the lowest such row on.
 // What is added to a row without one is -0, the number that leaves every sum as it was: +0 makes a -0 of y's a +0.
 //
-// Bound by memory where rows are many: 32768 x 1024 to 1024, rank 16, rows of 8 adapters, take 97 us on MI355X, 41 in
+// Bound by memory where rows are many: 32768 x 1024 to 1024, rank 16, rows of 8 adapters, take 97 to 107 us on MI355X, 41 in
 // adapter_down (134 MB of rows, 34 of codes: 4.1 TB/s) and 57 in the product (34 MB of codes, 134 of outputs;
 // 69 G int8 operations). A pass of its own for the codes, one for the low-rank parts and one for y took 186. 1500 x 1000
 // to 1001 with GELU 8 + 11 us, 512 x 1024 beside 4096 outputs at rank 64 4.5 + 7.4: loads' latency, a workgroup a CU
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(64 * GV_WAVES) void gemv_w8a8_adapters(
 }
 
 // The same in one launch, the rows quantized and their low-rank parts formed by every workgroup (16 rows, K = 384,
-// N = 1536, rank 8: 5.9 us, where two launches take 8.3 and up to 15 for 16 different adapters).
+// N = 1536, rank 8: 5.8 us, where two launches take 11, and 22 for 16 different adapters).
 template <int EPI, int QCH>
 __global__ __launch_bounds__(64 * GVQ_WAVES) void gemv_w8a8_q_adapters(
     const float *__restrict__ a, const int8_t *__restrict__ Wf, const float *__restrict__ wS,

@@ -15,9 +15,10 @@
 // Bound by the products, 12 len^2 hd flops a head in three f16 parts, and by what stands between them (per score an
 // exponential, a split into two parts, the maximum). Two blocks of 32 queries a wavefront give the products independent
 // sums to run on and halve the loads of keys from LDS, where the registers allow it (heads of 32 and 64). On MI355X,
-// flops of the formula (4 len^2 hd) a second: 64 x 512 rows of 12 heads of 64 179 us, 288 TF; 8192 rows 547 us, 377 TF
+// flops of the formula (4 len^2 hd) a second: 64 x 512 rows of 12 heads of 64 183 us, 282 TF; 8192 rows 550 us, 375 TF
 // (a third of a large f16 product's rate is 361); 20011 rows of documents of 1 to 1024, 16 heads of 128 that share 4 key
-// heads, longest first 296 us, 275 TF (317 as they come). 1 x 512 rows take 12.3 us and 1 x 16 5.1, a call's latency.
+// heads, longest first 302 us, 270 TF. 1 x 512 rows take 12.3 us and 1 x 16 5.0, a call's latency. Values decide too: scores
+// of twice the spread take up to 3% longer now that small weights hold bits, which the products' zeros had saved.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -584,10 +584,14 @@ void launch_linear(enchip_ctx *c, const Weight &w, const int8_t *aq, const float
 
 // Few rows in one launch (gemv_w8a8_q_adapters): every workgroup of 32 columns quantizes its 8 rows and forms their
 // low-rank parts again, so A is small (its 16 rt rows of a slot, once a row a workgroup) and the launch about two
-// workgroups a CU at rt = 1. LDS stays under 64 KiB. One launch against two, us, rows of mixed adapters (of one):
-//   16 rows, K = 384, N = 1536, rank 8   6.2, 15.3 (10.8)    16 rows, K = 768, N = 768, rank 32   10.6, 22.7 (16.2)
-//   32 rows, K = 768, N = 2304, rank 16 (288 workgroups)  12.3, 23.5 (16.4); rank 32 19.0, 23.4 (17.1): two
-//   32 rows, K = 1024, N = 4096, rank 16 (512 workgroups)  17.0, 25.7 (17.1); rank 32 27.2, 26.2 (17.9): two
+// workgroups a CU at rt = 1. LDS stays under 64 KiB. One launch against two, us, every row another adapter of 32
+// (all rows one adapter's):
+//   16 rows, K = 384, N = 1536, rank 8    6.0 against 22.4 (5.8 against 11.1)
+//   16 rows, K = 768, N = 768, rank 32    10.8 against 29.2 (10.7 against 13.8)
+//   32 rows, K = 768, N = 2304, rank 16 (288 workgroups)     12.8 against 29.5 (12.4 against 14.0)
+//   32 rows, K = 1024, N = 4096, rank 16 (512 workgroups)    19.1 against 38.2 (17.6 against 15.0)
+// and past it two: 32 rows, K = 768, N = 2304, rank 32 36.5 (15.0), K = 1024, N = 4096, rank 32 45.4 (16.0), where one took
+// 19.0 and 27.2 with 8 adapters. Two would win only where most rows share an adapter, which the host does not know.
 bool one_launch(const enchip_ctx *c, const Weight &w, const AdapterSet &set, int64_t M, const float *d_a) {
     const int64_t groups = (w.N + 31) / 32 * ((M + enchip::GVQ_ROWS - 1) / enchip::GVQ_ROWS);
     return M <= c->small_m && M <= 32 && w.K <= 1024 && w.K % 4 == 0 && (uintptr_t)d_a % 16 == 0 &&
