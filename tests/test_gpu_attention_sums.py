@@ -26,22 +26,24 @@ def say(msg):
     print(f"[case] {msg}", flush=True)
 
 
-def run(ctx, x, heads, hd, scale, before, after, n):
+def run(ctx, x, heads, hd, scale, before, after, n, kv=None, pad=0):
     """n rows among spans of no rows, every head the same columns of x [n, 3 hd]."""
     import torch
 
-    W = heads * hd
+    W, kv = heads * hd, kv or heads
     one = torch.from_numpy(x).cuda()
-    d = torch.cat([one[:, i * hd:(i + 1) * hd].repeat(1, heads) for i in range(3)], dim=1).contiguous()
-    out = torch.full((n, W), 3.0, device="cuda")
+    d = torch.cat([one[:, i * hd:(i + 1) * hd].repeat(1, k) for i, k in enumerate((heads, kv, kv))], dim=1).contiguous()
+    ld, ldo = d.shape[1], W + pad
+    out = torch.full((n, ldo), 3.0, device="cuda")
     spans = [(0, 0)] * before + [(0, n)] + [(n, n)] * after
     sp = torch.tensor(spans, dtype=torch.int32, device="cuda") if before + after else None
     p = d.data_ptr()
     torch.cuda.synchronize()
-    ctx.attention_bias_dev(None, p, 3 * W, p + 4 * W, 3 * W, p + 8 * W, 3 * W, out.data_ptr(), W, len(spans), n, heads, heads, hd, scale,
+    ctx.attention_bias_dev(None, p, ld, p + 4 * W, ld, p + 4 * (W + kv * hd), ld, out.data_ptr(), ldo, len(spans), n, heads, kv, hd, scale,
                            0 if sp is None else sp.data_ptr())
     torch.cuda.synchronize()
-    got = out.reshape(n, heads, hd)
+    assert (out[:, W:] == 3.0).all()
+    got = out[:, :W].reshape(n, heads, hd)
     assert (got == got[:, :1]).all()  # no head differs from another
     return got[:, 0].cpu().numpy()
 
@@ -140,3 +142,23 @@ def test_the_fused_attention_without_a_bias(ctx, hd, heads, gap, sign):
     got = out.reshape(n, heads, hd)
     assert (got == got[:, :1]).all()
     held(got[:, 0].cpu().numpy(), x, n, hd, scale, sink, 2.0 ** -32)
+
+
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_long_rows_into_outputs_of_any_pitch(ctx, hd, form):
+    # what is set aside stands in the outputs' place
+    n, scale, sink = 8192 + 37, hd ** -0.5, 4000
+    say(f"attention_bias {n} rows, outputs 3 floats apart, hd={hd}, {form}")
+    x = one_above(n, hd, scale, sink, 17.0)
+    want = run(ctx, x, hd=hd, scale=scale, n=n, **FORMS[form])
+    assert (run(ctx, x, hd=hd, scale=scale, n=n, pad=3, **FORMS[form]) == want).all()
+
+
+@pytest.mark.parametrize("form", ["whole", "ordered"])
+@pytest.mark.parametrize("hd,heads,kv", [(32, 64, 8), (64, 64, 16), (128, 48, 12), (64, 48, 24)])
+def test_long_rows_of_heads_that_share_keys(ctx, hd, heads, kv, form):
+    n, scale, sink = 8192 + 37, hd ** -0.5, 4000
+    say(f"attention_bias {n} rows, {heads} heads of {hd} on {kv}, {form}")
+    x = one_above(n, hd, scale, sink, 17.0)
+    held(run(ctx, x, hd=hd, scale=scale, n=n, kv=kv, **dict(FORMS[form], heads=heads)), x, n, hd, scale, sink, 2.0 ** -36)
