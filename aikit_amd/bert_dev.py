@@ -140,6 +140,7 @@ class DeviceBert:
                                torch.from_numpy(np.ascontiguousarray(s)).to(dev))
             self.handles.append(entry)
         self._bufs = {}
+        self._captured = []  # buffers that a graph holds the addresses of
         self._emb = None
         # Optional callback mark(label) called before each device operation this object
         # enqueues (and with "end" after the last), for per-operation timing; None: off.
@@ -188,7 +189,7 @@ class DeviceBert:
                 if name in entry:
                     self.ctx.release_weight(entry[name][0])
         self.handles = []
-        self._bufs = {}
+        self._bufs, self._captured = {}, []
 
     def bias_attention(self, spans=None) -> bool:
         """Whether the attention is enchip_attention_bias_dev's."""
@@ -241,6 +242,8 @@ class DeviceBert:
         if scores and b["scores"].numel() < S * self.H * L * L:  # beside the others, whose addresses a graph may hold
             with self._on(stream):
                 b["scores"] = t.empty((S, self.H, L, L), **f)
+        if t.cuda.is_current_stream_capturing() and not any(c is b for c in self._captured):
+            self._captured.append(b)
         return b
 
     def _ints(self, name: str, t, shape) -> int:
@@ -260,7 +263,8 @@ class DeviceBert:
 
     def forward(self, h, S: int, L: int, stream: int = 0, spans=None, pos=None, ids=None) -> None:
         """Runs every layer on h ([S*L, D] f32 on the device), in place, on `stream`. One shape's activations are
-        kept: a call on another stream is ordered behind the last one's by the caller.
+        kept, and until close() those of shapes that torch.cuda.graph captured: a call on another stream is ordered
+        behind the last one's by the caller.
 
         spans (int32 [n, 2] on the device): the sequences are these spans of the S*L rows, first row and one past
         the last, ascending (enchip_attention_bias_dev; a list of a fixed number of them is filled up with S*L, S*L); what h holds in rows of none means nothing. pos (int32

@@ -172,3 +172,37 @@ def test_more_spans_than_one_call_pools(ctx, model):
     assert (many[-1] == 5.0).all() and (many[:n][empty] == 0).all()
     # the order of the attention's sums goes by L / n: codes on a rounding border, the encoders' bar of 0.9999
     assert (np.linalg.norm(many[some] - few[:-1], axis=1) <= (2e-4) ** 0.5).all()
+
+
+def test_a_captured_shape_keeps_its_buffers(ctx, model):
+    # a graph's replay writes where its shape's buffers were: they are nobody else's after other shapes have run
+    import torch
+
+    st = torch.cuda.Stream()
+    S, L = SHAPES[0]
+    x, h = hidden(torch, S, L), hidden(torch, S, L)
+    p = torch.zeros((S, D), device="cuda")
+    torch.cuda.synchronize()
+    model.embed(h, S, L, p, st.cuda_stream)
+    torch.cuda.synchronize()
+    want = p.cpu().numpy()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        model.embed(h, S, L, p, st.cuda_stream)
+    say("a captured shape, other shapes, tensors of its buffers' sizes, its replays")
+    for rep in range(3):
+        for S2, L2 in SHAPES[1:] + [(1, 17)]:
+            h2, p2 = hidden(torch, S2, L2), torch.zeros((S2, D), device="cuda")
+            torch.cuda.synchronize()
+            model.embed(h2, S2, L2, p2, st.cuda_stream)
+        with torch.cuda.stream(st):
+            mine = [torch.full((S * L, w), 7.0, device="cuda") for w in (3 * D, D, I, D, D) for _ in range(3)]
+            h.copy_(x)
+            p.zero_()
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(p.cpu().numpy(), want), rep
+        for t in mine:
+            assert (t == 7.0).all(), rep
+    del gr
